@@ -108,7 +108,7 @@ def _pow2(e):
 def _scale_exp(amax, frac, shift):
     """Smallest k >= -126 with amax <= frac * 2^(shift + k), as int32."""
     f, e = torch.frexp(amax)
-    return (e.int() - shift + (f > frac).int()).clamp_(min=-126)
+    return torch.where(amax > 0, e.int() - shift + (f > frac).int(), -126).clamp_(min=-126)
 
 
 def _blocks(x):
