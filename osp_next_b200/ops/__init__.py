@@ -14,6 +14,7 @@ import torch
 
 from . import reference as ref
 from ._ext import ext, available  # noqa: F401
+from .fp8 import Fp8Tensor, adamw8_decode, adamw8_state, adamw_multi_, fp8_matmul, fp8_quantize  # noqa: F401
 
 _BF16 = torch.bfloat16
 
@@ -442,6 +443,8 @@ def hif8_quant_dequant(x, scale_max: float = 15.0):
 
 ERROR_NAMES = {
     101: "GEMM producer wait", 102: "GEMM MMA wait", 103: "GEMM epilogue wait", 104: "GEMM teardown",
+    111: "fp8 product producer wait", 112: "fp8 product MMA wait", 113: "fp8 product epilogue wait",
+    114: "fp8 product teardown",
     201: "attention producer wait", 202: "attention MMA wait", 203: "attention softmax wait",
     204: "attention teardown", 205: "attention shared-memory alignment",
     301: "NVLink peer barrier timeout", 302: "NVLink peer barrier slot mismatch",

@@ -1,0 +1,345 @@
+// AdamW over a list of tensors in one launch per 480 of them (the framework's per-tensor kernel
+// is adamw in misc.cu), with the moments in fp32 or in 8 bits.
+//
+//   g' = g grad_scale;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8-bit moments: each run of 128 elements of a tensor has one power-of-two scale per moment
+// (byte e = log2 + 127, the smallest that brings the largest magnitude into range).  m is e4m3;
+// v is the top byte of an IEEE half without its sign (5 exponent bits, 3 mantissa bits,
+// largest value 61440, 255 = NaN): the square needs twice the exponent range and no sign.
+// Both are rounded stochastically: at b2 = 0.999 a step changes v by a thousandth, far below
+// half a step of 3 mantissa bits (3 to 6 %), so nearest rounding would never let v move; with
+// probability in proportion to the remainder the stored averages stay unbiased.  A positive v
+// is never stored as 0, which would divide the next m by eps alone.  The update itself uses
+// the unrounded moments.
+//
+// Bound by memory: 16 bytes per element with fp32 p and g and 8-bit moments (28 with fp32
+// ones).  A warp takes 128 elements at a time, so the block maximum is one warp reduction and
+// each of its loads and stores is one contiguous segment.  The list travels in the kernel's
+// parameters (up to 32 KB): no table is copied or kept between calls.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cmath>
+
+#include "common.cuh"
+#include "fp8.cuh"
+#include "tma_host.h"
+
+namespace osp {
+namespace adamw8 {
+
+constexpr int kCap = 480;                 // tensors per launch: 480 x 64 B + constants < 32764 B
+constexpr int kChunkBlocks = 32;          // 128-element runs per CTA visit (8 warps x 4)
+constexpr uint32_t kMix1 = 0x6A09E667u, kMix2 = 0xBB67AE85u, kMix3 = 0x3C6EF373u;   // fractions of sqrt 2, 3, 5
+
+// c1 = 1 - b1, c2 = 1 - b2, keep = 1 - lr wd, rate = lr / (1 - b1^t), bc2s = sqrt(1 - b2^t): formed in
+// 64 bits on the host (1 - fp32(0.999) alone would be off by a 75000th).
+struct Consts {
+  float b1, b2, c1, c2, eps, keep, rate, bc2s, gscale;
+};
+struct Args {
+  void* p[kCap];
+  const void* g[kCap];
+  void* m[kCap];
+  void* v[kCap];
+  uint8_t* ms[kCap];
+  uint8_t* vs[kCap];
+  int64_t n[kCap];
+  int chunk_end[kCap];                    // chunks of tensors 0..i
+  uint32_t key[kCap];
+  int tensors;
+  Consts c;
+};
+static_assert(sizeof(Args) <= 32764, "kernel parameters");
+
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x = (x ^ (x >> 16)) * kMix1;
+  x = (x ^ (x >> 15)) * kMix2;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 ld4(const __nv_bfloat16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void st4(__nv_bfloat16* p, float4 v) {
+  uint2 u;
+  u.x = pack_bf16x2(v.x, v.y);
+  u.y = pack_bf16x2(v.z, v.w);
+  *reinterpret_cast<uint2*>(p) = u;
+}
+__device__ __forceinline__ float ld1(const float* p) { return *p; }
+__device__ __forceinline__ float ld1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void st1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st1(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+
+// Four elements, of which `left` (1..4) exist; `wide`: aligned for one vector access.
+template <typename T>
+__device__ __forceinline__ void load(const T* p, bool wide, int left, float* o) {
+  if (wide && left >= 4) {
+    const float4 f = ld4(p);
+    o[0] = f.x; o[1] = f.y; o[2] = f.z; o[3] = f.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = j < left ? ld1(p + j) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store(T* p, bool wide, int left, const float* o) {
+  if (wide && left >= 4) {
+    st4(p, make_float4(o[0], o[1], o[2], o[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) st1(p + j, o[j]);
+  }
+}
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, bool wide, int left) {
+  if (wide && left >= 4) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t u = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < left) u |= (uint32_t)p[j] << (8 * j);
+  return u;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, bool wide, int left, uint32_t u) {
+  if (wide && left >= 4) {
+    *reinterpret_cast<uint32_t*>(p) = u;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = (uint8_t)(u >> (8 * j));
+  }
+}
+
+__device__ __forceinline__ void decode_m(uint32_t u, uint32_t byte, float* o) {
+  const float s = __uint_as_float(byte << 23);
+  const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u & 0xFFFF), __NV_E4M3);
+  const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> 16), __NV_E4M3);
+  const float2 fa = __half22float2(__half2(a)), fb = __half22float2(__half2(b));
+  o[0] = fa.x * s; o[1] = fa.y * s; o[2] = fb.x * s; o[3] = fb.y * s;
+}
+__device__ __forceinline__ void decode_v(uint32_t u, uint32_t byte, float* o) {
+  const float s = __uint_as_float(byte << 23);
+  const uint32_t lo = __byte_perm(u, 0, 0x4140) << 7, hi = __byte_perm(u, 0, 0x4342) << 7;
+  const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  o[0] = fa.x * s; o[1] = fa.y * s; o[2] = fb.x * s; o[3] = fb.y * s;
+}
+
+// Stochastic rounding on the fp32 bits: add 20 random bits (16 and four zeros) below the three
+// mantissa bits kept, then cut.  Magnitudes below the least normal 2^-E are lifted by 2^-E
+// first, where the kept bits have the subnormal step.
+__device__ __forceinline__ uint32_t encode_m(float m, float inv, uint32_t r16) {
+  const float y = m * inv, a = fabsf(y);
+  const bool small = a < 0.015625f;                                   // 2^-6
+  const uint32_t t = __float_as_uint(small ? a + 0.015625f : a) + (r16 << 4);
+  return ((t >> 20) - (small ? 968u : 960u)) | ((__float_as_uint(y) >> 24) & 0x80u);
+}
+__device__ __forceinline__ uint32_t encode_v(float v, float inv, uint32_t r16) {
+  const float a = v * inv;
+  const bool small = a < 6.103515625e-05f;                            // 2^-14
+  const uint32_t t = __float_as_uint(small ? a + 6.103515625e-05f : a) + (r16 << 4);
+  const uint32_t code = (t >> 20) - (small ? 904u : 896u);
+  return max(code, v > 0.f ? 1u : 0u);
+}
+// Scale byte of a block of v: 61440 = 1.875 * 2^15.
+__device__ __forceinline__ uint32_t scale_byte_v(uint32_t vmax) {
+  return (uint32_t)max((int)((vmax + 0x0FFFFFu) >> 23) - 15, 1);
+}
+
+template <typename PT, typename GT, bool STATE8>
+__global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ Args args) {
+  const Consts c = args.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = args.chunk_end[args.tensors - 1];
+  for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    int lo = 0, hi = args.tensors - 1;               // first tensor with chunk < chunk_end
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (chunk < args.chunk_end[mid]) hi = mid;
+      else lo = mid + 1;
+    }
+    const int64_t n = args.n[lo];
+    const int64_t blk0 = (int64_t)(chunk - (lo ? args.chunk_end[lo - 1] : 0)) * kChunkBlocks;
+    PT* p = reinterpret_cast<PT*>(args.p[lo]);
+    const GT* g = reinterpret_cast<const GT*>(args.g[lo]);
+    const bool wide_p = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(PT)) == 0;
+    const bool wide_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(GT)) == 0;
+    const uint32_t key = args.key[lo];
+    for (int b = warp; b < kChunkBlocks; b += 8) {
+      const int64_t blk = blk0 + b;
+      const int64_t i = blk * 128 + lane * 4;
+      if (blk * 128 >= n) break;                     // whole warp
+      const int left = (int)min((int64_t)4, n - i);  // below 1: this lane has none
+      float pv[4], gv[4], mv[4], vv[4];
+      load(p + i, wide_p, left, pv);
+      load(g + i, wide_g, left, gv);
+      if constexpr (STATE8) {
+        uint8_t* mq = reinterpret_cast<uint8_t*>(args.m[lo]);
+        uint8_t* vq = reinterpret_cast<uint8_t*>(args.v[lo]);
+        const bool wide_m = reinterpret_cast<uintptr_t>(mq) % 4 == 0, wide_v = reinterpret_cast<uintptr_t>(vq) % 4 == 0;
+        decode_m(load_codes(mq + i, wide_m, left), args.ms[lo][blk], mv);
+        decode_v(load_codes(vq + i, wide_v, left), args.vs[lo][blk], vv);
+        uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // written with explicit roundings (no contraction), so that the stored codes are
+          // reproducible from the formula
+          const float gj = __fmul_rn(gv[j], c.gscale);
+          mv[j] = __fadd_rn(__fmul_rn(mv[j], c.b1), __fmul_rn(gj, c.c1));
+          vv[j] = __fadd_rn(__fmul_rn(vv[j], c.b2), __fmul_rn(__fmul_rn(gj, gj), c.c2));
+          mtop = max(mtop, __float_as_uint(mv[j]) & 0x7FFFFFFFu);
+          vtop = max(vtop, __float_as_uint(vv[j]) & 0x7FFFFFFFu);
+          const float den = sqrtf(vv[j]) / c.bc2s + c.eps;
+          pv[j] = pv[j] * c.keep - c.rate * (mv[j] / den);
+        }
+        store(p + i, wide_p, left, pv);
+        const bool bad = __any_sync(0xffffffffu, max(mtop, vtop) >= fp8::kInfBits);
+        if (bad) {
+          mtop = vtop = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a = __float_as_uint(mv[j]) & 0x7FFFFFFFu, b2 = __float_as_uint(vv[j]) & 0x7FFFFFFFu;
+            mtop = max(mtop, a >= fp8::kInfBits ? 0u : a);
+            vtop = max(vtop, b2 >= fp8::kInfBits ? 0u : b2);
+          }
+        }
+        const uint32_t mb = fp8::scale_byte(__reduce_max_sync(0xffffffffu, mtop));
+        const uint32_t vb = scale_byte_v(__reduce_max_sync(0xffffffffu, vtop));
+        const float minv = fp8::inv_scale(mb), vinv = fp8::inv_scale(vb);
+        uint32_t mu = 0, vu = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t r = mix((uint32_t)(i + j) + key);
+          uint32_t cm = encode_m(mv[j], minv, r & 0xFFFFu), cv = encode_v(vv[j], vinv, r >> 16);
+          if (bad) {
+            if (!isfinite(mv[j])) cm = 0x7Fu | (cm & 0x80u);
+            if (!isfinite(vv[j])) cv = 255u;
+          }
+          mu |= (cm & 0xFFu) << (8 * j);
+          vu |= (cv & 0xFFu) << (8 * j);
+        }
+        store_codes(mq + i, wide_m, left, mu);
+        store_codes(vq + i, wide_v, left, vu);
+        if (lane == 0) {
+          args.ms[lo][blk] = (uint8_t)mb;
+          args.vs[lo][blk] = (uint8_t)vb;
+        }
+      } else {
+        float* m = reinterpret_cast<float*>(args.m[lo]);
+        float* v = reinterpret_cast<float*>(args.v[lo]);
+        const bool wide_m = reinterpret_cast<uintptr_t>(m) % 16 == 0, wide_v = reinterpret_cast<uintptr_t>(v) % 16 == 0;
+        load(m + i, wide_m, left, mv);
+        load(v + i, wide_v, left, vv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float gj = gv[j] * c.gscale;
+          mv[j] = c.b1 * mv[j] + c.c1 * gj;
+          vv[j] = c.b2 * vv[j] + c.c2 * gj * gj;
+          pv[j] = pv[j] * c.keep - c.rate * (mv[j] / (sqrtf(vv[j]) / c.bc2s + c.eps));
+        }
+        store(p + i, wide_p, left, pv);
+        store(m + i, wide_m, left, mv);
+        store(v + i, wide_v, left, vv);
+      }
+    }
+  }
+}
+
+template <typename PT, typename GT>
+static void launch(const Args& a, bool state8, int device, cudaStream_t stream) {
+  const int chunks = a.chunk_end[a.tensors - 1];
+  const int grid = std::min(chunks, num_sms(device) * 8);
+  if (state8) step_kernel<PT, GT, true><<<grid, 256, 0, stream>>>(a);
+  else step_kernel<PT, GT, false><<<grid, 256, 0, stream>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+}  // namespace adamw8
+
+// In place on every tensor of the lists; ms / vs empty: fp32 moments.
+void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vector<at::Tensor> m,
+                 std::vector<at::Tensor> v, std::vector<at::Tensor> ms, std::vector<at::Tensor> vs, double lr,
+                 double b1, double b2, double eps, double wd, int64_t step, double gscale, int64_t seed) {
+  using namespace adamw8;
+  const size_t count = p.size();
+  const bool state8 = !ms.empty() || !vs.empty();
+  TORCH_CHECK(g.size() == count && m.size() == count && v.size() == count &&
+              (!state8 || (ms.size() == count && vs.size() == count)), "adamw_multi_: lists of one length");
+  if (count == 0) return;
+  TORCH_CHECK(step >= 1, "adamw_multi_: step counts from 1");
+  const auto pt = p[0].scalar_type(), gt = g[0].scalar_type();
+  TORCH_CHECK(pt == at::kFloat || pt == at::kBFloat16, "adamw_multi_: parameters fp32 or bf16");
+  TORCH_CHECK(gt == at::kFloat || gt == at::kBFloat16, "adamw_multi_: gradients fp32 or bf16");
+  TORCH_CHECK(p[0].is_cuda(), "adamw_multi_: CUDA tensors");
+  const int dev = p[0].get_device();
+  const auto mt = state8 ? at::kFloat8_e4m3fn : at::kFloat, vt = state8 ? at::kByte : at::kFloat;
+  auto good = [&](const at::Tensor& t, at::ScalarType dt, int64_t n) {
+    return t.is_cuda() && t.get_device() == dev && t.scalar_type() == dt && t.is_contiguous() && t.numel() == n;
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const int64_t n = p[i].numel();
+    TORCH_CHECK(good(p[i], pt, n) && good(g[i], gt, n) && good(m[i], mt, n) && good(v[i], vt, n),
+                "adamw_multi_: tensor ", std::to_string(i), ": p, g and moments contiguous, of one size and device, p and g of one "
+                "type throughout, moments ", state8 ? "e4m3 and uint8" : "fp32");
+    if (state8)
+      TORCH_CHECK(good(ms[i], at::kByte, (n + 127) / 128) && good(vs[i], at::kByte, (n + 127) / 128),
+                  "adamw_multi_: tensor ", std::to_string(i), ": one uint8 scale per 128 elements and moment");
+  }
+  c10::cuda::CUDAGuard guard(p[0].device());
+  auto stream = c10::cuda::getCurrentCUDAStream();
+  Args a;
+  a.c.b1 = (float)b1;
+  a.c.b2 = (float)b2;
+  a.c.c1 = (float)(1.0 - b1);
+  a.c.c2 = (float)(1.0 - b2);
+  a.c.eps = (float)eps;
+  a.c.keep = (float)(1.0 - lr * wd);
+  a.c.rate = (float)(lr / (1.0 - std::pow(b1, (double)step)));
+  a.c.bc2s = (float)std::sqrt(1.0 - std::pow(b2, (double)step));
+  a.c.gscale = (float)gscale;
+  a.tensors = 0;
+  int64_t chunks = 0;
+  auto flush = [&]() {
+    if (a.tensors == 0) return;
+    if (pt == at::kFloat) {
+      if (gt == at::kFloat) launch<float, float>(a, state8, dev, stream);
+      else launch<float, __nv_bfloat16>(a, state8, dev, stream);
+    } else {
+      if (gt == at::kFloat) launch<__nv_bfloat16, float>(a, state8, dev, stream);
+      else launch<__nv_bfloat16, __nv_bfloat16>(a, state8, dev, stream);
+    }
+    a.tensors = 0;
+    chunks = 0;
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const int64_t n = p[i].numel();
+    if (n == 0) continue;
+    const int64_t mine = ((n + 127) / 128 + kChunkBlocks - 1) / kChunkBlocks;
+    TORCH_CHECK(mine < (int64_t(1) << 30), "adamw_multi_: tensor ", std::to_string(i), " too large");
+    if (a.tensors == kCap || chunks + mine >= (int64_t(1) << 31)) flush();
+    const int t = a.tensors++;
+    chunks += mine;
+    a.p[t] = p[i].data_ptr();
+    a.g[t] = g[i].data_ptr();
+    a.m[t] = m[i].data_ptr();
+    a.v[t] = v[i].data_ptr();
+    a.ms[t] = state8 ? ms[i].data_ptr<uint8_t>() : nullptr;
+    a.vs[t] = state8 ? vs[i].data_ptr<uint8_t>() : nullptr;
+    a.n[t] = n;
+    a.chunk_end[t] = (int)chunks;
+    a.key[t] = mix((uint32_t)i * kMix3 + (uint32_t)seed);
+  }
+  flush();
+}
+
+}  // namespace osp

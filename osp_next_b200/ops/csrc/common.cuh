@@ -19,6 +19,7 @@ constexpr uint64_t kWaitLimitNs = 2000000000ull;   // 2 s
 enum : int {
   kErrNone = 0,
   kErrGemmProducer = 101, kErrGemmMma = 102, kErrGemmEpilogue = 103, kErrGemmTeardown = 104,
+  kErrFp8Producer = 111, kErrFp8Mma = 112, kErrFp8Epilogue = 113, kErrFp8Teardown = 114,
   kErrAttnProducer = 201, kErrAttnMma = 202, kErrAttnSoftmax = 203, kErrAttnTeardown = 204,
   kErrAttnLayout = 205,
   kErrP2P = 301, kErrP2PTag = 302,

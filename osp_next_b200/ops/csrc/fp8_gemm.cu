@@ -1,0 +1,441 @@
+// Block-scaled fp8 product for sm_100a:  D[M,N] = act( sum_kb sa[m,kb] sb[n,kb] sum_{k in kb} a[m,k] b[n,k] + bias[n] )
+// with e4m3 codes and power-of-two scales in the format of fp8.cuh, both operands K-major.
+//
+// The scales are applied by the tensor core: tcgen05.mma kind::mxf8f6f4.block_scale multiplies
+// each group of 32 along K by a power of two per row of A and per row of B, read from TMEM.
+// A block of 128 is four such groups with one scale, so the four MMAs of a block name the same
+// byte of the scale words.  Products and sums stay in the fp32 accumulator over the whole of K;
+// there is no second accumulation in registers, and the epilogue sees the finished sum.
+//
+// Structure (one CTA per SM, 320 threads), as in the bf16 product:
+//   warp 0      TMA producer: 128 x 128 codes of A and BN x 128 of B per stage (128B swizzle);
+//               with every fourth block, the 512-byte scale chunks of the next four
+//   warp 1      one thread issues tcgen05.cp (scale chunk -> TMEM, once per four blocks) and
+//               tcgen05.mma 128 x BN x 32, into one of two accumulators
+//   warps 2..9  epilogue: two groups of four warps, half of the tile's columns each
+// TMEM (512 columns): two accumulators of 256 columns and 16 columns of scales do not fit, so
+// at BN = 256 the accumulators overlap by 16 columns: accumulator 0 is 0..255, accumulator 1
+// 240..495, scales 496..511.  The epilogue reads the shared columns first and tells the MMA
+// warp so; the next tile then starts while the rest is still being read.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "common.cuh"
+#include "fp8.cuh"
+#include "tma_host.h"
+
+namespace osp {
+namespace fp8 {
+
+constexpr int kBM = 128;
+constexpr int kBK = 128;                      // one scale block, one 128-byte swizzle span
+constexpr int kGroupM = 16;
+constexpr int kThreads = 320;
+constexpr int kStageRow = 80;                 // bytes per staged output row (64 + 16 pad)
+constexpr int kStageBytes = 32 * kStageRow;
+constexpr uint32_t kScaleCol = 496;           // TMEM columns of the scales: A 496..499, B 500..507
+
+template <int BN> struct Shape {
+  static constexpr int kChunksB = BN > 128 ? 2 : 1;             // 128-row scale chunks of a B tile
+  static constexpr uint32_t kA = kBM * kBK, kB = BN * kBK;
+  static constexpr uint32_t kScales = kChunkBytes * (1 + kChunksB);
+  static constexpr int kStages = 196608 / (kA + kB) > 8 ? 8 : 196608 / (kA + kB);
+  static constexpr uint32_t kAccStride = BN == 256 ? 240 : BN;  // column offset of accumulator 1
+  static constexpr bool kOverlap = BN == 256;
+  static constexpr int smem_bytes() {
+    return 1024 + kStages * (int)(kA + kB + kScales) + (2 * kStages + 7) * 8 + 16 + 128 + 8 * kStageBytes;
+  }
+};
+
+struct Args {
+  int M, N, KB;              // KB: blocks of 128 along K
+  const uint8_t* sa;         // packed scales of A, of B
+  const uint8_t* sb;
+  const float* bias;         // [N] or null
+  int act;                   // 0 none, 1 gelu_tanh
+  void* out;                 // [M, N] bf16 or f32
+  __nv_bfloat16* aux;        // [M, N] pre-activation or null
+  int vec;                   // rows of out (and aux) start on 16 bytes
+  int* err;
+};
+
+__device__ __forceinline__ void bulk_load(uint64_t* bar, void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// One 512-byte scale chunk -> 4 TMEM columns, repeated in each quarter of the lanes.
+__device__ __forceinline__ void cp_scales(uint32_t tmem, uint32_t saddr) {
+  // no swizzle; 8-row core matrices of 16-byte rows, 128 bytes apart
+  const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1u << 46);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(d) : "memory");
+}
+__device__ __forceinline__ void umma_mxf8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate) : "memory");
+}
+// e4m3 x e4m3 with power-of-two scales; the scale-byte numbers go into bits 4 (B) and 29 (A).
+__host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N) {
+  return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int& mb, int& nb) {
+  const int per_group = kGroupM * num_n;
+  const int g = t / per_group;
+  const int first_m = g * kGroupM;
+  const int gsize = min(num_m - first_m, kGroupM);
+  const int r = t - g * per_group;
+  mb = first_m + r % gsize;
+  nb = r / gsize;
+}
+
+__device__ __forceinline__ float gelu_tanh_f(float x) {
+  return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
+}
+
+__device__ __forceinline__ void store_scalar(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_scalar(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+
+// A warp's 32 rows x 32 columns of results (one row per lane) -> out, through shared memory so
+// that a row's 64 bytes (bf16) are written as one segment; fp32 rows are full lines as they are.
+template <typename OutT>
+__device__ __forceinline__ void store_chunk(OutT* out, const float* v, uint8_t* stg, int lane, long row0, int col0,
+                                            int M, int N, bool vec) {
+  if (!vec || col0 + 32 > N) {
+    const long row = row0 + lane;
+    if (row < M) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < N) store_scalar(out + row * N + col0 + j, v[j]);
+    }
+    return;
+  }
+  if constexpr (sizeof(OutT) == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint4 w;
+      w.x = pack_bf16x2(v[8 * j + 0], v[8 * j + 1]);
+      w.y = pack_bf16x2(v[8 * j + 2], v[8 * j + 3]);
+      w.z = pack_bf16x2(v[8 * j + 4], v[8 * j + 5]);
+      w.w = pack_bf16x2(v[8 * j + 6], v[8 * j + 7]);
+      *reinterpret_cast<uint4*>(stg + lane * kStageRow + j * 16) = w;
+    }
+    __syncwarp();
+    const int q = lane >> 2, cc = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = i * 8 + q;
+      if (row0 + rr < M)
+        *reinterpret_cast<uint4*>(out + (row0 + rr) * N + col0 + cc * 8) =
+            *reinterpret_cast<const uint4*>(stg + rr * kStageRow + cc * 16);
+    }
+    __syncwarp();
+  } else if (row0 + lane < M) {
+    float4* o4 = reinterpret_cast<float4*>(out + (row0 + lane) * N + col0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o4[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+}
+
+template <int BN, typename OutT>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
+  using S = Shape<BN>;
+  constexpr int STAGES = S::kStages;
+  constexpr uint32_t IDESC = idesc_mxf8(kBM, BN);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + STAGES * S::kA;
+  uint8_t* sS = sB + STAGES * S::kB;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sS + STAGES * S::kScales);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;      // [2] accumulator finished
+  uint64_t* tempty = tfull + 2;          // [2] accumulator read
+  uint64_t* tearly = tempty + 2;         // [2] its columns shared with the other one read
+  uint64_t* done = tearly + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* epi_stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(abort_flag + 1) + 127) & ~uintptr_t(127));
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const int num_m = (args.M + kBM - 1) / kBM;
+  const int num_n = (args.N + BN - 1) / BN;
+  const int num_tiles = num_m * num_n;
+  const int num_kb = args.KB;
+  const int kgroups = (num_kb + 3) >> 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 8); mbar_init(&tearly[a], 4); }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0) {
+      const int last_chunk = (args.N + 127) / 128 - 1;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+        int mb, nb;
+        tile_coords(t, num_m, num_n, mb, nb);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrFp8Producer)) { *abort_flag = 1; break; }
+          const bool with_scales = (kb & 3) == 0;
+          mbar_expect_tx(&full[stage], S::kA + S::kB + (with_scales ? S::kScales : 0));
+          tma_load_2d(&tmA, &full[stage], sA + stage * S::kA, kb * kBK, mb * kBM);
+          tma_load_2d(&tmB, &full[stage], sB + stage * S::kB, kb * kBK, nb * BN);
+          if (with_scales) {
+            uint8_t* d = sS + stage * S::kScales;
+            bulk_load(&full[stage], d, args.sa + ((long)mb * kgroups + (kb >> 2)) * kChunkBytes, kChunkBytes);
+#pragma unroll
+            for (int c = 0; c < S::kChunksB; ++c) {
+              // a tile's second chunk may lie past the end of N: its rows are zeros, any scale will do
+              const int chunk = min(nb * BN / 128 + c, last_chunk);
+              bulk_load(&full[stage], d + (1 + c) * kChunkBytes,
+                        args.sb + ((long)chunk * kgroups + (kb >> 2)) * kChunkBytes, kChunkBytes);
+            }
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // after an abort nobody has waited for the last loads: let them land before the block ends
+      if (*abort_flag) {
+        for (int s = 0; s < STAGES; ++s) {
+          // stages before `stage` were filled in this round, the others in the one before it
+          const uint32_t p = s < stage ? phase : phase ^ 1;
+          mbar_wait(&full[s], p, args.err, kErrFp8Teardown);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      const uint32_t t_sa = tmem_base + kScaleCol;
+      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x, ++it) {
+        const int acc = it & 1;
+        const uint32_t acc_phase = (it >> 1) & 1;
+        bool ok = mbar_wait(&tempty[acc], acc_phase ^ 1, args.err, kErrFp8Mma);
+        // the previous tile's accumulator (use (it - 1) / 2 of it) shares columns with this one
+        if (ok && S::kOverlap && it > 0) ok = mbar_wait(&tearly[acc ^ 1], ((it - 1) >> 1) & 1, args.err, kErrFp8Mma);
+        if (!ok) { *abort_flag = 1; break; }
+        tc_fence_after();
+        // a 64-column tile takes the half of its 128-row scale chunk that is its own
+        uint32_t t_sb = t_sa + 4;
+        if (BN == 64) {
+          int mb, nb;
+          tile_coords(t, num_m, num_n, mb, nb);
+          t_sb += 2 * (nb & 1);
+        }
+        const uint32_t d_tmem = tmem_base + acc * S::kAccStride;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, args.err, kErrFp8Mma)) { ok = false; break; }
+          tc_fence_after();
+          if ((kb & 3) == 0) {
+            // cp and mma of one thread execute in order: the scales are in place for the
+            // MMAs below, and the MMAs before them have read the old ones
+            const uint32_t s_addr = smem_u32(sS + stage * S::kScales);
+            cp_scales(t_sa, s_addr);
+#pragma unroll
+            for (int c = 0; c < S::kChunksB; ++c) cp_scales(t_sa + 4 + 4 * c, s_addr + (1 + c) * kChunkBytes);
+          }
+          const uint32_t a_addr = smem_u32(sA + stage * S::kA);
+          const uint32_t b_addr = smem_u32(sB + stage * S::kB);
+          const uint32_t idesc = IDESC | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+#pragma unroll
+          for (int k = 0; k < kBK / 32; ++k)
+            umma_mxf8(d_tmem, sdesc_sw128(a_addr + k * 32, 16, 1024), sdesc_sw128(b_addr + k * 32, 16, 1024), idesc,
+                      t_sa, t_sb, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        umma_commit(&tfull[acc]);
+        if (!ok) { *abort_flag = 1; break; }
+      }
+      umma_commit(done);
+      mbar_wait(done, 0, args.err, kErrFp8Teardown);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (warps 2..9)
+    constexpr int PER = BN / 64;                // 32-column chunks of each of the two groups
+    const int quarter = warp & 3;               // TMEM lanes 32 * quarter ..
+    const int eg = (warp - 2) >> 2;
+    uint8_t* stg = epi_stage + (warp - 2) * kStageBytes;
+    int it = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, ++it) {
+      if (*abort_flag) break;
+      int mb, nb;
+      tile_coords(t, num_m, num_n, mb, nb);
+      const int acc = it & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (it >> 1) & 1, args.err, kErrFp8Epilogue))) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const long row0 = (long)mb * kBM + quarter * 32;
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * S::kAccStride;
+#pragma unroll 1
+      for (int i = 0; i < PER; ++i) {
+        // accumulator 0 shares its last columns, accumulator 1 its first: those go first
+        const int c = eg * PER + ((S::kOverlap && acc == 0) ? PER - 1 - i : i);
+        const int col0 = nb * BN + c * 32;
+        uint32_t r[32];
+        tmem_ld32(t_row + c * 32, r);
+        tmem_ld_wait();
+        if (S::kOverlap && i == 0 && eg == (acc ^ 1)) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tearly[acc]);
+        }
+        if (col0 >= args.N) continue;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        if (args.bias) {
+          if (col0 + 32 <= args.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __ldg(args.bias + col0 + j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col0 + j < args.N) v[j] += __ldg(args.bias + col0 + j);
+          }
+        }
+        if (args.aux) store_chunk(args.aux, v, stg, lane, row0, col0, args.M, args.N, args.vec);
+        if (args.act == 1) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = gelu_tanh_f(v[j]);
+        }
+        store_chunk(reinterpret_cast<OutT*>(args.out), v, stg, lane, row0, col0, args.M, args.N, args.vec);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// 2-D map over e4m3 codes [rows, Kp]: boxes of 128 bytes x box_rows, 128B swizzle, zeros outside.
+static CUtensorMap make_tmap(const at::Tensor& t, uint32_t box_rows) {
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {(cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
+  const cuuint64_t strides[1] = {(cuuint64_t)t.size(1)};
+  const cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows}, estr[2] = {1, 1};
+  const CUresult r = encode_tiled_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.data_ptr(), dims, strides, box, estr,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", std::to_string((int)r));
+  return m;
+}
+
+template <int BN, typename OutT>
+static void launch(const at::Tensor& a, const at::Tensor& b, const Args& args, cudaStream_t stream) {
+  const CUtensorMap tmA = make_tmap(a, kBM), tmB = make_tmap(b, BN);
+  auto kern = gemm_kernel<BN, OutT>;
+  constexpr int smem = Shape<BN>::smem_bytes();
+  static_assert(smem <= 232448, "shared memory");
+  smem_opt_in(reinterpret_cast<const void*>(kern), smem);
+  const int tiles = ((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
+  kern<<<std::min(tiles, num_sms(a.get_device())), kThreads, smem, stream>>>(tmA, tmB, args);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+}  // namespace fp8
+
+static void check_operand(const char* name, const at::Tensor& t, const at::Tensor& s, int64_t kp, int dev) {
+  TORCH_CHECK(t.is_cuda() && s.is_cuda() && t.get_device() == dev && s.get_device() == dev, "fp8_matmul: ", name,
+              " on the device of a");
+  TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn && t.dim() == 2 && t.is_contiguous() && t.size(1) == kp &&
+              kp % 128 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              "fp8_matmul: ", name, " e4m3 codes [rows, ", std::to_string(kp), "], contiguous, 16-byte aligned, K a multiple of 128");
+  TORCH_CHECK(s.scalar_type() == at::kByte && s.is_contiguous() &&
+              s.numel() == (t.size(0) + 127) / 128 * ((kp + 511) / 512) * 512 &&
+              reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0, "fp8_matmul: packed scales of ", name);
+}
+
+// out[M, N] = act(A B^T + bias); a [M, Kp], b [N, Kp] e4m3 with packed scales sa, sb
+void fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
+              const c10::optional<at::Tensor>& bias, at::Tensor& out, int64_t act,
+              const c10::optional<at::Tensor>& aux) {
+  TORCH_CHECK(a.is_cuda() && a.dim() == 2, "fp8_matmul: a on the GPU");
+  const int dev = a.get_device();
+  const int64_t kp = a.size(1);
+  check_operand("a", a, sa, kp, dev);
+  check_operand("b", b, sb, kp, dev);
+  TORCH_CHECK(a.size(0) < (int64_t(1) << 31) - 256 && b.size(0) < (int64_t(1) << 31) - 256, "fp8_matmul: sizes below 2^31");
+  fp8::Args args{};
+  args.M = (int)a.size(0);
+  args.N = (int)b.size(0);
+  args.KB = (int)(kp / 128);
+  args.sa = sa.data_ptr<uint8_t>();
+  args.sb = sb.data_ptr<uint8_t>();
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->is_cuda() && bias->get_device() == dev && bias->scalar_type() == at::kFloat &&
+                bias->is_contiguous() && bias->numel() == args.N, "fp8_matmul: bias f32 [N]");
+    args.bias = bias->data_ptr<float>();
+  }
+  TORCH_CHECK(out.is_cuda() && out.get_device() == dev && out.is_contiguous() && out.dim() == 2 &&
+              out.size(0) == args.M && out.size(1) == args.N, "fp8_matmul: contiguous out [M, N]");
+  const bool f32 = out.scalar_type() == at::kFloat;
+  TORCH_CHECK(f32 || out.scalar_type() == at::kBFloat16, "fp8_matmul: out bf16 or f32");
+  TORCH_CHECK(act == 0 || act == 1, "fp8_matmul: act");
+  args.act = (int)act;
+  args.out = out.data_ptr();
+  args.vec = args.N % 8 == 0 && reinterpret_cast<uintptr_t>(args.out) % 16 == 0;
+  if (aux.has_value()) {
+    TORCH_CHECK(aux->is_cuda() && aux->get_device() == dev && aux->scalar_type() == at::kBFloat16 &&
+                aux->is_contiguous() && aux->sizes() == out.sizes(), "fp8_matmul: aux bf16 [M, N]");
+    args.aux = reinterpret_cast<__nv_bfloat16*>(aux->data_ptr());
+    args.vec = args.vec && reinterpret_cast<uintptr_t>(args.aux) % 16 == 0;
+  }
+  args.err = error_word(dev);
+  if (args.M == 0 || args.N == 0) return;
+  TORCH_CHECK(args.KB > 0, "fp8_matmul: K of at least 1");
+  c10::cuda::CUDAGuard guard(a.device());
+  auto stream = c10::cuda::getCurrentCUDAStream();
+  const long sms = num_sms(dev);
+  const long tiles256 = (long)((args.M + 127) / 128) * ((args.N + 255) / 256);
+  const int bn = args.N <= 64 ? 64 : (args.N <= 128 || tiles256 < sms) ? 128 : 256;
+  if (f32) {
+    if (bn == 256) fp8::launch<256, float>(a, b, args, stream);
+    else if (bn == 128) fp8::launch<128, float>(a, b, args, stream);
+    else fp8::launch<64, float>(a, b, args, stream);
+  } else {
+    if (bn == 256) fp8::launch<256, __nv_bfloat16>(a, b, args, stream);
+    else if (bn == 128) fp8::launch<128, __nv_bfloat16>(a, b, args, stream);
+    else fp8::launch<64, __nv_bfloat16>(a, b, args, stream);
+  }
+}
+
+}  // namespace osp

@@ -224,3 +224,124 @@ def hif8_round_torch_oracle(x: torch.Tensor) -> torch.Tensor:
     ae = e.abs()
     m = torch.where(ae <= 3, 3.0, torch.where(ae <= 7, 2.0, torch.where(ae <= 15, 1.0, 0.0)))
     return torch.sign(x) * torch.floor(x.abs() * torch.pow(2.0, m - e) + 0.5) * torch.pow(2.0, e - m)
+
+
+# ----------------------------------------------------------------------------- block-128 fp8
+
+_FP8_BLOCK = 128
+
+
+def _two_to(k: torch.Tensor) -> torch.Tensor:
+    """Exact 2^k in fp32 for whole numbers -126 <= k <= 127."""
+    return ((k.int() + 127) << 23).view(torch.float32)
+
+
+def _pow2_scale(amax: torch.Tensor, mantissa: float, exponent: int) -> torch.Tensor:
+    """Smallest k >= -126 with amax / 2^k <= mantissa * 2^exponent (mantissa in [1/2, 1))."""
+    f, e = torch.frexp(amax)
+    k = e.int() - exponent + (f > mantissa).int()
+    return torch.where(amax > 0, k, torch.full_like(k, -126)).clamp(min=-126)
+
+
+def fp8_quantize(x: torch.Tensor, block_rows: int = 1):
+    """(e4m3 codes [R, Kp], packed scale bytes) of a matrix; format in :mod:`.fp8`."""
+    R, K = x.shape
+    kb, rt, kg = -(-K // _FP8_BLOCK), -(-R // 128), -(-K // 512)
+    xf = F.pad(x.detach().float(), (0, kb * _FP8_BLOCK - K)).view(R, kb, _FP8_BLOCK)
+    amax = torch.where(torch.isfinite(xf), xf.abs(), torch.zeros_like(xf)).amax(2) if R * kb else xf.new_zeros(R, kb)
+    if block_rows > 1:
+        tiles = F.pad(amax, (0, 0, 0, rt * 128 - R)).view(rt, 128, kb)
+        amax = (tiles.amax(1, keepdim=True).expand(rt, 128, kb) if rt * kb else tiles).reshape(rt * 128, kb)[:R]
+    k = _pow2_scale(amax, 0.875, 9)
+    codes = (xf * _two_to(-k)[:, :, None]).to(torch.float8_e4m3fn).view(R, kb * _FP8_BLOCK)
+    flat = torch.zeros(rt * 128, kg * 4, dtype=torch.uint8, device=x.device)
+    flat[:R, :kb] = (k + 127).to(torch.uint8)
+    return codes, flat.view(rt, 4, 32, kg, 4).permute(0, 3, 2, 1, 4).contiguous()
+
+
+def fp8_dequantize(data: torch.Tensor, scale: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """fp32 [rows, cols] that codes and packed scales stand for."""
+    kb = data.shape[1] // _FP8_BLOCK
+    flat = scale.permute(0, 3, 2, 1, 4).reshape(scale.shape[0] * 128, scale.shape[1] * 4)
+    s = _two_to(flat[:rows, :kb].int() - 127)
+    return (data.float().view(rows, kb, _FP8_BLOCK) * s[:, :, None]).view(rows, kb * _FP8_BLOCK)[:, :cols]
+
+
+def fp8_matmul(a, b, bias: Optional[torch.Tensor], act: Optional[str], out_dtype):
+    """(act(a·bᵀ + bias), its pre-activation in bf16) of two quantised matrices, in fp32."""
+    pre = a.dequantize() @ b.dequantize().t()
+    if bias is not None:
+        pre = pre + bias.detach().float()
+    return (gelu_tanh(pre) if act else pre).to(out_dtype), pre.to(torch.bfloat16)
+
+
+# ----------------------------------------------------------------------------- AdamW on lists
+
+_U32 = 0xFFFFFFFF
+
+
+def _mix32(x: torch.Tensor) -> torch.Tensor:
+    """32 mixed bits of int64 values below 2^32 (two multiply-xorshift rounds; the odd
+    multipliers are the first bits of the fractions of sqrt 2 and sqrt 3)."""
+    x = ((x ^ (x >> 16)) * 0x6A09E667) & _U32
+    x = ((x ^ (x >> 15)) * 0xBB67AE85) & _U32
+    return x ^ (x >> 16)
+
+
+def adamw8_decode(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
+    """fp32 moments of one tensor's 8-bit state."""
+    n = exp_avg.numel()
+    sm = _two_to(exp_avg_scale.int() - 127).repeat_interleave(_FP8_BLOCK)[:n].view(exp_avg.shape)
+    sv = _two_to(exp_avg_sq_scale.int() - 127).repeat_interleave(_FP8_BLOCK)[:n].view(exp_avg.shape)
+    v = (exp_avg_sq.to(torch.int16) << 7).view(torch.float16).float()
+    return exp_avg.float() * sm, v * sv
+
+
+def adamw8_encode(m: torch.Tensor, v: torch.Tensor, bits: torch.Tensor):
+    """8-bit state of fp32 moments, rounded stochastically by ``bits`` (int64, 32 random bits
+    per element: the low half for m, the high half for v)."""
+    n, shape = m.numel(), m.shape
+    nb = -(-n // _FP8_BLOCK)
+
+    def blocks(t):
+        return F.pad(t.reshape(-1), (0, nb * _FP8_BLOCK - n)).view(nb, _FP8_BLOCK)
+
+    def one(x, r, mantissa, exponent, low, normal):
+        x, r = blocks(x), blocks(r).int()
+        fin = torch.isfinite(x)
+        a = torch.where(fin, x.abs(), torch.zeros_like(x))
+        k = _pow2_scale(a.amax(1) if nb else a.new_zeros(0), mantissa, exponent)
+        a = a * _two_to(-k)[:, None]
+        small = a < low
+        t = torch.where(small, a + low, a).view(torch.int32) + (r << 4)
+        return fin, (t >> 20) - torch.where(small, normal + 8, normal), (k + 127).to(torch.uint8), x
+
+    fin, code, ms, x = one(m, bits & 0xFFFF, 0.875, 9, 2.0 ** -6, 960)
+    mq = torch.where(fin, code, 127) + torch.signbit(x).int() * 128
+    fin, code, vs, x = one(v, bits >> 16, 0.9375, 16, 2.0 ** -14, 896)
+    vq = torch.where(fin, torch.maximum(code, (x > 0).int()), 255)
+
+    def back(t):
+        return t.to(torch.uint8).view(-1)[:n].view(shape)
+    return back(mq).view(torch.float8_e4m3fn), back(vq), ms, vs
+
+
+def adamw_multi_(params, grads, exp_avgs, exp_avg_sqs, mscales, vscales, lr, beta1, beta2, eps, weight_decay, step,
+                 grad_scale=1.0, seed=0):
+    """In-place AdamW on lists of tensors, moments in fp32 or (with scales) in 8 bits."""
+    bc1, bc2 = 1 - beta1 ** step, math.sqrt(1 - beta2 ** step)
+    for t, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        gf = g.float() * grad_scale
+        mf, vf = (m, v) if mscales is None else adamw8_decode(m, v, mscales[t], vscales[t])
+        mf = mf * beta1 + gf * (1 - beta1)
+        vf = vf * beta2 + (gf * gf) * (1 - beta2)
+        p.copy_(p.float() * (1 - lr * weight_decay) - lr / bc1 * (mf / (vf.sqrt() / bc2 + eps)))
+        if mscales is None:
+            m.copy_(mf)
+            v.copy_(vf)
+            continue
+        i = torch.arange(p.numel(), dtype=torch.int64, device=p.device)
+        key = int(_mix32(torch.tensor((t * 0x3C6EF373 + seed) & _U32)))
+        state = adamw8_encode(mf, vf, _mix32((i + key) & _U32).view(p.shape))
+        for dst, src in zip((m, v, mscales[t], vscales[t]), state):
+            dst.copy_(src)

@@ -1,0 +1,139 @@
+"""Linear layers in block-scaled fp8 (format and kernels: :mod:`osp_next_b200.ops.fp8`).
+
+Forward: y = x_q·W_qᵀ + b, x quantised in blocks 1 x 128 along its features, W in tiles
+128 x 128.  Backward: dx = dy_q·W_q with the same codes of W read the other way, dW = dy_q'ᵀ·x_q'
+with dy and x quantised in blocks of 128 tokens (straight-through estimator: the quantisers
+have gradient 1).  All three products run on the block-scaled tensor-core kernel; the bias
+gradient is summed from dy itself.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from .. import ops
+
+
+def _grad_dtype(dt: torch.dtype) -> torch.dtype:
+    return torch.bfloat16 if dt == torch.bfloat16 else torch.float32
+
+
+def _out_dtype(x: torch.Tensor) -> torch.dtype:
+    """bf16 on the GPU (the DiT's activations), the input's own type on the CPU."""
+    return torch.float32 if not x.is_cuda and x.dtype == torch.float32 else torch.bfloat16
+
+
+class _FP8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act):
+        x2 = x.reshape(-1, x.shape[-1])
+        need_x, need_w = ctx.needs_input_grad[:2]
+        # one read of x gives the forward operand and the one of dW; the same for W and dx
+        xq = ops.fp8_quantize(x2, layout="both" if need_w else "rows")
+        wq = ops.fp8_quantize(weight, block_rows=ops.fp8.BLOCK, layout="both" if need_x else "rows")
+        xr, xc = xq if need_w else (xq, None)
+        wr, wc = wq if need_x else (wq, None)
+        y = ops.fp8_matmul(xr, wr, bias, act, _out_dtype(x), aux=act is not None)
+        y, pre = y if act else (y, None)
+        ctx.save_for_backward(pre, *(t for q in (xc, wc) if q is not None for t in (q.data, q.scale)))
+        ctx.kept = [None if q is None else (q.rows, q.cols, q.block_rows) for q in (xc, wc)]
+        ctx.meta = (x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    def backward(ctx, gy):
+        pre, *saved = ctx.saved_tensors
+        it = iter(saved)
+        xc, wc = [None if k is None else ops.Fp8Tensor(next(it), next(it), *k) for k in ctx.kept]
+        xshape, xdt, wdt, bdt = ctx.meta
+        g = gy.reshape(-1, gy.shape[-1])
+        if pre is not None:
+            g = _gelu_tanh_bwd(g, pre)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        if need_x or need_w:
+            gq = ops.fp8_quantize(g, layout="both" if need_x and need_w else "rows" if need_x else "cols")
+            gr, gc = gq if need_x and need_w else (gq, gq)
+            if need_x:
+                dx = ops.fp8_matmul(gr, wc, out_dtype=_grad_dtype(xdt)).to(xdt).view(xshape)
+            if need_w:
+                dw = ops.fp8_matmul(gc, xc, out_dtype=_grad_dtype(wdt)).to(wdt)
+        if need_b:
+            db = ops.bias_grad(g).to(bdt)
+        return dx, dw, db, None
+
+
+def _gelu_tanh_bwd(g, pre):
+    if g.is_cuda and g.numel() % 4 == 0:
+        return ops.gelu_tanh_bwd(g, pre)
+    with torch.enable_grad():
+        p = pre.detach().float().requires_grad_(True)
+        (d,) = torch.autograd.grad(F.gelu(p, approximate="tanh"), p, g.float())
+    return d.to(torch.bfloat16)
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               act: Optional[str] = None) -> torch.Tensor:
+    """``act(x·Wᵀ + b)`` (bf16; fp32 for fp32 CPU tensors) in block-scaled fp8 with an fp8
+    backward pass.
+
+    x [..., K] and weight [N, K] in bf16, fp16 or fp32, bias [N]; act None or ``"gelu_tanh"``.
+    Both operands are quantised in the call (a weight that does not change is better kept as
+    ``ops.fp8_quantize(weight, block_rows=128)`` for ``ops.fp8_matmul``)."""
+    if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"fp8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"fp8_linear: bias [{weight.shape[0]}], got {tuple(bias.shape)}")
+    return _FP8LinearFn.apply(x, weight, bias, act)
+
+
+class FP8Linear(nn.Linear):
+    """Drop-in ``nn.Linear`` in block-scaled fp8 (forward and backward).
+
+    Under autograd both operands are quantised every call.  For sampling, :meth:`freeze_weight`
+    quantises the weight once and later no-grad calls use that copy until :meth:`thaw_weight`,
+    ``train()`` or ``load_state_dict``: the layer never guesses whether a weight changed."""
+    is_fp8 = True
+
+    def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
+        self._frozen = None
+
+    def freeze_weight(self):
+        self._frozen = ops.fp8_quantize(self.weight.detach(), block_rows=ops.fp8.BLOCK)
+        return self
+
+    def thaw_weight(self):
+        self._frozen = None
+        return self
+
+    def train(self, mode: bool = True):
+        if mode:
+            self.thaw_weight()
+        return super().train(mode)
+
+    def _load_from_state_dict(self, *a, **k):
+        self.thaw_weight()
+        super()._load_from_state_dict(*a, **k)
+
+    def _apply(self, fn, *a, **k):
+        self.thaw_weight()
+        return super()._apply(fn, *a, **k)
+
+    def forward(self, x, act: Optional[str] = None):
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad
+                                        or (self.bias is not None and self.bias.requires_grad)):
+            return fp8_linear(x, self.weight, self.bias, act)
+        w = self._frozen if self._frozen is not None else ops.fp8_quantize(self.weight, block_rows=ops.fp8.BLOCK)
+        return ops.fp8_matmul(x, w, self.bias, act, _out_dtype(x))
+
+
+def freeze_fp8_weights(module: nn.Module) -> nn.Module:
+    """Quantise the weight of every :class:`FP8Linear` in ``module`` once (sampling)."""
+    for m in module.modules():
+        if isinstance(m, FP8Linear):
+            m.freeze_weight()
+    return module
