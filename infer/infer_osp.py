@@ -57,6 +57,9 @@ def main(config):
     for n, p in model.named_parameters():
         if "norm" in n or "modulation" in n:
             p.data = p.data.float()
+    if mcfg.get("quant") == "fp8":                       # the weights stay as they are from here on
+        from osp_next_b200.quant import freeze_fp8_weights
+        freeze_fp8_weights(model)
     attach_sp(model, sp_rt)
     model.enable_text_kv_cache(True)
     scheduler = B.build_scheduler(config)

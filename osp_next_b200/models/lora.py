@@ -67,8 +67,8 @@ class LoraLinear(nn.Module):
             return _LoraDualFn.apply(x, self.base_layer.weight, self.base_layer.bias,
                                      self.lora_A[self.adapter].weight, self.lora_B[self.adapter].weight,
                                      self.scaling, act)
-        y = self.base_layer(x) if not isinstance(self.base_layer, nn.Linear) else \
-            Fn.linear(x, self.base_layer.weight, self.base_layer.bias)
+        own = not isinstance(self.base_layer, nn.Linear) or getattr(self.base_layer, "is_fp8", False)
+        y = self.base_layer(x) if own else Fn.linear(x, self.base_layer.weight, self.base_layer.bias)
         if not self.disabled:
             a = Fn.linear(x, self.lora_A[self.adapter].weight)
             b = Fn.linear(a, self.lora_B[self.adapter].weight)

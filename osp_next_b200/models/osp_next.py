@@ -130,11 +130,11 @@ class OSPNextSelfAttention(nn.Module):
         B, n, _ = x.shape
         H, D = self.num_heads, self.head_dim
         lora = any(hasattr(m, "lora_A") for m in (self.q, self.k, self.v))
-        if Fn._fused(x, self.q.weight) and self.qk_norm and not lora and not _hif8(self):
+        if Fn._fused(x, self.q.weight) and self.qk_norm and not lora and not _hif8(self) and not _fp8(self):
             W, b = self.packed_qkv()
             qkv = Fn.ops.linear(x, W, b)
             return Fn.ops.qk_norm_rope(qkv, self.norm_q.weight, self.norm_k.weight, ctx.pos, ctx.freqs, H, self.eps)
-        if (lora and not _hif8(self) and self.qk_norm and ctx.pos is not None
+        if (lora and not _hif8(self) and not _fp8(self) and self.qk_norm and ctx.pos is not None
                 and Fn._fused(x, self.q.weight, *[p for m in (self.q, self.k, self.v) for p in _lora_params(m)])):
             # LoRA folded into the packed QKV GEMM (second operand pair), then the fused q/k
             # norm + RoPE, as the plain path
@@ -153,7 +153,10 @@ class OSPNextSelfAttention(nn.Module):
             # wrapped projections (LoRA, HiF8) run their own forward (HiF8: one quantisation of
             # x and one GEMM for all three); the q/k RMSNorm and the RoPE stay on the fused
             # kernel (forward and backward) whatever the Linear type
-            if _hif8(self) and all(getattr(m, "is_hif8", False) for m in (self.q, self.k, self.v)):
+            if all(getattr(m, "is_fp8", False) for m in (self.q, self.k, self.v)):
+                from ..quant.fp8 import fp8_multi_linear
+                qkv = fp8_multi_linear(x, (self.q, self.k, self.v))
+            elif _hif8(self) and all(getattr(m, "is_hif8", False) for m in (self.q, self.k, self.v)):
                 from ..quant.hif8 import hif8_multi_linear
                 qkv = hif8_multi_linear(x, (self.q, self.k, self.v))
             else:
@@ -199,10 +202,15 @@ def _hif8(attn) -> bool:
     return getattr(attn.q, "is_hif8", False)
 
 
+def _fp8(attn) -> bool:
+    """Projections in block-scaled fp8, also under a LoRA adapter."""
+    return any(getattr(getattr(m, "base_layer", m), "is_fp8", False) for m in (attn.q, attn.k, attn.v))
+
+
 def _lin(mod, x, act=None):
     """Plain Linears go through the functional layer (fused GEMM / dtype handling); LoRA
     Linears without autograd fold their branch into the same GEMM; other wrapped ones
-    (HiF8, LoRA under autograd) run their own forward."""
+    (HiF8, fp8, LoRA under autograd) run their own forward."""
     if type(mod) is nn.Linear:
         return Fn.linear(x, mod.weight, mod.bias, act=act)
     if _lora_fusable(mod, x):
@@ -210,6 +218,8 @@ def _lin(mod, x, act=None):
         x2 = x.reshape(-1, x.shape[-1])
         W, b, extra = fused_lora_operands((mod,), x2)
         return Fn.ops.linear(x2, W, b, act=act, extra=extra).view(*x.shape[:-1], W.shape[0])
+    if getattr(mod, "is_fp8", False):
+        return mod(x, act)
     y = mod(x)
     return Fn.F.gelu(y, approximate="tanh") if act == "gelu_tanh" else y
 
@@ -313,6 +323,8 @@ class OSPNextAttentionBlock(nn.Module):
         if getattr(f0, "is_hif8", False):
             from ..quant.hif8 import hif8_multi_linear
             h = hif8_multi_linear(xm, (f0,), act="gelu_tanh")       # GELU in the GEMM epilogue
+        elif getattr(f0, "is_fp8", False):
+            h = f0(xm, act="gelu_tanh")                             # GELU in the product's epilogue
         elif _plain(f0) or _lora_fusable(f0, xm):
             h = _lin(f0, xm, act="gelu_tanh")
         elif hasattr(f0, "lora_A"):
@@ -342,7 +354,7 @@ class OSPNextAttentionBlock(nn.Module):
 
 
 def _plain(m) -> bool:
-    """A plain nn.Linear (no LoRA / HiF8 wrapper) can use the fused GEMM epilogues."""
+    """A plain nn.Linear (no LoRA / HiF8 / fp8 wrapper) can use the fused GEMM epilogues."""
     return type(m) is nn.Linear
 
 
@@ -353,6 +365,9 @@ def _linear_factory(quant, smf, smb):
         def mk(i, o, bias=True):
             return HIF8Linear(i, o, bias=bias, scale_max_forward=smf, scale_max_backward=smb)
         return mk
+    if quant == "fp8":
+        from ..quant.fp8 import FP8Linear
+        return FP8Linear
     return nn.Linear
 
 

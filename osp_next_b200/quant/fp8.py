@@ -101,13 +101,14 @@ class FP8Linear(nn.Linear):
     def __init__(self, in_features, out_features, bias=True, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
         self._frozen = None
+        self._pack = None
 
     def freeze_weight(self):
         self._frozen = ops.fp8_quantize(self.weight.detach(), block_rows=ops.fp8.BLOCK)
         return self
 
     def thaw_weight(self):
-        self._frozen = None
+        self._frozen = self._pack = None
         return self
 
     def train(self, mode: bool = True):
@@ -129,6 +130,33 @@ class FP8Linear(nn.Linear):
             return fp8_linear(x, self.weight, self.bias, act)
         w = self._frozen if self._frozen is not None else ops.fp8_quantize(self.weight, block_rows=ops.fp8.BLOCK)
         return ops.fp8_matmul(x, w, self.bias, act, _out_dtype(x))
+
+
+def fp8_multi_linear(x: torch.Tensor, linears, act: Optional[str] = None) -> torch.Tensor:
+    """[FP8Linear_1(x) | ... | FP8Linear_n(x)] of layers that read one input (q/k/v): x is
+    quantised once and one product runs on the stacked weights.  With output sizes that are
+    multiples of 128 (whole weight tiles) the values are those of the separate layers; others
+    are run one by one."""
+    if len(linears) == 1:
+        return linears[0](x, act)
+    has_bias = [m.bias is not None for m in linears]
+    if any(m.out_features % ops.fp8.BLOCK for m in linears) or any(has_bias) != all(has_bias):
+        return torch.cat([m(x, act) for m in linears], -1)
+    bias = torch.cat([m.bias for m in linears]) if all(has_bias) else None
+    params = [p for m in linears for p in (m.weight, m.bias) if p is not None]
+    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
+        return fp8_linear(x, torch.cat([m.weight for m in linears]), bias, act)
+    parts = [m._frozen for m in linears]
+    if all(p is not None for p in parts):
+        pack = linears[0]._pack        # (the frozen weights it was stacked from, the stack)
+        if pack is None or len(pack[0]) != len(parts) or any(a is not b for a, b in zip(pack[0], parts)):
+            w = ops.Fp8Tensor(torch.cat([p.data for p in parts]), torch.cat([p.scale for p in parts]),
+                              sum(p.rows for p in parts), parts[0].cols, ops.fp8.BLOCK)
+            pack = linears[0]._pack = (parts, w)
+        w = pack[1]
+    else:
+        w = ops.fp8_quantize(torch.cat([m.weight.detach() for m in linears]), block_rows=ops.fp8.BLOCK)
+    return ops.fp8_matmul(x, w, bias, act, _out_dtype(x))
 
 
 def freeze_fp8_weights(module: nn.Module) -> nn.Module:

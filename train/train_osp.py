@@ -106,7 +106,8 @@ def main(config, on_step=None):
         if config.get("ema_decay", 0) else None
     opt = FusedAdamW([p for p in model.parameters() if p.requires_grad], lr=opt_cfg.get("lr", 1e-5),
                      betas=tuple(opt_cfg.get("betas", (0.9, 0.999))), eps=opt_cfg.get("eps", 1e-15),
-                     weight_decay=opt_cfg.get("weight_decay", 0.0))
+                     weight_decay=opt_cfg.get("weight_decay", 0.0), state_bits=opt_cfg.get("state_bits", 32),
+                     multi_tensor=opt_cfg.get("multi_tensor"))
     shard_group = None
     if mesh is not None:
         shard_group = (mesh["fsdp"] if "ddp" in (mesh.mesh_dim_names or ()) else mesh).get_group()

@@ -232,7 +232,8 @@ def main(config):
     ema = FSDPEMAModel(policy, config.get("ema_decay", 0.9999), config.get("ema_update_interval", 1),
                        lora_only=True) if config.get("ema_decay", 0) else None
     opt = FusedAdamW(lora_params, lr=oc.get("lr", 1e-5), betas=tuple(oc.get("betas", (0.9, 0.999))),
-                     eps=oc.get("eps", 1e-8), weight_decay=oc.get("weight_decay", 1e-4))
+                     eps=oc.get("eps", 1e-8), weight_decay=oc.get("weight_decay", 1e-4),
+                     state_bits=oc.get("state_bits", 32), multi_tensor=oc.get("multi_tensor"))
     clipper = AdaptiveGradClipper(init_max_grad_norm=config.get("init_max_grad_norm", 1.0),
                                   model_parallel_group=shard_group)
     ref_model = AdapterDisabled(policy)
