@@ -33,28 +33,30 @@ namespace osp {
 namespace adamw8 {
 
 constexpr int kCap = 480;                 // tensors per launch: 480 x 64 B + constants < 32764 B
+constexpr int kSmallCap = 64;
 constexpr int kChunkBlocks = 32;          // 128-element runs per CTA visit (8 warps x 4)
 constexpr uint32_t kMix1 = 0x6A09E667u, kMix2 = 0xBB67AE85u, kMix3 = 0x3C6EF373u;   // fractions of sqrt 2, 3, 5
 
-// c1 = 1 - b1, c2 = 1 - b2, keep = 1 - lr wd, rate = lr / (1 - b1^t), bc2s = sqrt(1 - b2^t): formed in
+// c1 = 1 - b1, c2 = 1 - b2, keep = 1 - lr wd, rate = lr / (1 - b1^t), inv_bc2s = 1 / sqrt(1 - b2^t): formed in
 // 64 bits on the host (1 - fp32(0.999) alone would be off by a 75000th).
 struct Consts {
-  float b1, b2, c1, c2, eps, keep, rate, bc2s, gscale;
+  float b1, b2, c1, c2, eps, keep, rate, inv_bc2s, gscale;
 };
+template <int CAP>
 struct Args {
-  void* p[kCap];
-  const void* g[kCap];
-  void* m[kCap];
-  void* v[kCap];
-  uint8_t* ms[kCap];
-  uint8_t* vs[kCap];
-  int64_t n[kCap];
-  int chunk_end[kCap];                    // chunks of tensors 0..i
-  uint32_t key[kCap];
+  void* p[CAP];
+  const void* g[CAP];
+  void* m[CAP];
+  void* v[CAP];
+  uint8_t* ms[CAP];
+  uint8_t* vs[CAP];
+  int64_t n[CAP];
+  int chunk_end[CAP];                     // chunks of tensors 0..i
+  uint32_t key[CAP];
   int tensors;
   Consts c;
 };
-static_assert(sizeof(Args) <= 32764, "kernel parameters");
+static_assert(sizeof(Args<kCap>) <= 32764, "kernel parameters");
 
 __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   x = (x ^ (x >> 16)) * kMix1;
@@ -102,22 +104,17 @@ __device__ __forceinline__ void store(T* p, bool wide, int left, const float* o)
       if (j < left) st1(p + j, o[j]);
   }
 }
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, bool wide, int left) {
-  if (wide && left >= 4) return *reinterpret_cast<const uint32_t*>(p);
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int left) {
   uint32_t u = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (j < left) u |= (uint32_t)p[j] << (8 * j);
   return u;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, bool wide, int left, uint32_t u) {
-  if (wide && left >= 4) {
-    *reinterpret_cast<uint32_t*>(p) = u;
-  } else {
+__device__ __forceinline__ void store_codes(uint8_t* p, int left, uint32_t u) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < left) p[j] = (uint8_t)(u >> (8 * j));
-  }
+  for (int j = 0; j < 4; ++j)
+    if (j < left) p[j] = (uint8_t)(u >> (8 * j));
 }
 
 __device__ __forceinline__ void decode_m(uint32_t u, uint32_t byte, float* o) {
@@ -156,8 +153,86 @@ __device__ __forceinline__ uint32_t scale_byte_v(uint32_t vmax) {
   return (uint32_t)max((int)((vmax + 0x0FFFFFu) >> 23) - 15, 1);
 }
 
-template <typename PT, typename GT, bool STATE8>
-__global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ Args args) {
+// sqrt and division of the update by the hardware approximations (relative errors of a few
+// 2^-23, on a term that is lr times a number near 1); the precise forms cost some 30
+// instructions per element, which is what bounded the 8-bit step.
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float stepped(float p, float m, float v, const Consts& c) {
+  return p * c.keep - c.rate * __fdividef(m, sqrt_fast(v) * c.inv_bc2s + c.eps);
+}
+
+__device__ __forceinline__ void update32(float* pv, const float* gv, float* mv, float* vv, const Consts& c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float gj = gv[j] * c.gscale;
+    mv[j] = c.b1 * mv[j] + c.c1 * gj;
+    vv[j] = c.b2 * vv[j] + c.c2 * gj * gj;
+    pv[j] = stepped(pv[j], mv[j], vv[j], c);
+  }
+}
+
+// One block of 128 over a warp: codes mu, vu of four elements per lane and the block's scale
+// bytes mb, vb in, their new values out; p updated.  `i`: index of the lane's first element.
+__device__ __forceinline__ void update8(float* pv, const float* gv, uint32_t& mu, uint32_t& vu, uint32_t& mb,
+                                        uint32_t& vb, uint32_t i, uint32_t key, const Consts& c) {
+  float mv[4], vv[4];
+  decode_m(mu, mb, mv);
+  decode_v(vu, vb, vv);
+  uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // written with explicit roundings (no contraction), so that the stored codes are
+    // reproducible from the formula
+    const float gj = __fmul_rn(gv[j], c.gscale);
+    mv[j] = __fadd_rn(__fmul_rn(mv[j], c.b1), __fmul_rn(gj, c.c1));
+    vv[j] = __fadd_rn(__fmul_rn(vv[j], c.b2), __fmul_rn(__fmul_rn(gj, gj), c.c2));
+    mtop = max(mtop, __float_as_uint(mv[j]) & 0x7FFFFFFFu);
+    vtop = max(vtop, __float_as_uint(vv[j]) & 0x7FFFFFFFu);
+    pv[j] = stepped(pv[j], mv[j], vv[j], c);
+  }
+  mtop = __reduce_max_sync(0xffffffffu, mtop);
+  vtop = __reduce_max_sync(0xffffffffu, vtop);
+  const bool bad = max(mtop, vtop) >= fp8::kInfBits;
+  if (bad) {                                         // whole warp: maxima of what is finite
+    mtop = vtop = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = __float_as_uint(mv[j]) & 0x7FFFFFFFu, b = __float_as_uint(vv[j]) & 0x7FFFFFFFu;
+      mtop = max(mtop, a >= fp8::kInfBits ? 0u : a);
+      vtop = max(vtop, b >= fp8::kInfBits ? 0u : b);
+    }
+    mtop = __reduce_max_sync(0xffffffffu, mtop);
+    vtop = __reduce_max_sync(0xffffffffu, vtop);
+  }
+  mb = fp8::scale_byte(mtop);
+  vb = scale_byte_v(vtop);
+  const float minv = fp8::inv_scale(mb), vinv = fp8::inv_scale(vb);
+  mu = vu = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t r = mix(i + j + key);
+    uint32_t cm = encode_m(mv[j], minv, r & 0xFFFFu), cv = encode_v(vv[j], vinv, r >> 16);
+    if (bad) {
+      if (!isfinite(mv[j])) cm = 0x7Fu | (cm & 0x80u);
+      if (!isfinite(vv[j])) cv = 255u;
+      cm &= 0xFFu;
+      cv &= 0xFFu;
+    }
+    mu |= cm << (8 * j);
+    vu |= cv << (8 * j);
+  }
+}
+
+// A CTA takes chunks of 32 blocks; a warp takes 4 of them, 8 blocks apart.  Where the chunk is
+// whole and every tensor starts on a vector, the warp has the loads of all 4 in flight before
+// it computes; ends and odd addresses go block by block, element by element.
+template <typename PT, typename GT, bool STATE8, int CAP>
+__global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ Args<CAP> args) {
+  constexpr int U = kChunkBlocks / 8;
   const Consts c = args.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunks = args.chunk_end[args.tensors - 1];
@@ -168,100 +243,153 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ Args 
       if (chunk < args.chunk_end[mid]) hi = mid;
       else lo = mid + 1;
     }
-    const int64_t n = args.n[lo];
     const int64_t blk0 = (int64_t)(chunk - (lo ? args.chunk_end[lo - 1] : 0)) * kChunkBlocks;
-    PT* p = reinterpret_cast<PT*>(args.p[lo]);
-    const GT* g = reinterpret_cast<const GT*>(args.g[lo]);
-    const bool wide_p = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(PT)) == 0;
-    const bool wide_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(GT)) == 0;
-    const uint32_t key = args.key[lo];
-    for (int b = warp; b < kChunkBlocks; b += 8) {
-      const int64_t blk = blk0 + b;
-      const int64_t i = blk * 128 + lane * 4;
-      if (blk * 128 >= n) break;                     // whole warp
-      const int left = (int)min((int64_t)4, n - i);  // below 1: this lane has none
-      float pv[4], gv[4], mv[4], vv[4];
-      load(p + i, wide_p, left, pv);
-      load(g + i, wide_g, left, gv);
-      if constexpr (STATE8) {
-        uint8_t* mq = reinterpret_cast<uint8_t*>(args.m[lo]);
-        uint8_t* vq = reinterpret_cast<uint8_t*>(args.v[lo]);
-        const bool wide_m = reinterpret_cast<uintptr_t>(mq) % 4 == 0, wide_v = reinterpret_cast<uintptr_t>(vq) % 4 == 0;
-        decode_m(load_codes(mq + i, wide_m, left), args.ms[lo][blk], mv);
-        decode_v(load_codes(vq + i, wide_v, left), args.vs[lo][blk], vv);
-        uint32_t mtop = 0, vtop = 0;
+    const int64_t e0 = blk0 * 128;
+    const int64_t n = args.n[lo] - e0;               // elements from the chunk's start on
+    PT* p = reinterpret_cast<PT*>(args.p[lo]) + e0;
+    const GT* g = reinterpret_cast<const GT*>(args.g[lo]) + e0;
+    const uint32_t key = args.key[lo] + (uint32_t)e0;
+    uintptr_t low = (reinterpret_cast<uintptr_t>(p) * (4 / sizeof(PT))) | (reinterpret_cast<uintptr_t>(g) * (4 / sizeof(GT)));
+    if constexpr (STATE8) {
+      uint8_t* mq = reinterpret_cast<uint8_t*>(args.m[lo]) + e0;
+      uint8_t* vq = reinterpret_cast<uint8_t*>(args.v[lo]) + e0;
+      uint8_t* ms = args.ms[lo] + blk0;
+      uint8_t* vs = args.vs[lo] + blk0;
+      low |= (reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(vq)) * 4;
+      if (low % 16 == 0 && n >= kChunkBlocks * 128) {
+        float pv[U][4], gv[U][4];
+        uint32_t mu[U], vu[U], mb[U], vb[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // written with explicit roundings (no contraction), so that the stored codes are
-          // reproducible from the formula
-          const float gj = __fmul_rn(gv[j], c.gscale);
-          mv[j] = __fadd_rn(__fmul_rn(mv[j], c.b1), __fmul_rn(gj, c.c1));
-          vv[j] = __fadd_rn(__fmul_rn(vv[j], c.b2), __fmul_rn(__fmul_rn(gj, gj), c.c2));
-          mtop = max(mtop, __float_as_uint(mv[j]) & 0x7FFFFFFFu);
-          vtop = max(vtop, __float_as_uint(vv[j]) & 0x7FFFFFFFu);
-          const float den = sqrtf(vv[j]) / c.bc2s + c.eps;
-          pv[j] = pv[j] * c.keep - c.rate * (mv[j] / den);
+        for (int u = 0; u < U; ++u) {
+          const int blk = warp + 8 * u, i = blk * 128 + lane * 4;
+          load(p + i, true, 4, pv[u]);
+          load(g + i, true, 4, gv[u]);
+          mu[u] = *reinterpret_cast<const uint32_t*>(mq + i);
+          vu[u] = *reinterpret_cast<const uint32_t*>(vq + i);
+          mb[u] = ms[blk];
+          vb[u] = vs[blk];
         }
-        store(p + i, wide_p, left, pv);
-        const bool bad = __any_sync(0xffffffffu, max(mtop, vtop) >= fp8::kInfBits);
-        if (bad) {
-          mtop = vtop = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a = __float_as_uint(mv[j]) & 0x7FFFFFFFu, b2 = __float_as_uint(vv[j]) & 0x7FFFFFFFu;
-            mtop = max(mtop, a >= fp8::kInfBits ? 0u : a);
-            vtop = max(vtop, b2 >= fp8::kInfBits ? 0u : b2);
+        for (int u = 0; u < U; ++u) {
+          const int blk = warp + 8 * u, i = blk * 128 + lane * 4;
+          update8(pv[u], gv[u], mu[u], vu[u], mb[u], vb[u], (uint32_t)i, key, c);
+          store(p + i, true, 4, pv[u]);
+          *reinterpret_cast<uint32_t*>(mq + i) = mu[u];
+          *reinterpret_cast<uint32_t*>(vq + i) = vu[u];
+          if (lane == 0) {
+            ms[blk] = (uint8_t)mb[u];
+            vs[blk] = (uint8_t)vb[u];
           }
         }
-        const uint32_t mb = fp8::scale_byte(__reduce_max_sync(0xffffffffu, mtop));
-        const uint32_t vb = scale_byte_v(__reduce_max_sync(0xffffffffu, vtop));
-        const float minv = fp8::inv_scale(mb), vinv = fp8::inv_scale(vb);
-        uint32_t mu = 0, vu = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t r = mix((uint32_t)(i + j) + key);
-          uint32_t cm = encode_m(mv[j], minv, r & 0xFFFFu), cv = encode_v(vv[j], vinv, r >> 16);
-          if (bad) {
-            if (!isfinite(mv[j])) cm = 0x7Fu | (cm & 0x80u);
-            if (!isfinite(vv[j])) cv = 255u;
-          }
-          mu |= (cm & 0xFFu) << (8 * j);
-          vu |= (cv & 0xFFu) << (8 * j);
-        }
-        store_codes(mq + i, wide_m, left, mu);
-        store_codes(vq + i, wide_v, left, vu);
+        continue;
+      }
+      for (int blk = warp; blk < kChunkBlocks && blk * 128 < n; blk += 8) {
+        const int i = blk * 128 + lane * 4;
+        const int left = (int)min((int64_t)4, n - i);          // below 1: this lane has none
+        float pv[4], gv[4];
+        load(p + i, false, left, pv);
+        load(g + i, false, left, gv);
+        uint32_t mu = load_codes(mq + i, left), vu = load_codes(vq + i, left), mb = ms[blk], vb = vs[blk];
+        update8(pv, gv, mu, vu, mb, vb, (uint32_t)i, key, c);
+        store(p + i, false, left, pv);
+        store_codes(mq + i, left, mu);
+        store_codes(vq + i, left, vu);
         if (lane == 0) {
-          args.ms[lo][blk] = (uint8_t)mb;
-          args.vs[lo][blk] = (uint8_t)vb;
+          ms[blk] = (uint8_t)mb;
+          vs[blk] = (uint8_t)vb;
         }
-      } else {
-        float* m = reinterpret_cast<float*>(args.m[lo]);
-        float* v = reinterpret_cast<float*>(args.v[lo]);
-        const bool wide_m = reinterpret_cast<uintptr_t>(m) % 16 == 0, wide_v = reinterpret_cast<uintptr_t>(v) % 16 == 0;
-        load(m + i, wide_m, left, mv);
-        load(v + i, wide_v, left, vv);
+      }
+    } else {
+      float* m = reinterpret_cast<float*>(args.m[lo]) + e0;
+      float* v = reinterpret_cast<float*>(args.v[lo]) + e0;
+      low |= reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
+      if (low % 16 == 0 && n >= kChunkBlocks * 128) {
+        float pv[U][4], gv[U][4], mv[U][4], vv[U][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float gj = gv[j] * c.gscale;
-          mv[j] = c.b1 * mv[j] + c.c1 * gj;
-          vv[j] = c.b2 * vv[j] + c.c2 * gj * gj;
-          pv[j] = pv[j] * c.keep - c.rate * (mv[j] / (sqrtf(vv[j]) / c.bc2s + c.eps));
+        for (int u = 0; u < U; ++u) {
+          const int i = (warp + 8 * u) * 128 + lane * 4;
+          load(p + i, true, 4, pv[u]);
+          load(g + i, true, 4, gv[u]);
+          load(m + i, true, 4, mv[u]);
+          load(v + i, true, 4, vv[u]);
         }
-        store(p + i, wide_p, left, pv);
-        store(m + i, wide_m, left, mv);
-        store(v + i, wide_v, left, vv);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = (warp + 8 * u) * 128 + lane * 4;
+          update32(pv[u], gv[u], mv[u], vv[u], c);
+          store(p + i, true, 4, pv[u]);
+          store(m + i, true, 4, mv[u]);
+          store(v + i, true, 4, vv[u]);
+        }
+        continue;
+      }
+      for (int blk = warp; blk < kChunkBlocks && blk * 128 < n; blk += 8) {
+        const int i = blk * 128 + lane * 4;
+        const int left = (int)min((int64_t)4, n - i);
+        const bool wide = low % 16 == 0;
+        float pv[4], gv[4], mv[4], vv[4];
+        load(p + i, wide, left, pv);
+        load(g + i, wide, left, gv);
+        load(m + i, wide, left, mv);
+        load(v + i, wide, left, vv);
+        update32(pv, gv, mv, vv, c);
+        store(p + i, wide, left, pv);
+        store(m + i, wide, left, mv);
+        store(v + i, wide, left, vv);
       }
     }
   }
 }
 
-template <typename PT, typename GT>
-static void launch(const Args& a, bool state8, int device, cudaStream_t stream) {
+template <typename PT, typename GT, int CAP>
+static void launch(const Args<CAP>& a, bool state8, int device, cudaStream_t stream) {
   const int chunks = a.chunk_end[a.tensors - 1];
   const int grid = std::min(chunks, num_sms(device) * 8);
-  if (state8) step_kernel<PT, GT, true><<<grid, 256, 0, stream>>>(a);
-  else step_kernel<PT, GT, false><<<grid, 256, 0, stream>>>(a);
+  if (state8) step_kernel<PT, GT, true, CAP><<<grid, 256, 0, stream>>>(a);
+  else step_kernel<PT, GT, false, CAP><<<grid, 256, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+struct Lists {
+  const std::vector<at::Tensor>&p, &g, &m, &v, &ms, &vs;
+};
+
+// Fills parameter blocks of CAP tensors and launches each.
+template <int CAP>
+static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed, int dev, cudaStream_t stream) {
+  const bool pf = l.p[0].scalar_type() == at::kFloat, gf = l.g[0].scalar_type() == at::kFloat;
+  Args<CAP> a;
+  a.c = consts;
+  a.tensors = 0;
+  int64_t chunks = 0;
+  auto flush = [&]() {
+    if (a.tensors == 0) return;
+    if (pf && gf) launch<float, float, CAP>(a, state8, dev, stream);
+    else if (pf) launch<float, __nv_bfloat16, CAP>(a, state8, dev, stream);
+    else if (gf) launch<__nv_bfloat16, float, CAP>(a, state8, dev, stream);
+    else launch<__nv_bfloat16, __nv_bfloat16, CAP>(a, state8, dev, stream);
+    a.tensors = 0;
+    chunks = 0;
+  };
+  for (size_t i = 0; i < l.p.size(); ++i) {
+    const int64_t n = l.p[i].numel();
+    if (n == 0) continue;
+    const int64_t mine = ((n + 127) / 128 + kChunkBlocks - 1) / kChunkBlocks;
+    TORCH_CHECK(mine < (int64_t(1) << 30), "adamw_multi_: tensor ", std::to_string(i), " too large");
+    if (a.tensors == CAP || chunks + mine >= (int64_t(1) << 31)) flush();
+    const int t = a.tensors++;
+    chunks += mine;
+    a.p[t] = l.p[i].data_ptr();
+    a.g[t] = l.g[i].data_ptr();
+    a.m[t] = l.m[i].data_ptr();
+    a.v[t] = l.v[i].data_ptr();
+    a.ms[t] = state8 ? l.ms[i].data_ptr<uint8_t>() : nullptr;
+    a.vs[t] = state8 ? l.vs[i].data_ptr<uint8_t>() : nullptr;
+    a.n[t] = n;
+    a.chunk_end[t] = (int)chunks;
+    a.key[t] = mix((uint32_t)i * kMix3 + seed);
+  }
+  flush();
 }
 
 }  // namespace adamw8
@@ -297,49 +425,20 @@ void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vect
   }
   c10::cuda::CUDAGuard guard(p[0].device());
   auto stream = c10::cuda::getCurrentCUDAStream();
-  Args a;
-  a.c.b1 = (float)b1;
-  a.c.b2 = (float)b2;
-  a.c.c1 = (float)(1.0 - b1);
-  a.c.c2 = (float)(1.0 - b2);
-  a.c.eps = (float)eps;
-  a.c.keep = (float)(1.0 - lr * wd);
-  a.c.rate = (float)(lr / (1.0 - std::pow(b1, (double)step)));
-  a.c.bc2s = (float)std::sqrt(1.0 - std::pow(b2, (double)step));
-  a.c.gscale = (float)gscale;
-  a.tensors = 0;
-  int64_t chunks = 0;
-  auto flush = [&]() {
-    if (a.tensors == 0) return;
-    if (pt == at::kFloat) {
-      if (gt == at::kFloat) launch<float, float>(a, state8, dev, stream);
-      else launch<float, __nv_bfloat16>(a, state8, dev, stream);
-    } else {
-      if (gt == at::kFloat) launch<__nv_bfloat16, float>(a, state8, dev, stream);
-      else launch<__nv_bfloat16, __nv_bfloat16>(a, state8, dev, stream);
-    }
-    a.tensors = 0;
-    chunks = 0;
-  };
-  for (size_t i = 0; i < count; ++i) {
-    const int64_t n = p[i].numel();
-    if (n == 0) continue;
-    const int64_t mine = ((n + 127) / 128 + kChunkBlocks - 1) / kChunkBlocks;
-    TORCH_CHECK(mine < (int64_t(1) << 30), "adamw_multi_: tensor ", std::to_string(i), " too large");
-    if (a.tensors == kCap || chunks + mine >= (int64_t(1) << 31)) flush();
-    const int t = a.tensors++;
-    chunks += mine;
-    a.p[t] = p[i].data_ptr();
-    a.g[t] = g[i].data_ptr();
-    a.m[t] = m[i].data_ptr();
-    a.v[t] = v[i].data_ptr();
-    a.ms[t] = state8 ? ms[i].data_ptr<uint8_t>() : nullptr;
-    a.vs[t] = state8 ? vs[i].data_ptr<uint8_t>() : nullptr;
-    a.n[t] = n;
-    a.chunk_end[t] = (int)chunks;
-    a.key[t] = mix((uint32_t)i * kMix3 + (uint32_t)seed);
-  }
-  flush();
+  Consts c;
+  c.b1 = (float)b1;
+  c.b2 = (float)b2;
+  c.c1 = (float)(1.0 - b1);
+  c.c2 = (float)(1.0 - b2);
+  c.eps = (float)eps;
+  c.keep = (float)(1.0 - lr * wd);
+  c.rate = (float)(lr / (1.0 - std::pow(b1, (double)step)));
+  c.inv_bc2s = (float)(1.0 / std::sqrt(1.0 - std::pow(b2, (double)step)));
+  c.gscale = (float)gscale;
+  const Lists lists{p, g, m, v, ms, vs};
+  // a short list has a small parameter block: 4 KB instead of 30 KB to copy with the launch
+  if (count <= kSmallCap) run<kSmallCap>(lists, c, state8, (uint32_t)seed, dev, stream);
+  else run<kCap>(lists, c, state8, (uint32_t)seed, dev, stream);
 }
 
 }  // namespace osp
