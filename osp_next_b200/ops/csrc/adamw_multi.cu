@@ -34,7 +34,7 @@ namespace adamw8 {
 
 constexpr int kCap = 480;                 // tensors per launch: 480 x 64 B + constants < 32764 B
 constexpr int kSmallCap = 64;
-constexpr int kChunkBlocks = 32;          // 128-element runs per CTA visit (8 warps x 4)
+constexpr int kChunkBlocks = 16;          // 128-element runs per CTA visit (8 warps x 2)
 constexpr uint32_t kMix1 = 0x6A09E667u, kMix2 = 0xBB67AE85u, kMix3 = 0x3C6EF373u;   // fractions of sqrt 2, 3, 5
 
 // c1 = 1 - b1, c2 = 1 - b2, keep = 1 - lr wd, rate = lr / (1 - b1^t), inv_bc2s = 1 / sqrt(1 - b2^t): formed in
@@ -132,21 +132,25 @@ __device__ __forceinline__ void decode_v(uint32_t u, uint32_t byte, float* o) {
   o[0] = fa.x * s; o[1] = fa.y * s; o[2] = fb.x * s; o[3] = fb.y * s;
 }
 
-// Stochastic rounding on the fp32 bits: add 20 random bits (16 and four zeros) below the three
-// mantissa bits kept, then cut.  Magnitudes below the least normal 2^-E are lifted by 2^-E
-// first, where the kept bits have the subnormal step.
-__device__ __forceinline__ uint32_t encode_m(float m, float inv, uint32_t r16) {
-  const float y = m * inv, a = fabsf(y);
-  const bool small = a < 0.015625f;                                   // 2^-6
-  const uint32_t t = __float_as_uint(small ? a + 0.015625f : a) + (r16 << 4);
-  return ((t >> 20) - (small ? 968u : 960u)) | ((__float_as_uint(y) >> 24) & 0x80u);
+// Stochastic rounding of a scaled magnitude a on its fp32 bits: add 20 random bits (16 and
+// four zeros) below the three mantissa bits kept, then cut.  Below the least normal 2^-E the
+// kept bits of a + 2^-E have the subnormal step; its pattern less one exponent exceeds that of
+// a exactly there, so a maximum chooses between the two.  Returned with the eight bits that
+// matter on top; the exponent offset, a multiple of half a byte's range, is left to one XOR on
+// four packed codes (0x40 for m, 0x80 for v).
+__device__ __forceinline__ uint32_t round_bits(float a, float least, uint32_t r16) {
+  const uint32_t t = __viaddmax_u32(__float_as_uint(a + least), 0u - (1u << 23), __float_as_uint(a));
+  return (r16 * 16u + t) << 4;
 }
-__device__ __forceinline__ uint32_t encode_v(float v, float inv, uint32_t r16) {
-  const float a = v * inv;
-  const bool small = a < 6.103515625e-05f;                            // 2^-14
-  const uint32_t t = __float_as_uint(small ? a + 6.103515625e-05f : a) + (r16 << 4);
-  const uint32_t code = (t >> 20) - (small ? 904u : 896u);
-  return max(code, v > 0.f ? 1u : 0u);
+__device__ __forceinline__ uint32_t pack_top(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+// Largest magnitude of four as fp32 bits (NaN wins).
+__device__ __forceinline__ uint32_t top4(const float* x) {
+  float t;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(t) : "f"(x[0]), "f"(x[1]), "f"(x[2]));
+  asm("max.NaN.abs.f32 %0, %0, %1, %1;" : "+f"(t) : "f"(x[3]));
+  return __float_as_uint(t);
 }
 // Scale byte of a block of v: 61440 = 1.875 * 2^15.
 __device__ __forceinline__ uint32_t scale_byte_v(uint32_t vmax) {
@@ -182,7 +186,6 @@ __device__ __forceinline__ void update8(float* pv, const float* gv, uint32_t& mu
   float mv[4], vv[4];
   decode_m(mu, mb, mv);
   decode_v(vu, vb, vv);
-  uint32_t mtop = 0, vtop = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     // written with explicit roundings (no contraction), so that the stored codes are
@@ -190,20 +193,18 @@ __device__ __forceinline__ void update8(float* pv, const float* gv, uint32_t& mu
     const float gj = __fmul_rn(gv[j], c.gscale);
     mv[j] = __fadd_rn(__fmul_rn(mv[j], c.b1), __fmul_rn(gj, c.c1));
     vv[j] = __fadd_rn(__fmul_rn(vv[j], c.b2), __fmul_rn(__fmul_rn(gj, gj), c.c2));
-    mtop = max(mtop, __float_as_uint(mv[j]) & 0x7FFFFFFFu);
-    vtop = max(vtop, __float_as_uint(vv[j]) & 0x7FFFFFFFu);
     pv[j] = stepped(pv[j], mv[j], vv[j], c);
   }
-  mtop = __reduce_max_sync(0xffffffffu, mtop);
-  vtop = __reduce_max_sync(0xffffffffu, vtop);
+  uint32_t mtop = __reduce_max_sync(0xffffffffu, top4(mv));
+  uint32_t vtop = __reduce_max_sync(0xffffffffu, top4(vv));
   const bool bad = max(mtop, vtop) >= fp8::kInfBits;
   if (bad) {                                         // whole warp: maxima of what is finite
     mtop = vtop = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t a = __float_as_uint(mv[j]) & 0x7FFFFFFFu, b = __float_as_uint(vv[j]) & 0x7FFFFFFFu;
-      mtop = max(mtop, a >= fp8::kInfBits ? 0u : a);
-      vtop = max(vtop, b >= fp8::kInfBits ? 0u : b);
+      const uint32_t x = __float_as_uint(mv[j]) & 0x7FFFFFFFu, y = __float_as_uint(vv[j]) & 0x7FFFFFFFu;
+      mtop = max(mtop, x >= fp8::kInfBits ? 0u : x);
+      vtop = max(vtop, y >= fp8::kInfBits ? 0u : y);
     }
     mtop = __reduce_max_sync(0xffffffffu, mtop);
     vtop = __reduce_max_sync(0xffffffffu, vtop);
@@ -211,27 +212,35 @@ __device__ __forceinline__ void update8(float* pv, const float* gv, uint32_t& mu
   mb = fp8::scale_byte(mtop);
   vb = scale_byte_v(vtop);
   const float minv = fp8::inv_scale(mb), vinv = fp8::inv_scale(vb);
-  mu = vu = 0;
+  uint32_t um[4], uv[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t r = mix(i + j + key);
-    uint32_t cm = encode_m(mv[j], minv, r & 0xFFFFu), cv = encode_v(vv[j], vinv, r >> 16);
-    if (bad) {
-      if (!isfinite(mv[j])) cm = 0x7Fu | (cm & 0x80u);
-      if (!isfinite(vv[j])) cv = 255u;
-      cm &= 0xFFu;
-      cv &= 0xFFu;
+    const uint32_t m7 = round_bits(fabsf(mv[j]) * minv, 0.015625f, __byte_perm(r, 0, 0x4410));        // 2^-6
+    um[j] = (m7 & 0x7FFFFFFFu) | (__float_as_uint(mv[j]) & 0x80000000u);
+    uv[j] = round_bits(vv[j] * vinv, 6.103515625e-05f, __byte_perm(r, 0, 0x4432));                    // 2^-14
+  }
+  mu = pack_top(um[0], um[1], um[2], um[3]) ^ 0x40404040u;
+  vu = pack_top(uv[0], uv[1], uv[2], uv[3]) ^ 0x80808080u;
+  if ((vu - 0x01010101u) & ~vu & 0x80808080u) {      // some code is 0: a positive v takes 1
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (vv[j] > 0.f && ((vu >> (8 * j)) & 0xFFu) == 0) vu |= 1u << (8 * j);
+  }
+  if (bad) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!isfinite(mv[j])) mu |= 0x7Fu << (8 * j);
+      if (!isfinite(vv[j])) vu |= 0xFFu << (8 * j);
     }
-    mu |= cm << (8 * j);
-    vu |= cv << (8 * j);
   }
 }
 
-// A CTA takes chunks of 32 blocks; a warp takes 4 of them, 8 blocks apart.  Where the chunk is
-// whole and every tensor starts on a vector, the warp has the loads of all 4 in flight before
+// A CTA takes chunks of 16 blocks; a warp takes 2 of them, 8 blocks apart.  Where the chunk is
+// whole and every tensor starts on a vector, the warp has the loads of both in flight before
 // it computes; ends and odd addresses go block by block, element by element.
 template <typename PT, typename GT, bool STATE8, int CAP>
-__global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ Args<CAP> args) {
+__global__ void __launch_bounds__(256, 4) step_kernel(const __grid_constant__ Args<CAP> args) {
   constexpr int U = kChunkBlocks / 8;
   const Consts c = args.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -344,7 +353,7 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ Args<
 template <typename PT, typename GT, int CAP>
 static void launch(const Args<CAP>& a, bool state8, int device, cudaStream_t stream) {
   const int chunks = a.chunk_end[a.tensors - 1];
-  const int grid = std::min(chunks, num_sms(device) * 8);
+  const int grid = std::min(chunks, num_sms(device) * 16);
   if (state8) step_kernel<PT, GT, true, CAP><<<grid, 256, 0, stream>>>(a);
   else step_kernel<PT, GT, false, CAP><<<grid, 256, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();

@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "common.cuh"
 #include "fp8.cuh"
@@ -23,94 +24,163 @@ __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 
-// 8 consecutive elements of a row from column c; zeros from column K on.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c, int K, float* v) {
-  if (VEC && c + 8 <= K) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(row + c));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + c));
-      const T* h = reinterpret_cast<const T*>(&u);
+// 8 consecutive elements of a row as they are in memory (16 bytes of a 16-bit type, 32 of fp32).
+// `top` takes the larger magnitudes of two such pieces element by element, packed two to a
+// register for 16-bit types (NaN wins, so that it is seen in the result); `bits(j)` is the
+// magnitude of element j as fp32 bits.
+template <typename T> struct Piece {
+  uint4 r;
+  __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load_some(const T* p, int n) {
+    uint16_t h[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f(h[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f(row[c + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) h[i] = i < n ? reinterpret_cast<const uint16_t*>(p)[i] : 0;
+    r = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                   h[6] | (uint32_t)h[7] << 16);
   }
+  // keeps the packed form live here: unpacked copies are not carried from one use to the next
+  __device__ __forceinline__ void pin() { asm volatile("" : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)); }
+  __device__ __forceinline__ uint32_t reg(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+  __device__ __forceinline__ static float wide(uint32_t u, int half) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return __uint_as_float(half ? u & 0xFFFF0000u : u << 16);
+    } else {
+      const uint32_t h = half ? u >> 16 : u & 0xFFFFu;
+      return __half2float(__ushort_as_half((unsigned short)h));
+    }
+  }
+  __device__ __forceinline__ float get(int j) const { return wide(reg(j >> 1), j & 1); }
+  // packed magnitudes of two registers
+  __device__ __forceinline__ static uint32_t top(uint32_t a, uint32_t b) {
+    using P = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+    const P m = __hmax2_nan(__habs2(*reinterpret_cast<P*>(&a)), __habs2(*reinterpret_cast<P*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  __device__ __forceinline__ static uint32_t bits(uint32_t packed, int half) {
+    return __float_as_uint(wide(packed, half)) & 0x7FFFFFFFu;
+  }
+  __device__ __forceinline__ uint32_t max_bits() const {
+    const uint32_t m = top(top(r.x, r.y), top(r.z, r.w));
+    return max(bits(m, 0), bits(m, 1));
+  }
+};
+template <> struct Piece<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  }
+  __device__ __forceinline__ void load_some(const float* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ void pin() {}
+  __device__ __forceinline__ float get(int j) const { return v[j]; }
+  __device__ __forceinline__ uint32_t max_bits() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+  }
+};
+// The piece at column c of a row of K; zeros from column K on.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_piece(Piece<T>& o, const T* row, int c, int K) {
+  if (VEC && c + 8 <= K) o.load(row + c);
+  else o.load_some(row + c, K - c);
 }
-
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t b = abs_bits(v);
-  return b >= kInfBits ? 0u : b;
+template <typename T>
+__device__ __forceinline__ uint32_t finite_max_bits(const Piece<T>& p) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __float_as_uint(p.get(j)) & 0x7FFFFFFFu;
+    m = max(m, b >= kInfBits ? 0u : b);
+  }
+  return m;
 }
 
 // ---------------------------------------------------------------------------- rows
 // A lane owns 16 consecutive columns, so 8 lanes own a block (3 shuffles for its maximum), a
-// lane's codes are one 16-byte store and a warp's four scales one 4-byte word.
+// lane's codes are one 16-byte store and a warp's four scales one 4-byte word.  A warp takes two
+// such runs of 512 columns, with the loads of both in flight.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
                                                             uint8_t* __restrict__ scale, int R, int K, int Kp,
                                                             int kgroups, long total) {
   const int lane = threadIdx.x & 31;
-  const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (w >= total) return;
-  const long r = w / kgroups;
-  const int kg = (int)(w - r * kgroups);
-  uint32_t* word = reinterpret_cast<uint32_t*>(scale + scale_offset(r, 4 * kg, kgroups));
-  if (r >= R) {
-    if (lane == 0) *word = 0;
-    return;
-  }
-  const int c = kg * 512 + lane * 16;
-  float v[16];
-  load8<T, VEC>(x + r * ld, c, K, v);
-  load8<T, VEC>(x + r * ld, c + 8, K, v + 8);
-  uint32_t amax = 0;
+  const long w0 = ((long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2;
+  if (w0 >= total) return;
+  Piece<T> v[2][2];
+  long row[2];
+  int kg[2];
+  row[0] = w0 / kgroups;
+  kg[0] = (int)(w0 - row[0] * kgroups);
+  const bool wraps = kg[0] + 1 == kgroups;
+  row[1] = w0 + 1 < total ? row[0] + wraps : (long)1 << 40;      // past the end: nothing to write
+  kg[1] = wraps ? 0 : kg[0] + 1;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) amax = max(amax, abs_bits(v[i]));
-  const bool bad = __any_sync(0xffffffffu, amax >= kInfBits);
-  if (bad) {
-    amax = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) amax = max(amax, finite_bits(v[i]));
+  for (int u = 0; u < 2; ++u) {
+    const int c = kg[u] * 512 + lane * 16;
+    if (row[u] < R) {
+      load_piece<T, VEC>(v[u][0], x + row[u] * ld, c, K);
+      load_piece<T, VEC>(v[u][1], x + row[u] * ld, c + 8, K);
+    }
   }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const uint32_t byte = scale_byte(amax);
-  const float inv = inv_scale(byte);
+  for (int u = 0; u < 2; ++u) {
+    if (row[u] == (long)1 << 40) return;
+    uint32_t* word = reinterpret_cast<uint32_t*>(scale + scale_offset(row[u], 4 * kg[u], kgroups));
+    if (row[u] >= R) {
+      if (lane == 0) *word = 0;
+      continue;
+    }
+    const int c = kg[u] * 512 + lane * 16;
+    uint32_t amax = max(v[u][0].max_bits(), v[u][1].max_bits());
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] *= inv;
-  if (bad) {
+    for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const bool bad = __any_sync(0xffffffffu, amax >= kInfBits);
+    if (bad) {
+      amax = max(finite_max_bits(v[u][0]), finite_max_bits(v[u][1]));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = nan_if_inf(v[i]);
+      for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
+    const uint32_t byte = scale_byte(amax);
+    const float inv = inv_scale(byte);
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = v[u][i >> 1].get((i & 1) * 4 + j) * inv;
+        if (bad) y[j] = nan_if_inf(y[j]);
+      }
+      o[i] = cvt4(y[0], y[1], y[2], y[3]);
+    }
+    if (c < Kp) *reinterpret_cast<uint4*>(q + row[u] * Kp + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    uint32_t mine = c < Kp ? byte << (8 * (lane >> 3)) : 0u;
+    mine |= __shfl_xor_sync(0xffffffffu, mine, 8);
+    mine |= __shfl_xor_sync(0xffffffffu, mine, 16);
+    if (lane == 0) *word = mine;
   }
-  uint4 o;
-  o.x = cvt4(v[0], v[1], v[2], v[3]);
-  o.y = cvt4(v[4], v[5], v[6], v[7]);
-  o.z = cvt4(v[8], v[9], v[10], v[11]);
-  o.w = cvt4(v[12], v[13], v[14], v[15]);
-  if (c < Kp) *reinterpret_cast<uint4*>(q + r * Kp + c) = o;
-  uint32_t mine = c < Kp ? byte << (8 * (lane >> 3)) : 0u;
-  mine |= __shfl_xor_sync(0xffffffffu, mine, 8);
-  mine |= __shfl_xor_sync(0xffffffffu, mine, 16);
-  if (lane == 0) *word = mine;
 }
 
 // ---------------------------------------------------------------------------- tiles
 // One CTA per 128 x 128 tile; a thread holds 8 rows x 8 columns, a warp 32 x 64 (4 x 8
 // threads), so that row loads are 128-byte segments, row codes 64-byte and column codes
-// 32-byte ones without a pass through shared memory.
+// 32-byte ones without a pass through shared memory.  16-bit inputs stay packed in registers
+// (32 for a thread) and their maxima are taken two at a time; all 8 loads are in flight at once.
 template <typename T, bool VEC, bool TILE_SCALE, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(256) quantize_tiles_kernel(const T* __restrict__ x, long ld,
-                                                             uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-                                                             uint8_t* __restrict__ qt, uint8_t* __restrict__ scale_t,
-                                                             int R, int K, int Kp, int Rp) {
+__global__ void __launch_bounds__(256, 2)
+quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
+                      uint8_t* __restrict__ qt, uint8_t* __restrict__ scale_t, int R, int K, int Kp, int Rp) {
   __shared__ uint32_t rmax[2][128];
   __shared__ uint32_t cmax[4][128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -120,60 +190,64 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const T* __restrict
   const int kb = blockIdx.x, rb = blockIdx.y;
   const long r0 = (long)rb * 128 + rl;
   const int c0 = kb * 128 + cl;
-  float v[8][8];
+  Piece<T> v[8];
+  if (VEC && (rb + 1) * 128L <= R && (kb + 1) * 128 <= K) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (r0 + i < R) {
-      load8<T, VEC>(x + (r0 + i) * ld, c0, K, v[i]);
-    } else {
+    for (int i = 0; i < 8; ++i) v[i].load(x + (r0 + i) * ld + c0);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      if (r0 + i < R) load_piece<T, VEC>(v[i], x + (r0 + i) * ld, c0, K);
+      else v[i].zero();
     }
   }
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
-  const bool bad = __syncthreads_or(top >= kInfBits);
+  // maxima of the thread's rows (over 8 columns) and columns (over 8 rows), then over the warp
   uint32_t ra[8], ca[8];
+  auto gather = [&](bool finite) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ra[i] = ca[i] = 0;
-  if (!bad) {
+    for (int i = 0; i < 8; ++i) {
+      ra[i] = finite ? finite_max_bits(v[i]) : v[i].max_bits();
+      ca[i] = 0;
+    }
+    if constexpr (COLS && !TILE_SCALE) {
+      if (sizeof(T) == 2 && !finite) {
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+          for (int k = 0; k < 4; ++k) {
+            uint32_t m = Piece<T>::top(v[0].reg(k), v[1].reg(k));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = abs_bits(v[i][j]);
-        ra[i] = max(ra[i], b);
-        ca[j] = max(ca[j], b);
+            for (int i = 2; i < 8; ++i) m = Piece<T>::top(m, v[i].reg(k));
+#pragma unroll
+            for (int o = 8; o < 32; o <<= 1) m = Piece<T>::top(m, __shfl_xor_sync(0xffffffffu, m, o));
+            ca[2 * k] = Piece<T>::bits(m, 0);
+            ca[2 * k + 1] = Piece<T>::bits(m, 1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t b = __float_as_uint(v[i].get(j)) & 0x7FFFFFFFu;
+            ca[j] = max(ca[j], finite && b >= kInfBits ? 0u : b);
+          }
+#pragma unroll
+          for (int o = 8; o < 32; o <<= 1) ca[j] = max(ca[j], __shfl_xor_sync(0xffffffffu, ca[j], o));
+        }
       }
-  } else {
+      if (lane < 8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = finite_bits(v[i][j]);
-        ra[i] = max(ra[i], b);
-        ca[j] = max(ca[j], b);
+        for (int j = 0; j < 8; ++j) cmax[wr][cl + j] = ca[j];
       }
-  }
-  uint32_t rbyte[8], cbyte[8];
-  if constexpr (TILE_SCALE) {
-    uint32_t m = 0;
+    }
+    if constexpr (TILE_SCALE) {
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, ra[i]);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) rmax[0][warp] = m;
-    __syncthreads();
-    m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, rmax[0][i]);
-    m = scale_byte(m);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rbyte[i] = cbyte[i] = m;
-  } else {
-    if constexpr (ROWS) {
+      for (int i = 0; i < 8; ++i) m = max(m, ra[i]);
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (lane == 0) rmax[0][warp] = m;
+      ra[0] = m;
+    } else if constexpr (ROWS) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -183,68 +257,66 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const T* __restrict
         for (int i = 0; i < 8; ++i) rmax[wc][rl + i] = ra[i];
       }
     }
-    if constexpr (COLS) {
+  };
+  gather(false);
+  bool over = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int o = 8; o < 32; o <<= 1) ca[j] = max(ca[j], __shfl_xor_sync(0xffffffffu, ca[j], o));
-      if (lane < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cmax[wr][cl + j] = ca[j];
-      }
-    }
+  for (int i = 0; i < 8; ++i) over |= ra[i] >= kInfBits;
+  const bool bad = __syncthreads_or(over);
+  if (bad) {                                       // maxima of what is finite
+    gather(true);
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (ROWS) rbyte[i] = scale_byte(max(rmax[0][rl + i], rmax[1][rl + i]));
-      if constexpr (COLS)
-        cbyte[i] = scale_byte(max(max(cmax[0][cl + i], cmax[1][cl + i]), max(cmax[2][cl + i], cmax[3][cl + i])));
-    }
   }
-  if (bad) {
+  uint32_t tile_byte = 0;
+  if constexpr (TILE_SCALE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = nan_if_inf(v[i][j]);
+    for (int i = 0; i < 8; ++i) tile_byte = max(tile_byte, rmax[0][i]);
+    tile_byte = scale_byte(tile_byte);
   }
+  auto value = [&](int i, int j, float inv) {
+    const float y = v[i].get(j) * inv;
+    return bad ? nan_if_inf(y) : y;
+  };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i].pin();
   // scale bytes: 128 rows of this tile's block, and zeros for what the last chunk lacks
   if constexpr (ROWS) {
     const int kgroups = (gridDim.x + 3) >> 2;
-    if ((lane & 7) == 0 && wc == 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t byte = TILE_SCALE ? tile_byte : scale_byte(max(rmax[0][rl + i], rmax[1][rl + i]));
+      if ((lane & 7) == 0 && wc == 0) {
         uint8_t* s = scale + scale_offset(r0 + i, kb, kgroups);
-        *s = r0 + i < R ? (uint8_t)rbyte[i] : 0;
+        *s = r0 + i < R ? (uint8_t)byte : 0;
         if (kb == gridDim.x - 1)
           for (int j = 1; j < 4 - (kb & 3); ++j) s[j] = 0;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float inv = inv_scale(rbyte[i]);
+      const float inv = inv_scale(byte);
       uint2 o;
-      o.x = cvt4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-      o.y = cvt4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+      o.x = cvt4(value(i, 0, inv), value(i, 1, inv), value(i, 2, inv), value(i, 3, inv));
+      o.y = cvt4(value(i, 4, inv), value(i, 5, inv), value(i, 6, inv), value(i, 7, inv));
       if (r0 + i < R) *reinterpret_cast<uint2*>(q + (r0 + i) * Kp + c0) = o;
     }
   }
   if constexpr (COLS) {
     const int rgroups = (gridDim.y + 3) >> 2;
-    if (lane < 8 && wr == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < 8; ++i) v[i].pin();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t byte = TILE_SCALE ? tile_byte
+                                       : scale_byte(max(max(cmax[0][cl + j], cmax[1][cl + j]),
+                                                        max(cmax[2][cl + j], cmax[3][cl + j])));
+      if (lane < 8 && wr == 0) {
         uint8_t* s = scale_t + scale_offset(c0 + j, rb, rgroups);
-        *s = c0 + j < K ? (uint8_t)cbyte[j] : 0;
+        *s = c0 + j < K ? (uint8_t)byte : 0;
         if (rb == gridDim.y - 1)
           for (int i = 1; i < 4 - (rb & 3); ++i) s[i] = 0;
       }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float inv = inv_scale(cbyte[j]);
+      const float inv = inv_scale(byte);
       uint2 o;
-      o.x = cvt4(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
-      o.y = cvt4(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv);
+      o.x = cvt4(value(0, j, inv), value(1, j, inv), value(2, j, inv), value(3, j, inv));
+      o.y = cvt4(value(4, j, inv), value(5, j, inv), value(6, j, inv), value(7, j, inv));
       if (c0 + j < K) *reinterpret_cast<uint2*>(qt + (long)(c0 + j) * Rp + r0) = o;
     }
   }
@@ -272,7 +344,7 @@ static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
   if (!tile_scale && qt == nullptr) {
     const int kgroups = (K + 511) / 512;
     const long total = (long)Rp * kgroups;
-    const unsigned grid = (unsigned)((total + 7) / 8);
+    const unsigned grid = (unsigned)((total + 15) / 16);
     if (vec) fp8::quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(xp, ld, q, s, R, K, Kp, kgroups, total);
     else fp8::quantize_rows_kernel<T, false><<<grid, 256, 0, stream>>>(xp, ld, q, s, R, K, Kp, kgroups, total);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
