@@ -104,14 +104,19 @@ __device__ __forceinline__ void store(T* p, bool wide, int left, const float* o)
       if (j < left) st1(p + j, o[j]);
   }
 }
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int left) {
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, bool wide, int left) {
+  if (wide && left >= 4) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t u = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (j < left) u |= (uint32_t)p[j] << (8 * j);
   return u;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int left, uint32_t u) {
+__device__ __forceinline__ void store_codes(uint8_t* p, bool wide, int left, uint32_t u) {
+  if (wide && left >= 4) {
+    *reinterpret_cast<uint32_t*>(p) = u;
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (j < left) p[j] = (uint8_t)(u >> (8 * j));
@@ -236,124 +241,111 @@ __device__ __forceinline__ void update8(float* pv, const float* gv, uint32_t& mu
   }
 }
 
-// A CTA takes chunks of 16 blocks; a warp takes 2 of them, 8 blocks apart.  Where the chunk is
-// whole and every tensor starts on a vector, the warp has the loads of both in flight before
-// it computes; ends and odd addresses go block by block, element by element.
+// One tensor as a kernel sees it, and the state of one block of it in a lane's registers.
+template <typename PT, typename GT> struct View {
+  PT* p;
+  const GT* g;
+  void *m, *v;
+  uint8_t *ms, *vs;
+  int64_t n;
+  uint32_t key;
+  bool wide;                              // every pointer allows vectors of four elements
+};
+template <typename PT, typename GT, bool STATE8> struct Lane {
+  float p[4], g[4];
+  float m[STATE8 ? 1 : 4], v[STATE8 ? 1 : 4];
+  uint32_t mu, vu, mb, vb;
+
+  __device__ __forceinline__ void read(const View<PT, GT>& t, int64_t blk, int lane, bool wide, int left) {
+    const int64_t i = blk * 128 + lane * 4;
+    load(t.p + i, wide, left, p);
+    load(t.g + i, wide, left, g);
+    if constexpr (STATE8) {
+      mu = load_codes(static_cast<const uint8_t*>(t.m) + i, wide, left);
+      vu = load_codes(static_cast<const uint8_t*>(t.v) + i, wide, left);
+      mb = t.ms[blk];
+      vb = t.vs[blk];
+    } else {
+      load(static_cast<const float*>(t.m) + i, wide, left, m);
+      load(static_cast<const float*>(t.v) + i, wide, left, v);
+    }
+  }
+  __device__ __forceinline__ void step(const View<PT, GT>& t, int64_t blk, int lane, const Consts& c) {
+    if constexpr (STATE8) update8(p, g, mu, vu, mb, vb, (uint32_t)(blk * 128 + lane * 4), t.key, c);
+    else update32(p, g, m, v, c);
+  }
+  __device__ __forceinline__ void write(const View<PT, GT>& t, int64_t blk, int lane, bool wide, int left) const {
+    const int64_t i = blk * 128 + lane * 4;
+    store(t.p + i, wide, left, p);
+    if constexpr (STATE8) {
+      store_codes(static_cast<uint8_t*>(t.m) + i, wide, left, mu);
+      store_codes(static_cast<uint8_t*>(t.v) + i, wide, left, vu);
+      if (lane == 0) {
+        t.ms[blk] = (uint8_t)mb;
+        t.vs[blk] = (uint8_t)vb;
+      }
+    } else {
+      store(static_cast<float*>(t.m) + i, wide, left, m);
+      store(static_cast<float*>(t.v) + i, wide, left, v);
+    }
+  }
+};
+
+// One CTA per chunk of 16 blocks; a warp takes 2 neighbouring ones, with the loads of both in
+// flight.  Many short CTAs beat resident ones that loop over chunks: 64M elements took 172 us
+// this way, 209 to 227 in a loop (a warp's next loads there queue behind its byte-sized scale
+// stores), and dealing contiguous runs of chunks to resident CTAs with a register prefetch was
+// slower still.
 template <typename PT, typename GT, bool STATE8, int CAP>
 __global__ void __launch_bounds__(256, 4) step_kernel(const __grid_constant__ Args<CAP> args) {
   constexpr int U = kChunkBlocks / 8;
   const Consts c = args.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int chunks = args.chunk_end[args.tensors - 1];
-  for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    int lo = 0, hi = args.tensors - 1;               // first tensor with chunk < chunk_end
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (chunk < args.chunk_end[mid]) hi = mid;
-      else lo = mid + 1;
+  const int chunk = blockIdx.x;
+  int lo = 0, hi = args.tensors - 1;                 // first tensor with chunk < chunk_end
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (chunk < args.chunk_end[mid]) hi = mid;
+    else lo = mid + 1;
+  }
+  View<PT, GT> t;
+  t.p = static_cast<PT*>(args.p[lo]);
+  t.g = static_cast<const GT*>(args.g[lo]);
+  t.m = args.m[lo];
+  t.v = args.v[lo];
+  t.ms = args.ms[lo];
+  t.vs = args.vs[lo];
+  t.n = args.n[lo];
+  t.key = args.key[lo];
+  constexpr uintptr_t kState = STATE8 ? 3 : 15;
+  t.wide = ((reinterpret_cast<uintptr_t>(t.p) & (4 * sizeof(PT) - 1)) |
+            (reinterpret_cast<uintptr_t>(t.g) & (4 * sizeof(GT) - 1)) |
+            ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & kState)) == 0;
+  const int64_t blk = (int64_t)(chunk - (lo ? args.chunk_end[lo - 1] : 0)) * kChunkBlocks + warp * U;
+  Lane<PT, GT, STATE8> x[U];
+  if (t.wide && (blk + U) * 128 <= t.n) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u].read(t, blk + u, lane, true, 4);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u].step(t, blk + u, lane, c);
+      x[u].write(t, blk + u, lane, true, 4);
     }
-    const int64_t blk0 = (int64_t)(chunk - (lo ? args.chunk_end[lo - 1] : 0)) * kChunkBlocks;
-    const int64_t e0 = blk0 * 128;
-    const int64_t n = args.n[lo] - e0;               // elements from the chunk's start on
-    PT* p = reinterpret_cast<PT*>(args.p[lo]) + e0;
-    const GT* g = reinterpret_cast<const GT*>(args.g[lo]) + e0;
-    const uint32_t key = args.key[lo] + (uint32_t)e0;
-    uintptr_t low = (reinterpret_cast<uintptr_t>(p) * (4 / sizeof(PT))) | (reinterpret_cast<uintptr_t>(g) * (4 / sizeof(GT)));
-    if constexpr (STATE8) {
-      uint8_t* mq = reinterpret_cast<uint8_t*>(args.m[lo]) + e0;
-      uint8_t* vq = reinterpret_cast<uint8_t*>(args.v[lo]) + e0;
-      uint8_t* ms = args.ms[lo] + blk0;
-      uint8_t* vs = args.vs[lo] + blk0;
-      low |= (reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(vq)) * 4;
-      if (low % 16 == 0 && n >= kChunkBlocks * 128) {
-        float pv[U][4], gv[U][4];
-        uint32_t mu[U], vu[U], mb[U], vb[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int blk = warp + 8 * u, i = blk * 128 + lane * 4;
-          load(p + i, true, 4, pv[u]);
-          load(g + i, true, 4, gv[u]);
-          mu[u] = *reinterpret_cast<const uint32_t*>(mq + i);
-          vu[u] = *reinterpret_cast<const uint32_t*>(vq + i);
-          mb[u] = ms[blk];
-          vb[u] = vs[blk];
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int blk = warp + 8 * u, i = blk * 128 + lane * 4;
-          update8(pv[u], gv[u], mu[u], vu[u], mb[u], vb[u], (uint32_t)i, key, c);
-          store(p + i, true, 4, pv[u]);
-          *reinterpret_cast<uint32_t*>(mq + i) = mu[u];
-          *reinterpret_cast<uint32_t*>(vq + i) = vu[u];
-          if (lane == 0) {
-            ms[blk] = (uint8_t)mb[u];
-            vs[blk] = (uint8_t)vb[u];
-          }
-        }
-        continue;
-      }
-      for (int blk = warp; blk < kChunkBlocks && blk * 128 < n; blk += 8) {
-        const int i = blk * 128 + lane * 4;
-        const int left = (int)min((int64_t)4, n - i);          // below 1: this lane has none
-        float pv[4], gv[4];
-        load(p + i, false, left, pv);
-        load(g + i, false, left, gv);
-        uint32_t mu = load_codes(mq + i, left), vu = load_codes(vq + i, left), mb = ms[blk], vb = vs[blk];
-        update8(pv, gv, mu, vu, mb, vb, (uint32_t)i, key, c);
-        store(p + i, false, left, pv);
-        store_codes(mq + i, left, mu);
-        store_codes(vq + i, left, vu);
-        if (lane == 0) {
-          ms[blk] = (uint8_t)mb;
-          vs[blk] = (uint8_t)vb;
-        }
-      }
-    } else {
-      float* m = reinterpret_cast<float*>(args.m[lo]) + e0;
-      float* v = reinterpret_cast<float*>(args.v[lo]) + e0;
-      low |= reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
-      if (low % 16 == 0 && n >= kChunkBlocks * 128) {
-        float pv[U][4], gv[U][4], mv[U][4], vv[U][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = (warp + 8 * u) * 128 + lane * 4;
-          load(p + i, true, 4, pv[u]);
-          load(g + i, true, 4, gv[u]);
-          load(m + i, true, 4, mv[u]);
-          load(v + i, true, 4, vv[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = (warp + 8 * u) * 128 + lane * 4;
-          update32(pv[u], gv[u], mv[u], vv[u], c);
-          store(p + i, true, 4, pv[u]);
-          store(m + i, true, 4, mv[u]);
-          store(v + i, true, 4, vv[u]);
-        }
-        continue;
-      }
-      for (int blk = warp; blk < kChunkBlocks && blk * 128 < n; blk += 8) {
-        const int i = blk * 128 + lane * 4;
-        const int left = (int)min((int64_t)4, n - i);
-        const bool wide = low % 16 == 0;
-        float pv[4], gv[4], mv[4], vv[4];
-        load(p + i, wide, left, pv);
-        load(g + i, wide, left, gv);
-        load(m + i, wide, left, mv);
-        load(v + i, wide, left, vv);
-        update32(pv, gv, mv, vv, c);
-        store(p + i, wide, left, pv);
-        store(m + i, wide, left, mv);
-        store(v + i, wide, left, vv);
-      }
+  } else {                                           // a tensor's end, and odd addresses
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) {
+      if ((blk + u) * 128 >= t.n) break;             // whole warp
+      const int left = (int)min((int64_t)4, t.n - (blk + u) * 128 - lane * 4);   // below 1: this lane has none
+      x[0].read(t, blk + u, lane, t.wide, left);
+      x[0].step(t, blk + u, lane, c);
+      x[0].write(t, blk + u, lane, t.wide, left);
     }
   }
 }
 
 template <typename PT, typename GT, int CAP>
-static void launch(const Args<CAP>& a, bool state8, int device, cudaStream_t stream) {
-  const int chunks = a.chunk_end[a.tensors - 1];
-  const int grid = std::min(chunks, num_sms(device) * 16);
+static void launch(const Args<CAP>& a, bool state8, cudaStream_t stream) {
+  const int grid = a.chunk_end[a.tensors - 1];       // chunks, below 2^31
   if (state8) step_kernel<PT, GT, true, CAP><<<grid, 256, 0, stream>>>(a);
   else step_kernel<PT, GT, false, CAP><<<grid, 256, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -365,7 +357,7 @@ struct Lists {
 
 // Fills parameter blocks of CAP tensors and launches each.
 template <int CAP>
-static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed, int dev, cudaStream_t stream) {
+static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed, cudaStream_t stream) {
   const bool pf = l.p[0].scalar_type() == at::kFloat, gf = l.g[0].scalar_type() == at::kFloat;
   Args<CAP> a;
   a.c = consts;
@@ -373,10 +365,10 @@ static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed
   int64_t chunks = 0;
   auto flush = [&]() {
     if (a.tensors == 0) return;
-    if (pf && gf) launch<float, float, CAP>(a, state8, dev, stream);
-    else if (pf) launch<float, __nv_bfloat16, CAP>(a, state8, dev, stream);
-    else if (gf) launch<__nv_bfloat16, float, CAP>(a, state8, dev, stream);
-    else launch<__nv_bfloat16, __nv_bfloat16, CAP>(a, state8, dev, stream);
+    if (pf && gf) launch<float, float, CAP>(a, state8, stream);
+    else if (pf) launch<float, __nv_bfloat16, CAP>(a, state8, stream);
+    else if (gf) launch<__nv_bfloat16, float, CAP>(a, state8, stream);
+    else launch<__nv_bfloat16, __nv_bfloat16, CAP>(a, state8, stream);
     a.tensors = 0;
     chunks = 0;
   };
@@ -446,8 +438,8 @@ void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vect
   c.gscale = (float)gscale;
   const Lists lists{p, g, m, v, ms, vs};
   // a short list has a small parameter block: 4 KB instead of 30 KB to copy with the launch
-  if (count <= kSmallCap) run<kSmallCap>(lists, c, state8, (uint32_t)seed, dev, stream);
-  else run<kCap>(lists, c, state8, (uint32_t)seed, dev, stream);
+  if (count <= kSmallCap) run<kSmallCap>(lists, c, state8, (uint32_t)seed, stream);
+  else run<kCap>(lists, c, state8, (uint32_t)seed, stream);
 }
 
 }  // namespace osp
