@@ -167,7 +167,7 @@ def check_product(y, a, b, bias=None, act=None):
 
 PRODUCTS = [(1, 16, 64), (1, 300, 5120), (2, 129, 640), (7, 1000, 130), (33, 128, 2048), (64, 512, 128),
             (65, 640, 384), (128, 256, 512), (130, 64, 900), (200, 72, 1111), (300, 777, 1024), (513, 1536, 640),
-            (1025, 250, 257), (2500, 2304, 512), (12, 1, 128), (5, 13824, 200)]
+            (1025, 250, 257), (2500, 2304, 512), (4700, 1300, 1111), (19000, 200, 129), (12, 1, 128), (5, 13824, 200)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
