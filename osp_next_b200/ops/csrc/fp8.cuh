@@ -44,9 +44,6 @@ __device__ __forceinline__ uint32_t cvt2(float a, float b) {
 __device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d) {
   return cvt2(a, b) | (cvt2(c, d) << 16);
 }
-// What a value becomes before conversion in a block with non-finite elements: infinities
-// turn into NaN (e4m3 has no infinity, and a silent 448 would hide an overflow).
-__device__ __forceinline__ float nan_if_inf(float y) { return isinf(y) ? __uint_as_float(0x7FFFFFFFu) : y; }
 
 }  // namespace fp8
 }  // namespace osp

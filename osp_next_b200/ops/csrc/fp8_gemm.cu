@@ -46,7 +46,8 @@ template <int BN> struct Shape {
   static constexpr uint32_t kAccStride = BN == 256 ? 240 : BN;  // column offset of accumulator 1
   static constexpr bool kOverlap = BN == 256;
   static constexpr int smem_bytes() {
-    return 1024 + kStages * (int)(kA + kB + kScales) + (2 * kStages + 7) * 8 + 16 + 128 + 8 * kStageBytes;
+    return 1024 + kStages * (int)(kA + kB + kScales) + (2 * kStages + 7) * 8 + 16 + 128 + 8 * kStageBytes +
+           16 * BN;      // bias: BN / 2 columns for each of 8 warps
   }
 };
 
@@ -58,7 +59,7 @@ struct Args {
   int act;                   // 0 none, 1 gelu_tanh
   void* out;                 // [M, N] bf16 or f32
   __nv_bfloat16* aux;        // [M, N] pre-activation or null
-  int vec;                   // rows of out (and aux) and the bias start on 16 bytes
+  int vec;                   // rows of out (and aux) start on 16 bytes
   int* err;
 };
 
@@ -107,7 +108,8 @@ __device__ __forceinline__ void store_scalar(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_scalar(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 
 // A warp's 32 rows x 32 columns of results (one row per lane) -> out, through shared memory so
-// that a row's 64 bytes (bf16) are written as one segment; fp32 rows are full lines as they are.
+// that 64 bytes of a row are written as one segment (16 bytes by 32 lanes to 32 rows took twice
+// the time of the whole product at K = 1536 in fp32).
 template <typename OutT>
 __device__ __forceinline__ void store_chunk(OutT* out, const float* v, uint8_t* stg, int lane, long row0, int col0,
                                             int M, int N, bool vec) {
@@ -140,31 +142,39 @@ __device__ __forceinline__ void store_chunk(OutT* out, const float* v, uint8_t* 
             *reinterpret_cast<const uint4*>(stg + rr * kStageRow + cc * 16);
     }
     __syncwarp();
-  } else if (row0 + lane < M) {
-    float4* o4 = reinterpret_cast<float4*>(out + (row0 + lane) * N + col0);
+  } else {
+    const int q = lane >> 2, cc = lane & 3;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o4[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    for (int h = 0; h < 2; ++h) {                     // 16 columns at a time: 64 bytes of a row
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(stg + lane * kStageRow + j * 16) =
+            make_float4(v[16 * h + 4 * j], v[16 * h + 4 * j + 1], v[16 * h + 4 * j + 2], v[16 * h + 4 * j + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rr = i * 8 + q;
+        if (row0 + rr < M)
+          *reinterpret_cast<float4*>(out + (row0 + rr) * N + col0 + 16 * h + cc * 4) =
+              *reinterpret_cast<const float4*>(stg + rr * kStageRow + cc * 16);
+      }
+      __syncwarp();
+    }
   }
 }
 
-// Bias, activation and store of a warp's 32 x 32 accumulator chunk.
+// Bias (the chunk's 32, in shared memory), activation and store of a warp's 32 x 32 chunk.
 template <typename OutT>
-__device__ __forceinline__ void finish_chunk(const Args& args, const uint32_t* r, uint8_t* stg, int lane, long row0,
-                                             int col0) {
+__device__ __forceinline__ void finish_chunk(const Args& args, const uint32_t* r, const float* bias, uint8_t* stg,
+                                             int lane, long row0, int col0) {
   float v[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
   if (args.bias) {
-    if (args.vec && col0 + 32 <= args.N) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 b = __ldg(reinterpret_cast<const float4*>(args.bias + col0) + j);
-        v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col0 + j < args.N) v[j] += __ldg(args.bias + col0 + j);
+    for (int j = 0; j < 8; ++j) {
+      const float4 b = reinterpret_cast<const float4*>(bias)[j];
+      v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
     }
   }
   if (args.aux) store_chunk(args.aux, v, stg, lane, row0, col0, args.M, args.N, args.vec);
@@ -317,12 +327,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     const int quarter = warp & 3;               // TMEM lanes 32 * quarter ..
     const int eg = (warp - 2) >> 2;
     uint8_t* stg = epi_stage + (warp - 2) * kStageBytes;
+    float* sbias = reinterpret_cast<float*>(epi_stage + 8 * kStageBytes) + (warp - 2) * PER * 32;
     int it = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, ++it) {
       if (*abort_flag) break;
       int mb, nb;
       tile_coords(t, num_m, num_n, mb, nb);
       const int acc = it & 1;
+      // the bias of the warp's columns, fetched while the MMAs run: beside the operands' traffic a
+      // load takes thousands of cycles, which per chunk made the epilogue longer than the MMAs
+      if (args.bias) {
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < PER; ++c) {
+          const int col = nb * BN + (eg * PER + c) * 32 + lane;
+          sbias[c * 32 + lane] = col < args.N ? __ldg(args.bias + col) : 0.f;
+        }
+        __syncwarp();
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (it >> 1) & 1, args.err, kErrFp8Epilogue))) {
         *abort_flag = 1;
         break;
@@ -343,7 +365,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           __syncwarp();
           if (lane == 0) mbar_arrive(&tearly[acc]);
         }
-        if (col0 < args.N) finish_chunk<OutT>(args, r, stg, lane, row0, col0);
+        if (col0 < args.N) finish_chunk<OutT>(args, r, sbias + (c - eg * PER) * 32, stg, lane, row0, col0);
       }
       tc_fence_before();
       __syncwarp();
@@ -425,8 +447,7 @@ void fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, co
   TORCH_CHECK(act == 0 || act == 1, "fp8_matmul: act");
   args.act = (int)act;
   args.out = out.data_ptr();
-  args.vec = args.N % 8 == 0 && reinterpret_cast<uintptr_t>(args.out) % 16 == 0 &&
-             reinterpret_cast<uintptr_t>(args.bias) % 16 == 0;
+  args.vec = args.N % 8 == 0 && reinterpret_cast<uintptr_t>(args.out) % 16 == 0;
   if (aux.has_value()) {
     TORCH_CHECK(aux->is_cuda() && aux->get_device() == dev && aux->scalar_type() == at::kBFloat16 &&
                 aux->is_contiguous() && aux->sizes() == out.sizes(), "fp8_matmul: aux bf16 [M, N]");

@@ -24,10 +24,16 @@ __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 
-// 8 consecutive elements of a row as they are in memory (16 bytes of a 16-bit type, 32 of fp32).
-// `top` takes the larger magnitudes of two such pieces element by element, packed two to a
-// register for 16-bit types (NaN wins, so that it is seen in the result); `bits(j)` is the
-// magnitude of element j as fp32 bits.
+// The larger of two magnitudes given as fp32 bits.  Maxima are first taken so that a NaN wins
+// (SEE_NAN), which shows with infinities as a result >= kInfBits; a block that has one turns its
+// infinities into NaN and takes its maxima again so that NaN loses.
+template <bool SEE_NAN> __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+  if constexpr (SEE_NAN) return max(a, b);
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+
+// 8 consecutive elements of a row as they are in memory (16 bytes of a 16-bit type, 32 of fp32);
+// maxima of 16-bit types are taken two at a time in packed registers.
 template <typename T> struct Piece {
   uint4 r;
   __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
@@ -38,6 +44,16 @@ template <typename T> struct Piece {
     for (int i = 0; i < 8; ++i) h[i] = i < n ? reinterpret_cast<const uint16_t*>(p)[i] : 0;
     r = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
                    h[6] | (uint32_t)h[7] << 16);
+  }
+  // infinities become NaN (e4m3 has none, and a silent 448 would hide an overflow)
+  __device__ __forceinline__ void spoil_inf() {
+    constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+    uint32_t* u = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((u[i] & 0x7FFFu) == kInf) u[i] |= 1u;
+      if (((u[i] >> 16) & 0x7FFFu) == kInf) u[i] |= 0x10000u;
+    }
   }
   // keeps the packed form live here: unpacked copies are not carried from one use to the next
   __device__ __forceinline__ void pin() { asm volatile("" : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)); }
@@ -51,18 +67,27 @@ template <typename T> struct Piece {
     }
   }
   __device__ __forceinline__ float get(int j) const { return wide(reg(j >> 1), j & 1); }
-  // packed magnitudes of two registers
-  __device__ __forceinline__ static uint32_t top(uint32_t a, uint32_t b) {
-    using P = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
-    const P m = __hmax2_nan(__habs2(*reinterpret_cast<P*>(&a)), __habs2(*reinterpret_cast<P*>(&b)));
-    return *reinterpret_cast<const uint32_t*>(&m);
+  // the larger magnitudes of two registers (their signs are of no meaning)
+  template <bool SEE_NAN> __device__ __forceinline__ static uint32_t top(uint32_t a, uint32_t b) {
+    uint32_t m;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      if constexpr (SEE_NAN) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+      else asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    } else {
+      if constexpr (SEE_NAN) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+      else asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    }
+    return m;
   }
   __device__ __forceinline__ static uint32_t bits(uint32_t packed, int half) {
     return __float_as_uint(wide(packed, half)) & 0x7FFFFFFFu;
   }
-  __device__ __forceinline__ uint32_t max_bits() const {
-    const uint32_t m = top(top(r.x, r.y), top(r.z, r.w));
-    return max(bits(m, 0), bits(m, 1));
+  template <bool SEE_NAN> __device__ __forceinline__ uint32_t packed_max() const {
+    return top<SEE_NAN>(top<SEE_NAN>(r.x, r.y), top<SEE_NAN>(r.z, r.w));
+  }
+  template <bool SEE_NAN> __device__ __forceinline__ uint32_t max_bits() const {
+    const uint32_t m = packed_max<SEE_NAN>();
+    return larger<SEE_NAN>(bits(m, 0), bits(m, 1));
   }
 };
 template <> struct Piece<float> {
@@ -80,12 +105,17 @@ template <> struct Piece<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
   }
+  __device__ __forceinline__ void spoil_inf() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (isinf(v[i])) v[i] = __uint_as_float(0x7FFFFFFFu);
+  }
   __device__ __forceinline__ void pin() {}
   __device__ __forceinline__ float get(int j) const { return v[j]; }
-  __device__ __forceinline__ uint32_t max_bits() const {
+  template <bool SEE_NAN> __device__ __forceinline__ uint32_t max_bits() const {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 8; ++i) m = larger<SEE_NAN>(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
     return m;
   }
 };
@@ -95,17 +125,6 @@ __device__ __forceinline__ void load_piece(Piece<T>& o, const T* row, int c, int
   if (VEC && c + 8 <= K) o.load(row + c);
   else o.load_some(row + c, K - c);
 }
-template <typename T>
-__device__ __forceinline__ uint32_t finite_max_bits(const Piece<T>& p) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t b = __float_as_uint(p.get(j)) & 0x7FFFFFFFu;
-    m = max(m, b >= kInfBits ? 0u : b);
-  }
-  return m;
-}
-
 // ---------------------------------------------------------------------------- rows
 // A lane owns 16 consecutive columns, so 8 lanes own a block (3 shuffles for its maximum), a
 // lane's codes are one 16-byte store and a warp's four scales one 4-byte word.  A warp takes two
@@ -142,14 +161,16 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
       continue;
     }
     const int c = kg[u] * 512 + lane * 16;
-    uint32_t amax = max(v[u][0].max_bits(), v[u][1].max_bits());
+    uint32_t amax = max(v[u][0].template max_bits<true>(), v[u][1].template max_bits<true>());
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const bool bad = __any_sync(0xffffffffu, amax >= kInfBits);
-    if (bad) {
-      amax = max(finite_max_bits(v[u][0]), finite_max_bits(v[u][1]));
+    if (__any_sync(0xffffffffu, amax >= kInfBits)) {
+      v[u][0].spoil_inf();
+      v[u][1].spoil_inf();
+      amax = larger<false>(v[u][0].template max_bits<false>(), v[u][1].template max_bits<false>());
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      for (int o = 1; o < 8; o <<= 1) amax = larger<false>(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (amax >= kInfBits) amax = 0;              // nothing finite
     }
     const uint32_t byte = scale_byte(amax);
     const float inv = inv_scale(byte);
@@ -158,10 +179,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
     for (int i = 0; i < 4; ++i) {
       float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[j] = v[u][i >> 1].get((i & 1) * 4 + j) * inv;
-        if (bad) y[j] = nan_if_inf(y[j]);
-      }
+      for (int j = 0; j < 4; ++j) y[j] = v[u][i >> 1].get((i & 1) * 4 + j) * inv;
       o[i] = cvt4(y[0], y[1], y[2], y[3]);
     }
     if (c < Kp) *reinterpret_cast<uint4*>(q + row[u] * Kp + c) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -177,23 +195,27 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // threads), so that row loads are 128-byte segments, row codes 64-byte and column codes
 // 32-byte ones without a pass through shared memory.  16-bit inputs stay packed in registers
 // (32 for a thread) and their maxima are taken two at a time; all 8 loads are in flight at once.
+// Maxima meet in shared memory, one thread per row and column forms its scale, and every
+// thread reads back the 16 factors that it needs.
 template <typename T, bool VEC, bool TILE_SCALE, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
                       uint8_t* __restrict__ qt, uint8_t* __restrict__ scale_t, int R, int K, int Kp, int Rp) {
-  __shared__ uint32_t rmax[2][128];
-  __shared__ uint32_t cmax[4][128];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ uint32_t top[2][4][128];              // [0]: rows over 2 warps, [1]: columns over 4
+  __shared__ __align__(16) float factor[2][128];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wr = warp >> 1, wc = warp & 1;
   const int rl = wr * 32 + (lane >> 3) * 8;        // first row of this thread in the tile
   const int cl = wc * 64 + (lane & 7) * 8;         // first column
   const int kb = blockIdx.x, rb = blockIdx.y;
   const long r0 = (long)rb * 128 + rl;
   const int c0 = kb * 128 + cl;
+  const bool inner = (rb + 1) * 128L <= R && (kb + 1) * 128 <= K;      // a whole tile
   Piece<T> v[8];
-  if (VEC && (rb + 1) * 128L <= R && (kb + 1) * 128 <= K) {
+  if (VEC && inner) {
+    const T* p = x + r0 * ld + c0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i].load(x + (r0 + i) * ld + c0);
+    for (int i = 0; i < 8; ++i, p += ld) v[i].load(p);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -202,122 +224,129 @@ quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
     }
   }
   // maxima of the thread's rows (over 8 columns) and columns (over 8 rows), then over the warp
-  uint32_t ra[8], ca[8];
-  auto gather = [&](bool finite) {
+  auto gather = [&](auto see) {
+    constexpr bool SEE = decltype(see)::value;
+    using P = Piece<T>;
+    uint32_t seen = 0;
+    if constexpr (TILE_SCALE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ra[i] = finite ? finite_max_bits(v[i]) : v[i].max_bits();
-      ca[i] = 0;
-    }
-    if constexpr (COLS && !TILE_SCALE) {
-      if (sizeof(T) == 2 && !finite) {
-        if constexpr (sizeof(T) == 2) {
+      for (int i = 0; i < 8; ++i) seen = larger<SEE>(seen, v[i].template max_bits<SEE>());
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t m = Piece<T>::top(v[0].reg(k), v[1].reg(k));
+      for (int o = 1; o < 32; o <<= 1) seen = larger<SEE>(seen, __shfl_xor_sync(0xffffffffu, seen, o));
+      if (lane == 0) top[0][0][warp] = seen;
+    } else if constexpr (sizeof(T) == 2) {
+      if constexpr (ROWS) {
 #pragma unroll
-            for (int i = 2; i < 8; ++i) m = Piece<T>::top(m, v[i].reg(k));
+        for (int i = 0; i < 8; i += 2) {
+          const uint32_t a = v[i].template packed_max<SEE>(), b = v[i + 1].template packed_max<SEE>();
+          // the two rows side by side
+          uint32_t m = P::template top<SEE>(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
 #pragma unroll
-            for (int o = 8; o < 32; o <<= 1) m = Piece<T>::top(m, __shfl_xor_sync(0xffffffffu, m, o));
-            ca[2 * k] = Piece<T>::bits(m, 0);
-            ca[2 * k + 1] = Piece<T>::bits(m, 1);
-          }
+          for (int o = 1; o < 8; o <<= 1) m = P::template top<SEE>(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const uint32_t m0 = P::bits(m, 0), m1 = P::bits(m, 1);
+          seen = max(seen, max(m0, m1));
+          if ((lane & 7) == 0) *reinterpret_cast<uint2*>(&top[0][wc][rl + i]) = make_uint2(m0, m1);
         }
-      } else {
+      }
+      if constexpr (COLS) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t m = P::template top<SEE>(v[0].reg(k), v[1].reg(k));
+#pragma unroll
+          for (int i = 2; i < 8; ++i) m = P::template top<SEE>(m, v[i].reg(k));
+#pragma unroll
+          for (int o = 8; o < 32; o <<= 1) m = P::template top<SEE>(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const uint32_t m0 = P::bits(m, 0), m1 = P::bits(m, 1);
+          seen = max(seen, max(m0, m1));
+          if (lane < 8) *reinterpret_cast<uint2*>(&top[1][wr][cl + 2 * k]) = make_uint2(m0, m1);
+        }
+      }
+    } else {
+      if constexpr (ROWS) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t m = v[i].template max_bits<SEE>();
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) m = larger<SEE>(m, __shfl_xor_sync(0xffffffffu, m, o));
+          seen = max(seen, m);
+          if ((lane & 7) == 0) top[0][wc][rl + i] = m;
+        }
+      }
+      if constexpr (COLS) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          uint32_t m = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __float_as_uint(v[i].get(j)) & 0x7FFFFFFFu;
-            ca[j] = max(ca[j], finite && b >= kInfBits ? 0u : b);
-          }
+          for (int i = 0; i < 8; ++i) m = larger<SEE>(m, __float_as_uint(v[i].get(j)) & 0x7FFFFFFFu);
 #pragma unroll
-          for (int o = 8; o < 32; o <<= 1) ca[j] = max(ca[j], __shfl_xor_sync(0xffffffffu, ca[j], o));
+          for (int o = 8; o < 32; o <<= 1) m = larger<SEE>(m, __shfl_xor_sync(0xffffffffu, m, o));
+          seen = max(seen, m);
+          if (lane < 8) top[1][wr][cl + j] = m;
         }
       }
-      if (lane < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cmax[wr][cl + j] = ca[j];
-      }
     }
-    if constexpr (TILE_SCALE) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, ra[i]);
-      m = __reduce_max_sync(0xffffffffu, m);
-      if (lane == 0) rmax[0][warp] = m;
-      ra[0] = m;
-    } else if constexpr (ROWS) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) ra[i] = max(ra[i], __shfl_xor_sync(0xffffffffu, ra[i], o));
-      if ((lane & 7) == 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rmax[wc][rl + i] = ra[i];
-      }
-    }
+    return seen;
   };
-  gather(false);
-  bool over = false;
+  const uint32_t seen = gather(std::true_type());
+  if (__syncthreads_or(seen >= kInfBits)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) over |= ra[i] >= kInfBits;
-  const bool bad = __syncthreads_or(over);
-  if (bad) {                                       // maxima of what is finite
-    gather(true);
+    for (int i = 0; i < 8; ++i) v[i].spoil_inf();
+    gather(std::false_type());
     __syncthreads();
   }
-  uint32_t tile_byte = 0;
-  if constexpr (TILE_SCALE) {
+  // one thread per row (the first 128) and per column: its scale byte, and zeros for what the
+  // last chunk of four blocks lacks
+  {
+    const int side = tid >> 7, i = tid & 127;
+    if ((side == 0 && ROWS) || (side == 1 && COLS)) {
+      uint32_t m;
+      if constexpr (TILE_SCALE) {
+        m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tile_byte = max(tile_byte, rmax[0][i]);
-    tile_byte = scale_byte(tile_byte);
-  }
-  auto value = [&](int i, int j, float inv) {
-    const float y = v[i].get(j) * inv;
-    return bad ? nan_if_inf(y) : y;
-  };
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i].pin();
-  // scale bytes: 128 rows of this tile's block, and zeros for what the last chunk lacks
-  if constexpr (ROWS) {
-    const int kgroups = (gridDim.x + 3) >> 2;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t byte = TILE_SCALE ? tile_byte : scale_byte(max(rmax[0][rl + i], rmax[1][rl + i]));
-      if ((lane & 7) == 0 && wc == 0) {
-        uint8_t* s = scale + scale_offset(r0 + i, kb, kgroups);
-        *s = r0 + i < R ? (uint8_t)byte : 0;
-        if (kb == gridDim.x - 1)
-          for (int j = 1; j < 4 - (kb & 3); ++j) s[j] = 0;
+        for (int w = 0; w < 8; ++w) m = larger<false>(m, top[0][0][w]);
+      } else {
+        m = larger<false>(top[side][0][i], top[side][1][i]);
+        if (side == 1) m = larger<false>(m, larger<false>(top[1][2][i], top[1][3][i]));
       }
-      const float inv = inv_scale(byte);
+      if (m >= kInfBits) m = 0;                    // nothing finite
+      const uint32_t byte = scale_byte(m);
+      factor[side][i] = inv_scale(byte);
+      const int blk = side ? rb : kb, blocks = side ? gridDim.y : gridDim.x;
+      const long line = side ? kb * 128L + i : rb * 128L + i;
+      uint8_t* s = (side ? scale_t : scale) + scale_offset(line, blk, (blocks + 3) >> 2);
+      *s = line < (side ? K : R) ? (uint8_t)byte : 0;
+      if (blk == blocks - 1)
+        for (int j = 1; j < 4 - (blk & 3); ++j) s[j] = 0;
+    }
+  }
+  __syncthreads();
+  if constexpr (ROWS) {
+    float f[8];
+    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&factor[0][rl]);
+    *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&factor[0][rl + 4]);
+    uint8_t* p = q + r0 * Kp + c0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, p += Kp) {
+      v[i].pin();
       uint2 o;
-      o.x = cvt4(value(i, 0, inv), value(i, 1, inv), value(i, 2, inv), value(i, 3, inv));
-      o.y = cvt4(value(i, 4, inv), value(i, 5, inv), value(i, 6, inv), value(i, 7, inv));
-      if (r0 + i < R) *reinterpret_cast<uint2*>(q + (r0 + i) * Kp + c0) = o;
+      o.x = cvt4(v[i].get(0) * f[i], v[i].get(1) * f[i], v[i].get(2) * f[i], v[i].get(3) * f[i]);
+      o.y = cvt4(v[i].get(4) * f[i], v[i].get(5) * f[i], v[i].get(6) * f[i], v[i].get(7) * f[i]);
+      if (inner || r0 + i < R) *reinterpret_cast<uint2*>(p) = o;
     }
   }
   if constexpr (COLS) {
-    const int rgroups = (gridDim.y + 3) >> 2;
+    float f[8];
+    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&factor[1][cl]);
+    *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&factor[1][cl + 4]);
+    uint8_t* p = qt + (long)c0 * Rp + r0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].pin();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t byte = TILE_SCALE ? tile_byte
-                                       : scale_byte(max(max(cmax[0][cl + j], cmax[1][cl + j]),
-                                                        max(cmax[2][cl + j], cmax[3][cl + j])));
-      if (lane < 8 && wr == 0) {
-        uint8_t* s = scale_t + scale_offset(c0 + j, rb, rgroups);
-        *s = c0 + j < K ? (uint8_t)byte : 0;
-        if (rb == gridDim.y - 1)
-          for (int i = 1; i < 4 - (rb & 3); ++i) s[i] = 0;
-      }
-      const float inv = inv_scale(byte);
+    for (int j = 0; j < 8; ++j, p += Rp) {
       uint2 o;
-      o.x = cvt4(value(0, j, inv), value(1, j, inv), value(2, j, inv), value(3, j, inv));
-      o.y = cvt4(value(4, j, inv), value(5, j, inv), value(6, j, inv), value(7, j, inv));
-      if (c0 + j < K) *reinterpret_cast<uint2*>(qt + (long)(c0 + j) * Rp + r0) = o;
+      o.x = cvt4(v[0].get(j) * f[j], v[1].get(j) * f[j], v[2].get(j) * f[j], v[3].get(j) * f[j]);
+      o.y = cvt4(v[4].get(j) * f[j], v[5].get(j) * f[j], v[6].get(j) * f[j], v[7].get(j) * f[j]);
+      if (inner || c0 + j < K) *reinterpret_cast<uint2*>(p) = o;
     }
   }
 }
