@@ -26,6 +26,7 @@ class _Counted:
         def call(*a, **k):
             _LAUNCHES[0] += 1
             return fn(*a, **k)
+        setattr(self, name, call)      # later look-ups of this name find it directly
         return call
 
 

@@ -52,11 +52,11 @@ void adamw(at::Tensor& p, const at::Tensor& g, at::Tensor& m, at::Tensor& v, dou
 void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vector<at::Tensor> m,
                  std::vector<at::Tensor> v, std::vector<at::Tensor> ms, std::vector<at::Tensor> vs, double lr,
                  double b1, double b2, double eps, double wd, int64_t step, double gscale, int64_t seed);
-void fp8_quantize(const at::Tensor& x, const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& s,
-                  const c10::optional<at::Tensor>& qt, const c10::optional<at::Tensor>& st, bool tile_scale);
-void fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
-              const c10::optional<at::Tensor>& bias, at::Tensor& out, int64_t act,
-              const c10::optional<at::Tensor>& aux);
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols);
+std::vector<at::Tensor> fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
+                                 const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux);
+std::vector<at::Tensor> fp8_linear(const at::Tensor& x, const at::Tensor& b, const at::Tensor& sb,
+                                   const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux);
 void sde_step(const at::Tensor& x, const at::Tensor& v, const c10::optional<at::Tensor>& xi,
               const c10::optional<at::Tensor>& prev_in, at::Tensor& prev_out, const c10::optional<at::Tensor>& mean_out,
               at::Tensor& logp, double sigma, double dt, double smin, double smax);
@@ -160,6 +160,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_multi", &osp::adamw_multi);
   m.def("fp8_quantize", &osp::fp8_quantize);
   m.def("fp8_gemm", &osp::fp8_gemm);
+  m.def("fp8_linear", &osp::fp8_linear);
   m.def("sde_step", &osp::sde_step);
   m.def("wait_probe", &osp::wait_probe);
   m.def("gemm_p2p", &osp::gemm_p2p);

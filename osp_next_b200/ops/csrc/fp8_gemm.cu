@@ -13,11 +13,13 @@
 //   warp 1      one thread issues tcgen05.cp (scale chunk -> TMEM, once per four blocks) and
 //               tcgen05.mma 128 x BN x 32, into one of two accumulators
 //   warps 2..9  epilogue: two groups of four warps, half of the tile's columns each
+// A product of few rows runs in another form (skinny_kernel).
 // TMEM (512 columns): two accumulators of 256 columns and 16 columns of scales do not fit, so
 // at BN = 256 the accumulators overlap by 16 columns: accumulator 0 is 0..255, accumulator 1
 // 240..495, scales 496..511.  The epilogue reads the shared columns first and tells the MMA
 // warp so; the next tile then starts while the rest is still being read.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContextLight.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAException.h>
@@ -28,6 +30,9 @@
 #include "tma_host.h"
 
 namespace osp {
+
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols);
+
 namespace fp8 {
 
 constexpr int kBM = 128;
@@ -67,6 +72,9 @@ __device__ __forceinline__ void bulk_load(uint64_t* bar, void* dst, const void* 
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// A product launched right behind the quantiser of its left operand starts while that still runs
+// (programmatic dependent launch) and waits here before it reads the codes.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // One 512-byte scale chunk -> 4 TMEM columns, repeated in each quarter of the lanes.
 __device__ __forceinline__ void cp_scales(uint32_t tmem, uint32_t saddr) {
   // no swizzle; 8-row core matrices of 16-byte rows, 128 bytes apart
@@ -237,6 +245,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
       const int last_chunk = (args.N + 127) / 128 - 1;
+      grid_dependency_wait();
       int stage = 0;
       uint32_t phase = 0;
       for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
@@ -262,14 +271,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      // after an abort nobody has waited for the last loads: let them land before the block ends
-      if (*abort_flag) {
-        for (int s = 0; s < STAGES; ++s) {
-          // stages before `stage` were filled in this round, the others in the one before it
-          const uint32_t p = s < stage ? phase : phase ^ 1;
-          mbar_wait(&full[s], p, args.err, kErrFp8Teardown);
-        }
-      }
+      // the last loads have landed before the block ends, whoever gave up waiting for them: stages
+      // before `stage` were filled in this round, the others in the one before (or never)
+      for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], s < stage ? phase : phase ^ 1, args.err, kErrFp8Teardown);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
@@ -381,6 +385,195 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   }
 }
 
+// ---------------------------------------------------------------------------- few rows
+// Up to 128 rows of A: the time is that of reading B, the weight.  The roles are exchanged, D^T =
+// B A^T, so that 128 rows of the weight fill the tensor core's M and the BNX (16 to 128) rows of A
+// its N.  CTAs of 100 KB share an SM in pairs; where the tiles are too few to fill the GPU a cluster
+// of up to 8 CTAs splits K and adds its parts through distributed shared memory, in rank order
+// (the result does not depend on timing, and no workspace is needed).  The weight's first
+// stages are loaded before the wait for the quantiser of A.
+// 192 threads: warp 0 TMA producer, warp 1 MMA issuer, warps 2..5 epilogue.
+template <int BNX> struct Skinny {
+  static constexpr uint32_t kW = 128 * kBK, kX = BNX * kBK, kScales = 2 * kChunkBytes;
+  static constexpr int kStages = 101 * 1024 / (kW + kX + kScales);
+  static constexpr uint32_t kTmemCols = BNX + 8 <= 32 ? 32 : BNX + 8 <= 64 ? 64 : BNX + 8 <= 128 ? 128 : 256;
+  static constexpr int smem_bytes() { return 1024 + kStages * (int)(kW + kX + kScales) + (2 * kStages + 1) * 8 + 16; }
+  static_assert(kStages * (int)(kW + kX) >= BNX * 128 * 4, "the parts of a split fit the ring");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float at `p` in this CTA's shared memory, read from CTA `rank` of the cluster.
+__device__ __forceinline__ float load_from_cta(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+template <int BNX, typename OutT>
+__global__ void __launch_bounds__(192, 2)
+skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Args args,
+              int splits) {
+  using S = Skinny<BNX>;
+  constexpr int STAGES = S::kStages;
+  constexpr uint32_t IDESC = idesc_mxf8(128, BNX);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sW = smem;
+  uint8_t* sX = sW + STAGES * S::kW;
+  uint8_t* sS = sX + STAGES * S::kX;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sS + STAGES * S::kScales);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  float* part = reinterpret_cast<float*>(smem);          // [M][128], over the ring when it is done with
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int split = splits > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / splits;
+  const int kgroups = (args.KB + 3) >> 2;
+  const int kb0 = 4 * (int)((long)kgroups * split / splits);
+  const int kb1 = min(args.KB, 4 * (int)((long)kgroups * (split + 1) / splits));
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(tfull, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load_w = [&](int kb, int stage) {
+        const bool first = (kb & 3) == 0;
+        mbar_expect_tx(&full[stage], S::kW + S::kX + (first ? S::kScales : 0));
+        tma_load_2d(&tmW, &full[stage], sW + stage * S::kW, kb * kBK, tile * 128);
+        if (first)
+          bulk_load(&full[stage], sS + stage * S::kScales, args.sb + ((long)tile * kgroups + (kb >> 2)) * kChunkBytes,
+                    kChunkBytes);
+      };
+      auto load_x = [&](int kb, int stage) {
+        tma_load_2d(&tmX, &full[stage], sX + stage * S::kX, kb * kBK, 0);
+        if ((kb & 3) == 0)
+          bulk_load(&full[stage], sS + stage * S::kScales + kChunkBytes, args.sa + (long)(kb >> 2) * kChunkBytes,
+                    kChunkBytes);
+      };
+      const int ahead = min(STAGES, kb1 - kb0);
+      for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+      grid_dependency_wait();
+      for (int i = 0; i < ahead; ++i) load_x(kb0 + i, i);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase, args.err, kErrFp8Producer)) break;
+        load_w(kb, stage);
+        load_x(kb, stage);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      // the last loads have landed before the ring is reused and the block ends
+      for (int s = 0; s < ahead; ++s) mbar_wait(&full[s], s < stage ? phase ^ 1 : phase, args.err, kErrFp8Teardown);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t t_sa = tmem_base + BNX, t_sb = t_sa + 4;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, args.err, kErrFp8Mma)) break;
+        tc_fence_after();
+        if ((kb & 3) == 0) {
+          const uint32_t s_addr = smem_u32(sS + stage * S::kScales);
+          cp_scales(t_sa, s_addr);
+          cp_scales(t_sb, s_addr + kChunkBytes);
+        }
+        const uint32_t w_addr = smem_u32(sW + stage * S::kW), x_addr = smem_u32(sX + stage * S::kX);
+        const uint32_t idesc = IDESC | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+#pragma unroll
+        for (int k = 0; k < kBK / 32; ++k)
+          umma_mxf8(tmem_base, sdesc_sw128(w_addr + k * 32, 16, 1024), sdesc_sw128(x_addr + k * 32, 16, 1024), idesc,
+                    t_sa, t_sb, (kb > kb0 || k > 0) ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      umma_commit(tfull);
+    }
+    __syncwarp();
+  }
+
+  const int quarter = warp & 3;
+  const int local = quarter * 32 + lane;                 // row of the weight tile
+  const int n = tile * 128 + local;
+  const float bias = (warp >= 2 && args.bias && n < args.N) ? __ldg(args.bias + n) : 0.f;
+  auto put = [&](int m, float v) {
+    v += bias;
+    const long o = (long)m * args.N + n;
+    if (args.aux) args.aux[o] = __float2bfloat16(v);
+    store_scalar(reinterpret_cast<OutT*>(args.out) + o, args.act ? gelu_tanh_f(v) : v);
+  };
+  if (warp >= 2) {
+    __syncwarp();
+    mbar_wait(tfull, 0, args.err, kErrFp8Epilogue);
+    __syncwarp();
+    tc_fence_after();
+    const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+    for (int m0 = 0; m0 < args.M; m0 += 16) {
+      uint32_t r[16];
+      tmem_ld16(t_row + m0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (m0 + j >= args.M) break;
+        if (splits > 1) part[(m0 + j) * 128 + local] = __uint_as_float(r[j]);
+        else if (n < args.N) put(m0 + j, __uint_as_float(r[j]));
+      }
+    }
+  }
+  if (splits > 1) {
+    cluster_sync();
+    if (warp >= 2 && n < args.N) {
+      for (int m = split; m < args.M; m += splits) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += load_from_cta(part + m * 128 + local, s);
+        put(m, v);
+      }
+    }
+    cluster_sync();                                      // no CTA leaves while its part may be read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
+
 // 2-D map over e4m3 codes [rows, Kp]: boxes of 128 bytes x box_rows, 128B swizzle, zeros outside.
 static CUtensorMap make_tmap(const at::Tensor& t, uint32_t box_rows) {
   CUtensorMap m;
@@ -394,16 +587,66 @@ static CUtensorMap make_tmap(const at::Tensor& t, uint32_t box_rows) {
   return m;
 }
 
+// `behind`: the stream's last kernel is the quantiser of `a` (see grid_dependency_wait).
+template <typename... P, typename... A>
+static void launch_kernel(void (*kern)(P...), int grid, int threads, int smem, int cluster, bool behind,
+                          cudaStream_t stream, A&&... a) {
+  smem_opt_in(reinterpret_cast<const void*>(kern), smem);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (behind) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(a)...));
+}
+
 template <int BN, typename OutT>
-static void launch(const at::Tensor& a, const at::Tensor& b, const Args& args, cudaStream_t stream) {
-  const CUtensorMap tmA = make_tmap(a, kBM), tmB = make_tmap(b, BN);
-  auto kern = gemm_kernel<BN, OutT>;
+static void launch(const at::Tensor& a, const at::Tensor& b, const Args& args, bool behind, cudaStream_t stream) {
   constexpr int smem = Shape<BN>::smem_bytes();
   static_assert(smem <= 232448, "shared memory");
-  smem_opt_in(reinterpret_cast<const void*>(kern), smem);
   const int tiles = ((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
-  kern<<<std::min(tiles, num_sms(a.get_device())), kThreads, smem, stream>>>(tmA, tmB, args);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_kernel(gemm_kernel<BN, OutT>, std::min(tiles, num_sms(a.get_device())), kThreads, smem, 1, behind, stream,
+                make_tmap(a, kBM), make_tmap(b, BN), args);
+}
+
+template <int BNX, typename OutT>
+static void launch_skinny(const at::Tensor& a, const at::Tensor& b, const Args& args, bool behind,
+                          cudaStream_t stream) {
+  // as many parts of K as fill two CTAs per SM, at most 8 (a portable cluster), whole scale
+  // chunks each; then no more parts than the longest of them needs
+  const int tiles = (args.N + 127) / 128, kgroups = (args.KB + 3) / 4;
+  const int most = std::max(1, std::min({8, kgroups, 2 * num_sms(a.get_device()) / tiles}));
+  const int longest = (kgroups + most - 1) / most;
+  const int splits = (kgroups + longest - 1) / longest;
+  launch_kernel(skinny_kernel<BNX, OutT>, tiles * splits, 192, Skinny<BNX>::smem_bytes(), splits, behind, stream,
+                make_tmap(a, BNX), make_tmap(b, 128), args, splits);
+}
+
+template <typename OutT>
+static void product(const at::Tensor& a, const at::Tensor& b, const Args& args, bool behind, cudaStream_t stream) {
+  if (args.M <= 16) return launch_skinny<16, OutT>(a, b, args, behind, stream);
+  if (args.M <= 32) return launch_skinny<32, OutT>(a, b, args, behind, stream);
+  if (args.M <= 64) return launch_skinny<64, OutT>(a, b, args, behind, stream);
+  if (args.M <= 128) return launch_skinny<128, OutT>(a, b, args, behind, stream);
+  // an MMA of 128 columns takes nearly the time of one of 256 (145 and 158 cycles in the loop):
+  // narrow tiles only where one round of them covers the result
+  const long tiles128 = (long)((args.M + 127) / 128) * ((args.N + 127) / 128);
+  if (args.N <= 64) launch<64, OutT>(a, b, args, behind, stream);
+  else if (args.N <= 128 || tiles128 <= num_sms(a.get_device())) launch<128, OutT>(a, b, args, behind, stream);
+  else launch<256, OutT>(a, b, args, behind, stream);
 }
 
 }  // namespace fp8
@@ -419,58 +662,62 @@ static void check_operand(const char* name, const at::Tensor& t, const at::Tenso
               reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0, "fp8_matmul: packed scales of ", name);
 }
 
-// out[M, N] = act(A B^T + bias); a [M, Kp], b [N, Kp] e4m3 with packed scales sa, sb
-void fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
-              const c10::optional<at::Tensor>& bias, at::Tensor& out, int64_t act,
-              const c10::optional<at::Tensor>& aux) {
+// {act(A B^T + bias) [M, N], its pre-activation in bf16 if asked for}; a [M, Kp], b [N, Kp] e4m3 with
+// packed scales sa, sb
+static std::vector<at::Tensor> multiply(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b,
+                                        const at::Tensor& sb, const c10::optional<at::Tensor>& bias_, int64_t act,
+                                        bool f32, bool aux, bool behind) {
   TORCH_CHECK(a.is_cuda() && a.dim() == 2, "fp8_matmul: a on the GPU");
   const int dev = a.get_device();
   const int64_t kp = a.size(1);
   check_operand("a", a, sa, kp, dev);
   check_operand("b", b, sb, kp, dev);
   TORCH_CHECK(a.size(0) < (int64_t(1) << 31) - 256 && b.size(0) < (int64_t(1) << 31) - 256, "fp8_matmul: sizes below 2^31");
+  TORCH_CHECK(act == 0 || act == 1, "fp8_matmul: act");
+  c10::cuda::CUDAGuard guard(a.device());
   fp8::Args args{};
   args.M = (int)a.size(0);
   args.N = (int)b.size(0);
   args.KB = (int)(kp / 128);
   args.sa = sa.data_ptr<uint8_t>();
   args.sb = sb.data_ptr<uint8_t>();
-  if (bias.has_value()) {
-    TORCH_CHECK(bias->is_cuda() && bias->get_device() == dev && bias->scalar_type() == at::kFloat &&
-                bias->is_contiguous() && bias->numel() == args.N, "fp8_matmul: bias f32 [N]");
-    args.bias = bias->data_ptr<float>();
+  at::Tensor bias;
+  if (bias_.has_value()) {
+    TORCH_CHECK(bias_->is_cuda() && bias_->get_device() == dev && bias_->dim() == 1 && bias_->numel() == args.N,
+                "fp8_matmul: bias [N] on the device of a");
+    bias = bias_->to(at::kFloat).contiguous();
+    args.bias = bias.data_ptr<float>();
   }
-  TORCH_CHECK(out.is_cuda() && out.get_device() == dev && out.is_contiguous() && out.dim() == 2 &&
-              out.size(0) == args.M && out.size(1) == args.N, "fp8_matmul: contiguous out [M, N]");
-  const bool f32 = out.scalar_type() == at::kFloat;
-  TORCH_CHECK(f32 || out.scalar_type() == at::kBFloat16, "fp8_matmul: out bf16 or f32");
-  TORCH_CHECK(act == 0 || act == 1, "fp8_matmul: act");
+  std::vector<at::Tensor> out;
+  out.push_back(at::empty({args.M, args.N}, a.options().dtype(f32 ? at::kFloat : at::kBFloat16)));
   args.act = (int)act;
-  args.out = out.data_ptr();
-  args.vec = args.N % 8 == 0 && reinterpret_cast<uintptr_t>(args.out) % 16 == 0;
-  if (aux.has_value()) {
-    TORCH_CHECK(aux->is_cuda() && aux->get_device() == dev && aux->scalar_type() == at::kBFloat16 &&
-                aux->is_contiguous() && aux->sizes() == out.sizes(), "fp8_matmul: aux bf16 [M, N]");
-    args.aux = reinterpret_cast<__nv_bfloat16*>(aux->data_ptr());
-    args.vec = args.vec && reinterpret_cast<uintptr_t>(args.aux) % 16 == 0;
+  args.out = out[0].data_ptr();
+  args.vec = args.N % 8 == 0;
+  if (aux) {
+    out.push_back(at::empty({args.M, args.N}, a.options().dtype(at::kBFloat16)));
+    args.aux = reinterpret_cast<__nv_bfloat16*>(out[1].data_ptr());
   }
   args.err = error_word(dev);
-  if (args.M == 0 || args.N == 0) return;
+  if (args.M == 0 || args.N == 0) return out;
   TORCH_CHECK(args.KB > 0, "fp8_matmul: K of at least 1");
-  c10::cuda::CUDAGuard guard(a.device());
   auto stream = c10::cuda::getCurrentCUDAStream();
-  const long sms = num_sms(dev);
-  const long tiles256 = (long)((args.M + 127) / 128) * ((args.N + 255) / 256);
-  const int bn = args.N <= 64 ? 64 : (args.N <= 128 || tiles256 < sms) ? 128 : 256;
-  if (f32) {
-    if (bn == 256) fp8::launch<256, float>(a, b, args, stream);
-    else if (bn == 128) fp8::launch<128, float>(a, b, args, stream);
-    else fp8::launch<64, float>(a, b, args, stream);
-  } else {
-    if (bn == 256) fp8::launch<256, __nv_bfloat16>(a, b, args, stream);
-    else if (bn == 128) fp8::launch<128, __nv_bfloat16>(a, b, args, stream);
-    else fp8::launch<64, __nv_bfloat16>(a, b, args, stream);
-  }
+  if (f32) fp8::product<float>(a, b, args, behind, stream);
+  else fp8::product<__nv_bfloat16>(a, b, args, behind, stream);
+  return out;
+}
+
+std::vector<at::Tensor> fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
+                                 const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux) {
+  return multiply(a, sa, b, sb, bias, act, f32, aux, false);
+}
+
+// The same of x [..., K] in bf16, fp16 or fp32, quantised here.
+std::vector<at::Tensor> fp8_linear(const at::Tensor& x, const at::Tensor& b, const at::Tensor& sb,
+                                   const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux) {
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, "fp8_matmul: a [..., K] on the GPU");
+  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  const auto q = fp8_quantize(x2, false, true, false);
+  return multiply(q[0], q[1], b, sb, bias, act, f32, aux, x2.numel() > 0);
 }
 
 }  // namespace osp

@@ -7,6 +7,7 @@
 //
 // Both are bound by memory: 2 or 4 bytes read and 1 (+ 1/128) written per element and side.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContextLight.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAException.h>
@@ -133,6 +134,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
                                                             uint8_t* __restrict__ scale, int R, int K, int Kp,
                                                             int kgroups, long total) {
+  // a product behind this kernel may start its own preparations (it waits before it reads q)
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31;
   const long w0 = ((long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2;
   if (w0 >= total) return;
@@ -353,13 +356,10 @@ quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
 
 }  // namespace fp8
 
-static void check_side(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s, int64_t rows, int64_t cols) {
-  const int64_t cp = (cols + 127) / 128 * 128;
-  TORCH_CHECK(q.is_cuda() && q.get_device() == x.get_device() && q.scalar_type() == at::kFloat8_e4m3fn &&
-              q.is_contiguous() && q.dim() == 2 && q.size(0) == rows && q.size(1) == cp,
-              "fp8_quantize: codes e4m3 [", std::to_string(rows), ", ", std::to_string(cp), "]");
-  TORCH_CHECK(s.is_cuda() && s.get_device() == x.get_device() && s.scalar_type() == at::kByte && s.is_contiguous() &&
-              s.numel() == (rows + 127) / 128 * ((cols + 511) / 512) * 512, "fp8_quantize: packed scales");
+// Codes and packed scales of a [rows, cols] matrix on x's device.
+static void alloc_side(const at::Tensor& x, int64_t rows, int64_t cols, at::Tensor& q, at::Tensor& s) {
+  q = at::empty({rows, (cols + 127) / 128 * 128}, x.options().dtype(at::kFloat8_e4m3fn));
+  s = at::empty({(rows + 127) / 128, (cols + 511) / 512, 32, 4, 4}, x.options().dtype(at::kByte));
 }
 
 template <typename T>
@@ -401,28 +401,37 @@ static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// x [R, K] (rows contiguous, any row stride) -> q [R, Kp], s and / or those of x^T, qt [K, Rp], st
-void fp8_quantize(const at::Tensor& x, const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& s,
-                  const c10::optional<at::Tensor>& qt, const c10::optional<at::Tensor>& st, bool tile_scale) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1), "fp8_quantize: x [R, K] on the GPU, rows contiguous");
+// Codes and scales of x [R, K] (`rows`) and / or of its transpose (`cols`); any strides.  Sides
+// that were not asked for come back undefined.
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x_, bool tile_scale, bool rows, bool cols) {
+  TORCH_CHECK(x_.is_cuda() && x_.dim() == 2, "fp8_quantize: x [R, K] on the GPU");
+  at::Tensor x = x_;
   const int64_t R = x.size(0), K = x.size(1);
   TORCH_CHECK(R < (int64_t(1) << 31) - 128 && K < (int64_t(1) << 31) - 512, "fp8_quantize: sizes below 2^31");
-  TORCH_CHECK(q.has_value() == s.has_value() && qt.has_value() == st.has_value() && (q.has_value() || qt.has_value()),
-              "fp8_quantize: codes and scales of at least one side");
-  if (q.has_value()) check_side(x, *q, *s, R, K);
-  if (qt.has_value()) check_side(x, *qt, *st, K, R);
-  if (R == 0 || K == 0) return;
   c10::cuda::CUDAGuard guard(x.device());
+  std::vector<at::Tensor> out(4);
+  if (rows) alloc_side(x, R, K, out[0], out[1]);
+  if (cols) alloc_side(x, K, R, out[2], out[3]);
+  if (R == 0 || K == 0) return out;
+  bool swap = false;
+  if (K > 1 && x.stride(1) != 1) {
+    if (R > 1 && x.stride(0) != 1) {
+      x = x.contiguous();
+    } else {                        // a transposed view: its rows are the columns of what is stored
+      x = x.t();
+      swap = true;
+    }
+  }
+  auto ptr = [&](int i) { return out[i].defined() ? reinterpret_cast<uint8_t*>(out[i].data_ptr()) : nullptr; };
+  uint8_t *q = ptr(swap ? 2 : 0), *s = ptr(swap ? 3 : 1), *qt = ptr(swap ? 0 : 2), *st = ptr(swap ? 1 : 3);
   auto stream = c10::cuda::getCurrentCUDAStream();
-  auto ptr = [](const c10::optional<at::Tensor>& t) {
-    return t.has_value() ? reinterpret_cast<uint8_t*>(t->data_ptr()) : nullptr;
-  };
   switch (x.scalar_type()) {
-    case at::kBFloat16: quantize_t<__nv_bfloat16>(x, ptr(q), ptr(s), ptr(qt), ptr(st), tile_scale, stream); break;
-    case at::kHalf: quantize_t<__half>(x, ptr(q), ptr(s), ptr(qt), ptr(st), tile_scale, stream); break;
-    case at::kFloat: quantize_t<float>(x, ptr(q), ptr(s), ptr(qt), ptr(st), tile_scale, stream); break;
+    case at::kBFloat16: quantize_t<__nv_bfloat16>(x, q, s, qt, st, tile_scale, stream); break;
+    case at::kHalf: quantize_t<__half>(x, q, s, qt, st, tile_scale, stream); break;
+    case at::kFloat: quantize_t<float>(x, q, s, qt, st, tile_scale, stream); break;
     default: TORCH_CHECK(false, "fp8_quantize: x bf16, fp16 or fp32");
   }
+  return out;
 }
 
 }  // namespace osp

@@ -50,12 +50,6 @@ class Fp8Tensor:
         return f"Fp8Tensor([{self.rows}, {self.cols}], block {self.block_rows}x{BLOCK}, {self.data.device})"
 
 
-def _empty(rows: int, cols: int, device):
-    kp = -(-cols // BLOCK) * BLOCK
-    return (torch.empty(rows, kp, dtype=torch.float8_e4m3fn, device=device),
-            torch.empty(-(-rows // 128), -(-cols // 512), 32, 4, 4, dtype=torch.uint8, device=device))
-
-
 def fp8_quantize(x: torch.Tensor, block_rows: int = 1, layout: str = "rows"):
     """Block-128 fp8 of a matrix x [R, K] (bf16, fp16 or fp32; any strides).
 
@@ -77,21 +71,10 @@ def fp8_quantize(x: torch.Tensor, block_rows: int = 1, layout: str = "rows"):
                            *((R, K) if s == "rows" else (K, R)), block_rows)
                  for s in ("rows", "cols") if layout in (s, "both")]
         return tuple(sides) if layout == "both" else sides[0]
-    x = x.detach()
-    rows = cols = None
-    if layout != "cols":
-        rows = Fp8Tensor(*_empty(R, K, x.device), R, K, block_rows)
-    if layout != "rows":
-        cols = Fp8Tensor(*_empty(K, R, x.device), K, R, block_rows)
-    a, b = rows, cols
-    if K > 1 and x.stride(1) != 1:
-        if R > 1 and x.stride(0) != 1:
-            x = x.contiguous()
-        else:                       # a transposed view: its rows are the columns of what is stored
-            x, a, b = x.t(), cols, rows
-    ext().fp8_quantize(x, None if a is None else a.data, None if a is None else a.scale,
-                       None if b is None else b.data, None if b is None else b.scale, block_rows != 1)
-    return (rows, cols) if layout == "both" else (rows if cols is None else cols)
+    q, qs, t, ts = ext().fp8_quantize(x, block_rows != 1, layout != "cols", layout != "rows")
+    rows = None if q is None else Fp8Tensor(q, qs, R, K, block_rows)
+    cols = None if t is None else Fp8Tensor(t, ts, K, R, block_rows)
+    return (rows, cols) if layout == "both" else (cols if rows is None else rows)
 
 
 def fp8_matmul(a, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
@@ -108,27 +91,28 @@ def fp8_matmul(a, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, act: Option
         raise ValueError(f"fp8_matmul: act None or 'gelu_tanh', got {act!r}")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"fp8_matmul: out_dtype bf16 or fp32, got {out_dtype}")
-    lead = None
-    if not isinstance(a, Fp8Tensor):
-        if a.dim() == 0 or a.shape[-1] != b.cols:
-            raise ValueError(f"fp8_matmul: a {tuple(a.shape)} against K = {b.cols}")
-        lead = a.shape[:-1]
-        a = fp8_quantize(a if a.dim() == 2 else a.reshape(-1, a.shape[-1]))
-    if a.cols != b.cols:
-        raise ValueError(f"fp8_matmul: K differs: {a.cols} and {b.cols}")
-    M, N = a.rows, b.rows
-    if bias is not None and tuple(bias.shape) != (N,):
-        raise ValueError(f"fp8_matmul: bias [{N}], got {tuple(bias.shape)}")
-    if not a.data.is_cuda or a.cols == 0:      # an empty sum: act(bias)
+    quantized = isinstance(a, Fp8Tensor)
+    shape = a.shape
+    if len(shape) == 0 or shape[-1] != b.cols:
+        raise ValueError(f"fp8_matmul: a {tuple(shape)} against K = {b.cols}")
+    if bias is not None and bias.shape != (b.rows,):
+        raise ValueError(f"fp8_matmul: bias [{b.rows}], got {tuple(bias.shape)}")
+    if not b.data.is_cuda or b.cols == 0:      # the reference; with K = 0 an empty sum: act(bias)
+        if not quantized:
+            a = fp8_quantize(a.reshape(a.shape[:-1].numel(), b.cols))
         out, pre = ref.fp8_matmul(a, b, bias, act, out_dtype)
     else:
-        out = torch.empty(M, N, dtype=out_dtype, device=a.data.device)
-        pre = torch.empty(M, N, dtype=torch.bfloat16, device=a.data.device) if aux else None
-        bb = None if bias is None else bias.detach().float().contiguous()
-        ext().fp8_gemm(a.data, a.scale, b.data, b.scale, bb, out, 1 if act else 0, pre)
-    if lead is not None and len(lead) != 1:
-        out = out.view(*lead, N)
-        pre = None if pre is None else pre.view(*lead, N)
+        args = (b.data, b.scale, bias, 1 if act else 0, out_dtype == torch.float32, aux)
+        if quantized:
+            out, *pre = ext().fp8_gemm(a.data, a.scale, *args)
+        elif a.dtype in _IN_TYPES:
+            out, *pre = ext().fp8_linear(a, *args)
+        else:
+            raise TypeError(f"fp8_matmul: bf16, fp16 or fp32, got {a.dtype}")
+        pre = pre[0] if aux else None
+    if len(shape) != 2:
+        out = out.view(*shape[:-1], b.rows)
+        pre = None if pre is None else pre.view(*shape[:-1], b.rows)
     return (out, pre) if aux else out
 
 
