@@ -351,14 +351,15 @@ static void launch(const Args<CAP>& a, bool state8, cudaStream_t stream) {
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+using Ptrs = std::vector<const at::Tensor*>;
 struct Lists {
-  const std::vector<at::Tensor>&p, &g, &m, &v, &ms, &vs;
+  const Ptrs &p, &g, &m, &v, &ms, &vs;
 };
 
 // Fills parameter blocks of CAP tensors and launches each.
 template <int CAP>
 static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed, cudaStream_t stream) {
-  const bool pf = l.p[0].scalar_type() == at::kFloat, gf = l.g[0].scalar_type() == at::kFloat;
+  const bool pf = l.p[0]->scalar_type() == at::kFloat, gf = l.g[0]->scalar_type() == at::kFloat;
   Args<CAP> a;
   a.c = consts;
   a.tensors = 0;
@@ -373,19 +374,19 @@ static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed
     chunks = 0;
   };
   for (size_t i = 0; i < l.p.size(); ++i) {
-    const int64_t n = l.p[i].numel();
+    const int64_t n = l.p[i]->numel();
     if (n == 0) continue;
     const int64_t mine = ((n + 127) / 128 + kChunkBlocks - 1) / kChunkBlocks;
     TORCH_CHECK(mine < (int64_t(1) << 30), "adamw_multi_: tensor ", std::to_string(i), " too large");
     if (a.tensors == CAP || chunks + mine >= (int64_t(1) << 31)) flush();
     const int t = a.tensors++;
     chunks += mine;
-    a.p[t] = l.p[i].data_ptr();
-    a.g[t] = l.g[i].data_ptr();
-    a.m[t] = l.m[i].data_ptr();
-    a.v[t] = l.v[i].data_ptr();
-    a.ms[t] = state8 ? l.ms[i].data_ptr<uint8_t>() : nullptr;
-    a.vs[t] = state8 ? l.vs[i].data_ptr<uint8_t>() : nullptr;
+    a.p[t] = l.p[i]->data_ptr();
+    a.g[t] = l.g[i]->data_ptr();
+    a.m[t] = l.m[i]->data_ptr();
+    a.v[t] = l.v[i]->data_ptr();
+    a.ms[t] = state8 ? l.ms[i]->data_ptr<uint8_t>() : nullptr;
+    a.vs[t] = state8 ? l.vs[i]->data_ptr<uint8_t>() : nullptr;
     a.n[t] = n;
     a.chunk_end[t] = (int)chunks;
     a.key[t] = mix((uint32_t)i * kMix3 + seed);
@@ -396,8 +397,9 @@ static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed
 }  // namespace adamw8
 
 // In place on every tensor of the lists; ms / vs empty: fp32 moments.
-void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vector<at::Tensor> m,
-                 std::vector<at::Tensor> v, std::vector<at::Tensor> ms, std::vector<at::Tensor> vs, double lr,
+void adamw_multi(const std::vector<const at::Tensor*>& p, const std::vector<const at::Tensor*>& g,
+                 const std::vector<const at::Tensor*>& m, const std::vector<const at::Tensor*>& v,
+                 const std::vector<const at::Tensor*>& ms, const std::vector<const at::Tensor*>& vs, double lr,
                  double b1, double b2, double eps, double wd, int64_t step, double gscale, int64_t seed) {
   using namespace adamw8;
   const size_t count = p.size();
@@ -406,17 +408,17 @@ void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vect
               (!state8 || (ms.size() == count && vs.size() == count)), "adamw_multi_: lists of one length");
   if (count == 0) return;
   TORCH_CHECK(step >= 1, "adamw_multi_: step counts from 1");
-  const auto pt = p[0].scalar_type(), gt = g[0].scalar_type();
+  const auto pt = p[0]->scalar_type(), gt = g[0]->scalar_type();
   TORCH_CHECK(pt == at::kFloat || pt == at::kBFloat16, "adamw_multi_: parameters fp32 or bf16");
   TORCH_CHECK(gt == at::kFloat || gt == at::kBFloat16, "adamw_multi_: gradients fp32 or bf16");
-  TORCH_CHECK(p[0].is_cuda(), "adamw_multi_: CUDA tensors");
-  const int dev = p[0].get_device();
+  TORCH_CHECK(p[0]->is_cuda(), "adamw_multi_: CUDA tensors");
+  const c10::Device dev = p[0]->device();
   const auto mt = state8 ? at::kFloat8_e4m3fn : at::kFloat, vt = state8 ? at::kByte : at::kFloat;
-  auto good = [&](const at::Tensor& t, at::ScalarType dt, int64_t n) {
-    return t.is_cuda() && t.get_device() == dev && t.scalar_type() == dt && t.is_contiguous() && t.numel() == n;
+  auto good = [&](const at::Tensor* t, at::ScalarType dt, int64_t n) {
+    return t->device() == dev && t->scalar_type() == dt && t->numel() == n && t->is_contiguous();
   };
   for (size_t i = 0; i < count; ++i) {
-    const int64_t n = p[i].numel();
+    const int64_t n = p[i]->numel();
     TORCH_CHECK(good(p[i], pt, n) && good(g[i], gt, n) && good(m[i], mt, n) && good(v[i], vt, n),
                 "adamw_multi_: tensor ", std::to_string(i), ": p, g and moments contiguous, of one size and device, p and g of one "
                 "type throughout, moments ", state8 ? "e4m3 and uint8" : "fp32");
@@ -424,7 +426,7 @@ void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vect
       TORCH_CHECK(good(ms[i], at::kByte, (n + 127) / 128) && good(vs[i], at::kByte, (n + 127) / 128),
                   "adamw_multi_: tensor ", std::to_string(i), ": one uint8 scale per 128 elements and moment");
   }
-  c10::cuda::CUDAGuard guard(p[0].device());
+  c10::cuda::CUDAGuard guard(dev);
   auto stream = c10::cuda::getCurrentCUDAStream();
   Consts c;
   c.b1 = (float)b1;

@@ -49,8 +49,9 @@ void hif8_round(const at::Tensor& x, at::Tensor& out, double s);
 void hif8_qdq(const at::Tensor& x, at::Tensor& out, double scale_max);
 void adamw(at::Tensor& p, const at::Tensor& g, at::Tensor& m, at::Tensor& v, double lr, double b1, double b2,
            double eps, double wd, int64_t step, double gscale);
-void adamw_multi(std::vector<at::Tensor> p, std::vector<at::Tensor> g, std::vector<at::Tensor> m,
-                 std::vector<at::Tensor> v, std::vector<at::Tensor> ms, std::vector<at::Tensor> vs, double lr,
+void adamw_multi(const std::vector<const at::Tensor*>& p, const std::vector<const at::Tensor*>& g,
+                 const std::vector<const at::Tensor*>& m, const std::vector<const at::Tensor*>& v,
+                 const std::vector<const at::Tensor*>& ms, const std::vector<const at::Tensor*>& vs, double lr,
                  double b1, double b2, double eps, double wd, int64_t step, double gscale, int64_t seed);
 std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols);
 std::vector<at::Tensor> fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
@@ -157,7 +158,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("hif8_round", &osp::hif8_round);
   m.def("hif8_qdq", &osp::hif8_qdq);
   m.def("adamw", &osp::adamw);
-  m.def("adamw_multi", &osp::adamw_multi);
+  // hundreds of tensors per list: borrowed from the Python lists (which the caller holds) instead
+  // of copied with a reference count each
+  m.def("adamw_multi", [](pybind11::list p, pybind11::list g, pybind11::list mo, pybind11::list v, pybind11::list ms,
+                          pybind11::list vs, double lr, double b1, double b2, double eps, double wd, int64_t step,
+                          double gscale, int64_t seed) {
+    auto borrow = [](const pybind11::list& l) {
+      std::vector<const at::Tensor*> out(l.size());
+      for (size_t i = 0; i < out.size(); ++i) {
+        PyObject* o = PyList_GET_ITEM(l.ptr(), (Py_ssize_t)i);
+        TORCH_CHECK(THPVariable_Check(o), "adamw_multi_: lists of tensors");
+        out[i] = &THPVariable_Unpack(o);
+      }
+      return out;
+    };
+    osp::adamw_multi(borrow(p), borrow(g), borrow(mo), borrow(v), borrow(ms), borrow(vs), lr, b1, b2, eps, wd, step,
+                     gscale, seed);
+  });
   m.def("fp8_quantize", &osp::fp8_quantize);
   m.def("fp8_gemm", &osp::fp8_gemm);
   m.def("fp8_linear", &osp::fp8_linear);

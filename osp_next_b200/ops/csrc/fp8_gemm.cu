@@ -356,24 +356,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       tc_fence_after();
       const long row0 = (long)mb * kBM + quarter * 32;
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * S::kAccStride;
-#pragma unroll 1
+      // chunk i's column in the tile: accumulator 0 shares its last columns, accumulator 1 its
+      // first, and those go first
+      auto chunk = [&](int i) { return eg * PER + ((S::kOverlap && acc == 0) ? PER - 1 - i : i); };
+      uint32_t r[2][32];
+      tmem_ld32(t_row + chunk(0) * 32, r[0]);
+#pragma unroll
       for (int i = 0; i < PER; ++i) {
-        // accumulator 0 shares its last columns, accumulator 1 its first: those go first
-        const int c = eg * PER + ((S::kOverlap && acc == 0) ? PER - 1 - i : i);
-        const int col0 = nb * BN + c * 32;
-        uint32_t r[32];
-        tmem_ld32(t_row + c * 32, r);
         tmem_ld_wait();
         if (S::kOverlap && i == 0 && eg == (acc ^ 1)) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&tearly[acc]);
         }
-        if (col0 < args.N) finish_chunk<OutT>(args, r, sbias + (c - eg * PER) * 32, stg, lane, row0, col0);
+        if (i + 1 < PER) {                                // on its way while this one is stored
+          tmem_ld32(t_row + chunk(i + 1) * 32, r[(i + 1) & 1]);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tempty[acc]);
+        }
+        const int c = chunk(i), col0 = nb * BN + c * 32;
+        if (col0 < args.N) finish_chunk<OutT>(args, r[i & 1], sbias + (c - eg * PER) * 32, stg, lane, row0, col0);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[acc]);
     }
   }
 
@@ -386,9 +391,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 }
 
 // ---------------------------------------------------------------------------- few rows
-// Up to 128 rows of A: the time is that of reading B, the weight.  The roles are exchanged, D^T =
-// B A^T, so that 128 rows of the weight fill the tensor core's M and the BNX (16 to 128) rows of A
-// its N.  CTAs of 100 KB share an SM in pairs; where the tiles are too few to fill the GPU a cluster
+// Up to 64 rows of A: the time is that of reading B, the weight.  The roles are exchanged, D^T =
+// B A^T, so that 128 rows of the weight fill the tensor core's M and the BNX (16 to 64) rows of A its
+// N.  CTAs of 100 KB share an SM in pairs; where the tiles are too few to fill the GPU a cluster
 // of up to 8 CTAs splits K and adds its parts through distributed shared memory, in rank order
 // (the result does not depend on timing, and no workspace is needed).  The weight's first
 // stages are loaded before the wait for the quantiser of A.
@@ -396,7 +401,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 template <int BNX> struct Skinny {
   static constexpr uint32_t kW = 128 * kBK, kX = BNX * kBK, kScales = 2 * kChunkBytes;
   static constexpr int kStages = 101 * 1024 / (kW + kX + kScales);
-  static constexpr uint32_t kTmemCols = BNX + 8 <= 32 ? 32 : BNX + 8 <= 64 ? 64 : BNX + 8 <= 128 ? 128 : 256;
+  static constexpr uint32_t kTmemCols = BNX + 8 <= 32 ? 32 : BNX + 8 <= 64 ? 64 : 128;
   static constexpr int smem_bytes() { return 1024 + kStages * (int)(kW + kX + kScales) + (2 * kStages + 1) * 8 + 16; }
   static_assert(kStages * (int)(kW + kX) >= BNX * 128 * 4, "the parts of a split fit the ring");
 };
@@ -640,7 +645,6 @@ static void product(const at::Tensor& a, const at::Tensor& b, const Args& args, 
   if (args.M <= 16) return launch_skinny<16, OutT>(a, b, args, behind, stream);
   if (args.M <= 32) return launch_skinny<32, OutT>(a, b, args, behind, stream);
   if (args.M <= 64) return launch_skinny<64, OutT>(a, b, args, behind, stream);
-  if (args.M <= 128) return launch_skinny<128, OutT>(a, b, args, behind, stream);
   // an MMA of 128 columns takes nearly the time of one of 256 (145 and 158 cycles in the loop):
   // narrow tiles only where one round of them covers the result
   const long tiles128 = (long)((args.M + 127) / 128) * ((args.N + 127) / 128);

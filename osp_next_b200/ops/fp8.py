@@ -139,9 +139,9 @@ def adamw_multi_(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_
     if not params[0].is_cuda:
         return ref.adamw_multi_(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, lr, beta1,
                                 beta2, eps, weight_decay, step, grad_scale, seed)
-    ext().adamw_multi(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales if state8 else [],
-                      exp_avg_sq_scales if state8 else [], float(lr), float(beta1), float(beta2), float(eps),
-                      float(weight_decay), int(step), float(grad_scale), int(seed))
+    lists = [x if type(x) is list else list(x) for x in lists] + ([] if state8 else [[], []])
+    ext().adamw_multi(*lists, float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
+                      int(step), float(grad_scale), int(seed))
 
 
 def adamw8_state(p: torch.Tensor):
