@@ -53,7 +53,7 @@ void adamw_multi(const std::vector<const at::Tensor*>& p, const std::vector<cons
                  const std::vector<const at::Tensor*>& m, const std::vector<const at::Tensor*>& v,
                  const std::vector<const at::Tensor*>& ms, const std::vector<const at::Tensor*>& vs, double lr,
                  double b1, double b2, double eps, double wd, int64_t step, double gscale, int64_t seed);
-std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols);
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols, bool sums);
 std::vector<at::Tensor> fp8_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
                                  const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux);
 std::vector<at::Tensor> fp8_linear(const at::Tensor& x, const at::Tensor& b, const at::Tensor& sb,

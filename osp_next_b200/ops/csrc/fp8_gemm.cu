@@ -31,7 +31,7 @@
 
 namespace osp {
 
-std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols);
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool tile_scale, bool rows, bool cols, bool sums);
 
 namespace fp8 {
 
@@ -403,7 +403,8 @@ template <int BNX> struct Skinny {
   static constexpr int kStages = 101 * 1024 / (kW + kX + kScales);
   static constexpr uint32_t kTmemCols = BNX + 8 <= 32 ? 32 : BNX + 8 <= 64 ? 64 : 128;
   static constexpr int smem_bytes() { return 1024 + kStages * (int)(kW + kX + kScales) + (2 * kStages + 1) * 8 + 16; }
-  static_assert(kStages * (int)(kW + kX) >= BNX * 128 * 4, "the parts of a split fit the ring");
+  static constexpr int kPartRow = BNX + 4;               // floats of a weight row's part, padded
+  static_assert(kStages * (int)(kW + kX) >= kPartRow * 128 * 4, "the parts of a split fit the ring");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -414,12 +415,13 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The float at `p` in this CTA's shared memory, read from CTA `rank` of the cluster.
-__device__ __forceinline__ float load_from_cta(const float* p, uint32_t rank) {
+// Four floats at `p` in this CTA's shared memory, read from CTA `rank` of the cluster.
+__device__ __forceinline__ float4 load_from_cta(const float* p, uint32_t rank) {
   uint32_t a;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
   return v;
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
@@ -447,7 +449,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ C
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
-  float* part = reinterpret_cast<float*>(smem);          // [M][128], over the ring when it is done with
+  float* part = reinterpret_cast<float*>(smem);          // [128][kPartRow], over the ring when it is done with
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int split = splits > 1 ? (int)cluster_rank() : 0;
@@ -552,21 +554,36 @@ skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ C
       uint32_t r[16];
       tmem_ld16(t_row + m0, r);
       tmem_ld_wait();
+      if (splits > 1) {
+        float4* p = reinterpret_cast<float4*>(part + local * S::kPartRow + m0);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (m0 + j >= args.M) break;
-        if (splits > 1) part[(m0 + j) * 128 + local] = __uint_as_float(r[j]);
-        else if (n < args.N) put(m0 + j, __uint_as_float(r[j]));
+        for (int j = 0; j < 4; ++j)
+          p[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                             __uint_as_float(r[4 * j + 3]));
+      } else if (n < args.N) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (m0 + j < args.M) put(m0 + j, __uint_as_float(r[j]));
       }
     }
   }
   if (splits > 1) {
     cluster_sync();
     if (warp >= 2 && n < args.N) {
-      for (int m = split; m < args.M; m += splits) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += load_from_cta(part + m * 128 + local, s);
-        put(m, v);
+      // rows of A dealt to the CTAs four at a time; all parts of four rows in flight together
+      for (int m = 4 * split; m < args.M; m += 4 * splits) {
+        float4 t[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < splits) t[s] = load_from_cta(part + local * S::kPartRow + m, s);
+        float4 v = t[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+          if (s < splits) { v.x += t[s].x; v.y += t[s].y; v.z += t[s].z; v.w += t[s].w; }
+        put(m, v.x);
+        if (m + 1 < args.M) put(m + 1, v.y);
+        if (m + 2 < args.M) put(m + 2, v.z);
+        if (m + 3 < args.M) put(m + 3, v.w);
       }
     }
     cluster_sync();                                      // no CTA leaves while its part may be read
@@ -720,7 +737,7 @@ std::vector<at::Tensor> fp8_linear(const at::Tensor& x, const at::Tensor& b, con
                                    const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux) {
   TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, "fp8_matmul: a [..., K] on the GPU");
   const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  const auto q = fp8_quantize(x2, false, true, false);
+  const auto q = fp8_quantize(x2, false, true, false, false);
   return multiply(q[0], q[1], b, sb, bias, act, f32, aux, x2.numel() > 0);
 }
 

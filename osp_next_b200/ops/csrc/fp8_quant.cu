@@ -200,12 +200,16 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // (32 for a thread) and their maxima are taken two at a time; all 8 loads are in flight at once.
 // Maxima meet in shared memory, one thread per row and column forms its scale, and every
 // thread reads back the 16 factors that it needs.
-template <typename T, bool VEC, bool TILE_SCALE, bool ROWS, bool COLS>
+// SUMS: also the sums of x over the tile's 128 rows, part [R / 128, K] (a bias gradient's first
+// step, without another read of x).
+template <typename T, bool VEC, bool TILE_SCALE, bool ROWS, bool COLS, bool SUMS>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-                      uint8_t* __restrict__ qt, uint8_t* __restrict__ scale_t, int R, int K, int Kp, int Rp) {
+                      uint8_t* __restrict__ qt, uint8_t* __restrict__ scale_t, float* __restrict__ part, int R, int K,
+                      int Kp, int Rp) {
   __shared__ uint32_t top[2][4][128];              // [0]: rows over 2 warps, [1]: columns over 4
   __shared__ __align__(16) float factor[2][128];
+  __shared__ float sums[SUMS ? 4 : 1][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wr = warp >> 1, wc = warp & 1;
   const int rl = wr * 32 + (lane >> 3) * 8;        // first row of this thread in the tile
@@ -291,6 +295,19 @@ quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
     return seen;
   };
   const uint32_t seen = gather(std::true_type());
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i].pin();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a += v[i].get(j);
+      a += __shfl_xor_sync(0xffffffffu, a, 8);
+      a += __shfl_xor_sync(0xffffffffu, a, 16);
+      if (lane < 8) sums[wr][cl + j] = a;
+    }
+  }
   if (__syncthreads_or(seen >= kInfBits)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].spoil_inf();
@@ -320,6 +337,10 @@ quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
       *s = line < (side ? K : R) ? (uint8_t)byte : 0;
       if (blk == blocks - 1)
         for (int j = 1; j < 4 - (blk & 3); ++j) s[j] = 0;
+    }
+    if constexpr (SUMS) {
+      if (side == 1 && kb * 128 + i < K)
+        part[(long)rb * K + kb * 128 + i] = sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i];
     }
   }
   __syncthreads();
@@ -363,8 +384,8 @@ static void alloc_side(const at::Tensor& x, int64_t rows, int64_t cols, at::Tens
 }
 
 template <typename T>
-static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st, bool tile_scale,
-                       cudaStream_t stream) {
+static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st, float* part,
+                       bool tile_scale, cudaStream_t stream) {
   const int R = (int)x.size(0), K = (int)x.size(1);
   const int Kp = (K + 127) / 128 * 128, Rp = (R + 127) / 128 * 128;
   const long ld = x.stride(0);
@@ -381,13 +402,14 @@ static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
   }
   const dim3 grid(Kp / 128, Rp / 128);
   TORCH_CHECK(grid.y <= 65535, "fp8_quantize: more than 8388480 rows");
-#define OSP_TILES(VEC, TS, RO, CO) \
-  fp8::quantize_tiles_kernel<T, VEC, TS, RO, CO><<<grid, 256, 0, stream>>>(xp, ld, q, s, qt, st, R, K, Kp, Rp)
-#define OSP_TILES_SIDES(VEC, TS)                      \
-  do {                                                \
-    if (q && qt) OSP_TILES(VEC, TS, true, true);      \
-    else if (q) OSP_TILES(VEC, TS, true, false);      \
-    else OSP_TILES(VEC, TS, false, true);             \
+#define OSP_TILES(VEC, TS, RO, CO, SU) \
+  fp8::quantize_tiles_kernel<T, VEC, TS, RO, CO, SU><<<grid, 256, 0, stream>>>(xp, ld, q, s, qt, st, part, R, K, Kp, Rp)
+#define OSP_TILES_SIDES(VEC, TS)                             \
+  do {                                                       \
+    if (part) OSP_TILES(VEC, false, true, true, true);       \
+    else if (q && qt) OSP_TILES(VEC, TS, true, true, false); \
+    else if (q) OSP_TILES(VEC, TS, true, false, false);      \
+    else OSP_TILES(VEC, TS, false, true, false);             \
   } while (0)
   if (vec) {
     if (tile_scale) OSP_TILES_SIDES(true, true);
@@ -402,20 +424,23 @@ static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
 }
 
 // Codes and scales of x [R, K] (`rows`) and / or of its transpose (`cols`); any strides.  Sides
-// that were not asked for come back undefined.
-std::vector<at::Tensor> fp8_quantize(const at::Tensor& x_, bool tile_scale, bool rows, bool cols) {
+// that were not asked for come back undefined.  `sums` (both sides, blocks of one row): also the
+// column sums of x over each 128 rows, fp32 [ceil(R / 128), K].
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x_, bool tile_scale, bool rows, bool cols, bool sums) {
   TORCH_CHECK(x_.is_cuda() && x_.dim() == 2, "fp8_quantize: x [R, K] on the GPU");
   at::Tensor x = x_;
   const int64_t R = x.size(0), K = x.size(1);
   TORCH_CHECK(R < (int64_t(1) << 31) - 128 && K < (int64_t(1) << 31) - 512, "fp8_quantize: sizes below 2^31");
   c10::cuda::CUDAGuard guard(x.device());
-  std::vector<at::Tensor> out(4);
+  TORCH_CHECK(!sums || (rows && cols && !tile_scale), "fp8_quantize: column sums go with both sides");
+  std::vector<at::Tensor> out(5);
   if (rows) alloc_side(x, R, K, out[0], out[1]);
   if (cols) alloc_side(x, K, R, out[2], out[3]);
+  if (sums) out[4] = at::empty({(R + 127) / 128, K}, x.options().dtype(at::kFloat));
   if (R == 0 || K == 0) return out;
   bool swap = false;
   if (K > 1 && x.stride(1) != 1) {
-    if (R > 1 && x.stride(0) != 1) {
+    if (sums || (R > 1 && x.stride(0) != 1)) {
       x = x.contiguous();
     } else {                        // a transposed view: its rows are the columns of what is stored
       x = x.t();
@@ -424,11 +449,12 @@ std::vector<at::Tensor> fp8_quantize(const at::Tensor& x_, bool tile_scale, bool
   }
   auto ptr = [&](int i) { return out[i].defined() ? reinterpret_cast<uint8_t*>(out[i].data_ptr()) : nullptr; };
   uint8_t *q = ptr(swap ? 2 : 0), *s = ptr(swap ? 3 : 1), *qt = ptr(swap ? 0 : 2), *st = ptr(swap ? 1 : 3);
+  float* part = sums ? out[4].data_ptr<float>() : nullptr;
   auto stream = c10::cuda::getCurrentCUDAStream();
   switch (x.scalar_type()) {
-    case at::kBFloat16: quantize_t<__nv_bfloat16>(x, q, s, qt, st, tile_scale, stream); break;
-    case at::kHalf: quantize_t<__half>(x, q, s, qt, st, tile_scale, stream); break;
-    case at::kFloat: quantize_t<float>(x, q, s, qt, st, tile_scale, stream); break;
+    case at::kBFloat16: quantize_t<__nv_bfloat16>(x, q, s, qt, st, part, tile_scale, stream); break;
+    case at::kHalf: quantize_t<__half>(x, q, s, qt, st, part, tile_scale, stream); break;
+    case at::kFloat: quantize_t<float>(x, q, s, qt, st, part, tile_scale, stream); break;
     default: TORCH_CHECK(false, "fp8_quantize: x bf16, fp16 or fp32");
   }
   return out;

@@ -71,10 +71,22 @@ def fp8_quantize(x: torch.Tensor, block_rows: int = 1, layout: str = "rows"):
                            *((R, K) if s == "rows" else (K, R)), block_rows)
                  for s in ("rows", "cols") if layout in (s, "both")]
         return tuple(sides) if layout == "both" else sides[0]
-    q, qs, t, ts = ext().fp8_quantize(x, block_rows != 1, layout != "cols", layout != "rows")
+    q, qs, t, ts, _ = ext().fp8_quantize(x, block_rows != 1, layout != "cols", layout != "rows", False)
     rows = None if q is None else Fp8Tensor(q, qs, R, K, block_rows)
     cols = None if t is None else Fp8Tensor(t, ts, K, R, block_rows)
     return (rows, cols) if layout == "both" else (cols if rows is None else rows)
+
+
+def fp8_quantize_with_sums(g: torch.Tensor):
+    """``fp8_quantize(g, layout="both")`` and the fp32 column sums of g [R, K] (an output gradient
+    and its bias gradient) from one read of g: (rows, cols, sums [K])."""
+    if not g.is_cuda:
+        return (*fp8_quantize(g, layout="both"), g.float().sum(0))
+    if g.dim() != 2 or g.dtype not in _IN_TYPES:
+        raise TypeError(f"fp8_quantize_with_sums: a matrix in bf16, fp16 or fp32, got {g.dtype} {tuple(g.shape)}")
+    R, K = g.shape
+    q, qs, t, ts, part = ext().fp8_quantize(g, False, True, True, True)
+    return Fp8Tensor(q, qs, R, K), Fp8Tensor(t, ts, K, R), part.sum(0)
 
 
 def fp8_matmul(a, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,

@@ -54,14 +54,17 @@ class _FP8LinearFn(torch.autograd.Function):
             g = _gelu_tanh_bwd(g, pre)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = dw = db = None
-        if need_x or need_w:
+        if need_x and need_w and need_b:
+            gr, gc, db = ops.fp8_quantize_with_sums(g)
+            db = db.to(bdt)
+        elif need_x or need_w:
             gq = ops.fp8_quantize(g, layout="both" if need_x and need_w else "rows" if need_x else "cols")
             gr, gc = gq if need_x and need_w else (gq, gq)
-            if need_x:
-                dx = ops.fp8_matmul(gr, wc, out_dtype=_grad_dtype(xdt)).to(xdt).view(xshape)
-            if need_w:
-                dw = ops.fp8_matmul(gc, xc, out_dtype=_grad_dtype(wdt)).to(wdt)
-        if need_b:
+        if need_x:
+            dx = ops.fp8_matmul(gr, wc, out_dtype=_grad_dtype(xdt)).to(xdt).view(xshape)
+        if need_w:
+            dw = ops.fp8_matmul(gc, xc, out_dtype=_grad_dtype(wdt)).to(wdt)
+        if need_b and db is None:
             db = ops.bias_grad(g).to(bdt)
         return dx, dw, db, None
 

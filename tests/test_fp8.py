@@ -117,6 +117,22 @@ def test_quantize_extremes(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("R,K", [(1, 1), (5, 130), (128, 256), (300, 515), (1000, 72)])
+def test_quantize_with_sums(device, dtype, R, K):
+    x = _randn(R, K + 8, device=device, seed=R, dtype=dtype)
+    for v in (x[:, :K], x[:, 8:], x.t()[:K].t()):
+        rows, cols, sums = ops.fp8_quantize_with_sums(v)
+        check_quantized(rows, v, 1)
+        check_quantized(cols, v.t(), 1)
+        # R additions in fp32
+        assert bool(((sums.double() - v.double().sum(0)).abs() <= R * 2.0 ** -24 * v.double().abs().sum(0)).all())
+    x[R // 2, 0], x[0, K // 2] = math.inf, math.nan
+    bad = ops.fp8_quantize_with_sums(x[:, :K])[2]
+    assert torch.equal(bad, x[:, :K].float().sum(0)) or torch.equal(bad.isfinite(), x[:, :K].float().sum(0).isfinite())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_quantize_empty(device):
     for R, K in ((0, 5), (5, 0), (0, 0)):
         t = ops.fp8_quantize(torch.zeros(R, K, device=device))
