@@ -203,6 +203,28 @@ def test_matmul(device, M, N, K):
     check_product(y, xq, wq, bias, "gelu_tanh")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(3, 130, 20160), (64, 256, 9000), (40, 5120, 5120), (256, 300, 14040),
+                                   (700, 512, 20161), (1000, 64, 5120), (3000, 2304, 2200)])
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+def test_matmul_long_sums_in_fp32(M, N, K, act):
+    """Sums of one sign, where cutting each of the K / 32 steps would add up: runs of 64 steps cut
+    the growing sum by at most 2^-23 of it each, half of that in the mean and half a run's sum
+    on average, 64 / 4 * 2^-23 = 2^-19 in all; as much again for the additions of the runs."""
+    x = _randn(M, K, device="cuda", seed=M, dtype=torch.bfloat16).abs()
+    w = _randn(N, K, device="cuda", seed=N, spread=0.2).abs() / K
+    bias = _randn(N, device="cuda").abs()
+    wq, xq = ops.fp8_quantize(w, block_rows=128), ops.fp8_quantize(x)
+    want = xq.dequantize().double() @ wq.dequantize().double().t() + bias.double()
+    y, pre = ops.fp8_matmul(x, wq, bias, act, torch.float32, aux=True)
+    if act:
+        want_pre, want = want, _gelu64(want)
+        assert bool(((pre.double() - want_pre).abs() <= 2.0 ** -8 * want_pre).all())
+    assert ((y.double() - want).norm() / want.norm()).item() < 2.0 ** -18
+    again = ops.fp8_matmul(x, wq, bias, act, torch.float32)
+    assert torch.equal(again, y)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("M,N,K", [(1, 200, 700), (70, 130, 515), (300, 260, 300)])
 def test_matmul_scales_by_row_and_block(device, M, N, K):
