@@ -7,12 +7,13 @@
 // byte of the scale words.  Products and sums stay in the fp32 accumulator over the whole of K;
 // there is no second accumulation in registers, and the epilogue sees the finished sum.
 //
-// Structure (one CTA per SM, 320 threads):
+// Structure (one CTA per SM, 384 threads):
 //   warp 0      TMA producer: 128 x 128 codes of A and BN x 128 of B per stage (128B swizzle);
 //               with every fourth block, the 512-byte scale chunks of the next four
 //   warp 1      one thread issues tcgen05.cp (scale chunk -> TMEM, once per four blocks) and
 //               tcgen05.mma 128 x BN x 32, into one of two accumulators
-//   warps 2..9  epilogue: two groups of four warps, half of the tile's columns each
+//   warps 4..11 epilogue: two groups of four warps, half of the tile's columns each (where they
+//               keep 128 sums a thread, with 208 registers, which warps 0..3 give up)
 // A product of few rows runs in another form (skinny_kernel).
 // TMEM (512 columns): two accumulators of 256 columns and 16 columns of scales do not fit, so
 // at BN = 256 the accumulators overlap by 16 columns: accumulator 0 is 0..255, accumulator 1
@@ -40,7 +41,7 @@ namespace fp8 {
 constexpr int kBM = 128;
 constexpr int kBK = 128;                      // one scale block, one 128-byte swizzle span
 constexpr int kGroupM = 16;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr int kStageRow = 80;                 // bytes per staged output row (64 + 16 pad)
 constexpr int kStageBytes = 32 * kStageRow;
 constexpr uint32_t kScaleCol = 496;           // TMEM columns of the scales: A 496..499, B 500..507
@@ -199,12 +200,17 @@ __device__ __forceinline__ void finish_chunk(const Args& args, float* v, const f
   store_chunk(reinterpret_cast<OutT*>(args.out), v, stg, lane, row0, col0, args.M, args.N, args.vec);
 }
 
+// Launched with 12 warps x 168 registers; 4 x 64 + 8 x 208 of them are what is used.
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+
 template <int BN, typename OutT, bool RUNS>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
   using S = Shape<BN>;
   constexpr int STAGES = S::kStages;
   constexpr uint32_t IDESC = idesc_mxf8(kBM, BN);
+  constexpr bool kSplitRegs = RUNS && BN == 256;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -248,100 +254,104 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      const int last_chunk = (args.N + 127) / 128 - 1;
-      grid_dependency_wait();
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
-        int mb, nb;
-        tile_coords(t, num_m, num_n, mb, nb);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrFp8Producer)) { *abort_flag = 1; break; }
-          const bool with_scales = (kb & 3) == 0;
-          mbar_expect_tx(&full[stage], S::kA + S::kB + (with_scales ? S::kScales : 0));
-          tma_load_2d(&tmA, &full[stage], sA + stage * S::kA, kb * kBK, mb * kBM);
-          tma_load_2d(&tmB, &full[stage], sB + stage * S::kB, kb * kBK, nb * BN);
-          if (with_scales) {
-            uint8_t* d = sS + stage * S::kScales;
-            bulk_load(&full[stage], d, args.sa + ((long)mb * kgroups + (kb >> 2)) * kChunkBytes, kChunkBytes);
-#pragma unroll
-            for (int c = 0; c < S::kChunksB; ++c) {
-              // a tile's second chunk may lie past the end of N: its rows are zeros, any scale will do
-              const int chunk = min(nb * BN / 128 + c, last_chunk);
-              bulk_load(&full[stage], d + (1 + c) * kChunkBytes,
-                        args.sb + ((long)chunk * kgroups + (kb >> 2)) * kChunkBytes, kChunkBytes);
-            }
-          }
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        }
-      }
-      // the last loads have landed before the block ends, whoever gave up waiting for them: stages
-      // before `stage` were filled in this round, the others in the one before (or never)
-      for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], s < stage ? phase : phase ^ 1, args.err, kErrFp8Teardown);
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int it = 0;
-      const uint32_t t_sa = tmem_base + kScaleCol;
-      // (tile, run) pairs in order; `it` counts them
-      for (int t = blockIdx.x, run = 0; t < num_tiles && !*abort_flag; ++it) {
-        const int kb0 = run * kRun, kb1 = runs == 1 ? num_kb : min(num_kb, kb0 + kRun);
-        const int acc = it & 1;
-        const uint32_t acc_phase = (it >> 1) & 1;
-        bool ok = mbar_wait(&tempty[acc], acc_phase ^ 1, args.err, kErrFp8Mma);
-        // the previous tile's accumulator (use (it - 1) / 2 of it) shares columns with this one
-        if (ok && S::kOverlap && it > 0) ok = mbar_wait(&tearly[acc ^ 1], ((it - 1) >> 1) & 1, args.err, kErrFp8Mma);
-        if (!ok) { *abort_flag = 1; break; }
-        tc_fence_after();
-        // tiles of 64 and 192 columns begin in the middle of a 128-row scale chunk every other time
-        uint32_t t_sb = t_sa + 4;
-        if (BN % 128 != 0) {
+  if (warp < 4) {
+    if constexpr (kSplitRegs) fewer_registers();         // by all warps of the warpgroup
+    if (warp == 0) {
+      // ---------------------------------------------------------------- producer
+      if (lane == 0) {
+        const int last_chunk = (args.N + 127) / 128 - 1;
+        grid_dependency_wait();
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
           int mb, nb;
           tile_coords(t, num_m, num_n, mb, nb);
-          t_sb += 2 * (nb & 1);
-        }
-        const uint32_t d_tmem = tmem_base + acc * S::kAccStride;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, args.err, kErrFp8Mma)) { ok = false; break; }
-          tc_fence_after();
-          if ((kb & 3) == 0) {
-            // cp and mma of one thread execute in order: the scales are in place for the
-            // MMAs below, and the MMAs before them have read the old ones
-            const uint32_t s_addr = smem_u32(sS + stage * S::kScales);
-            cp_scales(t_sa, s_addr);
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrFp8Producer)) { *abort_flag = 1; break; }
+            const bool with_scales = (kb & 3) == 0;
+            mbar_expect_tx(&full[stage], S::kA + S::kB + (with_scales ? S::kScales : 0));
+            tma_load_2d(&tmA, &full[stage], sA + stage * S::kA, kb * kBK, mb * kBM);
+            tma_load_2d(&tmB, &full[stage], sB + stage * S::kB, kb * kBK, nb * BN);
+            if (with_scales) {
+              uint8_t* d = sS + stage * S::kScales;
+              bulk_load(&full[stage], d, args.sa + ((long)mb * kgroups + (kb >> 2)) * kChunkBytes, kChunkBytes);
 #pragma unroll
-            for (int c = 0; c < S::kChunksB; ++c) cp_scales(t_sa + 4 + 4 * c, s_addr + (1 + c) * kChunkBytes);
+              for (int c = 0; c < S::kChunksB; ++c) {
+                // a tile's second chunk may lie past the end of N: its rows are zeros, any scale will do
+                const int chunk = min(nb * BN / 128 + c, last_chunk);
+                bulk_load(&full[stage], d + (1 + c) * kChunkBytes,
+                          args.sb + ((long)chunk * kgroups + (kb >> 2)) * kChunkBytes, kChunkBytes);
+              }
+            }
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
           }
-          const uint32_t a_addr = smem_u32(sA + stage * S::kA);
-          const uint32_t b_addr = smem_u32(sB + stage * S::kB);
-          const uint32_t idesc = IDESC | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
-#pragma unroll
-          for (int k = 0; k < kBK / 32; ++k)
-            umma_mxf8(d_tmem, sdesc_sw128(a_addr + k * 32, 16, 1024), sdesc_sw128(b_addr + k * 32, 16, 1024), idesc,
-                      t_sa, t_sb, (kb > kb0 || k > 0) ? 1u : 0u);
-          umma_commit(&empty[stage]);
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-        umma_commit(&tfull[acc]);
-        if (!ok) { *abort_flag = 1; break; }
-        if (++run == runs) { run = 0; t += gridDim.x; }
+        // the last loads have landed before the block ends, whoever gave up waiting for them: stages
+        // before `stage` were filled in this round, the others in the one before (or never)
+        for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], s < stage ? phase : phase ^ 1, args.err, kErrFp8Teardown);
       }
-      umma_commit(done);
-      mbar_wait(done, 0, args.err, kErrFp8Teardown);
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        int it = 0;
+        const uint32_t t_sa = tmem_base + kScaleCol;
+        // (tile, run) pairs in order; `it` counts them
+        for (int t = blockIdx.x, run = 0; t < num_tiles && !*abort_flag; ++it) {
+          const int kb0 = run * kRun, kb1 = runs == 1 ? num_kb : min(num_kb, kb0 + kRun);
+          const int acc = it & 1;
+          const uint32_t acc_phase = (it >> 1) & 1;
+          bool ok = mbar_wait(&tempty[acc], acc_phase ^ 1, args.err, kErrFp8Mma);
+          // the previous tile's accumulator (use (it - 1) / 2 of it) shares columns with this one
+          if (ok && S::kOverlap && it > 0) ok = mbar_wait(&tearly[acc ^ 1], ((it - 1) >> 1) & 1, args.err, kErrFp8Mma);
+          if (!ok) { *abort_flag = 1; break; }
+          tc_fence_after();
+          // tiles of 64 columns begin in the middle of a 128-row scale chunk every other time
+          uint32_t t_sb = t_sa + 4;
+          if (BN == 64) {
+            int mb, nb;
+            tile_coords(t, num_m, num_n, mb, nb);
+            t_sb += 2 * (nb & 1);
+          }
+          const uint32_t d_tmem = tmem_base + acc * S::kAccStride;
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(&full[stage], phase, args.err, kErrFp8Mma)) { ok = false; break; }
+            tc_fence_after();
+            if ((kb & 3) == 0) {
+              // cp and mma of one thread execute in order: the scales are in place for the
+              // MMAs below, and the MMAs before them have read the old ones
+              const uint32_t s_addr = smem_u32(sS + stage * S::kScales);
+              cp_scales(t_sa, s_addr);
+#pragma unroll
+              for (int c = 0; c < S::kChunksB; ++c) cp_scales(t_sa + 4 + 4 * c, s_addr + (1 + c) * kChunkBytes);
+            }
+            const uint32_t a_addr = smem_u32(sA + stage * S::kA);
+            const uint32_t b_addr = smem_u32(sB + stage * S::kB);
+            const uint32_t idesc = IDESC | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+#pragma unroll
+            for (int k = 0; k < kBK / 32; ++k)
+              umma_mxf8(d_tmem, sdesc_sw128(a_addr + k * 32, 16, 1024), sdesc_sw128(b_addr + k * 32, 16, 1024), idesc,
+                        t_sa, t_sb, (kb > kb0 || k > 0) ? 1u : 0u);
+            umma_commit(&empty[stage]);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          umma_commit(&tfull[acc]);
+          if (!ok) { *abort_flag = 1; break; }
+          if (++run == runs) { run = 0; t += gridDim.x; }
+        }
+        umma_commit(done);
+        mbar_wait(done, 0, args.err, kErrFp8Teardown);
+      }
     }
   } else {
-    // ---------------------------------------------------------------- epilogue (warps 2..9)
+    // ---------------------------------------------------------------- epilogue (warps 4..11)
+    if constexpr (kSplitRegs) more_registers();
     constexpr int PER = BN / 64;                // 32-column chunks of each of the two groups
     const int quarter = warp & 3;               // TMEM lanes 32 * quarter ..
-    const int eg = (warp - 2) >> 2;
-    uint8_t* stg = epi_stage + (warp - 2) * kStageBytes;
-    float* sbias = reinterpret_cast<float*>(epi_stage + 8 * kStageBytes) + (warp - 2) * PER * 32;
+    const int eg = (warp - 4) >> 2;
+    uint8_t* stg = epi_stage + (warp - 4) * kStageBytes;
+    float* sbias = reinterpret_cast<float*>(epi_stage + 8 * kStageBytes) + (warp - 4) * PER * 32;
     float sum[RUNS ? PER : 1][32];                        // the runs so far
     int it = 0;
     for (int t = blockIdx.x, run = 0; t < num_tiles; ++it) {
@@ -382,15 +392,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         if (lane == 0) mbar_arrive(&tempty[acc]);
       };
       if constexpr (RUNS) {
-        static_assert(!S::kOverlap, "the sums of 256 columns do not fit a thread's registers");
+        auto add_up = [&](auto backwards) {
 #pragma unroll
-        for (int c = 0; c < PER; ++c) {
-          uint32_t r[32];
-          tmem_ld32(t_row + (eg * PER + c) * 32, r);
-          tmem_ld_wait();
+          for (int i = 0; i < PER; ++i) {
+            constexpr bool kBack = decltype(backwards)::value;
+            const int c = kBack ? PER - 1 - i : i;
+            uint32_t r[32];
+            tmem_ld32(t_row + (eg * PER + c) * 32, r);
+            tmem_ld_wait();
+            shared_read(i);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[c][j] = run == 0 ? __uint_as_float(r[j]) : sum[c][j] + __uint_as_float(r[j]);
-        }
+            for (int j = 0; j < 32; ++j) sum[c][j] = run == 0 ? __uint_as_float(r[j]) : sum[c][j] + __uint_as_float(r[j]);
+          }
+        };
+        if (S::kOverlap && acc == 0) add_up(std::true_type());
+        else add_up(std::false_type());
         all_read();
         if (run + 1 == runs) {
 #pragma unroll
@@ -730,11 +746,9 @@ static void product(const at::Tensor& a, const at::Tensor& b, const Args& args, 
   const bool narrow = args.N <= 128 || tiles128 <= num_sms(a.get_device());
   if constexpr (sizeof(OutT) == 4) {
     if (args.KB > kRun) {
-      // sums of runs: 96 registers a thread with tiles of 192 columns, 128 with 256, which spill
-      // (1536 x 8960 over 14040: 2150 TFLOP/s; one run in tiles of 256: 2500; runs in tiles of 128: 1690)
       if (args.N <= 64) launch<64, OutT, true>(a, b, args, behind, stream);
       else if (narrow) launch<128, OutT, true>(a, b, args, behind, stream);
-      else launch<192, OutT, true>(a, b, args, behind, stream);
+      else launch<256, OutT, true>(a, b, args, behind, stream);
       return;
     }
   }
