@@ -92,6 +92,13 @@ __device__ __forceinline__ void umma_mxf8(uint32_t tmem_d, uint64_t adesc, uint6
       "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
       :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate) : "memory");
 }
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // e4m3 x e4m3 with power-of-two scales; the scale-byte numbers go into bits 4 (B) and 29 (A).
 __host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N) {
   return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
@@ -292,32 +299,37 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issuer
-      if (lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        int it = 0;
-        const uint32_t t_sa = tmem_base + kScaleCol;
-        // (tile, run) pairs in order; `it` counts them
-        for (int t = blockIdx.x, run = 0; t < num_tiles && !*abort_flag; ++it) {
-          const int kb0 = run * kRun, kb1 = runs == 1 ? num_kb : min(num_kb, kb0 + kRun);
-          const int acc = it & 1;
-          const uint32_t acc_phase = (it >> 1) & 1;
-          bool ok = mbar_wait(&tempty[acc], acc_phase ^ 1, args.err, kErrFp8Mma);
-          // the previous tile's accumulator (use (it - 1) / 2 of it) shares columns with this one
-          if (ok && S::kOverlap && it > 0) ok = mbar_wait(&tearly[acc ^ 1], ((it - 1) >> 1) & 1, args.err, kErrFp8Mma);
-          if (!ok) { *abort_flag = 1; break; }
+      // The whole warp runs the loop and one elected lane issues: the operands of the MMAs then stay
+      // in uniform registers, and the descriptors of a stage differ from the first's by an addend.
+      const uint64_t a_desc = sdesc_sw128(smem_u32(sA), 16, 1024), b_desc = sdesc_sw128(smem_u32(sB), 16, 1024);
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      const uint32_t t_sa = tmem_base + kScaleCol;
+      // (tile, run) pairs in order; `it` counts them
+      for (int t = blockIdx.x, run = 0; t < num_tiles && !*abort_flag; ++it) {
+        const int kb0 = run * kRun, kb1 = runs == 1 ? num_kb : min(num_kb, kb0 + kRun);
+        const int acc = it & 1;
+        const uint32_t acc_phase = (it >> 1) & 1;
+        bool ok = mbar_wait(&tempty[acc], acc_phase ^ 1, args.err, kErrFp8Mma);
+        // the previous tile's accumulator (use (it - 1) / 2 of it) shares columns with this one
+        if (ok && S::kOverlap && it > 0) ok = mbar_wait(&tearly[acc ^ 1], ((it - 1) >> 1) & 1, args.err, kErrFp8Mma);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) { *abort_flag = 1; break; }
+        tc_fence_after();
+        // tiles of 64 columns begin in the middle of a 128-row scale chunk every other time
+        uint32_t t_sb = t_sa + 4;
+        if (BN == 64) {
+          int mb, nb;
+          tile_coords(t, num_m, num_n, mb, nb);
+          t_sb += 2 * (nb & 1);
+        }
+        const uint32_t d_tmem = tmem_base + acc * S::kAccStride;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, args.err, kErrFp8Mma));
+          if (!ok) break;
           tc_fence_after();
-          // tiles of 64 columns begin in the middle of a 128-row scale chunk every other time
-          uint32_t t_sb = t_sa + 4;
-          if (BN == 64) {
-            int mb, nb;
-            tile_coords(t, num_m, num_n, mb, nb);
-            t_sb += 2 * (nb & 1);
-          }
-          const uint32_t d_tmem = tmem_base + acc * S::kAccStride;
-          for (int kb = kb0; kb < kb1; ++kb) {
-            if (!mbar_wait(&full[stage], phase, args.err, kErrFp8Mma)) { ok = false; break; }
-            tc_fence_after();
+          if (elect_one()) {
             if ((kb & 3) == 0) {
               // cp and mma of one thread execute in order: the scales are in place for the
               // MMAs below, and the MMAs before them have read the old ones
@@ -326,23 +338,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
               for (int c = 0; c < S::kChunksB; ++c) cp_scales(t_sa + 4 + 4 * c, s_addr + (1 + c) * kChunkBytes);
             }
-            const uint32_t a_addr = smem_u32(sA + stage * S::kA);
-            const uint32_t b_addr = smem_u32(sB + stage * S::kB);
+            const uint64_t ad = a_desc + stage * (S::kA >> 4), bd = b_desc + stage * (S::kB >> 4);
             const uint32_t idesc = IDESC | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
 #pragma unroll
             for (int k = 0; k < kBK / 32; ++k)
-              umma_mxf8(d_tmem, sdesc_sw128(a_addr + k * 32, 16, 1024), sdesc_sw128(b_addr + k * 32, 16, 1024), idesc,
-                        t_sa, t_sb, (kb > kb0 || k > 0) ? 1u : 0u);
+              umma_mxf8(d_tmem, ad + 2 * k, bd + 2 * k, idesc, t_sa, t_sb, (kb > kb0 || k > 0) ? 1u : 0u);
             umma_commit(&empty[stage]);
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            if (kb + 1 == kb1) umma_commit(&tfull[acc]);
           }
-          umma_commit(&tfull[acc]);
-          if (!ok) { *abort_flag = 1; break; }
-          if (++run == runs) { run = 0; t += gridDim.x; }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-        umma_commit(done);
-        mbar_wait(done, 0, args.err, kErrFp8Teardown);
+        if (!ok) { *abort_flag = 1; break; }
+        if (++run == runs) { run = 0; t += gridDim.x; }
       }
+      if (elect_one()) umma_commit(done);
+      mbar_wait(done, 0, args.err, kErrFp8Teardown);
     }
   } else {
     // ---------------------------------------------------------------- epilogue (warps 4..11)
