@@ -27,7 +27,7 @@
 
 #include "common.cuh"
 #include "fp8.cuh"
-#include "tma_host.h"
+#include "launch.h"
 
 namespace osp {
 namespace adamw8 {
@@ -299,6 +299,8 @@ template <typename PT, typename GT, bool STATE8> struct Lane {
 template <typename PT, typename GT, bool STATE8, int CAP>
 __global__ void __launch_bounds__(256, 4) step_kernel(const __grid_constant__ Args<CAP> args) {
   constexpr int U = kChunkBlocks / 8;
+  grid_dependency_wait();
+  allow_dependents();
   const Consts c = args.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunk = blockIdx.x;
@@ -346,9 +348,7 @@ __global__ void __launch_bounds__(256, 4) step_kernel(const __grid_constant__ Ar
 template <typename PT, typename GT, int CAP>
 static void launch(const Args<CAP>& a, bool state8, cudaStream_t stream) {
   const int grid = a.chunk_end[a.tensors - 1];       // chunks, below 2^31
-  if (state8) step_kernel<PT, GT, true, CAP><<<grid, 256, 0, stream>>>(a);
-  else step_kernel<PT, GT, false, CAP><<<grid, 256, 0, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_kernel(state8 ? step_kernel<PT, GT, true, CAP> : step_kernel<PT, GT, false, CAP>, grid, 256, 0, 1, stream, a);
 }
 
 using Ptrs = std::vector<const at::Tensor*>;

@@ -30,6 +30,7 @@
 
 #include "common.cuh"
 #include "fp8.cuh"
+#include "launch.h"
 #include "tma_host.h"
 
 namespace osp {
@@ -75,9 +76,6 @@ __device__ __forceinline__ void bulk_load(uint64_t* bar, void* dst, const void* 
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-// A product launched right behind the quantiser of its left operand starts while that still runs
-// (programmatic dependent launch) and waits here before it reads the codes.
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // One 512-byte scale chunk -> 4 TMEM columns, repeated in each quarter of the lanes.
 __device__ __forceinline__ void cp_scales(uint32_t tmem, uint32_t saddr) {
   // no swizzle; 8-row core matrices of 16-byte rows, 128 bytes apart
@@ -260,6 +258,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_wait();
+  allow_dependents();
 
   if (warp < 4) {
     if constexpr (kSplitRegs) fewer_registers();         // by all warps of the warpgroup
@@ -267,8 +267,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       // ---------------------------------------------------------------- producer
       if (lane == 0) {
         const int last_chunk = (args.N + 127) / 128 - 1;
-        grid_dependency_wait();
-        int stage = 0;
+          int stage = 0;
         uint32_t phase = 0;
         for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
           int mb, nb;
@@ -499,7 +498,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 template <int BNX, typename OutT>
 __global__ void __launch_bounds__(192, 2)
 skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Args args,
-              int splits) {
+              int splits, bool weight_first) {
   using S = Skinny<BNX>;
   constexpr int STAGES = S::kStages;
   constexpr uint32_t IDESC = idesc_mxf8(128, BNX);
@@ -541,6 +540,11 @@ skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // only the producer of the weight's first stages goes ahead, if nothing before can have written it
+  if (warp != 0 || !weight_first) {
+    grid_dependency_wait();
+    allow_dependents();
+  }
 
   if (warp == 0) {
     if (lane == 0) {
@@ -697,43 +701,17 @@ static CUtensorMap make_tmap(const at::Tensor& t, uint32_t box_rows) {
   return m;
 }
 
-// `behind`: the stream's last kernel is the quantiser of `a` (see grid_dependency_wait).
-template <typename... P, typename... A>
-static void launch_kernel(void (*kern)(P...), int grid, int threads, int smem, int cluster, bool behind,
-                          cudaStream_t stream, A&&... a) {
-  smem_opt_in(reinterpret_cast<const void*>(kern), smem);
-  cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  if (cluster > 1) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = cluster;
-    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (behind) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(a)...));
-}
-
 template <int BN, typename OutT, bool RUNS>
-static void launch(const at::Tensor& a, const at::Tensor& b, const Args& args, bool behind, cudaStream_t stream) {
+static void launch(const at::Tensor& a, const at::Tensor& b, const Args& args, cudaStream_t stream) {
   constexpr int smem = Shape<BN>::smem_bytes();
   static_assert(smem <= 232448, "shared memory");
   const int tiles = ((args.M + kBM - 1) / kBM) * ((args.N + BN - 1) / BN);
-  launch_kernel(gemm_kernel<BN, OutT, RUNS>, std::min(tiles, num_sms(a.get_device())), kThreads, smem, 1, behind, stream,
+  launch_kernel(gemm_kernel<BN, OutT, RUNS>, std::min(tiles, num_sms(a.get_device())), kThreads, smem, 1, stream,
                 make_tmap(a, kBM), make_tmap(b, BN), args);
 }
 
 template <int BNX, typename OutT>
-static void launch_skinny(const at::Tensor& a, const at::Tensor& b, const Args& args, bool behind,
+static void launch_skinny(const at::Tensor& a, const at::Tensor& b, const Args& args, bool weight_first,
                           cudaStream_t stream) {
   // as many parts of K as fill two CTAs per SM, at most 8 (a portable cluster), whole scale
   // chunks each; then no more parts than the longest of them needs
@@ -741,10 +719,12 @@ static void launch_skinny(const at::Tensor& a, const at::Tensor& b, const Args& 
   const int most = std::max(1, std::min({8, kgroups, 2 * num_sms(a.get_device()) / tiles}));
   const int longest = (kgroups + most - 1) / most;
   const int splits = (kgroups + longest - 1) / longest;
-  launch_kernel(skinny_kernel<BNX, OutT>, tiles * splits, 192, Skinny<BNX>::smem_bytes(), splits, behind, stream,
-                make_tmap(a, BNX), make_tmap(b, 128), args, splits);
+  launch_kernel(skinny_kernel<BNX, OutT>, tiles * splits, 192, Skinny<BNX>::smem_bytes(), splits, stream,
+                make_tmap(a, BNX), make_tmap(b, 128), args, splits, weight_first);
 }
 
+// `behind`: the stream's last kernel is the quantiser of `a`, whose own predecessors have completed
+// when a kernel starts behind it: the weight, which it does not write, may be read at once.
 template <typename OutT>
 static void product(const at::Tensor& a, const at::Tensor& b, const Args& args, bool behind, cudaStream_t stream) {
   if (args.M <= 16) return launch_skinny<16, OutT>(a, b, args, behind, stream);
@@ -756,15 +736,15 @@ static void product(const at::Tensor& a, const at::Tensor& b, const Args& args, 
   const bool narrow = args.N <= 128 || tiles128 <= num_sms(a.get_device());
   if constexpr (sizeof(OutT) == 4) {
     if (args.KB > kRun) {
-      if (args.N <= 64) launch<64, OutT, true>(a, b, args, behind, stream);
-      else if (narrow) launch<128, OutT, true>(a, b, args, behind, stream);
-      else launch<256, OutT, true>(a, b, args, behind, stream);
+      if (args.N <= 64) launch<64, OutT, true>(a, b, args, stream);
+      else if (narrow) launch<128, OutT, true>(a, b, args, stream);
+      else launch<256, OutT, true>(a, b, args, stream);
       return;
     }
   }
-  if (args.N <= 64) launch<64, OutT, false>(a, b, args, behind, stream);
-  else if (narrow) launch<128, OutT, false>(a, b, args, behind, stream);
-  else launch<256, OutT, false>(a, b, args, behind, stream);
+  if (args.N <= 64) launch<64, OutT, false>(a, b, args, stream);
+  else if (narrow) launch<128, OutT, false>(a, b, args, stream);
+  else launch<256, OutT, false>(a, b, args, stream);
 }
 
 }  // namespace fp8

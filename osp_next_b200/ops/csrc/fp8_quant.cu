@@ -17,6 +17,7 @@
 
 #include "common.cuh"
 #include "fp8.cuh"
+#include "launch.h"
 
 namespace osp {
 namespace fp8 {
@@ -134,8 +135,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
                                                             uint8_t* __restrict__ scale, int R, int K, int Kp,
                                                             int kgroups, long total) {
-  // a product behind this kernel may start its own preparations (it waits before it reads q)
-  asm volatile("griddepcontrol.launch_dependents;");
+  grid_dependency_wait();
+  allow_dependents();
   const int lane = threadIdx.x & 31;
   const long w0 = ((long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2;
   if (w0 >= total) return;
@@ -210,6 +211,8 @@ quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
   __shared__ uint32_t top[2][4][128];              // [0]: rows over 2 warps, [1]: columns over 4
   __shared__ __align__(16) float factor[2][128];
   __shared__ float sums[SUMS ? 4 : 1][128];
+  grid_dependency_wait();
+  allow_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wr = warp >> 1, wc = warp & 1;
   const int rl = wr * 32 + (lane >> 3) * 8;        // first row of this thread in the tile
@@ -395,15 +398,15 @@ static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
     const int kgroups = (K + 511) / 512;
     const long total = (long)Rp * kgroups;
     const unsigned grid = (unsigned)((total + 15) / 16);
-    if (vec) fp8::quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(xp, ld, q, s, R, K, Kp, kgroups, total);
-    else fp8::quantize_rows_kernel<T, false><<<grid, 256, 0, stream>>>(xp, ld, q, s, R, K, Kp, kgroups, total);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    launch_kernel(vec ? fp8::quantize_rows_kernel<T, true> : fp8::quantize_rows_kernel<T, false>, grid, 256, 0, 1,
+                  stream, xp, ld, q, s, R, K, Kp, kgroups, total);
     return;
   }
   const dim3 grid(Kp / 128, Rp / 128);
   TORCH_CHECK(grid.y <= 65535, "fp8_quantize: more than 8388480 rows");
 #define OSP_TILES(VEC, TS, RO, CO, SU) \
-  fp8::quantize_tiles_kernel<T, VEC, TS, RO, CO, SU><<<grid, 256, 0, stream>>>(xp, ld, q, s, qt, st, part, R, K, Kp, Rp)
+  launch_kernel(fp8::quantize_tiles_kernel<T, VEC, TS, RO, CO, SU>, grid, 256, 0, 1, stream, xp, ld, q, s, qt, st, \
+                part, R, K, Kp, Rp)
 #define OSP_TILES_SIDES(VEC, TS)                             \
   do {                                                       \
     if (part) OSP_TILES(VEC, false, true, true, true);       \
@@ -420,7 +423,6 @@ static void quantize_t(const at::Tensor& x, uint8_t* q, uint8_t* s, uint8_t* qt,
   }
 #undef OSP_TILES_SIDES
 #undef OSP_TILES
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 // Codes and scales of x [R, K] (`rows`) and / or of its transpose (`cols`); any strides.  Sides
