@@ -71,8 +71,9 @@ def parse():
     p.add_argument("--no-e2e", action="store_true")
     p.add_argument("--mode", choices=["infer", "train"], default="infer",
                    help="infer: the sec/video headline; train: flow-matching training tokens/s")
-    p.add_argument("--quant", choices=["none", "hif8"], default="none",
-                   help="train mode: HiF8 fake-quant linears (BASELINE config 4) or plain bf16")
+    p.add_argument("--quant", choices=["none", "hif8", "fp8"], default="none",
+                   help="train mode: HiF8 fake-quant linears, block-scaled fp8 linears with 8-bit AdamW moments, "
+                        "or plain bf16")
     p.add_argument("--loss-log", default=None, help="train mode: append per-step losses (JSONL) here")
     p.add_argument("--fsdp-comm", choices=["p2p", "nccl"], default="p2p",
                    help="train mode: FSDP block all-gather / reduce-scatter over NVLink peer memory or NCCL")
@@ -301,6 +302,9 @@ def train_config(args, world, out_dir):
     cfg["model_config"].pop("pretrained_model_dir_or_checkpoint", None)
     if getattr(args, "quant", "none") == "hif8":
         cfg["model_config"].update(quant="hif8")
+    if getattr(args, "quant", "none") == "fp8":
+        cfg["model_config"].update(quant="fp8")
+        cfg["optimizer_config"] = dict(cfg.get("optimizer_config", {}), state_bits=8)
     if getattr(args, "loss_log", None):
         cfg["metrics_file"] = args.loss_log
     dc = dict(cfg.get("data_config", {}))
@@ -355,7 +359,7 @@ def run_train(args, rank, world, local, impl):
     return {"metric": f"train tokens/s OSP-Next-{args.model}{q} flow matching {args.frames}f "
                       f"{args.height}x{args.width}", "unit": "tokens/s", "n_gpus": world, "steps": args.steps,
             "warmup": args.warmup, "higher_is_better": True, "scaling": "weak" if world > 4 else "strong",
-            "dtype": "bf16", "impl": impl,
+            "dtype": "fp8" if args.quant == "fp8" else "bf16", "impl": impl,
             "data": "synthetic (random-init weights, N(0,1) latents and text embeddings, logit-normal t)",
             "layout": {"fsdp_comm": args.fsdp_comm if impl == "ours" else "nccl"},
             "config": {"model": f"OSP-Next-{args.model}", "global_batch": max(1, world // ssp),
