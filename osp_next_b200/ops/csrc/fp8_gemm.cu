@@ -4,8 +4,13 @@
 // The scales are applied by the tensor core: tcgen05.mma kind::mxf8f6f4.block_scale multiplies
 // each group of 32 along K by a power of two per row of A and per row of B, read from TMEM.
 // A block of 128 is four such groups with one scale, so the four MMAs of a block name the same
-// byte of the scale words.  Products and sums stay in the fp32 accumulator over the whole of K;
-// there is no second accumulation in registers, and the epilogue sees the finished sum.
+// byte of the scale words.  Sums stay in the fp32 accumulator in TMEM over the whole of K (over runs
+// of 16 blocks where the result is fp32, see kRun), with no rescaling in registers between blocks.
+//
+// What bounds it: large products run at the power cap, 2500 to 2640 TFLOP/s at an SM clock of 1.33 to
+// 1.5 GHz with 136 cycles per 128 x 256 x 32 MMA (128 at the full rate); the same tiles on CTA pairs
+// (cta_group::2) were slower (2390).  An MMA of fewer columns costs nearly as much, so 256 columns are
+// taken where they fill the GPU: 4096 x 5120 x 5120 takes 84 us, in tiles of 128 columns 119, of 64 194.
 //
 // Structure (one CTA per SM, 384 threads):
 //   warp 0      TMA producer: 128 x 128 codes of A and BN x 128 of B per stage (128B swizzle);
@@ -13,7 +18,7 @@
 //   warp 1      one thread issues tcgen05.cp (scale chunk -> TMEM, once per four blocks) and
 //               tcgen05.mma 128 x BN x 32, into one of two accumulators
 //   warps 4..11 epilogue: two groups of four warps, half of the tile's columns each (where they
-//               keep 128 sums a thread, with 208 registers, which warps 0..3 give up)
+//               keep 128 sums a thread, with 208 registers, of which warps 0..3 give up a part)
 // A product of few rows runs in another form (skinny_kernel).
 // TMEM (512 columns): two accumulators of 256 columns and 16 columns of scales do not fit, so
 // at BN = 256 the accumulators overlap by 16 columns: accumulator 0 is 0..255, accumulator 1
@@ -458,7 +463,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 // N.  CTAs of 100 KB share an SM in pairs; where the tiles are too few to fill the GPU a cluster
 // of up to 8 CTAs splits K and adds its parts through distributed shared memory, in rank order
 // (the result does not depend on timing, and no workspace is needed).  The weight's first
-// stages are loaded before the wait for the quantiser of A.
+// stages are loaded before the wait for the quantiser of A.  1 x 5120 -> 30720: 27.9 us with the
+// quantiser, 0.86 of the copy rate on the weight's bytes; 128 rows take 27.5 us here (cold caches)
+// and 21.5 in gemm_kernel's tiles, 64 rows about the same in both.
 // 192 threads: warp 0 TMA producer, warp 1 MMA issuer, warps 2..5 epilogue.
 template <int BNX> struct Skinny {
   static constexpr uint32_t kW = 128 * kBK, kX = BNX * kBK, kScales = 2 * kChunkBytes;
@@ -730,8 +737,9 @@ static void product(const at::Tensor& a, const at::Tensor& b, const Args& args, 
   if (args.M <= 16) return launch_skinny<16, OutT>(a, b, args, behind, stream);
   if (args.M <= 32) return launch_skinny<32, OutT>(a, b, args, behind, stream);
   if (args.M <= 64) return launch_skinny<64, OutT>(a, b, args, behind, stream);
-  // an MMA of 128 columns takes nearly the time of one of 256 (145 and 158 cycles in the loop):
-  // narrow tiles only where one round of them covers the result
+  // an MMA of 128 columns takes nearly the time of one of 256: narrow tiles only where one round of
+  // them covers the result (128 x 4096 -> 5120: 17.6 us in tiles of 128 columns, 20.3 of 256; 512 rows,
+  // two rounds against one: 28.2 and 22.5)
   const long tiles128 = (long)((args.M + 127) / 128) * ((args.N + 127) / 128);
   const bool narrow = args.N <= 128 || tiles128 <= num_sms(a.get_device());
   if constexpr (sizeof(OutT) == 4) {
