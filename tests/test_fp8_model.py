@@ -111,7 +111,7 @@ def test_optimizer_checkpoints_hold_fp32_moments(device):
     sd = opt.state_dict()
     for st in sd["state"].values():
         assert set(st) == {"step", "exp_avg", "exp_avg_sq"} and st["exp_avg"].dtype == torch.float32
-    # into 8 bits again: the codes are what they were
+    # into 8 bits again: the same values (a block whose largest was rounded down may take a smaller scale)
     opt2 = FusedAdamW(twin.parameters(), lr=1e-3, state_bits=8)
     opt2.load_state_dict(copy.deepcopy(sd))
     for a, b in zip(opt.state.values(), opt2.state.values()):
@@ -170,3 +170,72 @@ def test_trainer_with_fp8_and_8bit_moments(tmp_path, monkeypatch):
     recs = [json.loads(line) for line in open(os.path.join(out, "metrics.jsonl"))]
     assert [r["iter"] for r in recs] == [1, 2, 3, 4]
     assert all(r["loss"] == r["loss"] and r["loss"] < 100 for r in recs)
+
+
+def _fsdp_worker(rank, world, port, out_dir):
+    import torch.distributed as dist
+    from torch.distributed.checkpoint.state_dict import (StateDictOptions, get_optimizer_state_dict,
+                                                         set_optimizer_state_dict)
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.fsdp import fully_shard
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    opts = StateDictOptions(full_state_dict=True)
+
+    def build():
+        torch.manual_seed(0)
+        net = torch.nn.Sequential(torch.nn.Linear(70, 51), torch.nn.Linear(51, 3))     # odd rows: uneven shards
+        return fully_shard(net, mesh=init_device_mesh("cpu", (world,)))
+
+    def steps(net, opt, first, n):
+        for i in range(first, first + n):
+            for j, p in enumerate(net.parameters()):
+                full = torch.randn(p.shape, generator=torch.Generator().manual_seed(100 * i + j))
+                p.grad = torch.distributed.tensor.distribute_tensor(full, p.device_mesh, p.placements)
+            opt.step()
+    net = build()
+    opt = FusedAdamW(net.parameters(), lr=1e-2, state_bits=8)
+    steps(net, opt, 0, 3)
+    full = get_optimizer_state_dict(net, opt, options=opts)
+    opt.zero_grad(set_to_none=True)              # as on resume: no gradients yet
+    again = FusedAdamW(net.parameters(), lr=1e-2, state_bits=8)
+    set_optimizer_state_dict(net, again, copy.deepcopy(full), options=opts)
+    names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+    for a, b in zip(opt.state.values(), again.state.values()):
+        assert a["step"] == b["step"]
+        assert all(torch.equal(x, y) for x, y in zip(*(ops.adamw8_decode(*(s[k] for k in names)) for s in (a, b))))
+    state = {n: {k: v for k, v in st.items()} for n, st in full["state"].items()}
+    shapes = {n: tuple(p.shape) for n, p in net.named_parameters()}
+    assert all(tuple(st[k].shape) == shapes[n] for n, st in state.items() for k in ("exp_avg", "exp_avg_sq"))
+    steps(net, again, 3, 1)
+    torch.save({"state": state, "params": [p.full_tensor() for p in net.parameters()]},
+               os.path.join(out_dir, f"r{rank}.pt"))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_8bit_moments_on_sharded_parameters(tmp_path):
+    """Two ranks with uneven FSDP shards: the full checkpoint has the moments of the whole tensors,
+    those of the shards stepped alone, and loading it gives back the same values."""
+    import torch.multiprocessing as mp
+    from test_distributed_cpu import _port
+    mp.start_processes(_fsdp_worker, args=(2, _port(), str(tmp_path)), nprocs=2, join=True, start_method="spawn")
+    outs = [torch.load(tmp_path / f"r{r}.pt") for r in range(2)]
+    for a, b in zip(outs[0]["params"], outs[1]["params"]):
+        assert torch.equal(a, b) and bool(a.isfinite().all())
+    # each rank's shards by themselves (rows dealt as FSDP deals them), put together
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(70, 51), torch.nn.Linear(51, 3))
+    parts = []
+    for rank in range(2):
+        shards = [torch.nn.Parameter(p.detach().chunk(2)[rank].clone()) for p in net.parameters()]
+        opt = FusedAdamW(shards, lr=1e-2, state_bits=8)
+        for i in range(3):
+            for j, (p, full) in enumerate(zip(shards, net.parameters())):
+                g = torch.randn(full.shape, generator=torch.Generator().manual_seed(100 * i + j))
+                p.grad = g.chunk(2)[rank].contiguous()
+            opt.step()
+        parts.append([st for st in opt.state_dict()["state"].values()])
+    for (n, _), a, b in zip(net.named_parameters(), *parts):
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(outs[0]["state"][n][k], torch.cat([a[k], b[k]])), (n, k)
