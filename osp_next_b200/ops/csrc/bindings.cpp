@@ -58,6 +58,12 @@ std::vector<at::Tensor> fp8_gemm(const at::Tensor& a, const at::Tensor& sa, cons
                                  const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux);
 std::vector<at::Tensor> fp8_linear(const at::Tensor& x, const at::Tensor& b, const at::Tensor& sb,
                                    const c10::optional<at::Tensor>& bias, int64_t act, bool f32, bool aux);
+std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor& w,
+                                           const c10::optional<at::Tensor>& bias, int64_t act, bool aux, bool need_x,
+                                           bool need_w);
+std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& g, const c10::optional<at::Tensor>& xc,
+                                            const c10::optional<at::Tensor>& xs, const c10::optional<at::Tensor>& wc,
+                                            const c10::optional<at::Tensor>& ws, bool need_b, bool dx_f32, bool dw_f32);
 void sde_step(const at::Tensor& x, const at::Tensor& v, const c10::optional<at::Tensor>& xi,
               const c10::optional<at::Tensor>& prev_in, at::Tensor& prev_out, const c10::optional<at::Tensor>& mean_out,
               at::Tensor& logp, double sigma, double dt, double smin, double smax);
@@ -178,6 +184,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_quantize", &osp::fp8_quantize);
   m.def("fp8_gemm", &osp::fp8_gemm);
   m.def("fp8_linear", &osp::fp8_linear);
+  m.def("fp8_linear_forward", &osp::fp8_linear_forward);
+  m.def("fp8_linear_backward", &osp::fp8_linear_backward);
   m.def("sde_step", &osp::sde_step);
   m.def("wait_probe", &osp::wait_probe);
   m.def("gemm_p2p", &osp::gemm_p2p);

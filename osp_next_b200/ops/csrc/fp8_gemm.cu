@@ -26,6 +26,7 @@
 // warp so; the next tile then starts while the rest is still being read.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/sum.h>
 #include <ATen/cuda/CUDAContextLight.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAException.h>
@@ -141,15 +142,7 @@ __device__ __forceinline__ void store_scalar(__nv_bfloat16* p, float v) { *p = _
 template <typename OutT>
 __device__ __forceinline__ void store_chunk(OutT* out, const float* v, uint8_t* stg, int lane, long row0, int col0,
                                             int M, int N, bool vec) {
-  if (!vec || col0 + 32 > N) {
-    const long row = row0 + lane;
-    if (row < M) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col0 + j < N) store_scalar(out + row * N + col0 + j, v[j]);
-    }
-    return;
-  }
+  const bool whole = vec && col0 + 32 <= N;           // 16-byte stores fit
   if constexpr (sizeof(OutT) == 2) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -161,13 +154,19 @@ __device__ __forceinline__ void store_chunk(OutT* out, const float* v, uint8_t* 
       *reinterpret_cast<uint4*>(stg + lane * kStageRow + j * 16) = w;
     }
     __syncwarp();
-    const int q = lane >> 2, cc = lane & 3;
+    if (whole) {
+      const int q = lane >> 2, cc = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int rr = i * 8 + q;
-      if (row0 + rr < M)
-        *reinterpret_cast<uint4*>(out + (row0 + rr) * N + col0 + cc * 8) =
-            *reinterpret_cast<const uint4*>(stg + rr * kStageRow + cc * 16);
+      for (int i = 0; i < 4; ++i) {
+        const int rr = i * 8 + q;
+        if (row0 + rr < M)
+          *reinterpret_cast<uint4*>(out + (row0 + rr) * N + col0 + cc * 8) =
+              *reinterpret_cast<const uint4*>(stg + rr * kStageRow + cc * 16);
+      }
+    } else if (col0 + lane < N) {                       // any row length: a row's 32 elements by 32 lanes
+#pragma unroll 8
+      for (int rr = 0; rr < 32; ++rr)
+        if (row0 + rr < M) out[(row0 + rr) * N + col0 + lane] = reinterpret_cast<const OutT*>(stg + rr * kStageRow)[lane];
     }
     __syncwarp();
   } else {
@@ -179,12 +178,20 @@ __device__ __forceinline__ void store_chunk(OutT* out, const float* v, uint8_t* 
         *reinterpret_cast<float4*>(stg + lane * kStageRow + j * 16) =
             make_float4(v[16 * h + 4 * j], v[16 * h + 4 * j + 1], v[16 * h + 4 * j + 2], v[16 * h + 4 * j + 3]);
       __syncwarp();
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int rr = i * 8 + q;
-        if (row0 + rr < M)
-          *reinterpret_cast<float4*>(out + (row0 + rr) * N + col0 + 16 * h + cc * 4) =
-              *reinterpret_cast<const float4*>(stg + rr * kStageRow + cc * 16);
+        for (int i = 0; i < 4; ++i) {
+          const int rr = i * 8 + q;
+          if (row0 + rr < M)
+            *reinterpret_cast<float4*>(out + (row0 + rr) * N + col0 + 16 * h + cc * 4) =
+                *reinterpret_cast<const float4*>(stg + rr * kStageRow + cc * 16);
+        }
+      } else if (col0 + 16 * h + (lane & 15) < N) {
+#pragma unroll 8
+        for (int rr = lane >> 4; rr < 32; rr += 2)
+          if (row0 + rr < M)
+            out[(row0 + rr) * N + col0 + 16 * h + (lane & 15)] =
+                reinterpret_cast<const OutT*>(stg + rr * kStageRow)[lane & 15];
       }
       __syncwarp();
     }
@@ -824,6 +831,35 @@ std::vector<at::Tensor> fp8_linear(const at::Tensor& x, const at::Tensor& b, con
   const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
   const auto q = fp8_quantize(x2, false, true, false, false);
   return multiply(q[0], q[1], b, sb, bias, act, f32, aux, x2.numel() > 0);
+}
+
+// A training step of a linear in two calls (the same steps as the functions above, without a
+// Python call for each): x [M, K], w [N, K], none of the sizes zero.
+// -> {y, pre-activation if asked for, x^T as blocks of tokens (need_w), w^T (need_x)}, codes and scales
+std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor& w,
+                                           const c10::optional<at::Tensor>& bias, int64_t act, bool aux, bool need_x,
+                                           bool need_w) {
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.numel() > 0 && w.numel() > 0,
+              "fp8_linear: x [M, K], w [N, K], not empty");
+  const auto wq = fp8_quantize(w, true, true, need_x, false);
+  const auto xq = fp8_quantize(x, false, true, need_w, false);
+  const auto y = multiply(xq[0], xq[1], wq[0], wq[1], bias, act, false, aux, true);
+  return {y[0], aux ? y[1] : at::Tensor(), xq[2], xq[3], wq[2], wq[3]};
+}
+
+// -> {dx [M, K], dw [N, K], db [N]} of g [M, N], those that are needed
+std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& g, const c10::optional<at::Tensor>& xc,
+                                            const c10::optional<at::Tensor>& xs, const c10::optional<at::Tensor>& wc,
+                                            const c10::optional<at::Tensor>& ws, bool need_b, bool dx_f32, bool dw_f32) {
+  const bool need_x = wc.has_value(), need_w = xc.has_value();
+  TORCH_CHECK(need_x || need_w, "fp8_linear: gradients of x or w");
+  const bool sums = need_b && need_x && need_w;
+  const auto q = fp8_quantize(g, false, need_x, need_w, sums);
+  std::vector<at::Tensor> out(3);
+  if (need_x) out[0] = multiply(q[0], q[1], *wc, *ws, c10::nullopt, 0, dx_f32, false, true)[0];
+  if (need_w) out[1] = multiply(q[2], q[3], *xc, *xs, c10::nullopt, 0, dw_f32, false, !need_x)[0];
+  if (sums) out[2] = q[4].sum(0);
+  return out;
 }
 
 }  // namespace osp

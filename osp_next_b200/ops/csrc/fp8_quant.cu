@@ -37,11 +37,33 @@ template <bool SEE_NAN> __device__ __forceinline__ uint32_t larger(uint32_t a, u
   return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
 }
 
+// N 32-bit words from any address that is a multiple of the element size: the aligned 16-byte groups
+// that hold them (each holds some of them, so none lies outside the allocation), shifted into
+// place.  Rows whose stride is not a multiple of 16 bytes read this way; element by element
+// they took several times as long.
+template <int N> __device__ __forceinline__ void load_shifted(const void* p, uint32_t* out) {
+  const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+  const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+  uint32_t w[N + 4];
+#pragma unroll
+  for (int i = 0; i <= N / 4; ++i) {
+    const uint4 u = i < N / 4 || o ? __ldg(g + i) : make_uint4(0, 0, 0, 0);
+    w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+  }
+#pragma unroll
+  for (int i = 0; i < N + 2; ++i) w[i] = o & 8u ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < N + 1; ++i) w[i] = o & 4u ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = o & 2u ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+}
+
 // 8 consecutive elements of a row as they are in memory (16 bytes of a 16-bit type, 32 of fp32);
 // maxima of 16-bit types are taken two at a time in packed registers.
 template <typename T> struct Piece {
   uint4 r;
   __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load_anywhere(const T* p) { load_shifted<4>(p, reinterpret_cast<uint32_t*>(&r)); }
   __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load_some(const T* p, int n) {
     uint16_t h[8];
@@ -102,6 +124,7 @@ template <> struct Piece<float> {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
+  __device__ __forceinline__ void load_anywhere(const float* p) { load_shifted<8>(p, reinterpret_cast<uint32_t*>(v)); }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
@@ -127,8 +150,12 @@ template <> struct Piece<float> {
 // The piece at column c of a row of K; zeros from column K on.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_piece(Piece<T>& o, const T* row, int c, int K) {
-  if (VEC && c + 8 <= K) o.load(row + c);
-  else o.load_some(row + c, K - c);
+  if (c + 8 <= K) {
+    if constexpr (VEC) o.load(row + c);
+    else o.load_anywhere(row + c);
+  } else {
+    o.load_some(row + c, K - c);
+  }
 }
 // ---------------------------------------------------------------------------- rows
 // A lane owns 16 consecutive columns, so 8 lanes own a block (3 shuffles for its maximum), a
@@ -225,10 +252,13 @@ quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
   const int c0 = kb * 128 + cl;
   const bool inner = (rb + 1) * 128L <= R && (kb + 1) * 128 <= K;      // a whole tile
   Piece<T> v[8];
-  if (VEC && inner) {
+  if (inner) {
     const T* p = x + r0 * ld + c0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i, p += ld) v[i].load(p);
+    for (int i = 0; i < 8; ++i, p += ld) {
+      if constexpr (VEC) v[i].load(p);
+      else v[i].load_anywhere(p);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

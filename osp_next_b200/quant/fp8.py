@@ -32,40 +32,43 @@ class _FP8LinearFn(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1])
         need_x, need_w = ctx.needs_input_grad[:2]
         # one read of x gives the forward operand and the one of dW; the same for W and dx
-        xq = ops.fp8_quantize(x2, layout="both" if need_w else "rows")
-        wq = ops.fp8_quantize(weight, block_rows=ops.fp8.BLOCK, layout="both" if need_x else "rows")
-        xr, xc = xq if need_w else (xq, None)
-        wr, wc = wq if need_x else (wq, None)
-        y = ops.fp8_matmul(xr, wr, bias, act, _out_dtype(x), aux=act is not None)
-        y, pre = y if act else (y, None)
-        ctx.save_for_backward(pre, *(t for q in (xc, wc) if q is not None for t in (q.data, q.scale)))
-        ctx.kept = [None if q is None else (q.rows, q.cols, q.block_rows) for q in (xc, wc)]
-        ctx.meta = (x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        if x.is_cuda and x2.numel() and weight.numel():
+            y, pre, *saved = ops.ext().fp8_linear_forward(x2, weight, bias, 1 if act else 0, act is not None, need_x,
+                                                          need_w)
+        else:
+            xr, xc = ops.fp8_quantize(x2, layout="both")
+            wr, wc = ops.fp8_quantize(weight, block_rows=ops.fp8.BLOCK, layout="both")
+            y, pre = ops.fp8_matmul(xr, wr, bias, act, _out_dtype(x), aux=True)
+            saved = [xc.data, xc.scale, wc.data, wc.scale]
+        ctx.save_for_backward(pre if act else None, *saved)
+        ctx.meta = (x.shape, x.dtype, weight.shape, weight.dtype, None if bias is None else bias.dtype)
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     def backward(ctx, gy):
         pre, *saved = ctx.saved_tensors
-        it = iter(saved)
-        xc, wc = [None if k is None else ops.Fp8Tensor(next(it), next(it), *k) for k in ctx.kept]
-        xshape, xdt, wdt, bdt = ctx.meta
+        xshape, xdt, wshape, wdt, bdt = ctx.meta
         g = gy.reshape(-1, gy.shape[-1])
         if pre is not None:
             g = _gelu_tanh_bwd(g, pre)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = dw = db = None
-        if need_x and need_w and need_b:
-            gr, gc, db = ops.fp8_quantize_with_sums(g)
-            db = db.to(bdt)
-        elif need_x or need_w:
-            gq = ops.fp8_quantize(g, layout="both" if need_x and need_w else "rows" if need_x else "cols")
-            gr, gc = gq if need_x and need_w else (gq, gq)
-        if need_x:
-            dx = ops.fp8_matmul(gr, wc, out_dtype=_grad_dtype(xdt)).to(xdt).view(xshape)
-        if need_w:
-            dw = ops.fp8_matmul(gc, xc, out_dtype=_grad_dtype(wdt)).to(wdt)
-        if need_b and db is None:
-            db = ops.bias_grad(g).to(bdt)
+        if need_x or need_w:
+            xdo, wdo = _grad_dtype(xdt), _grad_dtype(wdt)
+            if g.is_cuda and g.numel() and xshape[-1]:
+                dx, dw, db = ops.ext().fp8_linear_backward(g, *saved, need_b, xdo == torch.float32,
+                                                           wdo == torch.float32)
+            else:
+                gr, gc = ops.fp8_quantize(g, layout="both")
+                tokens, (N, K) = g.shape[0], wshape
+                if need_x:
+                    dx = ops.fp8_matmul(gr, ops.Fp8Tensor(saved[2], saved[3], K, N, ops.fp8.BLOCK), out_dtype=xdo)
+                if need_w:
+                    dw = ops.fp8_matmul(gc, ops.Fp8Tensor(saved[0], saved[1], K, tokens), out_dtype=wdo)
+            dx = None if dx is None else dx.to(xdt).view(xshape)
+            dw = None if dw is None else dw.to(wdt)
+        if need_b:
+            db = (ops.bias_grad(g) if db is None else db).to(bdt)
         return dx, dw, db, None
 
 
