@@ -15,7 +15,7 @@
 // the unrounded moments.
 //
 // It has to move 16 bytes per element with fp32 p and g and 8-bit moments (28 with fp32 ones); 177M
-// elements in 820 tensors take 556 us, 0.78 of the copy rate, held up by some 76 instructions
+// elements in 820 tensors take 499 us, 0.87 of the copy rate, held up by some 64 instructions
 // per element.  A warp takes 128 elements at a time, so the block maximum is one warp reduction
 // and each of its loads and stores is one contiguous segment.  The list travels in the kernel's
 // parameters (up to 32 KB): no table is copied or kept between calls.
@@ -35,7 +35,8 @@ namespace adamw8 {
 
 constexpr int kCap = 480;                 // tensors per launch: 480 x 64 B + constants < 32764 B
 constexpr int kSmallCap = 64;
-constexpr int kChunkBlocks = 16;          // 128-element runs per CTA visit (8 warps x 2)
+constexpr int kGroups = 512;              // steps of the table from a chunk to its tensor
+constexpr int kChunkBlocks = 32;          // 128-element runs per CTA (8 warps x 4)
 constexpr uint32_t kMix1 = 0x6A09E667u, kMix2 = 0xBB67AE85u, kMix3 = 0x3C6EF373u;   // fractions of sqrt 2, 3, 5
 
 // c1 = 1 - b1, c2 = 1 - b2, keep = 1 - lr wd, rate = lr / (1 - b1^t), inv_bc2s = 1 / sqrt(1 - b2^t): formed in
@@ -54,6 +55,8 @@ struct Args {
   int64_t n[CAP];
   int chunk_end[CAP];                     // chunks of tensors 0..i
   uint32_t key[CAP];
+  uint16_t group[kGroups + 1];            // tensor of chunk g << shift; the last tensor from the end on
+  int shift;
   int tensors;
   Consts c;
 };
@@ -292,20 +295,22 @@ template <typename PT, typename GT, bool STATE8> struct Lane {
   }
 };
 
-// One CTA per chunk of 16 blocks; a warp takes 2 neighbouring ones, with the loads of both in
-// flight.  Many short CTAs beat resident ones that loop over chunks: 64M elements took 172 us
-// this way, 209 to 227 in a loop (a warp's next loads there queue behind its byte-sized scale
-// stores), and dealing contiguous runs of chunks to resident CTAs with a register prefetch was
-// slower still.
+// One CTA per chunk of 32 blocks; a warp takes 4 neighbouring ones, with the loads of all in
+// flight (177M elements in 820 tensors, before the table of groups: 548 us, with 2 a warp 591).
+// Many short CTAs beat resident ones that loop over chunks: 64M elements took 172 us, 209 to 227
+// in a loop (a warp's next loads there queue behind its byte-sized scale stores), and dealing
+// contiguous runs of chunks to resident CTAs with a register prefetch was slower still.
 template <typename PT, typename GT, bool STATE8, int CAP>
-__global__ void __launch_bounds__(256, 4) step_kernel(const __grid_constant__ Args<CAP> args) {
+__global__ void __launch_bounds__(256, 3) step_kernel(const __grid_constant__ Args<CAP> args) {
   constexpr int U = kChunkBlocks / 8;
   grid_dependency_wait();
   allow_dependents();
   const Consts c = args.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunk = blockIdx.x;
-  int lo = 0, hi = args.tensors - 1;                 // first tensor with chunk < chunk_end
+  // first tensor with chunk < chunk_end: one of those that the chunk's group touches, mostly one or
+  // two (a search over the whole list: 177M elements in 820 tensors took 536 us, not 492)
+  int lo = args.group[chunk >> args.shift], hi = args.group[(chunk >> args.shift) + 1];
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (chunk < args.chunk_end[mid]) hi = mid;
@@ -367,6 +372,13 @@ static void run(const Lists& l, const Consts& consts, bool state8, uint32_t seed
   int64_t chunks = 0;
   auto flush = [&]() {
     if (a.tensors == 0) return;
+    a.shift = 0;
+    while ((chunks - 1) >> a.shift >= kGroups) ++a.shift;
+    const int groups = (int)((chunks - 1) >> a.shift) + 1;
+    for (int g = 0, t = 0; g <= groups; ++g) {
+      while (t < a.tensors - 1 && (int64_t)g << a.shift >= a.chunk_end[t]) ++t;
+      a.group[g] = (uint16_t)t;
+    }
     if (pf && gf) launch<float, float, CAP>(a, state8, stream);
     else if (pf) launch<float, __nv_bfloat16, CAP>(a, state8, stream);
     else if (gf) launch<__nv_bfloat16, float, CAP>(a, state8, stream);
