@@ -28,6 +28,13 @@ def _c(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
+def _vec(t, align: int):
+    """``t`` contiguous and from an address that is a multiple of ``align`` bytes, for kernels that
+    read vectors: a gradient from autograd can be a contiguous view that starts at any element."""
+    t = _c(t)
+    return t if t.data_ptr() % align == 0 else t.clone()
+
+
 # ----------------------------------------------------------------------------- norms
 
 def ln_modulate(x, shift, scale, eps: float = 1e-6):
@@ -221,15 +228,16 @@ def bias_grad(g):
     g2 = g.reshape(-1, g.shape[-1])
     if not _cuda(g2) or g2.shape[-1] % 8:
         return g2.float().sum(0)
-    g2 = _c(g2.to(_BF16))
+    g2 = _vec(g2.to(_BF16), 16)
     part = torch.empty((g2.shape[0] + 255) // 256, g2.shape[1], dtype=torch.float32, device=g2.device)
     ext().bias_grad(g2, part)
     return part.sum(0)
 
 
 def gelu_tanh_bwd(dh, pre):
+    pre = _vec(pre, 8)
     dpre = torch.empty_like(pre)
-    ext().gelu_tanh_bwd(_c(dh.to(_BF16)), _c(pre), dpre)
+    ext().gelu_tanh_bwd(_vec(dh.to(_BF16), 8), pre, dpre)
     return dpre
 
 

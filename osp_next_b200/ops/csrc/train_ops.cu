@@ -535,6 +535,8 @@ void gelu_tanh_bwd(const at::Tensor& dh, const at::Tensor& pre, at::Tensor& dpre
               dpre.scalar_type() == at::kBFloat16 && dh.is_contiguous() && pre.is_contiguous() &&
               dpre.is_contiguous() && dh.numel() == pre.numel() && dpre.numel() == pre.numel() &&
               pre.numel() % 4 == 0, "gelu_tanh_bwd: contiguous bf16 of equal size (multiple of 4)");
+  auto at8 = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0; };
+  TORCH_CHECK(at8(dh) && at8(pre) && at8(dpre), "gelu_tanh_bwd: tensors from 8-byte addresses");
   c10::cuda::CUDAGuard guard(dh.device());
   const long total4 = pre.numel() / 4;
   if (total4 == 0) return;
@@ -548,6 +550,7 @@ void gelu_tanh_bwd(const at::Tensor& dh, const at::Tensor& pre, at::Tensor& dpre
 void bias_grad(const at::Tensor& g, at::Tensor& part) {
   TORCH_CHECK(g.is_cuda() && g.scalar_type() == at::kBFloat16 && g.is_contiguous() && g.dim() == 2,
               "bias_grad: contiguous bf16 [M, N]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0, "bias_grad: g from a 16-byte address");
   const long M = g.size(0);
   const int N = (int)g.size(1);
   const long nchunk = (M + trn::kBiasRows - 1) / trn::kBiasRows;

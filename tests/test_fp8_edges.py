@@ -1,0 +1,89 @@
+"""Calls at the edges of the 8-bit operators: gradients that start at any address, empty sizes,
+second derivatives, weights that change after they were packed or frozen, long lists of tensors."""
+import pytest
+import torch
+
+from osp_next_b200 import ops
+from osp_next_b200.quant import fp8_linear
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _randn(*shape, device="cpu", seed=0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(device=device, dtype=dtype)
+
+
+# ----------------------------------------------------------------------------- addresses
+
+def test_vector_kernels_get_aligned_tensors(monkeypatch):
+    """A contiguous view that starts at any element reaches the kernels that read vectors of 4 and 8
+    bf16 as a copy from an aligned address, with the same values."""
+    seen = []
+
+    class Recorder:
+        def gelu_tanh_bwd(self, dh, pre, dpre):
+            seen.extend((t, 8) for t in (dh, pre, dpre))
+
+        def bias_grad(self, g, part):
+            seen.append((g, 16))
+    monkeypatch.setattr(ops, "ext", Recorder)
+    monkeypatch.setattr(ops, "_cuda", lambda *t: True)
+    flat = _randn(200, dtype=torch.bfloat16)
+    for start in range(9):
+        a, b = flat[start:start + 48].view(6, 8), flat[100 + start:148 + start].view(6, 8)
+        ops.gelu_tanh_bwd(a, b)
+        ops.bias_grad(a)
+        assert torch.equal(seen[-4][0], a) and torch.equal(seen[-3][0], b) and torch.equal(seen[-1][0], a)
+    assert all(t.is_contiguous() and t.data_ptr() % align == 0 for t, align in seen)
+    aligned = flat[:48].view(6, 8)
+    ops.bias_grad(aligned)
+    assert seen[-1][0].data_ptr() == aligned.data_ptr()          # no copy where none is needed
+
+
+def _gelu64(x):
+    return 0.5 * x * (1 + torch.tanh((2 / torch.pi) ** 0.5 * (x + 0.044715 * x ** 3)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_gelu_with_gradients_from_any_address(device):
+    """Two layers' outputs joined: the second's gradient is a contiguous view that starts 2 * 6 or
+    2 * 3 bytes into the joined one, of a multiple of four elements."""
+    for rows, n in (((1, 2), 6), ((1, 4), 3), ((3, 8), 5)):
+        xs = [_randn(r, 64, device=device, seed=r, dtype=torch.bfloat16).requires_grad_() for r in rows]
+        ws = [_randn(n, 64, device=device, seed=10 + i).div_(8).requires_grad_() for i in range(2)]
+        y = torch.cat([fp8_linear(x, w, act="gelu_tanh") for x, w in zip(xs, ws)])
+        dy = _randn(*y.shape, device=device, seed=3, dtype=torch.bfloat16)
+        got = torch.autograd.grad(y, xs, dy)
+        for x, w, d, g in zip(xs, ws, dy.split(rows), got):
+            wr, wc = ops.fp8_quantize(w, block_rows=128, layout="both")
+            pre = ops.fp8_matmul(x.detach(), wr, out_dtype=torch.float32).bfloat16().double().requires_grad_()
+            (dpre,) = torch.autograd.grad(_gelu64(pre), pre, d.double())
+            want = ops.fp8_quantize(dpre.bfloat16()).dequantize().double() @ wc.dequantize().double().t()
+            # a last bit of the derivative in bf16 can move its code by a step, at most 2^-3 of the value;
+            # a gradient read from another address is off by its own size
+            assert ((g.double() - want).norm() / want.norm()).item() < 2.0 ** -3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear_bias_gradient_from_any_address(device):
+    """The bias gradient of a layer without a weight gradient, from a gradient 2 bytes into its buffer."""
+    x = _randn(5, 32, device=device, dtype=torch.bfloat16)
+    w, b = _randn(16, 32, device=device), torch.zeros(16, device=device, requires_grad=True)
+    head = torch.zeros(1, device=device, dtype=torch.bfloat16, requires_grad=True)
+    y = torch.cat([head, fp8_linear(x, w, b).flatten()])
+    dy = _randn(*y.shape, device=device, seed=3, dtype=torch.bfloat16)
+    (got,) = torch.autograd.grad(y, [b], dy)
+    want = dy[1:].view(5, 16).double().sum(0)
+    assert bool(((got.double() - want).abs() <= 5 * 2.0 ** -24 * dy[1:].view(5, 16).double().abs().sum(0)).all())
+
+
+@pytest.mark.gpu
+def test_vector_kernels_refuse_other_addresses():
+    flat = torch.zeros(64, device="cuda", dtype=torch.bfloat16)
+    good, odd = flat[:32].view(4, 8), flat[1:33].view(4, 8)
+    for args in ((odd, good, good), (good, odd, good), (good, good, odd)):
+        with pytest.raises(RuntimeError):
+            ops.ext().gelu_tanh_bwd(*args)
+    with pytest.raises(RuntimeError):
+        ops.ext().bias_grad(odd, torch.zeros(1, 8, device="cuda"))
