@@ -387,7 +387,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
         for (int c = 0; c < PER; ++c) {
           const int col = nb * BN + (eg * PER + c) * 32 + lane;
-          sbias[c * 32 + lane] = col < args.N ? __ldg(args.bias + col) : 0.f;
+          sbias[c * 32 + lane] = col < args.N ? args.bias[col] : 0.f;
         }
         __syncwarp();
       }
@@ -629,7 +629,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ C
   const int quarter = warp & 3;
   const int local = quarter * 32 + lane;                 // row of the weight tile
   const int n = tile * 128 + local;
-  const float bias = (warp >= 2 && args.bias && n < args.N) ? __ldg(args.bias + n) : 0.f;
+  const float bias = (warp >= 2 && args.bias && n < args.N) ? args.bias[n] : 0.f;
   auto put = [&](int m, float v) {
     v += bias;
     const long o = (long)m * args.N + n;

@@ -47,7 +47,7 @@ template <int N> __device__ __forceinline__ void load_shifted(const void* p, uin
   uint32_t w[N + 4];
 #pragma unroll
   for (int i = 0; i <= N / 4; ++i) {
-    const uint4 u = i < N / 4 || o ? __ldg(g + i) : make_uint4(0, 0, 0, 0);
+    const uint4 u = i < N / 4 || o ? g[i] : make_uint4(0, 0, 0, 0);
     w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
   }
 #pragma unroll
@@ -62,7 +62,7 @@ template <int N> __device__ __forceinline__ void load_shifted(const void* p, uin
 // maxima of 16-bit types are taken two at a time in packed registers.
 template <typename T> struct Piece {
   uint4 r;
-  __device__ __forceinline__ void load(const T* p) { r = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void load_anywhere(const T* p) { load_shifted<4>(p, reinterpret_cast<uint32_t*>(&r)); }
   __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load_some(const T* p, int n) {
@@ -120,7 +120,7 @@ template <typename T> struct Piece {
 template <> struct Piece<float> {
   float v[8];
   __device__ __forceinline__ void load(const float* p) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
@@ -162,9 +162,8 @@ __device__ __forceinline__ void load_piece(Piece<T>& o, const T* row, int c, int
 // lane's codes are one 16-byte store and a warp's four scales one 4-byte word.  A warp takes two
 // such runs of 512 columns, with the loads of both in flight.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q,
-                                                            uint8_t* __restrict__ scale, int R, int K, int Kp,
-                                                            int kgroups, long total) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long ld, uint8_t* q, uint8_t* scale, int R,
+                                                            int K, int Kp, int kgroups, long total) {
   grid_dependency_wait();
   allow_dependents();
   const int lane = threadIdx.x & 31;
@@ -235,9 +234,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // step, without another read of x).
 template <typename T, bool VEC, bool TILE_SCALE, bool ROWS, bool COLS, bool SUMS>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
-quantize_tiles_kernel(const T* __restrict__ x, long ld, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
-                      uint8_t* __restrict__ qt, uint8_t* __restrict__ scale_t, float* __restrict__ part, int R, int K,
-                      int Kp, int Rp) {
+quantize_tiles_kernel(const T* x, long ld, uint8_t* q, uint8_t* scale, uint8_t* qt, uint8_t* scale_t, float* part,
+                      int R, int K, int Kp, int Rp) {
   __shared__ uint32_t top[2][4][128];              // [0]: rows over 2 warps, [1]: columns over 4
   __shared__ __align__(16) float factor[2][128];
   __shared__ float sums[SUMS ? 4 : 1][128];

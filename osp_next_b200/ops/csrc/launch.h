@@ -5,7 +5,10 @@
 //
 // Every kernel launched this way calls grid_dependency_wait() in every thread before that thread
 // touches global memory, and allow_dependents() after it: a kernel that starts early behind it
-// then knows that everything before the two of them has completed.
+// then knows that everything before the two of them has completed.  Such a kernel reads its inputs
+// by plain loads: a load through the read-only path promises data that nobody writes while the
+// kernel runs, which is not so before the wait, and the compiler need not keep it behind the wait.
+// So no read-only intrinsic and no restrict-qualified pointer, from which the compiler infers one.
 //
 // The wait costs a block time of its own even when there is nothing to wait for: a grid of
 // thousands of short blocks loses more than it gains (quantising 20161 x 5120 before a product of

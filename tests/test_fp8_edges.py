@@ -1,5 +1,9 @@
 """Calls at the edges of the 8-bit operators: gradients that start at any address, empty sizes,
 second derivatives, weights that change after they were packed or frozen, long lists of tensors."""
+import glob
+import os
+import re
+
 import pytest
 import torch
 
@@ -87,3 +91,20 @@ def test_vector_kernels_refuse_other_addresses():
             ops.ext().gelu_tanh_bwd(*args)
     with pytest.raises(RuntimeError):
         ops.ext().bias_grad(odd, torch.zeros(1, 8, device="cuda"))
+
+
+# ----------------------------------------------------------------------------- loads and launches
+
+def _csrc():
+    return os.path.join(os.path.dirname(ops.__file__), "csrc")
+
+
+def test_kernels_that_start_early_have_no_read_only_loads():
+    """A kernel launched while the one before it runs must not read through the read-only path: its
+    inputs may still be written, and such loads are not held behind the wait."""
+    early = [f for f in glob.glob(os.path.join(_csrc(), "*.cu")) if "launch_kernel(" in open(f).read()]
+    assert {os.path.basename(f) for f in early} >= {"fp8_gemm.cu", "fp8_quant.cu", "adamw_multi.cu"}
+    shared = [os.path.join(_csrc(), h) for h in ("common.cuh", "fp8.cuh", "launch.h")]
+    for f in early + shared:
+        code = re.sub(r"//[^\n]*", "", open(f).read())
+        assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict", code), os.path.basename(f)
