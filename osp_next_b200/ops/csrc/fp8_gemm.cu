@@ -489,7 +489,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// Every warp of the cluster's CTAs arrives converged (the barrier is of the aligned form, and the
+// code before it may have left a warp's lanes apart).
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Four floats at `p` in this CTA's shared memory, read from CTA `rank` of the cluster.

@@ -108,3 +108,29 @@ def test_kernels_that_start_early_have_no_read_only_loads():
     for f in early + shared:
         code = re.sub(r"//[^\n]*", "", open(f).read())
         assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict", code), os.path.basename(f)
+
+
+def test_cluster_barriers_are_reached_converged():
+    """``barrier.cluster`` in its aligned form is undefined for a warp whose lanes are apart."""
+    found = 0
+    for f in glob.glob(os.path.join(_csrc(), "*.cu")) + glob.glob(os.path.join(_csrc(), "*.cuh")):
+        code = re.sub(r"//[^\n]*", "", open(f).read())
+        for m in re.finditer(r"asm volatile\(\s*\"barrier\.cluster\.arrive\.[a-z.]*aligned", code):
+            assert code[:m.start()].rstrip().endswith("__syncwarp();"), os.path.basename(f)
+            found += 1
+    assert found
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 6, 13, 33, 64])
+@pytest.mark.parametrize("N", [1, 100, 129, 1000])
+def test_split_products_of_ragged_tiles(M, N):
+    """Few rows over a K split on a cluster, where a warp's last lanes have no column of the result.
+    Small integers: every sum is exact, whatever its order."""
+    g = torch.Generator().manual_seed(M + N)
+    x = torch.randint(-4, 5, (M, 4096), generator=g).to(device="cuda", dtype=torch.bfloat16)
+    w = torch.randint(-4, 5, (N, 4096), generator=g).to(device="cuda", dtype=torch.float32)
+    want = x.double() @ w.double().t()
+    y = ops.fp8_matmul(x, ops.fp8_quantize(w, block_rows=128), out_dtype=torch.float32)
+    assert torch.equal(y.double(), want)
+    ops.check_device_errors()
