@@ -135,6 +135,16 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
+        if not self.multi_tensor:
+            return
+        # torch casts the state to the parameter's type; the moments of 16-bit parameters are taken
+        # from the checkpoint again, as they were saved
+        numbers = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(numbers, (p for g in self.param_groups for p in g["params"])):
+            st = self.state.get(p, {})
+            for k in ("exp_avg", "exp_avg_sq"):
+                if k in st and st[k].dtype != torch.float32:
+                    st[k] = state_dict["state"][i][k].to(device=st[k].device, dtype=torch.float32)
         if self.state_bits != 8:
             return
         for p, st in self.state.items():

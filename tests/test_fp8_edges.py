@@ -1,5 +1,6 @@
 """Calls at the edges of the 8-bit operators: gradients that start at any address, empty sizes,
 second derivatives, weights that change after they were packed or frozen, long lists of tensors."""
+import copy
 import glob
 import os
 import re
@@ -8,6 +9,7 @@ import pytest
 import torch
 
 from osp_next_b200 import ops
+from osp_next_b200.parallel.optim import FusedAdamW
 from osp_next_b200.quant import fp8_linear
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -134,3 +136,68 @@ def test_split_products_of_ragged_tiles(M, N):
     y = ops.fp8_matmul(x, ops.fp8_quantize(w, block_rows=128), out_dtype=torch.float32)
     assert torch.equal(y.double(), want)
     ops.check_device_errors()
+
+
+# ----------------------------------------------------------------------------- optimizer
+
+def _trained(device, dtype, steps, **kw):
+    torch.manual_seed(0)
+    params = [torch.nn.Parameter(torch.randn(n, device=device).to(dtype)) for n in (300, 7)]
+    opt = FusedAdamW([{"params": params[:1]}, {"params": params[1:], "lr": 1e-3}], lr=1e-2, **kw)
+    _steps(params, opt, 0, steps)
+    return params, opt
+
+
+def _steps(params, opt, first, n):
+    for i in range(first, first + n):
+        for j, p in enumerate(params):
+            p.grad = 1e-3 * _randn(*p.shape, device=p.device, seed=100 * i + j, dtype=p.dtype)
+        opt.step()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("save_bits", [8, 32])
+@pytest.mark.parametrize("load_bits", [8, 32])
+def test_checkpoints_keep_fp32_moments_of_16_bit_parameters(device, dtype, save_bits, load_bits):
+    params, opt = _trained(device, dtype, 3, multi_tensor=True, state_bits=save_bits)
+    sd = copy.deepcopy(opt.state_dict())
+    saved = [dict(sd["state"][i]) for i in range(2)]
+    assert all(st[k].dtype == torch.float32 for st in saved for k in ("exp_avg", "exp_avg_sq"))
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    again = FusedAdamW([{"params": twins[:1]}, {"params": twins[1:]}], multi_tensor=True, state_bits=load_bits)
+    again.load_state_dict(copy.deepcopy(sd))
+    for p, st in zip(twins, saved):
+        got = again.state[p]
+        assert got["step"] == st["step"] == 3
+        if load_bits == 32:
+            assert all(torch.equal(got[k], st[k]) and got[k].dtype == torch.float32 for k in ("exp_avg", "exp_avg_sq"))
+        else:
+            m, v = ops.adamw8_decode(*(got[k] for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")))
+            # to the nearest of 3 mantissa bits (2^-4), or of the subnormal step: of the block's largest 2^-9 / 224
+            # below for m, 2^-17 / 2^15 for v, which keeps a positive value positive
+            for a, b, floor in ((m, st["exp_avg"], 2.0 ** -16), (v, st["exp_avg_sq"], 2.0 ** -30)):
+                assert bool(((a - b).abs() <= 2.0 ** -4 * b.abs() + floor * b.abs().max()).all())
+                # the same values again where they were 8-bit ones
+                assert save_bits == 32 or torch.equal(a, b)
+    _steps(params, opt, 3, 1)
+    _steps(twins, again, 3, 1)
+    if load_bits == save_bits == 32:                 # as if there had been no break
+        assert all(torch.equal(p, q) for p, q in zip(params, twins))
+    assert all(bool(q.isfinite().all()) for q in twins)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_per_tensor_moments_of_16_bit_parameters_load_into_lists(device):
+    """The per-tensor form keeps moments in the parameter's type: they come back in fp32."""
+    if device == "cuda":
+        pytest.skip("the per-tensor kernel takes fp32 parameters")
+    params, opt = _trained(device, torch.bfloat16, 2)
+    assert opt.state[params[0]]["exp_avg"].dtype == torch.bfloat16
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    again = FusedAdamW([{"params": twins[:1]}, {"params": twins[1:]}], multi_tensor=True)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for p, q in zip(params, twins):
+        assert again.state[q]["exp_avg"].dtype == torch.float32
+        assert torch.equal(again.state[q]["exp_avg"], opt.state[p]["exp_avg"].float())
+    _steps(twins, again, 2, 1)
