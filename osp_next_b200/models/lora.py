@@ -244,6 +244,8 @@ class LoraModel(nn.Module):
                 if isinstance(child, LoraLinear):
                     base = child.base_layer
                     base.weight.copy_(child.merged_weight())
+                    if getattr(base, "is_fp8", False):
+                        base.refreeze_weight()
                     setattr(mod, cname, base)
         return model
 

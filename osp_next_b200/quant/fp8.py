@@ -117,6 +117,10 @@ class FP8Linear(nn.Linear):
         self._frozen = self._pack = None
         return self
 
+    def refreeze_weight(self):
+        """After a change of the weight: a frozen layer quantises it again, another stays as it is."""
+        return self if self._frozen is None else self.freeze_weight()
+
     def train(self, mode: bool = True):
         if mode:
             self.thaw_weight()

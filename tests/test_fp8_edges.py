@@ -9,8 +9,9 @@ import pytest
 import torch
 
 from osp_next_b200 import ops
+from osp_next_b200.models.lora import LoraModel
 from osp_next_b200.parallel.optim import FusedAdamW
-from osp_next_b200.quant import fp8_linear
+from osp_next_b200.quant import FP8Linear, fp8_linear, fp8_multi_linear, freeze_fp8_weights
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -201,3 +202,35 @@ def test_per_tensor_moments_of_16_bit_parameters_load_into_lists(device):
         assert again.state[q]["exp_avg"].dtype == torch.float32
         assert torch.equal(again.state[q]["exp_avg"], opt.state[p]["exp_avg"].float())
     _steps(twins, again, 2, 1)
+
+
+# ----------------------------------------------------------------------------- weights that change
+
+class _Projections(torch.nn.Module):
+    def __init__(self, device):
+        super().__init__()
+        self.q, self.k = FP8Linear(64, 128, device=device), FP8Linear(64, 128, device=device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("frozen", [True, False])
+def test_merging_an_adapter_into_fp8_layers(device, frozen):
+    """The merged layers are those of the merged weights, frozen before or not, also stacked."""
+    torch.manual_seed(0)
+    lora = LoraModel(_Projections(device), r=4, lora_alpha=8.0, target_modules=["k"])
+    net = lora.base_model.model
+    x = _randn(3, 64, device=device, dtype=torch.bfloat16)
+    if frozen:
+        freeze_fp8_weights(net)
+        with torch.no_grad():
+            fp8_multi_linear(x, (net.q, net.k.base_layer))         # a stack of the weights as they are
+    with torch.no_grad():
+        net.k.lora_B["default"].weight.normal_()
+        want_k = net.k.merged_weight()
+        before = net.q(x)
+        merged = lora.merge_and_unload()
+        assert type(merged.k) is FP8Linear and torch.equal(merged.k.weight, want_k)
+        assert (merged.k._frozen is not None) == frozen
+        want = ops.fp8_matmul(x, ops.fp8_quantize(want_k, block_rows=128), merged.k.bias, out_dtype=merged.k(x).dtype)
+        assert torch.equal(merged.k(x), want) and torch.equal(merged.q(x), before)
+        assert torch.equal(fp8_multi_linear(x, (merged.q, merged.k)), torch.cat([before, want], -1))
