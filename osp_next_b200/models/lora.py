@@ -251,11 +251,15 @@ class LoraModel(nn.Module):
 
 
 # ---------------------------------------------------------------------------- fused inference path
-_PACK_CACHE: Dict[tuple, tuple] = {}
-
-
-def _key(ts):
-    return tuple((t.data_ptr(), t._version) for t in ts if t is not None)
+def _packed(mods, slot, ts, build):
+    """What ``build`` makes of the tensors ``ts`` of ``mods``: kept with the first of them until one
+    of the tensors changes (an optimizer step replaces what it made out of date)."""
+    key = tuple((t.data_ptr(), t._version) for t in ts if t is not None)
+    packs = mods[0].__dict__.setdefault("_packs", {})
+    hit = packs.get(slot)
+    if hit is None or hit[0] != key:
+        hit = packs[slot] = (key, build())
+    return hit[1]
 
 
 def fused_lora_operands(mods, x2d: torch.Tensor):
@@ -268,24 +272,18 @@ def fused_lora_operands(mods, x2d: torch.Tensor):
     from .. import ops
     base = [m.base_layer if isinstance(m, LoraLinear) else m for m in mods]
     lora = [m for m in mods if isinstance(m, LoraLinear) and not m.disabled]
-    wkey = ("w",) + _key([b.weight for b in base] + [b.bias for b in base])
-    hit = _PACK_CACHE.get(wkey)
-    if hit is None:
+
+    def base_operands():
         W = torch.cat([b.weight.detach() for b in base], 0).to(torch.bfloat16).contiguous() if len(base) > 1 \
             else base[0].weight.detach().to(torch.bfloat16).contiguous()
         bs = [b.bias for b in base]
-        bias = torch.cat([b.detach().float() for b in bs], 0).contiguous() if all(b is not None for b in bs) else None
-        hit = (W, bias)
-        if len(_PACK_CACHE) > 512:
-            _PACK_CACHE.clear()
-        _PACK_CACHE[wkey] = hit
-    W, bias = hit
+        return W, torch.cat([b.detach().float() for b in bs], 0).contiguous() if all(b is not None for b in bs) else None
+    W, bias = _packed(mods, ("w",) + tuple(id(b) for b in base), [b.weight for b in base] + [b.bias for b in base],
+                      base_operands)
     if not lora:
         return W, bias, None
-    akey = ("a",) + tuple(id(m) for m in mods) + _key([m.lora_A[m.adapter].weight for m in lora] +
-                                                      [m.lora_B[m.adapter].weight for m in lora])
-    hit = _PACK_CACHE.get(akey)
-    if hit is None:
+
+    def branch_operands():
         A = torch.cat([m.lora_A[m.adapter].weight.detach() for m in lora], 0).to(torch.bfloat16).contiguous()
         rs = sum(m.r for m in lora)
         Bd = torch.zeros(W.shape[0], rs, dtype=torch.bfloat16, device=W.device)
@@ -297,8 +295,9 @@ def fused_lora_operands(mods, x2d: torch.Tensor):
                     torch.bfloat16)
                 col += m.r
             row += n_out
-        hit = (A, Bd)
-        _PACK_CACHE[akey] = hit
-    A, Bd = hit
+        return A, Bd
+    A, Bd = _packed(mods, ("a",) + tuple((id(m), isinstance(m, LoraLinear) and not m.disabled) for m in mods),
+                    [m.lora_A[m.adapter].weight for m in lora] + [m.lora_B[m.adapter].weight for m in lora],
+                    branch_operands)
     a2 = ops.linear(x2d, A, None)
     return W, bias, (a2, Bd)

@@ -357,6 +357,11 @@ static void launch(const Args<CAP>& a, bool state8, cudaStream_t stream) {
   launch_kernel(state8 ? step_kernel<PT, GT, true, CAP> : step_kernel<PT, GT, false, CAP>, grid, 256, 0, 1, stream, a);
 }
 
+// An in-place write that autograd's version counter sees, as one by a torch function does.
+static void count_write(const at::Tensor* t) {
+  if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 using Ptrs = std::vector<const at::Tensor*>;
 struct Lists {
   const Ptrs &p, &g, &m, &v, &ms, &vs;
@@ -455,6 +460,8 @@ void adamw_multi(const std::vector<const at::Tensor*>& p, const std::vector<cons
   // a short list has a small parameter block: 4 KB instead of 30 KB to copy with the launch
   if (count <= kSmallCap) run<kSmallCap>(lists, c, state8, (uint32_t)seed, stream);
   else run<kCap>(lists, c, state8, (uint32_t)seed, stream);
+  for (const Ptrs* written : {&p, &m, &v, &ms, &vs})
+    for (const at::Tensor* t : *written) count_write(t);
 }
 
 }  // namespace osp

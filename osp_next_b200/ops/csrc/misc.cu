@@ -282,6 +282,9 @@ void adamw(at::Tensor& p, const at::Tensor& g, at::Tensor& m, at::Tensor& v, dou
                                              v.data_ptr<float>(), n, (float)lr, (float)b1, (float)b2, (float)eps,
                                              (float)wd, bc1, bc2s, (float)gscale);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  // an in-place write that autograd's version counter sees, as one by a torch function does
+  for (const at::Tensor* t : {&p, &m, &v})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 // ------------------------------------------------------------------------------------ GRPO SDE

@@ -57,7 +57,7 @@ class FSDPEMAModel:
     def ema_copy_to_model(self, model):
         for n, p in model.named_parameters():
             if n in self.shadow_params:
-                p.data.copy_(self.shadow_params[n].data)
+                p.detach().copy_(self.shadow_params[n].data)     # counted in p._version, unlike .data
 
     @torch.no_grad()
     def model_copy_to_ema(self, model):
@@ -72,5 +72,5 @@ class FSDPEMAModel:
     def restore(self, model):
         for n, p in model.named_parameters():
             if n in self.backup:
-                p.data.copy_(self.backup[n].data)
+                p.detach().copy_(self.backup[n].data)
         self.backup = {}

@@ -10,6 +10,9 @@ One launch per parameter shard by default; ``multi_tensor=True`` updates all of 
 few launches (``ops.adamw_multi_``).  ``state_bits=8`` keeps both moments in 8 bits, a quarter
 of the optimizer's memory (2.03 bytes per parameter for 8), and implies ``multi_tensor``.
 Checkpoints hold fp32 moments either way, so a run can change ``state_bits`` on resume.
+
+A step counts as an in-place change of each parameter (``_version``, through ``detach()``; ``.data``
+would hide it), as with torch's optimizers: what was packed from the old weights is built anew.
 """
 from __future__ import annotations
 
@@ -63,7 +66,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 st = self.state[p]
-                lp, lg = _local(p.data), _local(p.grad)
+                lp, lg = _local(p.detach()), _local(p.grad)
                 if not st:
                     st["step"] = torch.tensor(0.0)
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -104,7 +107,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 st["step"] = torch.tensor(0.0)
                 st.update(self._init_state(p))
             st["step"] += 1
-            lp, lg = _local(p.data), _local(p.grad)
+            lp, lg = _local(p.detach()), _local(p.grad)
             if not lp.is_contiguous():
                 raise ValueError("multi_tensor: parameters have to be contiguous")
             if lg.dtype not in (torch.float32, torch.bfloat16):

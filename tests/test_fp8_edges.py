@@ -9,7 +9,9 @@ import pytest
 import torch
 
 from osp_next_b200 import ops
-from osp_next_b200.models.lora import LoraModel
+from osp_next_b200.models.lora import LoraModel, inject_lora
+from osp_next_b200.models.osp_next import OSPNextModel
+from osp_next_b200.parallel.ema import FSDPEMAModel
 from osp_next_b200.parallel.optim import FusedAdamW
 from osp_next_b200.quant import FP8Linear, fp8_linear, fp8_multi_linear, freeze_fp8_weights
 
@@ -234,3 +236,76 @@ def test_merging_an_adapter_into_fp8_layers(device, frozen):
         want = ops.fp8_matmul(x, ops.fp8_quantize(want_k, block_rows=128), merged.k.bias, out_dtype=merged.k(x).dtype)
         assert torch.equal(merged.k(x), want) and torch.equal(merged.q(x), before)
         assert torch.equal(fp8_multi_linear(x, (merged.q, merged.k)), torch.cat([before, want], -1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kw", [{}, {"multi_tensor": True}, {"state_bits": 8}])
+def test_an_optimizer_step_counts_as_a_change_of_the_weights(device, kw):
+    """What is packed from weights looks at their version; torch's optimizers advance it, so do these."""
+    params = [torch.nn.Parameter(torch.ones(n, device=device)) for n in (300, 5)]
+    opt = FusedAdamW(params, lr=1e-2, **kw)
+    for _ in range(2):
+        before = [(p._version, p.detach().clone()) for p in params]
+        for p in params:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        assert all(p._version > v and not torch.equal(p.detach(), old) for p, (v, old) in zip(params, before))
+    ema = FSDPEMAModel(torch.nn.ParameterList(params))
+    start = [p._version for p in params]
+    ema.store(torch.nn.ParameterList(params))
+    ema.ema_copy_to_model(torch.nn.ParameterList(params))
+    swapped = [p._version for p in params]
+    ema.restore(torch.nn.ParameterList(params))
+    assert all(a < b < p._version for a, b, p in zip(start, swapped, params))
+
+
+@pytest.mark.gpu
+def test_list_step_counts_as_a_change_of_all_its_tensors():
+    p, g = [torch.ones(300, device="cuda")], [torch.ones(300, device="cuda")]
+    state = [[t] for t in ops.adamw8_state(p[0])]
+    versions = [x[0]._version for x in (p, g, *state)]
+    ops.adamw_multi_(p, g, *state, lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, step=1)
+    after = [x[0]._version for x in (p, g, *state)]
+    assert after[1] == versions[1]
+    assert all(a > b for i, (a, b) in enumerate(zip(after, versions)) if i != 1)
+    with torch.inference_mode():                     # tensors without a version
+        q = [torch.ones(300, device="cuda")]
+        ops.adamw_multi_(q, [torch.ones_like(q[0])], [torch.zeros_like(q[0])], [torch.zeros_like(q[0])], lr=1e-2,
+                         beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, step=1)
+        assert bool((q[0] < 1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{}, {"multi_tensor": True}, {"state_bits": 8}])
+@pytest.mark.parametrize("lora", [False, True])
+def test_no_grad_outputs_follow_the_optimizer(kw, lora):
+    """Packed q/k/v weights and folded adapters are those of the weights as they are: outputs equal
+    those of a model built from a copy of the weights."""
+    torch.manual_seed(0)
+
+    def build():
+        with torch.device("cuda"):
+            m = OSPNextModel(dim=256, ffn_dim=512, num_heads=2, num_layers=2, text_len=16,
+                             skiparse_model_type="dual_end", sparse_ratio=2, num_full_blocks=0)
+        if lora:
+            inject_lora(m, 4, 4.0, ["self_attn.q", "self_attn.k", "self_attn.v", "self_attn.o", "ffn.0", "ffn.2"])
+        return m
+    model = build()
+    torch.nn.init.normal_(model.head.head.weight, std=0.02)
+    params = [p for n, p in model.named_parameters() if not lora or "lora_" in n]
+    opt = FusedAdamW(params, lr=3e-2, **kw)
+    g = torch.Generator().manual_seed(1)
+    x, t, ctx = (torch.randn(1, 16, 3, 16, 16, generator=g).cuda(), torch.tensor([500.0], device="cuda"),
+                 torch.randn(1, 16, 4096, generator=g).cuda())
+    with torch.no_grad():
+        first = model(x, t, ctx)
+    for step in range(2):
+        for i, p in enumerate(params):
+            p.grad = _randn(*p.shape, device="cuda", seed=10 * step + i, dtype=p.dtype)
+        opt.step()
+        twin = build()
+        twin.load_state_dict(copy.deepcopy(model.state_dict()))
+        with torch.no_grad():
+            y = model(x, t, ctx)
+            assert torch.equal(y, twin(x, t, ctx)) and not torch.equal(y, first)
+    assert len(getattr(model.blocks[0].self_attn.q, "_packs", {})) <= 2          # nothing of the old weights is kept
