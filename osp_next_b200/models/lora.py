@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as Fn
+from ..utils.weights import weights_key
 
 
 class LoraLinear(nn.Module):
@@ -254,7 +255,7 @@ class LoraModel(nn.Module):
 def _packed(mods, slot, ts, build):
     """What ``build`` makes of the tensors ``ts`` of ``mods``: kept with the first of them until one
     of the tensors changes (an optimizer step replaces what it made out of date)."""
-    key = tuple((t.data_ptr(), t._version) for t in ts if t is not None)
+    key = weights_key(ts)
     packs = mods[0].__dict__.setdefault("_packs", {})
     hit = packs.get(slot)
     if hit is None or hit[0] != key:

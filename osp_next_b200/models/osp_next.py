@@ -30,6 +30,7 @@ import torch.nn as nn
 import torch.utils.checkpoint
 
 from ..utils.profiling import nvtx_range
+from ..utils.weights import weights_key
 from . import functional as Fn
 from .layout import (FULL, GROUP, TOKEN, ParallelSpec, TokenLayout, block_schedule,
                      make_layout, make_redistribution, token_positions)
@@ -119,7 +120,7 @@ class OSPNextSelfAttention(nn.Module):
     def packed_qkv(self):
         ws = (self.q.weight, self.k.weight, self.v.weight)
         bs = (self.q.bias, self.k.bias, self.v.bias)
-        key = tuple((t.data_ptr(), t._version) for t in ws + bs)
+        key = weights_key(ws + bs)
         if self._packed is None or self._packed[0] != key:
             W = torch.cat([w.detach() for w in ws], 0).to(torch.bfloat16).contiguous()
             b = torch.cat([x.detach() for x in bs], 0).float().contiguous()

@@ -10,6 +10,8 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from ..utils.weights import weights_changed
+
 
 def _local(t):
     return t.to_local() if hasattr(t, "to_local") else t
@@ -58,6 +60,7 @@ class FSDPEMAModel:
         for n, p in model.named_parameters():
             if n in self.shadow_params:
                 p.detach().copy_(self.shadow_params[n].data)     # counted in p._version, unlike .data
+        weights_changed()
 
     @torch.no_grad()
     def model_copy_to_ema(self, model):
@@ -73,4 +76,5 @@ class FSDPEMAModel:
         for n, p in model.named_parameters():
             if n in self.backup:
                 p.detach().copy_(self.backup[n].data)
+        weights_changed()
         self.backup = {}

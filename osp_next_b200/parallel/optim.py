@@ -22,6 +22,7 @@ import torch
 
 from .. import ops
 from ..ops import reference as ref
+from ..utils.weights import weights_changed
 
 
 def _local(t):
@@ -86,6 +87,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     bc2 = 1 - b2 ** step
                     denom = (v.sqrt() / (bc2 ** 0.5)).add_(group["eps"])
                     lp.addcdiv_(m, denom, value=-group["lr"] / bc1)
+        weights_changed()
         return loss
 
     # ------------------------------------------------------------------ lists of tensors

@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..ops import reference as ref
+from ..utils.weights import weights_key
 
 
 def _out_dtype(dt: torch.dtype) -> torch.dtype:
@@ -146,7 +147,7 @@ def hif8_multi_linear(x, linears, act=None):
         if len(linears) == 1:
             w_q = l0._cached_wq()
         else:                        # packed quantised weights, rebuilt when any weight changes
-            key = tuple((m.weight.data_ptr(), m.weight._version) for m in linears)
+            key = weights_key(m.weight for m in linears)
             hit = getattr(l0, "_packed_wq", None)
             if hit is None or hit[0] != key:
                 hit = (key, torch.cat([m._cached_wq() for m in linears], 0))
@@ -173,7 +174,7 @@ class HIF8Linear(nn.Linear):
         self._wq = None
 
     def _cached_wq(self):
-        key = (self.weight.data_ptr(), self.weight._version)
+        key = weights_key((self.weight,))
         if self._wq is None or self._wq[0] != key:
             self._wq = (key, quant(self.weight.detach(), self.scale_max_forward).to(torch.bfloat16))
         return self._wq[1]

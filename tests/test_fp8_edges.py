@@ -9,11 +9,12 @@ import pytest
 import torch
 
 from osp_next_b200 import ops
-from osp_next_b200.models.lora import LoraModel, inject_lora
+from osp_next_b200.models.lora import LoraLinear, LoraModel, fused_lora_operands, inject_lora
 from osp_next_b200.models.osp_next import OSPNextModel
 from osp_next_b200.parallel.ema import FSDPEMAModel
 from osp_next_b200.parallel.optim import FusedAdamW
-from osp_next_b200.quant import FP8Linear, fp8_linear, fp8_multi_linear, freeze_fp8_weights
+from osp_next_b200.quant import (FP8Linear, HIF8Linear, fp8_linear, fp8_multi_linear, freeze_fp8_weights,
+                                 hif8_multi_linear)
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -309,3 +310,45 @@ def test_no_grad_outputs_follow_the_optimizer(kw, lora):
             y = model(x, t, ctx)
             assert torch.equal(y, twin(x, t, ctx)) and not torch.equal(y, first)
     assert len(getattr(model.blocks[0].self_attn.q, "_packs", {})) <= 2          # nothing of the old weights is kept
+
+
+def test_packs_of_gathered_weights_follow_the_optimizer():
+    """FSDP writes the weights that it gathers without advancing their version, often where they
+    were before: an optimizer step and a swap of averaged weights count by themselves."""
+    layer = LoraLinear(torch.nn.Linear(64, 32), r=4, alpha=8.0)
+    shard = torch.nn.ParameterList([torch.nn.Parameter(torch.ones(4))])
+    opt, ema, x = FusedAdamW(shard, lr=1e-2), FSDPEMAModel(shard), _randn(3, 64)
+
+    def gathered():                                  # the same memory, the same version, other values
+        w = layer.lora_B["default"].weight
+        at = w.data_ptr(), w._version
+        w.data.normal_()
+        layer.base_layer.weight.data.normal_()
+        assert (w.data_ptr(), w._version) == at
+
+    def check():
+        W, _, (_, B) = fused_lora_operands([layer], x)
+        assert torch.equal(W, layer.base_layer.weight.detach().bfloat16())
+        assert torch.equal(B, (2 * layer.lora_B["default"].weight.detach()).bfloat16())
+        return W
+    check()
+    for write in (opt.step, lambda: ema.ema_copy_to_model(shard), lambda: ema.restore(shard)):
+        shard[0].grad = torch.ones(4)
+        write()
+        gathered()
+        W = check()
+        assert check() is W                          # and kept as long as nothing changes
+
+
+@pytest.mark.gpu
+def test_hif8_copies_of_gathered_weights_follow_the_optimizer():
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    opt = FusedAdamW([p])
+    layer, x = HIF8Linear(64, 32, bias=False, device="cuda"), _randn(3, 64, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        for f in (layer, lambda v: hif8_multi_linear(v, (layer, layer))):
+            before = f(x)
+            p.grad = torch.ones_like(p)
+            opt.step()
+            layer.weight.data.neg_()
+            assert torch.equal(f(x), -before) and bool(before.any())
