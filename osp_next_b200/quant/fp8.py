@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -45,6 +46,7 @@ class _FP8LinearFn(torch.autograd.Function):
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy):
         pre, *saved = ctx.saved_tensors
         xshape, xdt, wshape, wdt, bdt = ctx.meta
@@ -88,7 +90,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     x [..., K] and weight [N, K] in bf16, fp16 or fp32, bias [N]; act None or ``"gelu_tanh"``.
     Both operands are quantised in the call (a weight that does not change is better kept as
-    ``ops.fp8_quantize(weight, block_rows=128)`` for ``ops.fp8_matmul``)."""
+    ``ops.fp8_quantize(weight, block_rows=128)`` for ``ops.fp8_matmul``).  First derivatives only:
+    differentiating a gradient again raises."""
     if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"fp8_linear: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):

@@ -352,3 +352,18 @@ def test_hif8_copies_of_gathered_weights_follow_the_optimizer():
             opt.step()
             layer.weight.data.neg_()
             assert torch.equal(f(x), -before) and bool(before.any())
+
+
+# ----------------------------------------------------------------------------- second derivatives
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+def test_second_derivatives_raise(device, act):
+    """A penalty on a gradient would otherwise add nothing, without a word."""
+    x = _randn(4, 64, device=device, dtype=torch.bfloat16).requires_grad_()
+    w = _randn(8, 64, device=device, seed=1).requires_grad_()
+    (dx,) = torch.autograd.grad(fp8_linear(x, w, act=act).float().square().sum(), x, create_graph=True)
+    (plain,) = torch.autograd.grad(fp8_linear(x, w, act=act).float().square().sum(), x)
+    assert torch.equal(dx.detach(), plain)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.float().square().sum().backward()
