@@ -96,7 +96,10 @@ def fp8_matmul(a, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, act: Option
     ``a``: an :class:`Fp8Tensor` [M, K], or a matrix / batch [..., K] in bf16, fp16 or fp32 that
     is quantised here with blocks 1 x 128.  ``b``: an Fp8Tensor [N, K] (a weight, or either side
     of a gradient product).  ``act``: None or ``"gelu_tanh"``.  ``out_dtype``: bf16 or fp32.
-    ``aux=True`` also returns the value before ``act`` in bf16."""
+    ``aux=True`` also returns the value before ``act`` in bf16.
+
+    It records no graph: an ``a`` or ``bias`` that requires a gradient is refused unless gradients
+    are off (``quant.fp8_linear`` is the product under autograd)."""
     if not isinstance(b, Fp8Tensor):
         raise TypeError("fp8_matmul: b has to be an Fp8Tensor")
     if act not in (None, "gelu_tanh"):
@@ -104,6 +107,8 @@ def fp8_matmul(a, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, act: Option
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"fp8_matmul: out_dtype bf16 or fp32, got {out_dtype}")
     quantized = isinstance(a, Fp8Tensor)
+    if torch.is_grad_enabled() and ((not quantized and a.requires_grad) or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("fp8_matmul has no gradient: use quant.fp8_linear, or torch.no_grad()")
     shape = a.shape
     if len(shape) == 0 or shape[-1] != b.cols:
         raise ValueError(f"fp8_matmul: a {tuple(shape)} against K = {b.cols}")

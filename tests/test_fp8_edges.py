@@ -367,3 +367,18 @@ def test_second_derivatives_raise(device, act):
     assert torch.equal(dx.detach(), plain)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.float().square().sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_matmul_refuses_to_drop_a_gradient(device):
+    w = ops.fp8_quantize(_randn(8, 64, device=device), block_rows=128)
+    x, b = _randn(4, 64, device=device, dtype=torch.bfloat16), torch.zeros(8, device=device)
+    want = ops.fp8_matmul(x, w, b)
+    for args in ((x.clone().requires_grad_(), w, b), (x, w, b.clone().requires_grad_()),
+                 (ops.fp8_quantize(x), w, b.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.fp8_matmul(*args)
+        with torch.no_grad():
+            assert torch.equal(ops.fp8_matmul(*args), want)
+        with torch.inference_mode():
+            assert torch.equal(ops.fp8_matmul(*args), want)
