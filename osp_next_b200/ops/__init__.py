@@ -225,7 +225,7 @@ def linear_gelu_aux(x2, w, b, extra=None):
 def bias_grad(g):
     """Σ over rows of g [M, N] (the bias gradient of a Linear) in fp32, read straight from
     bf16: per-chunk column sums on the GPU, then a sum over the chunks (deterministic)."""
-    g2 = g.reshape(-1, g.shape[-1])
+    g2 = g.reshape(g.shape[:-1].numel(), g.shape[-1])
     if not _cuda(g2) or g2.shape[-1] % 8:
         return g2.float().sum(0)
     g2 = _vec(g2.to(_BF16), 16)

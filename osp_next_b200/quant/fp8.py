@@ -27,10 +27,15 @@ def _out_dtype(x: torch.Tensor) -> torch.dtype:
     return torch.float32 if not x.is_cuda and x.dtype == torch.float32 else torch.bfloat16
 
 
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [..., K] as a matrix, also without columns (where -1 would be ambiguous)."""
+    return x.reshape(x.shape[:-1].numel(), x.shape[-1])
+
+
 class _FP8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _rows(x)
         need_x, need_w = ctx.needs_input_grad[:2]
         # one read of x gives the forward operand and the one of dW; the same for W and dx
         if x.is_cuda and x2.numel() and weight.numel():
@@ -50,7 +55,7 @@ class _FP8LinearFn(torch.autograd.Function):
     def backward(ctx, gy):
         pre, *saved = ctx.saved_tensors
         xshape, xdt, wshape, wdt, bdt = ctx.meta
-        g = gy.reshape(-1, gy.shape[-1])
+        g = _rows(gy)
         if pre is not None:
             g = _gelu_tanh_bwd(g, pre)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]

@@ -382,3 +382,31 @@ def test_matmul_refuses_to_drop_a_gradient(device):
             assert torch.equal(ops.fp8_matmul(*args), want)
         with torch.inference_mode():
             assert torch.equal(ops.fp8_matmul(*args), want)
+
+
+# ----------------------------------------------------------------------------- empty sizes
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lead", [(), (3,), (2, 3), (0,), (2, 0)])
+@pytest.mark.parametrize("K,N", [(0, 5), (64, 0), (0, 0), (64, 8)])
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+def test_linear_without_rows_columns_or_outputs(device, lead, K, N, act):
+    """As nn.Linear: an empty sum is the bias, gradients of what is empty are zero."""
+    x = _randn(*lead, K, device=device, dtype=torch.bfloat16).requires_grad_()
+    w, b = _randn(N, K, device=device, seed=1).requires_grad_(), _randn(N, device=device, seed=2).requires_grad_()
+    y = fp8_linear(x, w, b, act)
+    assert y.shape == lead + (N,)
+    if K == 0:
+        want = _gelu64(b.detach().double()) if act else b.detach().double()
+        assert bool(((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20).all())
+    dx, dw, db = torch.autograd.grad(y.float().square().sum(), (x, w, b))
+    assert all(g.shape == t.shape and g.dtype == t.dtype for g, t in ((dx, x), (dw, w), (db, b)))
+    assert all(bool(g.isfinite().all()) for g in (dx, dw, db))
+    if x.numel() == 0 or N == 0:
+        assert not bool(dw.any()) and not bool(dx.any())
+    if 0 in lead:
+        assert not bool(db.any())
+    with torch.no_grad():
+        layer = FP8Linear(K, N, device=device) if K and N else None
+        if layer is not None:
+            assert layer(x).shape == y.shape
