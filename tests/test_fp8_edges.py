@@ -11,6 +11,7 @@ import torch
 from osp_next_b200 import ops
 from osp_next_b200.models.lora import LoraLinear, LoraModel, fused_lora_operands, inject_lora
 from osp_next_b200.models.osp_next import OSPNextModel
+from osp_next_b200.ops import reference as ref
 from osp_next_b200.parallel.ema import FSDPEMAModel
 from osp_next_b200.parallel.optim import FusedAdamW
 from osp_next_b200.quant import (FP8Linear, HIF8Linear, fp8_linear, fp8_multi_linear, freeze_fp8_weights,
@@ -410,3 +411,81 @@ def test_linear_without_rows_columns_or_outputs(device, lead, K, N, act):
         layer = FP8Linear(K, N, device=device) if K and N else None
         if layer is not None:
             assert layer(x).shape == y.shape
+
+
+# ----------------------------------------------------------------------------- AdamW over long lists
+
+HYPER = dict(lr=1.0, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01)
+
+
+def _param_bound(p, g, m, v, step, grad_scale):
+    """64-bit parameters after a step and how far fp32 may be off.  Roundings to 2^-24: three of p; of
+    the update three of each term of m, two of v, the constants, two products and a sum below the
+    line, a square root and a division approximate to 2^-22 each: below 2^-20 of it, with m taken as
+    the sum of its terms' magnitudes."""
+    p, g, m, v = (t.double() for t in (p, g * grad_scale, m, v))
+    b1, b2 = HYPER["beta1"], HYPER["beta2"]
+    rate, bc2 = HYPER["lr"] / (1 - b1 ** step), (1 - b2 ** step) ** 0.5
+    den = (b2 * v + (1 - b2) * g * g).sqrt() / bc2 + HYPER["eps"]
+    want = p * (1 - HYPER["lr"] * HYPER["weight_decay"]) - rate * (b1 * m + (1 - b1) * g) / den
+    return want, 2.0 ** -22 * (p.abs() + want.abs()) + 2.0 ** -20 * rate * (b1 * m.abs() + (1 - b1) * g.abs()) / den
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("step", [1, 2, 500])
+def test_adamw_parameters_to_fp32_accuracy(device, bits, step):
+    """Also where 1 - b2^t is small, which formed in fp32 would be off by 2^-14."""
+    n = 5000
+    p, g = _randn(n, device=device), 1e-3 * _randn(n, device=device, seed=1)
+    m, v = 1e-3 * _randn(n, device=device, seed=2), (1e-3 * _randn(n, device=device, seed=3)) ** 2
+    if bits == 8:
+        half = torch.full((n,), 0x80008000, dtype=torch.int64, device=device)
+        state = list(ref.adamw8_encode(m, v, half))
+        m, v = ops.adamw8_decode(*state)
+    else:
+        m, v = (m, v) if step > 1 else (torch.zeros_like(m), torch.zeros_like(v))
+        state = [m.clone(), v.clone()]
+    want, bound = _param_bound(p, g, m, v, step, 0.5)
+    ops.adamw_multi_([p], [g], *([t] for t in state), step=step, grad_scale=0.5, seed=3, **HYPER)
+    assert bool(((p.double() - want).abs() <= bound).all()), float(((p.double() - want).abs() / bound).max())
+
+
+LONG_LISTS = {   # tensors -> chunks of 4096 elements: more than 512 a launch, so that a step of the table has several
+    "few": [3_000_001, 1, 4096, 4097, 129] + [700 + 97 * i for i in range(20)] + [1_234_567, 5, 8192],
+    "small at the end": [2_500_000] + [1 + 61 * i for i in range(50)],
+    "many": [1 + 641 * (i % 29) for i in range(300)] + [2_000_003] + [4095 + i % 3 for i in range(170)] + [1_000_000],
+    "two launches": [9000 + 13 * i for i in range(700)],
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", list(LONG_LISTS))
+@pytest.mark.parametrize("pdtype,gdtype,bits", [(torch.float32, torch.float32, 8), (torch.bfloat16, torch.bfloat16, 8),
+                                                (torch.bfloat16, torch.float32, 8), (torch.float32, torch.bfloat16, 32)])
+def test_adamw_long_lists(sizes, pdtype, gdtype, bits):
+    """Every tensor by its own state, key and length: codes and scales as the CPU form has them."""
+    sizes = LONG_LISTS[sizes]
+    assert sum(-(-n // 4096) for n in sizes[:480]) > 512
+    p = [_randn(n, seed=i, dtype=pdtype) for i, n in enumerate(sizes)]
+    g = [(1e-3 * (1 + i % 7) * _randn(n, seed=5000 + i)).to(gdtype) for i, n in enumerate(sizes)]
+    if bits == 8:
+        state = [list(x) for x in zip(*(ops.adamw8_state(t) for t in p))]
+    else:
+        state = [[torch.zeros(n) for n in sizes] for _ in range(2)]
+    host = [p, g] + state
+    dev = [[t.cuda() for t in x] for x in host]
+    hyper = dict(HYPER, lr=1e-2)
+    for step in (1, 2):
+        for lists in (host, dev):
+            ops.adamw_multi_(*lists, step=step, grad_scale=0.7, seed=41 * step, **hyper)
+        for a, b in zip(host[2:], dev[2:]):
+            if bits == 8:
+                assert all(torch.equal(x.view(torch.uint8), y.cpu().view(torch.uint8)) for x, y in zip(a, b))
+            else:                                    # two products and a sum, which the kernel may contract
+                assert all(bool(((x - y.cpu()).abs() <= 2.0 ** -20 * x.abs() + 1e-9).all()) for x, y in zip(a, b))
+    # p moved by less than 0.1 a step: the update to 2^-20, its own roundings, in bf16 one place a step
+    rel = 2.0 ** -6 if pdtype == torch.bfloat16 else 2.0 ** -22
+    for x, y in zip(host[0], dev[0]):
+        x, y = x.double(), y.cpu().double()
+        assert bool(((x - y).abs() <= rel * x.abs() + 2.0 ** -20).all())
