@@ -54,7 +54,8 @@ constexpr int kStageBytes = 32 * kStageRow;
 constexpr uint32_t kScaleCol = 496;           // TMEM columns of the scales: A 496..499, B 500..507
 
 template <int BN> struct Shape {
-  static constexpr int kChunksB = BN > 128 ? 2 : 1;             // 128-row scale chunks of a B tile
+  static constexpr int kChunksB = BN > 128 ? 2 : 1;             // 128-row scale chunks of a B tile (at
+                                                                // BN = 64 a product has one tile of columns)
   static constexpr uint32_t kA = kBM * kBK, kB = BN * kBK;
   static constexpr uint32_t kScales = kChunkBytes * (1 + kChunksB);
   static constexpr int kStages = 196608 / (kA + kB) > 8 ? 8 : 196608 / (kA + kB);
@@ -279,7 +280,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       // ---------------------------------------------------------------- producer
       if (lane == 0) {
         const int last_chunk = (args.N + 127) / 128 - 1;
-          int stage = 0;
+        int stage = 0;
         uint32_t phase = 0;
         for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
           int mb, nb;
@@ -316,7 +317,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
-      const uint32_t t_sa = tmem_base + kScaleCol;
+      const uint32_t t_sa = tmem_base + kScaleCol, t_sb = t_sa + 4;
       // (tile, run) pairs in order; `it` counts them
       for (int t = blockIdx.x, run = 0; t < num_tiles && !*abort_flag; ++it) {
         const int kb0 = run * kRun, kb1 = runs == 1 ? num_kb : min(num_kb, kb0 + kRun);
@@ -328,13 +329,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) { *abort_flag = 1; break; }
         tc_fence_after();
-        // tiles of 64 columns begin in the middle of a 128-row scale chunk every other time
-        uint32_t t_sb = t_sa + 4;
-        if (BN == 64) {
-          int mb, nb;
-          tile_coords(t, num_m, num_n, mb, nb);
-          t_sb += 2 * (nb & 1);
-        }
         const uint32_t d_tmem = tmem_base + acc * S::kAccStride;
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, args.err, kErrFp8Mma));

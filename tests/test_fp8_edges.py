@@ -489,3 +489,22 @@ def test_adamw_long_lists(sizes, pdtype, gdtype, bits):
     for x, y in zip(host[0], dev[0]):
         x, y = x.double(), y.cpu().double()
         assert bool(((x - y).abs() <= rel * x.abs() + 2.0 ** -20).all())
+
+
+# ----------------------------------------------------------------------------- narrow products
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [65, 129, 5000])
+@pytest.mark.parametrize("N", [1, 40, 63, 64])
+def test_narrow_products(M, N):
+    """One tile of 64 columns, in both result types, over one run of blocks and over several.  Small
+    integers: every sum is exact, and so is its rounding."""
+    for K in (128, 1000, 4096):
+        g = torch.Generator().manual_seed(M + N + K)
+        x = torch.randint(-4, 5, (M, K), generator=g).to(device="cuda", dtype=torch.bfloat16)
+        w = torch.randint(-4, 5, (N, K), generator=g).to(device="cuda", dtype=torch.float32)
+        want = x.double() @ w.double().t()
+        wq = ops.fp8_quantize(w, block_rows=128)
+        for dt in (torch.float32, torch.bfloat16):
+            assert torch.equal(ops.fp8_matmul(x, wq, out_dtype=dt), want.to(dt))
+    ops.check_device_errors()
