@@ -66,7 +66,7 @@ class _FP8LinearFn(torch.autograd.Function):
                 dx, dw, db = ops.ext().fp8_linear_backward(g, *saved, need_b, xdo == torch.float32,
                                                            wdo == torch.float32)
             else:
-                gr, gc = ops.fp8_quantize(g, layout="both")
+                gr, gc, db = ops.fp8_quantize_with_sums(g)
                 tokens, (N, K) = g.shape[0], wshape
                 if need_x:
                     dx = ops.fp8_matmul(gr, ops.Fp8Tensor(saved[2], saved[3], K, N, ops.fp8.BLOCK), out_dtype=xdo)
@@ -74,8 +74,7 @@ class _FP8LinearFn(torch.autograd.Function):
                     dw = ops.fp8_matmul(gc, ops.Fp8Tensor(saved[0], saved[1], K, tokens), out_dtype=wdo)
             dx = None if dx is None else dx.to(xdt).view(xshape)
             dw = None if dw is None else dw.to(wdt)
-        if need_b:
-            db = (ops.bias_grad(g) if db is None else db).to(bdt)
+        db = (ops.bias_grad(g) if db is None else db).to(bdt) if need_b else None
         return dx, dw, db, None
 
 
