@@ -474,7 +474,8 @@ class OSPNextModel(nn.Module):
 
     def freqs(self, device):
         if self._freqs is None or self._freqs.device != torch.device(device):
-            self._freqs = ref.rope_freqs(self.rope_d).to(device)
+            with torch.inference_mode(False):        # kept: an ordinary tensor, also if sampling makes it first
+                self._freqs = ref.rope_freqs(self.rope_d).to(device)
         return self._freqs
 
     def enable_text_kv_cache(self, enabled: bool = True):
@@ -648,7 +649,9 @@ def _dev(t: torch.Tensor, device, dtype):
     if v is None or v[0] is not t:
         if len(_DEV_CACHE) > 4096:       # inputs are cached host tables; bound it all the same
             _DEV_CACHE.clear()
-        v = (t, t.to(device=device, dtype=dtype))
+        with torch.inference_mode(False):            # kept, as the RoPE table
+            d = t.to(device=device, dtype=dtype)
+            v = (t, d.clone() if d.is_inference() else d)
         _DEV_CACHE[key] = v
     return v[1]
 

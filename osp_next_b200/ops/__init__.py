@@ -307,15 +307,22 @@ def qk_norm_rope_bwd(raw, dq, dk, dv, wq, wk, pos, freqs, eps: float = 1e-6):
 _CS_CACHE = {}
 
 
+def _cos_sin(freqs, device):
+    a = freqs.to(device=device, dtype=torch.float64)
+    return torch.stack([a.cos(), a.sin()], -1).float().contiguous()
+
+
 def rope_cos_sin(freqs: torch.Tensor, device) -> torch.Tensor:
     """(cos, sin) table [L, D/2, 2] fp32 of an angle table, evaluated in fp64 once per
     table (cached), so the kernels rotate with table loads instead of sincos."""
+    if freqs.is_inference():         # no version to tell a change by: evaluated anew
+        return _cos_sin(freqs, device)
     key = (freqs.data_ptr(), freqs._version, tuple(freqs.shape), str(device))
     hit = _CS_CACHE.get(key)
     if hit is not None and hit[0] is freqs:
         return hit[1]
-    a = freqs.to(device=device, dtype=torch.float64)
-    cs = torch.stack([a.cos(), a.sin()], -1).float().contiguous()
+    with torch.inference_mode(False):
+        cs = _cos_sin(freqs, device)
     if len(_CS_CACHE) > 16:
         _CS_CACHE.clear()
     _CS_CACHE[key] = (freqs, cs)

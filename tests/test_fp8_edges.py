@@ -508,3 +508,116 @@ def test_narrow_products(M, N):
         for dt in (torch.float32, torch.bfloat16):
             assert torch.equal(ops.fp8_matmul(x, wq, out_dtype=dt), want.to(dt))
     ops.check_device_errors()
+
+
+# ----------------------------------------------------------------------------- sampling in fp8
+
+def _small_model(device, quant):
+    torch.manual_seed(0)
+    with torch.device(device):
+        m = OSPNextModel(dim=256, ffn_dim=512, num_heads=2, num_layers=2, text_len=16,
+                         skiparse_model_type="dual_end", sparse_ratio=2, num_full_blocks=0, quant=quant)
+    torch.nn.init.normal_(m.head.head.weight, std=0.02)
+    return m
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("quant", [None, "fp8"])
+def test_a_model_first_run_in_inference_mode(device, quant):
+    """Its tables are made there and kept: later steps, gradients among them, find ordinary tensors."""
+    model = _small_model(device, quant)
+    g = torch.Generator().manual_seed(1)
+    # a grid that no other test runs, so that the shared tables are made here
+    x, t, ctx = (torch.randn(1, 16, 3, 12, 20, generator=g).to(device), torch.tensor([500.0], device=device),
+                 torch.randn(1, 16, 4096, generator=g).to(device))
+    with torch.inference_mode():
+        y = model(x, t, ctx)
+        assert torch.equal(model(x, t, ctx), y)
+    with torch.no_grad():
+        assert torch.equal(model(x, t, ctx), y.clone())
+    model(x, t, ctx).float().square().mean().backward()
+    assert all(bool(p.grad.isfinite().all()) for p in model.parameters() if p.grad is not None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rope_table_of_an_inference_tensor(device):
+    with torch.inference_mode():
+        f = torch.arange(12.0, device=device).view(3, 4)
+        a = ops.rope_cos_sin(f, device).clone()
+        f.add_(1)
+        b = ops.rope_cos_sin(f, device)
+        assert torch.equal(b[..., 0], f.double().cos().float()) and not torch.equal(a, b)
+
+
+
+class _Text:
+    """Stands in for tokenizer and text encoder: a sequence of 16 made from the prompt's length."""
+    def __init__(self, device):
+        self.device, self.tokenizer = device, self._tokenize
+        self.dtype = torch.float32 if torch.device(device).type == "cpu" else torch.bfloat16
+
+    def _tokenize(self, texts, **kw):
+        return torch.tensor([[len(t)] for t in texts]), torch.ones(len(texts), 1)
+
+    def __call__(self, ids, mask):
+        return torch.cat([_randn(1, 16, 4096, device=self.device, seed=int(i), dtype=self.dtype) for i in ids])
+
+
+class _Frames:
+    """Stands in for the VAE: the first three channels of the latents."""
+    dtype = torch.float32
+
+    def decode(self, z):
+        return torch.tanh(z.float())[:, :3]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_inference_script_in_fp8(device, tmp_path, monkeypatch):
+    """``model_config.quant: fp8``: the weights are quantised once, every step runs on the frozen
+    copies, and the videos are those of layers that quantise their weight in each call."""
+    import torch.distributed as dist
+    from osp_next_b200.data.utils import video_io
+    from osp_next_b200.engine import builders
+    monkeypatch.syspath_prepend(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "infer"))
+    import infer_osp
+    for k, v in dict(MASTER_ADDR="127.0.0.1", MASTER_PORT="29637", RANK="0", WORLD_SIZE="1", LOCAL_RANK="0").items():
+        monkeypatch.setenv(k, v)
+    (tmp_path / "prompts.txt").write_text("a dog runs\nthe sea at night, seen from above\n")
+    cfg = {"model_name": "osp_next", "seed": 3, "prompt_txt": str(tmp_path / "prompts.txt"), "num_frames": 5,
+           "height": 64, "width": 64, "output_dir": str(tmp_path / "out"), "timeout_s": 120,
+           "weight_dtype": "fp32" if device == "cpu" else "bf16",
+           "model_config": dict(dim=256, ffn_dim=512, num_heads=2, num_layers=2, text_len=16, quant="fp8",
+                                skiparse_model_type="dual_end", sparse_ratio=2, num_full_blocks=0),
+           "scheduler_config": {"scheduler_name": "flow_matching", "num_inference_steps": 2, "guidance_scale": 5.0}}
+    built, videos, build_model = [], [], builders.build_model
+
+    def build(*a, **k):
+        built.append(build_model(*a, **k))
+        torch.manual_seed(5)
+        torch.nn.init.normal_(built[-1].head.head.weight, std=0.02)      # the head starts at zero
+        return built[-1]
+    monkeypatch.setattr(builders, "build_model", build)
+    monkeypatch.setattr(builders, "build_vae", lambda *a: _Frames())
+    monkeypatch.setattr(builders, "build_text_encoder", lambda c, dev: _Text(dev))
+    monkeypatch.setattr(video_io, "save_video", lambda v, path, fps: videos.append((os.path.basename(path), v)))
+
+    def run():
+        videos.clear()
+        infer_osp.main(copy.deepcopy(cfg))
+        if dist.is_initialized():
+            dist.destroy_process_group()
+        assert [n for n, _ in videos] == ["00000.mp4", "00001.mp4", "grid.mp4"]
+        return [v for n, v in videos if n != "grid.mp4"]
+    frozen = run()
+    layers = [m for m in built[-1].modules() if isinstance(m, FP8Linear)]
+    assert len(layers) == 20 and all(m._frozen is not None for m in layers)
+    assert all(v.shape == (2, 8, 8, 3) and v.dtype == torch.uint8 for v in frozen)
+    assert not torch.equal(frozen[0], frozen[1])
+    monkeypatch.setattr(FP8Linear, "freeze_weight", lambda self: self)
+    again = run()
+    assert all(torch.equal(a, b) for a, b in zip(frozen, again))
+    cfg["model_config"].pop("quant")
+    plain = run()
+    assert not all(torch.equal(a, b) for a, b in zip(frozen, plain))
+    # uint8 frames of tanh values: the quantisation moves them by a few of 255 in the mean
+    assert max((a.float() - b.float()).abs().mean().item() for a, b in zip(frozen, plain)) < 25
