@@ -621,3 +621,28 @@ def test_inference_script_in_fp8(device, tmp_path, monkeypatch):
     assert not all(torch.equal(a, b) for a, b in zip(frozen, plain))
     # uint8 frames of tanh values: the quantisation moves them by a few of 255 in the mean
     assert max((a.float() - b.float()).abs().mean().item() for a, b in zip(frozen, plain)) < 25
+
+
+# ----------------------------------------------------------------------------- long sums in fp32
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(1, 512), (40, 300), (100, 64), (130, 300), (5000, 512)])
+def test_a_large_first_term_costs_no_more_than_an_fp32_sum(M, N):
+    """Sums near 1.5 from their first product on, with small ones of both signs behind it: each step
+    of 32 products forms its sum in quarters of a place of 2^-23 and cuts it toward zero, by 3/8 of a
+    place in the mean, for as long as a run goes on (12 blocks, 48 steps: 18 places), and the sum of the
+    runs is rounded (1 more)."""
+    K = 2048
+    g = torch.Generator().manual_seed(M + N)
+
+    def small(rows):                                 # +- 2^-11 (8 .. 15) / 8: products far below 2^-23
+        v = torch.randint(8, 16, (rows, K), generator=g) / 8 * 2.0 ** -11
+        return v * (torch.randint(0, 2, (rows, K), generator=g) * 2 - 1)
+    x, w = small(M), small(N)
+    x[:, 0], w[:, 0] = 1.5, 1.0
+    a, b = ops.fp8_quantize(x.cuda()), ops.fp8_quantize(w.cuda())
+    want = a.dequantize().double() @ b.dequantize().double().t()
+    assert torch.equal(a.dequantize().cpu(), x) and torch.equal(b.dequantize().cpu(), w)
+    assert 1 < want.min().item() and want.max().item() < 2
+    places = (want - ops.fp8_matmul(a, b, out_dtype=torch.float32).double()) * 2 ** 23
+    assert abs(places.mean().item()) <= 19
