@@ -104,7 +104,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
 
 class FP8Linear(nn.Linear):
-    """Drop-in ``nn.Linear`` in block-scaled fp8 (forward and backward).
+    """``nn.Linear`` in block-scaled fp8 (forward and backward), with its parameters and state.
+    The output is bf16 on the GPU, whatever the input's type (see :func:`fp8_linear`).
 
     Under autograd both operands are quantised every call.  For sampling, :meth:`freeze_weight`
     quantises the weight once and later no-grad calls use that copy until :meth:`thaw_weight`,
