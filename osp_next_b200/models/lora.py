@@ -17,6 +17,7 @@ import contextlib
 import fnmatch
 import json
 import os
+import weakref
 from typing import Dict, Iterable, List, Optional
 
 import torch
@@ -252,11 +253,14 @@ class LoraModel(nn.Module):
 
 
 # ---------------------------------------------------------------------------- fused inference path
+_PACKS: "weakref.WeakKeyDictionary[nn.Module, dict]" = weakref.WeakKeyDictionary()
+
+
 def _packed(mods, slot, ts, build):
-    """What ``build`` makes of the tensors ``ts`` of ``mods``: kept with the first of them until one
-    of the tensors changes (an optimizer step replaces what it made out of date)."""
+    """What ``build`` makes of the tensors ``ts`` of ``mods``: kept as long as the first of them, and
+    until one of the tensors changes (an optimizer step replaces what it made out of date)."""
     key = weights_key(ts)
-    packs = mods[0].__dict__.setdefault("_packs", {})
+    packs = _PACKS.setdefault(mods[0], {})
     hit = packs.get(slot)
     if hit is None or hit[0] != key:
         hit = packs[slot] = (key, build())

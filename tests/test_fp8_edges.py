@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from osp_next_b200 import ops
-from osp_next_b200.models.lora import LoraLinear, LoraModel, fused_lora_operands, inject_lora
+from osp_next_b200.models.lora import _PACKS, LoraLinear, LoraModel, fused_lora_operands, inject_lora
 from osp_next_b200.models.osp_next import OSPNextModel
 from osp_next_b200.ops import reference as ref
 from osp_next_b200.parallel.ema import FSDPEMAModel
@@ -310,7 +310,7 @@ def test_no_grad_outputs_follow_the_optimizer(kw, lora):
         with torch.no_grad():
             y = model(x, t, ctx)
             assert torch.equal(y, twin(x, t, ctx)) and not torch.equal(y, first)
-    assert len(getattr(model.blocks[0].self_attn.q, "_packs", {})) <= 2          # nothing of the old weights is kept
+    assert len(_PACKS.get(model.blocks[0].self_attn.q, {})) <= 2          # nothing of the old weights is kept
 
 
 def test_packs_of_gathered_weights_follow_the_optimizer():
@@ -333,6 +333,7 @@ def test_packs_of_gathered_weights_follow_the_optimizer():
         assert torch.equal(B, (2 * layer.lora_B["default"].weight.detach()).bfloat16())
         return W
     check()
+    assert len(_PACKS[layer]) == 2 and copy.deepcopy(layer) not in _PACKS        # not in copies or checkpoints
     for write in (opt.step, lambda: ema.ema_copy_to_model(shard), lambda: ema.restore(shard)):
         shard[0].grad = torch.ones(4)
         write()
