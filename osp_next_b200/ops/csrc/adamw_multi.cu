@@ -15,7 +15,7 @@
 // the unrounded moments.
 //
 // It has to move 16 bytes per element with fp32 p and g and 8-bit moments (28 with fp32 ones); 177M
-// elements in 820 tensors take 499 us, 0.87 of the copy rate, held up by some 64 instructions
+// elements in 820 tensors take 498 us, 0.87 of the copy rate, held up by some 64 instructions
 // per element.  A warp takes 128 elements at a time, so the block maximum is one warp reduction
 // and each of its loads and stores is one contiguous segment.  The list travels in the kernel's
 // parameters (up to 32 KB): no table is copied or kept between calls.

@@ -129,12 +129,13 @@ __device__ __forceinline__ float gelu_tanh_f(float x) {
 
 // Accumulation over a long K.  The tensor core cuts the sum to its fp32 accumulator at each of the
 // K / 32 steps, always toward zero (by 3/8 of a last place in the mean: it forms the sum in quarters of
-// one): over K = 14040 tokens a weight gradient came out 5e-6 small.  An
-// fp32 result is therefore accumulated in runs of kRun blocks, which the epilogue adds up in its
-// registers, rounded to nearest (adding the runs up in L2 took the time half again).  Weight gradients of
-// 8960 x 1536 over 14040 tokens of very different sizes, 40 of them, against 64 bits: runs of 16 blocks
-// 6.4e-7 in the mean and 1.4e-6 at most in 155.6 us, of 12 blocks 4.5e-7 and 7.4e-7 in 158.7, of 8 blocks
-// 3.1e-7 and 6.9e-7 in 163.8; an fp32 product of the same operands 5.5e-7 and 7.9e-7.
+// one): over K = 14040 tokens a weight gradient came out 5e-6 small.  An fp32 result is therefore
+// accumulated in runs of kRun blocks, which the epilogue adds up in its registers, rounded to nearest
+// (adding the runs up in L2 took the time half again).  Weight gradients of 8960 x 1536 over 14040 tokens
+// of very different sizes, 40 of them, against 64 bits: runs of 16 blocks 6.4e-7 in the mean and 1.4e-6 at
+// most in 155.6 us, of 12 blocks 4.5e-7 and 7.4e-7 in 158.7, of 8 blocks 3.1e-7 and 6.9e-7 in 163.8; an
+// fp32 product of the same operands 5.5e-7 and 7.9e-7.  A second run costs most where it is short
+// (20000 x 8192 over 1664: 266 us in one, 281 in two; over 2048: 307 and 317).
 // bf16 results have one run: the cut (7e-6 over K = 20160) moves one in some 800 of them by a last
 // place, and runs would cost 3.5 % (13824 x 5120 over 20160 tokens: 1033 us, in runs 1068).
 constexpr int kRun = 12;
@@ -470,8 +471,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 // N.  CTAs of 100 KB share an SM in pairs; where the tiles are too few to fill the GPU a cluster
 // of up to 8 CTAs splits K and adds its parts through distributed shared memory, in rank order
 // (the result does not depend on timing, and no workspace is needed).  The weight's first
-// stages are loaded before the wait for the quantiser of A.  1 x 5120 -> 30720: 27.9 us with the
-// quantiser, 0.86 of the copy rate on the weight's bytes; 128 rows take 27.5 us here (cold caches)
+// stages are loaded before the wait for the quantiser of A.  1 x 5120 -> 30720: 28.4 us with the
+// quantiser, 0.85 of the copy rate on the weight's bytes; 128 rows take 27.5 us here (cold caches)
 // and 21.5 in gemm_kernel's tiles, 64 rows about the same in both.
 // 192 threads: warp 0 TMA producer, warp 1 MMA issuer, warps 2..5 epilogue.
 template <int BNX> struct Skinny {

@@ -7,8 +7,8 @@
 //
 // Both are bound by memory: 2 or 4 bytes read and 1 (+ 1/128) written per element and side.  Measured
 // against the copy rate of 6551 GB/s: rows of 80640 x 5120 bf16 in 181 us (1.04, part of the codes
-// still in L2), 20160 x 13824 bf16 both ways in 198 us (0.86), tiles of an fp32 8960 x 1536 weight both ways
-// in 16.5 us (0.76).
+// still in L2), 20160 x 13824 bf16 both ways in 206 us (0.83), tiles of an fp32 8960 x 1536 weight both ways
+// in 16.3 us (0.77).
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContextLight.h>
