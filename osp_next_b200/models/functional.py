@@ -20,6 +20,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 from ..ops import reference as ref
@@ -344,3 +345,40 @@ def attention(q, k, v, seg_q, seg_k, scale=None):
     if _fused(q, k, v):
         return ops.attention(q, k, v, seg_q, seg_k, scale)
     return _AttnFn.apply(q, k, v, seg_q, seg_k, scale)
+
+
+class _PackedAttnFn(torch.autograd.Function):
+    """Attention over packed sequences with both passes on the tcgen05 kernels; keeps
+    (q, k, v, o, log-sum-exp) and recomputes P."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, pack, causal, scale):
+        qb, kb, vb = q.to(_BF16), k.to(_BF16), v.to(_BF16)
+        o, lse = ops.packed_attention(qb, kb, vb, pack, causal, scale, return_lse=True)
+        ctx.save_for_backward(qb, kb, vb, o, lse)
+        ctx.meta = (pack, causal, scale, (q.dtype, k.dtype, v.dtype))
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        q, k, v, o, lse = ctx.saved_tensors
+        pack, causal, scale, dtypes = ctx.meta
+        grads = ops.packed_attention_bwd(q, k, v, o, go, lse, pack, causal, scale)
+        return (*(g.to(t) for g, t in zip(grads, dtypes)), None, None, None)
+
+
+def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=None):
+    """Attention inside the sequences of ``pack`` (see :func:`ops.packed_attention`), under autograd
+    too: q [Nq, heads, D], k and v [Nk, key heads, D] -> [Nq, heads, D], bf16 on the GPU.  The gradient
+    of a shared key head is the sum over its query heads.  ``rel_bias`` has no gradient and allows
+    none: with it, call without autograd.  First derivatives only."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if not q.is_cuda:
+        ops.packed.check_packed(q, k, v, pack, rel_bias)
+        return ref.packed_attention(q, k, v, pack, causal, scale, rel_bias)[0]
+    if _fused(q, k, v, rel_bias):
+        return ops.packed_attention(q.to(_BF16), k.to(_BF16), v.to(_BF16), pack, causal, scale, rel_bias)
+    if rel_bias is not None:
+        raise RuntimeError("packed_attention: no gradient with rel_bias on the GPU; use torch.no_grad()")
+    return _PackedAttnFn.apply(q, k, v, pack, causal, scale)

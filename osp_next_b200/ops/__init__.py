@@ -16,6 +16,7 @@ from . import reference as ref
 from ._ext import ext, available  # noqa: F401
 from .fp8 import (Fp8Tensor, adamw8_decode, adamw8_state, adamw_multi_, fp8_matmul, fp8_quantize,  # noqa: F401
                   fp8_quantize_with_sums)
+from .packed import SequencePack, packed_attention, packed_attention_bwd  # noqa: F401
 
 _BF16 = torch.bfloat16
 

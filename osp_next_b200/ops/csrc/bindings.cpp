@@ -43,6 +43,14 @@ void attention_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
                    const at::Tensor& dout, const at::Tensor& lse, const at::Tensor& seg_q, const at::Tensor& seg_k,
                    at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta, double scale, int64_t max_q,
                    int64_t max_k);
+std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                        const at::Tensor& items, const at::Tensor& joins, int64_t slots, bool causal,
+                                        double scale, const c10::optional<at::Tensor>& rel_bias, bool want_lse,
+                                        bool fill);
+std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                        const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse,
+                                        const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
+                                        int64_t slots, bool causal, double scale, bool fill);
 void cfg_euler(const at::Tensor& lat, const at::Tensor& cond, const at::Tensor& unc, at::Tensor& out, double g,
                double dt);
 void hif8_round(const at::Tensor& x, at::Tensor& out, double s);
@@ -160,6 +168,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_bwd", &osp::rms_norm_bwd);
   m.def("attention_fwd", &osp::attention_fwd);
   m.def("attention_bwd", &osp::attention_bwd);
+  m.def("packed_attn_fwd", &osp::packed_attn_fwd);
+  m.def("packed_attn_bwd", &osp::packed_attn_bwd);
   m.def("cfg_euler", &osp::cfg_euler);
   m.def("hif8_round", &osp::hif8_round);
   m.def("hif8_qdq", &osp::hif8_qdq);

@@ -1,0 +1,81 @@
+// What the packed attention kernels share: work items, tile geometry and tail rows.
+//
+// Sequences of different lengths lie one behind another (or at any distance) in q [Nq, Hq, D] and
+// k, v [Nk, Hkv, D]; G = Hq / Hkv query heads share a key head.  A tile of the tensor core's 128
+// rows holds the G heads of P = 128 / G positions, row = position * G + head, which one TMA box
+// {64 elements, G heads, P positions} lays out that way.  So a key tile is read once for its whole
+// group, a sequence of few queries fills a tile with G times as many rows, and the gradients of a
+// shared key head are sums over the rows of one accumulator: no atomics.  128 - G * P rows (2 for
+// G = 3, 6, 7, 9; 3 for G = 5) stay unused.
+//
+// The host lays the work out once per pack: a list of items for each kernel, longest first, so that
+// a grid of one CTA per item and key head ends with the short ones.
+//
+// Tiles that reach over a sequence's end hold rows of the next one.  Scores there are masked, but
+// 0 * NaN is NaN in a product that sums over those rows, so the producer warp overwrites the rows
+// behind the end with zeros in shared memory before it hands the tile on.
+#pragma once
+#include "common.cuh"
+#include "attn_math.cuh"
+
+namespace osp {
+namespace pa {
+
+constexpr int kRows = 128;           // rows of a tile: group heads x positions, or keys
+constexpr float kLog2e = 1.4426950408889634f;
+
+// One work item = 8 ints.
+struct FwdItem {       // forward (two tiles of P positions) and dQ (one tile)
+  int q_row;           // row of the first query
+  int n_q;             // queries of the item
+  int limit;           // keys that its first query sees if causal (may be negative)
+  int k_row;           // row of the sequence's first key
+  int n_keys;          // keys of the sequence
+  int kt0, kt1;        // key tiles of the item
+  int slot;            // place of its partial result, or -1
+};
+struct KeyItem {       // dK, dV of one tile of 128 keys
+  int k_row;           // row of its first key
+  int n_k;             // its keys
+  int first;           // first query (of the sequence) that sees its first key
+  int q_row;           // row of the query `first`
+  int n_q;             // queries from there on
+  int lead;            // key 0 is seen by query max(0, lead) of those, key i by query lead + i
+  int slot;            // place of its partial result, or -1
+  int pad;
+};
+
+__device__ __forceinline__ const int4* item_ptr(const int* list, int i) {
+  return reinterpret_cast<const int4*>(list) + 2 * i;
+}
+__device__ __forceinline__ FwdItem load_fwd_item(const int* list, int i) {
+  const int4 a = item_ptr(list, i)[0], b = item_ptr(list, i)[1];
+  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+__device__ __forceinline__ KeyItem load_key_item(const int* list, int i) {
+  const int4 a = item_ptr(list, i)[0], b = item_ptr(list, i)[1];
+  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+// Zeros into rows [row0, 128) of `boxes` boxes of 128 rows x 128 bytes, by one warp.  Whole rows, so
+// the swizzle inside a row does not matter.  The caller fences towards the async proxy.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int boxes, int row0, int lane) {
+  const int n = (kRows - row0) * 8;                // 16-byte pieces per box
+  for (int b = 0; b < boxes; ++b) {
+    uint4* p = reinterpret_cast<uint4*>(tile + b * kRows * 128 + row0 * 128);
+    for (int i = lane; i < n; i += 32) p[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// 8 fp32 values of a row, scaled, as 16 bytes of bf16.
+__device__ __forceinline__ uint4 pack8(const uint32_t* v, float mul) {
+  uint4 w;
+  w.x = pack_bf16x2(__uint_as_float(v[0]) * mul, __uint_as_float(v[1]) * mul);
+  w.y = pack_bf16x2(__uint_as_float(v[2]) * mul, __uint_as_float(v[3]) * mul);
+  w.z = pack_bf16x2(__uint_as_float(v[4]) * mul, __uint_as_float(v[5]) * mul);
+  w.w = pack_bf16x2(__uint_as_float(v[6]) * mul, __uint_as_float(v[7]) * mul);
+  return w;
+}
+
+}  // namespace pa
+}  // namespace osp

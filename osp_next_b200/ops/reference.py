@@ -345,3 +345,52 @@ def adamw_multi_(params, grads, exp_avgs, exp_avg_sqs, mscales, vscales, lr, bet
         state = adamw8_encode(mf, vf, _mix32((i + key) & _U32).view(p.shape))
         for dst, src in zip((m, v, mscales[t], vscales[t]), state):
             dst.copy_(src)
+
+
+# ----------------------------------------------------------------------------- packed sequences
+
+def packed_attention(q, k, v, pack, causal: bool, scale: float, rel_bias=None):
+    """(o like q, log-sum-exp fp32) of attention inside the sequences of a pack, in fp32 (64 bits for
+    64-bit inputs); differentiable.  Rows that see no key: 0 and -inf."""
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    group = q.shape[1] // k.shape[1]
+    o = torch.zeros(q.shape, dtype=acc, device=q.device)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=acc, device=q.device)
+    for a0, a, b0, b in zip(pack.starts.tolist(), pack.lengths.tolist(), pack.key_starts.tolist(),
+                            pack.key_lengths.tolist()):
+        if a == 0 or b == 0:
+            continue
+        qs = q[a0:a0 + a].to(acc).transpose(0, 1)                                   # [H, a, D]
+        ks = k[b0:b0 + b].to(acc).transpose(0, 1).repeat_interleave(group, 0)
+        vs = v[b0:b0 + b].to(acc).transpose(0, 1).repeat_interleave(group, 0)
+        s = (qs @ ks.transpose(1, 2)) * scale
+        place = torch.arange(b - a, b, device=q.device)[:, None]
+        key = torch.arange(b, device=q.device)[None]
+        if rel_bias is not None:
+            s = s + rel_bias.to(acc)[:, key - place + (rel_bias.shape[1] + 1) // 2 - 1]
+        if causal:
+            seen = key <= place
+            s = s.masked_fill(~seen, -math.inf)
+            full = seen.any(1)
+            p = torch.softmax(s.masked_fill(~full[:, None], 0.0), -1).masked_fill(~seen, 0.0)
+            # a sum over the keys that a row sees: 0 * NaN of a hidden value does not count
+            bad = ~torch.isfinite(vs)
+            out = p @ vs.masked_fill(bad, 0.0)
+            if bool(bad.any()):
+                out = out + torch.where(seen[None, :, :, None] & bad[:, None], p[..., None] * vs[:, None], 0.0).sum(2)
+        else:
+            out = torch.softmax(s, -1) @ vs
+        o[a0:a0 + a] = out.transpose(0, 1)
+        lse[a0:a0 + a] = torch.logsumexp(s.detach(), -1).t()
+    return o.to(q.dtype), lse.float() if acc == torch.float32 else lse
+
+
+def packed_attention_bwd(q, k, v, dout, pack, causal: bool, scale: float):
+    """(dq, dk, dv) of :func:`packed_attention` by autograd of the same math."""
+    with torch.enable_grad():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o, _ = packed_attention(*leaves, pack, causal, scale)
+        if not o.requires_grad:
+            return tuple(torch.zeros_like(t) for t in leaves)
+        grads = torch.autograd.grad(o, leaves, dout.to(o.dtype), allow_unused=True)
+    return tuple(torch.zeros_like(t) if g is None else g for t, g in zip(leaves, grads))
