@@ -300,8 +300,43 @@ def qk_norm_rope_packed(qkv, wq, wk, pos, freqs, num_heads: int, eps: float):
 
 
 def apply_rope(x, pos, freqs):
-    """x [B,n,H,D] → rotated fp32 (CPU / autograd path)."""
-    return ref.apply_rope(x, pos, freqs)
+    """x [B,n,H,D] rotated at (t, h, w) positions [n,3]: fp32 on the CPU, on the rotary kernel in x's own
+    type on the GPU (heads without q/k norm, forward and backward)."""
+    if not x.is_cuda or x.dtype not in (_BF16, torch.float16, torch.float32):
+        return ref.apply_rope(x, pos, freqs)
+    return rotary(x, None, pos.to(x.device), ops.rope_cos_sin(freqs, x.device), "interleaved",
+                  ref.rope_split(x.shape[-1]))[0]
+
+
+class _RotaryFn(torch.autograd.Function):
+    """Rotation of q and k in one launch; the gradient is the rotation back."""
+
+    @staticmethod
+    def forward(ctx, q, k, pos, table, layout, sections):
+        ctx.save_for_backward(pos, table)
+        ctx.meta = (layout, sections)
+        return ops.rotary(q, k, pos, table, layout, sections)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        pos, table = ctx.saved_tensors
+        layout, sections = ctx.meta
+        gq, gk = rotary(gq, gk, pos, table, layout, sections, inverse=True)
+        return gq, gk, None, None, None, None
+
+
+def rotary(q, k, pos, table, layout: str = "half", sections=None, inverse: bool = False):
+    """Rotary positions of q and k (k may be None; see :func:`ops.rotary`), under autograd too."""
+    if _fused(q, k) or not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k))):
+        return ops.rotary(q, k, pos, table, layout, sections, inverse)
+    if q.is_cuda:
+        t = table if not inverse else table * table.new_tensor([1.0, -1.0])
+        return _RotaryFn.apply(q, k, pos, t, layout, sections)
+    with torch.no_grad():
+        ops.rotary(q, k, pos, table, layout, sections)                # the same refusals
+    p = pos[:, None] if pos.dim() == 1 else pos
+    s = [table.shape[1]] if sections is None else list(sections)
+    return tuple(None if t is None else ref.rotary(t, p, table, layout, s, inverse) for t in (q, k))
 
 
 # ----------------------------------------------------------------------------- attention
@@ -382,3 +417,59 @@ def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=No
     if rel_bias is not None:
         raise RuntimeError("packed_attention: no gradient with rel_bias on the GPU; use torch.no_grad()")
     return _PackedAttnFn.apply(q, k, v, pack, causal, scale)
+
+
+# ----------------------------------------------------------------------------- gated feed-forward
+
+class _GatedFFNFn(torch.autograd.Function):
+    """Gated feed-forward block on the kernels of ops/csrc/gated_ffn.cu.  Keeps x, the weights and both
+    projections; h comes back from them in the epilogue of dh = dy W_down."""
+
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd, act):
+        x2 = ops.gated.matrix(x.reshape(x.shape[:-1].numel(), x.shape[-1]))
+        g, u, d = ops.gated.hidden_rows(wg), ops.gated.hidden_rows(wu), ops.gated.hidden_rows(wd)
+        h, gu = ops.ext().gated_linear_fwd(x2, g, u, ops.gated.ACTS[act], True)
+        y = ops.ext().ffn_product(h, d, None, None, False, False, False)
+        ctx.save_for_backward(x2, g, u, d, gu)
+        ctx.meta = (x.shape, x.dtype, wg.shape, wg.dtype, wu.dtype, wd.shape, wd.dtype, ops.gated.ACTS[act])
+        return y[:, :wd.shape[0]].reshape(*x.shape[:-1], wd.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x2, wg, wu, wd, gu = ctx.saved_tensors
+        xshape, xdt, wshape, gdt, udt, dshape, ddt, act = ctx.meta
+        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
+        dy = ops.gated.matrix(gy.reshape(gy.shape[:-1].numel(), gy.shape[-1]))
+        product = ops.ext().ffn_product
+        h, dgu = ops.ext().gated_linear_bwd(dy, wd, gu, act)
+        fp, (f, k) = wg.shape[0], wshape
+        dx = dwg = dwu = dwd = None
+        if need_x:
+            dx = product(dgu[:, :fp], wg, dgu[:, fp:], wu, False, True, xdt != _BF16)
+            dx = dx[:, :k].reshape(xshape).to(xdt)
+        if need_g or need_u:
+            part = dgu if need_g and need_u else dgu[:, :fp] if need_g else dgu[:, fp:]
+            dw = product(part, x2, None, None, True, True, gdt != _BF16 or udt != _BF16)
+            if need_g:
+                dwg = dw[:f, :k].to(gdt)
+            if need_u:
+                dwu = dw[-fp:][:f, :k].to(udt)
+        if need_d:
+            dwd = product(dy, h, None, None, True, True, ddt != _BF16)[:dshape[0], :f].to(ddt)
+        return dx, dwg, dwu, dwd, None
+
+
+def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
+    """``(act(x W_gate^T) * (x W_up^T)) W_down^T`` (see :func:`ops.gated_ffn`), under autograd too; bf16 on
+    the GPU, where gradients come in their tensor's type.  First derivatives only."""
+    if not x.is_cuda:
+        ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
+        return ref.gated_ffn(x, w_gate, w_up, w_down, act)
+    if _fused(x, w_gate, w_up, w_down):
+        return ops.gated_ffn(x, w_gate, w_up, w_down, act)
+    ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
+    if 0 in w_gate.shape or 0 in w_down.shape:                # empty sums
+        return ref.gated_ffn(x.to(_BF16), w_gate, w_up, w_down, act)
+    return _GatedFFNFn.apply(x, w_gate, w_up, w_down, act)

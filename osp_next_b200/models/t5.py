@@ -21,6 +21,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import functional as Fn
+from ..ops import SequencePack
+
 
 class T5LayerNorm(nn.Module):
     def __init__(self, dim, eps=1e-6):
@@ -63,6 +66,13 @@ class T5RelativeEmbedding(nn.Module):
         b = relative_position_bucket(rel, self.num_buckets, self.bidirectional, self.max_dist)
         return self.embedding(b).permute(2, 0, 1).unsqueeze(0).contiguous()     # [1, H, Lq, Lk]
 
+    def table(self, length):
+        """The bias by relative position alone, fp32 [H, 2 length - 1]: entry d + length - 1 is that of
+        key position - query position = d."""
+        rel = torch.arange(1 - length, length, device=self.embedding.weight.device)
+        b = relative_position_bucket(rel, self.num_buckets, self.bidirectional, self.max_dist)
+        return self.embedding(b).t().float().contiguous()
+
 
 class T5Attention(nn.Module):
     def __init__(self, dim, dim_attn, num_heads, dropout=0.1):
@@ -74,7 +84,11 @@ class T5Attention(nn.Module):
         self.o = nn.Linear(dim_attn, dim, bias=False)
         self.dropout = nn.Dropout(dropout)
 
-    def forward(self, x, context=None, mask=None, pos_bias=None):
+    def forward(self, x, context=None, mask=None, pos_bias=None, pack=None):
+        if pack is not None:        # packed rows [N, dim], pos_bias [heads, 2 M - 1] by relative position
+            q, k, v = (m(x).unflatten(-1, (self.num_heads, self.head_dim)) for m in (self.q, self.k, self.v))
+            o = Fn.packed_attention(q, k, v, pack, causal=False, scale=1.0, rel_bias=pos_bias)
+            return self.dropout(self.o(o.to(x.dtype).flatten(1)))
         ctx = x if context is None else context
         b, n, c = x.size(0), self.num_heads, self.head_dim
         q = self.q(x).view(b, -1, n, c).transpose(1, 2)
@@ -101,6 +115,10 @@ class T5FeedForward(nn.Module):
         self.dropout = nn.Dropout(dropout)
 
     def forward(self, x):
+        ws = (self.gate[0].weight, self.fc1.weight, self.fc2.weight)
+        if (x.is_cuda and x.dtype == torch.bfloat16 and all(w.dtype == torch.bfloat16 for w in ws)
+                and not (self.training and self.dropout.p > 0)):
+            return Fn.gated_ffn(x, *ws, act="gelu_tanh")        # one kernel up to the product, one down
         return self.dropout(self.fc2(self.dropout(self.fc1(x) * self.gate(x))))
 
 
@@ -121,9 +139,12 @@ class T5SelfAttention(nn.Module):
         self.ffn = T5FeedForward(dim, dim_ffn, dropout)
         self.pos_embedding = None if shared_pos else T5RelativeEmbedding(num_buckets, num_heads, True)
 
-    def forward(self, x, mask=None, pos_bias=None):
-        e = pos_bias if self.shared_pos else self.pos_embedding(x.size(1), x.size(1))
-        x = _fp16_clamp(x + self.attn(self.norm1(x), mask=mask, pos_bias=e))
+    def forward(self, x, mask=None, pos_bias=None, pack=None):
+        if pack is not None:
+            e = pos_bias if self.shared_pos else self.pos_embedding.table(max(pack.longest, 1))
+        else:
+            e = pos_bias if self.shared_pos else self.pos_embedding(x.size(1), x.size(1))
+        x = _fp16_clamp(x + self.attn(self.norm1(x), mask=mask, pos_bias=e, pack=pack))
         return _fp16_clamp(x + self.ffn(self.norm2(x)))
 
 
@@ -141,11 +162,15 @@ class T5Encoder(nn.Module):
         self.norm = T5LayerNorm(dim)
         self.apply(_init)
 
-    def forward(self, ids, mask=None):
+    def forward(self, ids, mask=None, pack=None):
+        """ids [B, L] and a mask -> [B, L, dim]; or, with a :class:`ops.SequencePack`, the tokens of its
+        sequences alone, ids [N] -> [N, dim] (no padding is computed)."""
         x = self.dropout(self.token_embedding(ids))
-        e = self.pos_embedding(x.size(1), x.size(1)) if self.shared_pos else None
+        e = None
+        if self.shared_pos:
+            e = self.pos_embedding.table(max(pack.longest, 1)) if pack is not None else self.pos_embedding(x.size(1), x.size(1))
         for blk in self.blocks:
-            x = blk(x, mask, pos_bias=e)
+            x = blk(x, mask, pos_bias=e, pack=pack)
         return self.dropout(self.norm(x))
 
 
@@ -220,10 +245,32 @@ class T5EncoderModel:
             ids, mask = self.tokenizer(ids_or_texts, return_mask=True, add_special_tokens=True)
         else:
             ids = ids_or_texts
+        real = mask.gt(0).cpu()
+        lengths = real.sum(1)
+        prefix = torch.equal(real, torch.arange(real.shape[1])[None] < lengths[:, None])
+        dev = torch.device(self.device)
+        if prefix and dev.type == "cuda" and self._packs():
+            return self._encode_packed(ids.to(dev), real, lengths.tolist())
         ids, mask = ids.to(self.device), mask.to(self.device)
-        seq_lens = mask.gt(0).sum(dim=1).long()
         ctx = self.model(ids, mask)
         out = torch.zeros(ids.shape[0], self.text_len, ctx.shape[-1], dtype=ctx.dtype, device=ctx.device)
-        for i, L in enumerate(seq_lens.tolist()):
+        for i, L in enumerate(lengths.tolist()):
             out[i, :L] = ctx[i, :L]
         return out
+
+    def _packs(self) -> bool:
+        """Whether the packed kernels take this encoder: bf16, heads of a multiple of 8 up to 128."""
+        attn = next((m for m in self.model.modules() if isinstance(m, T5Attention)), None)
+        return (attn is not None and attn.head_dim % 8 == 0 and attn.head_dim <= 128
+                and self.model.token_embedding.weight.dtype == torch.bfloat16)
+
+    def _encode_packed(self, ids, real, lengths):
+        """The prompts' tokens one behind another through the encoder, then zero-padded rows."""
+        if max(lengths, default=0) > self.text_len:
+            raise ValueError(f"a prompt of {max(lengths)} tokens, text_len is {self.text_len}")
+        at = real.flatten().nonzero()[:, 0].to(ids.device)           # places of the tokens in [B, L]
+        ctx = self.model(ids.flatten()[at], pack=SequencePack(lengths, device=ids.device))
+        L = real.shape[1]
+        out = torch.zeros(ids.shape[0] * self.text_len, ctx.shape[-1], dtype=ctx.dtype, device=ctx.device)
+        out[at // L * self.text_len + at % L] = ctx
+        return out.view(ids.shape[0], self.text_len, -1)

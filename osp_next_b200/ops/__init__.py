@@ -16,7 +16,9 @@ from . import reference as ref
 from ._ext import ext, available  # noqa: F401
 from .fp8 import (Fp8Tensor, adamw8_decode, adamw8_state, adamw_multi_, fp8_matmul, fp8_quantize,  # noqa: F401
                   fp8_quantize_with_sums)
+from .gated import gated_ffn, gated_linear  # noqa: F401
 from .packed import SequencePack, packed_attention, packed_attention_bwd  # noqa: F401
+from .rotary import rotary, rotary_angles, rotary_table  # noqa: F401
 
 _BF16 = torch.bfloat16
 
@@ -463,7 +465,7 @@ ERROR_NAMES = {
     111: "fp8 product producer wait", 112: "fp8 product MMA wait", 113: "fp8 product epilogue wait",
     114: "fp8 product teardown",
     201: "attention producer wait", 202: "attention MMA wait", 203: "attention softmax wait",
-    204: "attention teardown", 205: "attention shared-memory alignment",
+    204: "attention teardown", 205: "attention shared-memory alignment", 221: "rotary position outside the table",
     301: "NVLink peer barrier timeout", 302: "NVLink peer barrier slot mismatch",
     901: "probe mbarrier wait", 902: "probe flag wait",
 }

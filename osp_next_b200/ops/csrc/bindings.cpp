@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <map>
 #include <mutex>
+#include <string>
 #include <utility>
 
 #include "tma_host.h"
@@ -51,6 +52,13 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k
                                         const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, bool causal, double scale, bool fill);
+std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act,
+                                         bool keep);
+std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor& wd, const at::Tensor& gu, int64_t act);
+at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& a2,
+                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32);
+std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos,
+                                     const at::Tensor& table, std::vector<int64_t> sections, bool half, bool inverse);
 void cfg_euler(const at::Tensor& lat, const at::Tensor& cond, const at::Tensor& unc, at::Tensor& out, double g,
                double dt);
 void hif8_round(const at::Tensor& x, at::Tensor& out, double s);
@@ -100,7 +108,8 @@ static int* g_err[kMaxDevices] = {nullptr};
 static std::mutex g_err_mu;
 
 static void check_device(int device) {
-  TORCH_CHECK(device >= 0 && device < kMaxDevices, "device ordinal ", device, " out of range [0, ", kMaxDevices, ")");
+  TORCH_CHECK(device >= 0 && device < kMaxDevices, "device ordinal ", std::to_string(device), " out of range [0, ",
+              std::to_string(kMaxDevices), ")");
 }
 
 int* error_word(int device) {
@@ -170,6 +179,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_bwd", &osp::attention_bwd);
   m.def("packed_attn_fwd", &osp::packed_attn_fwd);
   m.def("packed_attn_bwd", &osp::packed_attn_bwd);
+  m.def("gated_linear_fwd", &osp::gated_linear_fwd);
+  m.def("gated_linear_bwd", &osp::gated_linear_bwd);
+  m.def("ffn_product", &osp::ffn_product);
+  m.def("rotary_apply", &osp::rotary_apply);
   m.def("cfg_euler", &osp::cfg_euler);
   m.def("hif8_round", &osp::hif8_round);
   m.def("hif8_qdq", &osp::hif8_qdq);

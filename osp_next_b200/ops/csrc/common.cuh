@@ -22,6 +22,7 @@ enum : int {
   kErrFp8Producer = 111, kErrFp8Mma = 112, kErrFp8Epilogue = 113, kErrFp8Teardown = 114,
   kErrAttnProducer = 201, kErrAttnMma = 202, kErrAttnSoftmax = 203, kErrAttnTeardown = 204,
   kErrAttnLayout = 205,
+  kErrRotaryPosition = 221,
   kErrP2P = 301, kErrP2PTag = 302,
   kErrProbeMbar = 901, kErrProbeFlag = 902,
 };

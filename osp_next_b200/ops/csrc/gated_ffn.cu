@@ -1,0 +1,450 @@
+// Gated feed-forward block:  h = act(x Wg^T) o (x Wu^T),  y = h Wd^T, and its gradients.
+//
+//   act(g) = g sigmoid(c (g)),  c(g) = g (SiLU) or 2 sqrt(2/pi) (g + 0.044715 g^3) (GELU, tanh form)
+//   forward   one kernel forms both projections: a tile of 256 accumulator columns holds 128 of g and
+//             the same 128 of u (TMA loads 128 rows of either weight behind one another, so no weight
+//             is packed), and the epilogue writes act(g) u, in training g and u too
+//   backward  dh = dy Wd with the epilogue  dg = dh u act'(g),  du = dh act(g),  h = act(g) u, which
+//             also brings h back for dWd (it is not kept); then dx = dg Wg + du Wu as one product over
+//             two operand pairs, [dWg; dWu] = [dg | du]^T x, dWd = dy^T h
+//
+// All are tiles of 128 x BN of one persistent kernel (a CTA per SM, 320 threads): warp 0 loads, warp 1
+// issues tcgen05.mma into one of two accumulators, warps 2..9 are two groups of epilogue warps that take
+// half of the tile's columns each.  Operands lie K-major or MN-major as the tensors are; results leave
+// through shared memory as whole 64-byte row segments.  Sums are fp32 in tensor memory; g, u, dg, du and
+// h are rounded to bf16 once, as operands of the next product have to be.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "common.cuh"
+#include <string>
+
+#include "tma_host.h"
+
+namespace osp {
+namespace ffn {
+
+constexpr int kBM = 128, kBK = 64, kGroupM = 16, kThreads = 320;
+constexpr int kRing = 196608;
+constexpr int kStageRow = 80;                 // bytes per staged row (64 + 16 pad)
+constexpr int kStageBytes = 32 * kStageRow;
+
+enum Mode : int { kPlain = 0, kGate = 1, kGateBwd = 2 };
+enum Act : int { kSilu = 0, kGeluTanh = 1 };
+
+struct Args {
+  int M, N, K, K2;             // result [M, N]; K2: depth of the second operand pair (kPlain)
+  int act;
+  __nv_bfloat16* out;          // kPlain: [M, N]; kGate: h [M, N]; kGateBwd: h [M, N]
+  float* out32;                // kPlain: the result in fp32 instead (gradients of fp32 weights), or null
+  __nv_bfloat16* gu;           // [M, 2 N]: g | u written (kGate, or null), read (kGateBwd)
+  __nv_bfloat16* dgu;          // [M, 2 N]: dg | du written (kGateBwd)
+  int* err;
+};
+
+__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+// act(g), and its derivative where asked for.  g sigmoid(z): tanh(a) = 2 sigmoid(2 a) - 1.
+template <bool kGrad>
+__device__ __forceinline__ float act_f(int act, float g, float& d) {
+  float z = g, dz = 1.0f;
+  if (act == kGeluTanh) {
+    const float k = 1.5957691216057308f;      // 2 sqrt(2 / pi)
+    const float g2 = g * g;
+    z = k * g * fmaf(0.044715f, g2, 1.0f);
+    if (kGrad) dz = k * fmaf(3.0f * 0.044715f, g2, 1.0f);
+  }
+  const float s = sigmoid_f(z);
+  // act' = s + g s (1 - s) z'; far from 0 (1 - s) s underflows before z' overflows
+  if (kGrad) d = s + (g * s) * ((1.0f - s) * dz);
+  return g * s;
+}
+
+__device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int& mb, int& nb) {
+  const int per_group = kGroupM * num_n;
+  const int g = t / per_group;
+  const int first_m = g * kGroupM;
+  const int gsize = min(num_m - first_m, kGroupM);
+  const int r = t - g * per_group;
+  mb = first_m + r % gsize;
+  nb = r / gsize;
+}
+
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+__device__ __forceinline__ void unpack8(const uint4& w, float* v) {
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// A warp's 32 rows x 32 columns (a row per lane) to dst [rows of `pitch`], in 64-byte row segments.
+__device__ __forceinline__ void store_tile(const float* v, uint8_t* stg, __nv_bfloat16* dst, long pitch, long row0,
+                                           int rows, int col0, int cols, int lane) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stg + lane * kStageRow + j * 16) = pack8(v + 8 * j);
+  __syncwarp();
+  const int q = lane >> 2, cc = lane & 3;
+  if (col0 + cc * 8 < cols) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = i * 8 + q;
+      if (row0 + rr < rows)
+        *reinterpret_cast<uint4*>(dst + (row0 + rr) * pitch + col0 + cc * 8) =
+            *reinterpret_cast<const uint4*>(stg + rr * kStageRow + cc * 16);
+    }
+  }
+  __syncwarp();
+}
+// The same way in: 32 columns of this lane's row, zeros outside.
+__device__ __forceinline__ void load_tile(float* v, uint8_t* stg, const __nv_bfloat16* src, long pitch, long row0,
+                                          int rows, int col0, int cols, int lane) {
+  const int q = lane >> 2, cc = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rr = i * 8 + q;
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (row0 + rr < rows && col0 + cc * 8 < cols)
+      w = *reinterpret_cast<const uint4*>(src + (row0 + rr) * pitch + col0 + cc * 8);
+    *reinterpret_cast<uint4*>(stg + rr * kStageRow + cc * 16) = w;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) unpack8(*reinterpret_cast<const uint4*>(stg + lane * kStageRow + j * 16), v + 8 * j);
+  __syncwarp();
+}
+
+// kGate: the tile's BN accumulator columns are BN / 2 of g and BN / 2 of u; A [M, K], B1 = Wg, B2 = Wu.
+// kPlain with K2 > 0: D = A1 B1^T + A2 B2^T.
+template <int BN, int MODE, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+     const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2, const Args args) {
+  constexpr uint32_t A_BYTES = kBM * kBK * 2, B_BYTES = BN * kBK * 2;
+  constexpr int STAGES = kRing / (A_BYTES + B_BYTES);
+  constexpr uint32_t MN_BOX = 64 * kBK * 2;
+  constexpr uint32_t IDESC = idesc_bf16(kBM, BN, B_MN, A_MN);
+  constexpr int OUT_N = MODE == kGate ? BN / 2 : BN;        // result columns of a tile
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_BYTES;
+  uint8_t* epi = sB + STAGES * B_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi + 8 * kStageBytes);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int num_m = (args.M + kBM - 1) / kBM;
+  const int num_n = (args.N + OUT_N - 1) / OUT_N;
+  const int num_tiles = num_m * num_n;
+  const int num_kb1 = (args.K + kBK - 1) / kBK;
+  const int num_kb = num_kb1 + (args.K2 + kBK - 1) / kBK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 8); }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    if (MODE == kGate || args.K2 > 0) prefetch_tmap(&tmB2);
+    if (args.K2 > 0) prefetch_tmap(&tmA2);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+        int mb, nb;
+        tile_coords(t, num_m, num_n, mb, nb);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, args.err, kErrGemmProducer)) { *abort_flag = 1; break; }
+          mbar_expect_tx(&full[stage], A_BYTES + B_BYTES);
+          const bool second = kb >= num_kb1;
+          const CUtensorMap* ta = second ? &tmA2 : &tmA;
+          const CUtensorMap* tb = second ? &tmB2 : &tmB;
+          const int kc = (second ? kb - num_kb1 : kb) * kBK;
+          uint8_t* a = sA + stage * A_BYTES;
+          uint8_t* b = sB + stage * B_BYTES;
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int c = 0; c < kBM / 64; ++c) tma_load_2d(ta, &full[stage], a + c * MN_BOX, mb * kBM + 64 * c, kc);
+          } else {
+            tma_load_2d(ta, &full[stage], a, kc, mb * kBM);
+          }
+          if constexpr (MODE == kGate) {
+            tma_load_2d(&tmB, &full[stage], b, kc, nb * OUT_N);
+            tma_load_2d(&tmB2, &full[stage], b + B_BYTES / 2, kc, nb * OUT_N);
+          } else if constexpr (B_MN) {
+#pragma unroll
+            for (int c = 0; c < BN / 64; ++c) tma_load_2d(tb, &full[stage], b + c * MN_BOX, nb * BN + 64 * c, kc);
+          } else {
+            tma_load_2d(tb, &full[stage], b, kc, nb * BN);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x, ++it) {
+        const int acc = it & 1;
+        if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1, args.err, kErrGemmMma)) { *abort_flag = 1; break; }
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * BN;
+        bool ok = true;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, args.err, kErrGemmMma)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a = smem_u32(sA + stage * A_BYTES), b = smem_u32(sB + stage * B_BYTES);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            const uint64_t ad = A_MN ? sdesc_sw128(a + k * 2048, MN_BOX, 1024) : sdesc_sw128(a + k * 32, 16, 1024);
+            const uint64_t bd = B_MN ? sdesc_sw128(b + k * 2048, MN_BOX, 1024) : sdesc_sw128(b + k * 32, 16, 1024);
+            umma_bf16(d, ad, bd, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          umma_commit(&empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        umma_commit(&tfull[acc]);
+        if (!ok) { *abort_flag = 1; break; }
+      }
+      umma_commit(done);
+      mbar_wait(done, 0, args.err, kErrGemmTeardown);
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
+    uint8_t* stg = epi + (warp - 2) * kStageBytes;
+    int it = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, ++it) {
+      if (*abort_flag) break;
+      int mb, nb;
+      tile_coords(t, num_m, num_n, mb, nb);
+      const int acc = it & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (it >> 1) & 1, args.err, kErrGemmEpilogue))) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const long row0 = (long)mb * kBM + quarter * 32;
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c = half * (OUT_N / 64); c < (half + 1) * (OUT_N / 64); ++c) {
+        const int col0 = nb * OUT_N + c * 32;
+        if (col0 >= args.N) continue;                       // uniform across the warp
+        uint32_t r[32];
+        tmem_ld32(t_row + c * 32, r);
+        float v[32];
+        if constexpr (MODE == kGate) {
+          uint32_t ru[32];
+          tmem_ld32(t_row + BN / 2 + c * 32, ru);
+          tmem_ld_wait();
+          float u[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) { v[j] = __uint_as_float(r[j]); u[j] = __uint_as_float(ru[j]); }
+          if (args.gu) {
+            store_tile(v, stg, args.gu, 2l * args.N, row0, args.M, col0, args.N, lane);
+            store_tile(u, stg, args.gu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float d;
+            v[j] = act_f<false>(args.act, v[j], d) * u[j];
+          }
+        } else if constexpr (MODE == kGateBwd) {
+          float g[32], u[32];
+          load_tile(g, stg, args.gu, 2l * args.N, row0, args.M, col0, args.N, lane);
+          load_tile(u, stg, args.gu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float d;
+            const float a = act_f<true>(args.act, g[j], d), dh = __uint_as_float(r[j]);
+            v[j] = a * u[j];
+            g[j] = dh * u[j] * d;
+            u[j] = dh * a;
+          }
+          store_tile(g, stg, args.dgu, 2l * args.N, row0, args.M, col0, args.N, lane);
+          store_tile(u, stg, args.dgu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
+        } else {
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        }
+        if (MODE == kPlain && args.out32) {
+          // a lane's row piece is a whole 128-byte line
+          if (row0 + lane < args.M) {
+            float4* o = reinterpret_cast<float4*>(args.out32 + (row0 + lane) * args.N + col0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col0 + 4 * j < args.N) o[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        } else {
+          store_tile(v, stg, args.out, args.N, row0, args.M, col0, args.N, lane);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+template <int BN>
+constexpr int smem_bytes() {
+  constexpr int stage = kBM * kBK * 2 + BN * kBK * 2;
+  return 1024 + kRing / stage * stage + 8 * kStageBytes + (2 * (kRing / stage) + 5) * 8 + 16;
+}
+
+// A row-major matrix; `mn`: its rows run along K, boxes are 64 columns x kBK rows.
+static CUtensorMap map_of(const at::Tensor& t, bool mn, int rows_box) {
+  return make_tmap_2d_bf16(t.data_ptr(), t.size(1), t.size(0), t.stride(0), 64, mn ? kBK : rows_box);
+}
+
+template <int BN, int MODE, bool A_MN, bool B_MN>
+static void launch(const at::Tensor& a, const at::Tensor& b, const at::Tensor* a2, const at::Tensor* b2, Args args,
+                   cudaStream_t stream) {
+  constexpr int b_rows = MODE == kGate ? BN / 2 : BN;
+  const CUtensorMap ma = map_of(a, A_MN, kBM), mb = map_of(b, B_MN, b_rows);
+  const CUtensorMap ma2 = a2 ? map_of(*a2, A_MN, kBM) : ma, mb2 = b2 ? map_of(*b2, B_MN, b_rows) : mb;
+  auto kern = gemm<BN, MODE, A_MN, B_MN>;
+  constexpr int smem = smem_bytes<BN>();
+  smem_opt_in(reinterpret_cast<const void*>(kern), smem);
+  constexpr int out_n = MODE == kGate ? BN / 2 : BN;
+  const long tiles = ((long)args.M + kBM - 1) / kBM * ((args.N + out_n - 1) / out_n);
+  kern<<<(unsigned)std::min<long>(tiles, num_sms(a.get_device())), kThreads, smem, stream>>>(ma, mb, ma2, mb2, args);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+static void check(const at::Tensor& t, const at::Tensor& x, int64_t rows, int64_t cols, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 &&
+              t.size(0) == rows && t.size(1) == cols, "gated_ffn: ", what, " bf16 [", std::to_string(rows), ", ", std::to_string(cols), "]");
+  TORCH_CHECK(cols % 8 == 0 && t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= cols &&
+              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "gated_ffn: ", what,
+              " in rows at multiples of 16 bytes");
+  TORCH_CHECK(rows < (1ll << 30) && cols < (1ll << 30), "gated_ffn: ", what, " too large");
+}
+
+static Args make_args(const at::Tensor& x, int64_t M, int64_t N, int64_t K, int64_t act) {
+  Args a{};
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.act = (int)act;
+  a.err = error_word(x.get_device());
+  return a;
+}
+
+}  // namespace ffn
+
+// {h [M, F]} or, with `keep`, {h, gu [M, 2 F]}: h = act(x wg^T) (x wu^T).
+std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act,
+                                         bool keep) {
+  using namespace ffn;
+  TORCH_CHECK(x.dim() == 2 && wg.dim() == 2, "gated_ffn: x [M, K], weights [F, K]");
+  const int64_t M = x.size(0), K = x.size(1), F = wg.size(0);
+  check(x, x, M, K, "x");
+  check(wg, x, F, K, "gate weight");
+  check(wu, x, F, K, "up weight");
+  TORCH_CHECK(F % 8 == 0 && K > 0, "gated_ffn: F a multiple of 8");
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor h = at::empty({M, F}, x.options()), gu;
+  if (keep) gu = at::empty({M, 2 * F}, x.options());
+  if (M > 0 && F > 0) {
+    Args a = make_args(x, M, F, K, act);
+    a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
+    a.gu = keep ? reinterpret_cast<__nv_bfloat16*>(gu.data_ptr()) : nullptr;
+    launch<256, kGate, false, false>(x, wg, nullptr, &wu, a, c10::cuda::getCurrentCUDAStream());
+  }
+  return {h, gu};
+}
+
+// {h [M, F], dgu [M, 2 F]} of dy [M, C], wd [C, F] and the kept gu [M, 2 F].
+std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor& wd, const at::Tensor& gu, int64_t act) {
+  using namespace ffn;
+  TORCH_CHECK(dy.dim() == 2 && wd.dim() == 2, "gated_ffn: dy [M, C], down weight [C, F]");
+  const int64_t M = dy.size(0), C = dy.size(1), F = wd.size(1);
+  check(dy, dy, M, C, "output gradient");
+  check(wd, dy, C, F, "down weight");
+  check(gu, dy, M, 2 * F, "kept projections");
+  TORCH_CHECK(gu.is_contiguous() && F % 8 == 0 && C > 0, "gated_ffn: contiguous kept projections, F a multiple of 8");
+  c10::cuda::CUDAGuard guard(dy.device());
+  at::Tensor h = at::empty({M, F}, dy.options()), dgu = at::empty({M, 2 * F}, dy.options());
+  if (M > 0 && F > 0) {
+    Args a = make_args(dy, M, F, C, act);
+    a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
+    a.gu = reinterpret_cast<__nv_bfloat16*>(gu.data_ptr());
+    a.dgu = reinterpret_cast<__nv_bfloat16*>(dgu.data_ptr());
+    launch<256, kGateBwd, false, true>(dy, wd, nullptr, nullptr, a, c10::cuda::getCurrentCUDAStream());
+  }
+  return {h, dgu};
+}
+
+// A B^T (+ A2 B2^T) in bf16 or fp32.  a [M, K] or, with a_mn, [K, M]; b [N, K] or, with b_mn, [K, N].
+at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& a2,
+                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32) {
+  using namespace ffn;
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2, "gated_ffn: matrices");
+  const int64_t M = a.size(a_mn ? 1 : 0), K = a.size(a_mn ? 0 : 1), N = b.size(b_mn ? 1 : 0);
+  check(a, a, a.size(0), a.size(1), "operand");
+  check(b, a, b_mn ? K : N, b_mn ? N : K, "operand");
+  TORCH_CHECK(N % 8 == 0 && a2.has_value() == b2.has_value(), "gated_ffn: result columns a multiple of 8");
+  c10::cuda::CUDAGuard guard(a.device());
+  Args args = make_args(a, M, N, K, 0);
+  if (a2.has_value()) {
+    check(*a2, a, a.size(0), a.size(1), "second operand");
+    check(*b2, a, b.size(0), b.size(1), "second operand");
+    args.K2 = (int)K;
+  }
+  at::Tensor out = at::empty({M, N}, f32 ? a.options().dtype(at::kFloat) : a.options());
+  if (M == 0 || N == 0) return out;
+  if (K == 0) return out.zero_();
+  if (f32) args.out32 = out.data_ptr<float>();
+  else args.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  const at::Tensor* pa = a2.has_value() ? &*a2 : nullptr;
+  const at::Tensor* pb = b2.has_value() ? &*b2 : nullptr;
+  auto stream = c10::cuda::getCurrentCUDAStream();
+  TORCH_CHECK(b_mn || !a_mn, "gated_ffn: operand order");
+  if (a_mn) launch<256, kPlain, true, true>(a, b, pa, pb, args, stream);
+  else if (b_mn) launch<256, kPlain, false, true>(a, b, pa, pb, args, stream);
+  else launch<256, kPlain, false, false>(a, b, pa, pb, args, stream);
+  return out;
+}
+
+}  // namespace osp

@@ -14,8 +14,12 @@
 // first column per key; in dq it is a limit per row.  Items of dkdv with far more than their share of
 // the work (the first keys of a long causal sequence) are split along the queries; their fp32 parts
 // are added in a fixed order by packed_join_kernel.
-#include <torch/extension.h>
-#include <ATen/cuda/CUDAContext.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "packed_attn.cuh"
@@ -655,7 +659,7 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k
   at::Tensor dq = make({s.Nq, s.Hq, s.D}), dk = make({s.Nk, s.Hkv, s.D}), dv = make({s.Nk, s.Hkv, s.D});
   if ((rows.size(0) == 0 && keys.size(0) == 0) || s.Hq == 0 || s.D == 0) return {dq, dk, dv};
   if (s.Nq == 0) return {dq, dk.zero_(), dv.zero_()};
-  auto stream = at::cuda::getCurrentCUDAStream();
+  auto stream = c10::cuda::getCurrentCUDAStream();
   at::Tensor delta = at::empty({s.Nq, s.Hq}, opt.dtype(at::kFloat));
   const long n = (long)s.Nq * s.Hq;
   if (n > 0) {

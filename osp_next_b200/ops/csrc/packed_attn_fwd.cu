@@ -12,8 +12,12 @@
 //
 // Items with many keys and few rows are split along the keys: each part leaves its normalised fp32
 // output and log-sum-exp in a workspace and packed_combine_kernel joins them.
-#include <torch/extension.h>
-#include <ATen/cuda/CUDAContext.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "attention_fwd.cuh"
@@ -440,7 +444,7 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k
   const CUtensorMap tq = pa::tile_map(q, q, s.D, s.G, a.P);
   const CUtensorMap tk = pa::tile_map(k, q, s.D, 1, pa::kRows), tv = pa::tile_map(v, q, s.D, 1, pa::kRows);
   dim3 grid((unsigned)(n * s.Hkv));
-  auto stream = at::cuda::getCurrentCUDAStream();
+  auto stream = c10::cuda::getCurrentCUDAStream();
   if (s.D > 64) {
     if (a.bias) launch_packed_fwd<128, true>(grid, tq, tk, tv, a, stream);
     else launch_packed_fwd<128, false>(grid, tq, tk, tv, a, stream);

@@ -1,6 +1,6 @@
 // Host checks and tensor maps of the packed attention launchers.
 #pragma once
-#include <torch/extension.h>
+#include <ATen/core/Tensor.h>
 
 #include "packed_attn.cuh"
 #include "tma_host.h"

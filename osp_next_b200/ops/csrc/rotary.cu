@@ -1,0 +1,242 @@
+// Rotary positions of q and k in one launch: interleaved or half layout, part of the head, positions of
+// one or several axes, cosines and sines from a table (rotary_table in ops/rotary.py evaluates it in 64
+// bits, scaled for long contexts or not).
+//
+//   pair i of a head: (a, b) -> (a c - b s, a s + b c),  (c, s) = table[pos[axis(i)], i]
+//   pairs: elements (2 i, 2 i + 1) interleaved, (i, i + R / 2) half layout; elements from R on are copied
+//
+// Bound by memory: each value is read and written once, and the R / 2 pairs of a token's table row
+// serve all heads of q and k.  A warp takes one token: its lanes hold the cosines and sines of the
+// vector pieces that they own in registers and pass over the heads, so that a table entry is read once
+// per token and not once per head.  The inverse (gradients) turns by -s.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+#include <string>
+
+#include "common.cuh"
+#include "tma_host.h"
+
+namespace osp {
+namespace rotary {
+
+struct Tensor {
+  const void* in;
+  void* out;                   // [n, heads, D], contiguous
+  long row, head;              // strides of `in` in elements
+  int heads;
+};
+
+struct Args {
+  Tensor t[2];
+  const int* pos;              // [n, axes]
+  const float2* table;         // [positions, R / 2]
+  long n;
+  int axes, positions;
+  int D, R;
+  int end[4];                  // axis a owns pairs end[a - 1] .. end[a] - 1
+  float sign;                  // 1, or -1 for the inverse
+  int* err;
+};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec { T v[V]; };
+
+__device__ __forceinline__ float2 pair_of(const Args& a, long token, int i, int first_pos, bool& bad) {
+  int axis = 0;
+  while (axis + 1 < a.axes && i >= a.end[axis]) ++axis;
+  const int p = a.axes == 1 ? first_pos : a.pos[token * a.axes + axis];
+  if (p < 0 || p >= a.positions) {          // no such position: NaN results and an error for the host
+    bad = true;
+    return make_float2(NAN, NAN);
+  }
+  const float2 cs = a.table[(long)p * (a.R / 2) + i];
+  return make_float2(cs.x, cs.y * a.sign);
+}
+
+// One piece = V elements of a pair's first half and V of its second (half layout), or V elements
+// (V / 2 pairs, interleaved; also the copied elements).  Pieces of a head: half layout R / 2 / V and
+// (D - R) / V to copy, interleaved D / V.
+template <typename T, int V, bool kHalf, int kPieces>
+__global__ void __launch_bounds__(256)
+rotate(const Args args) {
+  const long token = (long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (token >= args.n) return;
+  const int lane = threadIdx.x % 32;
+  const int R = args.R, D = args.D;
+  const int turned = kHalf ? R / 2 / V : R / V;
+  const int pieces = turned + (D - R) / V;
+  const int first_pos = args.axes == 1 ? args.pos[token] : 0;
+  bool bad = false;
+  // heads are dealt so that a warp is full: `per` lanes to a head, 32 / per heads at a time
+  int per = 1;
+  while (per < pieces && per < 32) per <<= 1;
+  const int sub = lane % per, group = lane / per, groups = 32 / per;
+  float2 cs[kPieces][V];
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const int p = sub + k * per;
+    if (p < turned) {
+#pragma unroll
+      for (int j = 0; j < (kHalf ? V : V / 2); ++j)
+        cs[k][j] = pair_of(args, token, p * (kHalf ? V : V / 2) + j, first_pos, bad);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const Tensor& t = args.t[w];
+    const T* in = reinterpret_cast<const T*>(t.in) + token * t.row;
+    T* out = reinterpret_cast<T*>(t.out) + token * t.heads * D;
+    for (int h = group; h < t.heads; h += groups) {
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) {
+        const int p = sub + k * per;
+        if (p >= pieces) continue;
+        const T* src = in + h * t.head;
+        T* dst = out + (long)h * D;
+        if (p >= turned) {
+          const int o = R + (p - turned) * V;
+          *reinterpret_cast<Vec<T, V>*>(dst + o) = *reinterpret_cast<const Vec<T, V>*>(src + o);
+        } else if (kHalf) {
+          const Vec<T, V> a = *reinterpret_cast<const Vec<T, V>*>(src + p * V);
+          const Vec<T, V> b = *reinterpret_cast<const Vec<T, V>*>(src + R / 2 + p * V);
+          Vec<T, V> x, y;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float fa = to_f(a.v[j]), fb = to_f(b.v[j]);
+            x.v[j] = from_f<T>(fa * cs[k][j].x - fb * cs[k][j].y);
+            y.v[j] = from_f<T>(fa * cs[k][j].y + fb * cs[k][j].x);
+          }
+          *reinterpret_cast<Vec<T, V>*>(dst + p * V) = x;
+          *reinterpret_cast<Vec<T, V>*>(dst + R / 2 + p * V) = y;
+        } else {
+          const Vec<T, V> a = *reinterpret_cast<const Vec<T, V>*>(src + p * V);
+          Vec<T, V> x;
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            const float fa = to_f(a.v[2 * j]), fb = to_f(a.v[2 * j + 1]);
+            x.v[2 * j] = from_f<T>(fa * cs[k][j].x - fb * cs[k][j].y);
+            x.v[2 * j + 1] = from_f<T>(fa * cs[k][j].y + fb * cs[k][j].x);
+          }
+          *reinterpret_cast<Vec<T, V>*>(dst + p * V) = x;
+        }
+      }
+    }
+  }
+  if (bad) record_error(args.err, kErrRotaryPosition);
+}
+
+template <typename T, int V, bool kHalf>
+static void launch(const Args& a, cudaStream_t stream) {
+  const unsigned blocks = (unsigned)((a.n + 7) / 8);
+  const int turned = kHalf ? a.R / 2 / V : a.R / V;
+  const int pieces = turned + (a.D - a.R) / V;
+  if (pieces <= 32) rotate<T, V, kHalf, 1><<<blocks, 256, 0, stream>>>(a);
+  else if (pieces <= 64) rotate<T, V, kHalf, 2><<<blocks, 256, 0, stream>>>(a);
+  else rotate<T, V, kHalf, 8><<<blocks, 256, 0, stream>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+template <typename T>
+static void launch_type(const Args& a, bool half, int vec, cudaStream_t stream) {
+  constexpr int W = 16 / sizeof(T);
+  if (half) {
+    if (vec == W) launch<T, W, true>(a, stream);
+    else if (vec == 2) launch<T, 2, true>(a, stream);
+    else launch<T, 1, true>(a, stream);
+  } else {
+    if (vec == W) launch<T, W, false>(a, stream);
+    else launch<T, 2, false>(a, stream);
+  }
+}
+
+}  // namespace rotary
+
+// Rotated copies of q [n, Hq, D] and, if given, k [n, Hk, D].  pos int32 [n, axes]; table fp32
+// [positions, R / 2, 2]; sections: pairs of each axis (their sum R / 2).
+std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos,
+                                     const at::Tensor& table, std::vector<int64_t> sections, bool half, bool inverse) {
+  using namespace rotary;
+  const char* what = "rotary: ";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, what, "CUDA q [tokens, heads, head_dim]");
+  const int64_t n = q.size(0), D = q.size(2), R = 2 * table.size(1);
+  TORCH_CHECK(pos.device() == q.device() && pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.dim() == 2 &&
+              pos.size(0) == n && pos.size(1) == (int64_t)sections.size() && pos.size(1) >= 1 && pos.size(1) <= 4,
+              what, "positions int32 [tokens, axes], 1 to 4 axes");
+  TORCH_CHECK(table.device() == q.device() && table.scalar_type() == at::kFloat && table.is_contiguous() &&
+              table.dim() == 3 && table.size(2) == 2 && table.size(0) < (1ll << 31), what,
+              "table fp32 [positions, pairs, 2]");
+  TORCH_CHECK(R <= D && D <= 256 && D % 2 == 0, what, "table of ", std::to_string(R / 2), " pairs for a head dim of ", std::to_string(D),
+              " (even, at most 256)");
+  c10::cuda::CUDAGuard guard(q.device());
+  Args a{};
+  std::vector<at::Tensor> out;
+  const int size = (int)q.element_size();
+  int vec = 16 / size;
+  const at::Tensor* in[2] = {&q, k.has_value() ? &*k : nullptr};
+  for (int i = 0; i < 2 && in[i]; ++i) {
+    const at::Tensor& x = *in[i];
+    TORCH_CHECK(x.device() == q.device() && x.scalar_type() == q.scalar_type() && x.dim() == 3 && x.size(0) == n &&
+                x.size(2) == D && (D == 0 || x.stride(2) == 1), what, "q and k [tokens, heads, head_dim] of one type");
+    out.push_back(at::empty({n, x.size(1), D}, x.options()));
+    a.t[i] = {x.data_ptr(), out.back().data_ptr(), x.stride(0), x.stride(1), (int)x.size(1)};
+    auto fits = [&](int v) {
+      return reinterpret_cast<uintptr_t>(x.data_ptr()) % (v * size) == 0 && x.stride(0) % v == 0 && x.stride(1) % v == 0;
+    };
+    while (vec > 1 && !fits(vec)) vec >>= 1;
+  }
+  if (n == 0 || D == 0 || R == 0) {
+    for (int i = 0; i < 2 && in[i]; ++i) out[i].copy_(*in[i]);
+    return out;
+  }
+  // every piece lies in the turned or in the copied part
+  while (vec > 1 && ((half ? R / 2 : R) % vec || (D - R) % vec)) vec >>= 1;
+  const int wide = 16 / size;
+  vec = vec == wide ? wide : vec >= 2 ? 2 : 1;
+  if (!half && vec == 1) {       // pairs at odd addresses: one aligned copy, then as usual
+    std::vector<at::Tensor> c;
+    for (int i = 0; i < 2 && in[i]; ++i) c.push_back(in[i]->clone(at::MemoryFormat::Contiguous));
+    return rotary_apply(c[0], c.size() > 1 ? c10::optional<at::Tensor>(c[1]) : c10::nullopt, pos, table, sections,
+                        half, inverse);
+  }
+  a.pos = pos.data_ptr<int>();
+  a.table = reinterpret_cast<const float2*>(table.data_ptr<float>());
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(a.table) % 8 == 0, what, "table at a multiple of 8 bytes");
+  a.n = n;
+  a.axes = (int)sections.size();
+  a.positions = (int)table.size(0);
+  a.D = (int)D;
+  a.R = (int)R;
+  int64_t end = 0;
+  for (size_t i = 0; i < sections.size(); ++i) {
+    TORCH_CHECK(sections[i] >= 0, what, "sections from 0 on");
+    a.end[i] = (int)(end += sections[i]);
+  }
+  TORCH_CHECK(end == R / 2, what, "sections of ", std::to_string(end), " pairs, table of ",
+              std::to_string(R / 2));
+  a.sign = inverse ? -1.0f : 1.0f;
+  a.err = error_word(q.get_device());
+  auto stream = c10::cuda::getCurrentCUDAStream();
+  switch (q.scalar_type()) {
+    case at::kBFloat16: launch_type<__nv_bfloat16>(a, half, vec, stream); break;
+    case at::kHalf: launch_type<__half>(a, half, vec, stream); break;
+    case at::kFloat: launch_type<float>(a, half, vec, stream); break;
+    default: TORCH_CHECK(false, what, "bf16, fp16 or fp32");
+  }
+  return out;
+}
+
+}  // namespace osp

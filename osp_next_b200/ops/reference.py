@@ -394,3 +394,43 @@ def packed_attention_bwd(q, k, v, dout, pack, causal: bool, scale: float):
             return tuple(torch.zeros_like(t) for t in leaves)
         grads = torch.autograd.grad(o, leaves, dout.to(o.dtype), allow_unused=True)
     return tuple(torch.zeros_like(t) if g is None else g for t, g in zip(leaves, grads))
+
+
+# ----------------------------------------------------------------------------- gated feed-forward, rotary
+
+def gated_act(g: torch.Tensor, act: str) -> torch.Tensor:
+    return F.silu(g) if act == "silu" else F.gelu(g, approximate="tanh")
+
+
+def gated_linear(x, w_gate, w_up, act: str):
+    """act(x W_gate^T) * (x W_up^T) in fp32 (64 bits for 64-bit inputs), rounded to x's type."""
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xf = x.to(acc)
+    return (gated_act(xf @ w_gate.to(acc).t(), act) * (xf @ w_up.to(acc).t())).to(x.dtype)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, act: str):
+    """The whole gated block in fp32 (64 bits for 64-bit inputs); differentiable."""
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    return (gated_linear(x.to(acc), w_gate, w_up, act) @ w_down.to(acc).t()).to(x.dtype)
+
+
+def rotary(x, pos, table, layout: str, sections, inverse: bool = False):
+    """x [..., n, H, D] rotated by table [positions, pairs, 2] at pos [n, axes]; differentiable."""
+    if pos.numel() and (int(pos.min()) < 0 or int(pos.max()) >= table.shape[0]):
+        raise IndexError(f"rotary: positions 0 to {table.shape[0] - 1}, got {int(pos.min())} to {int(pos.max())}")
+    axis = torch.repeat_interleave(torch.tensor(sections, device=pos.device))
+    pair = torch.arange(table.shape[1], device=pos.device)
+    cs = table[pos.long()[:, axis], pair[None]]                                     # [n, pairs, 2]
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    c, s = cs[:, None, :, 0].to(acc), cs[:, None, :, 1].to(acc)
+    s = -s if inverse else s
+    r = 2 * table.shape[1]
+    y = x.to(acc)
+    if layout == "half":
+        a, b = y[..., :r // 2], y[..., r // 2:r]
+        z = torch.cat([a * c - b * s, a * s + b * c, y[..., r:]], -1)
+    else:
+        a, b = y[..., 0:r:2], y[..., 1:r:2]
+        z = torch.cat([torch.stack([a * c - b * s, a * s + b * c], -1).flatten(-2), y[..., r:]], -1)
+    return z.to(x.dtype)

@@ -22,10 +22,12 @@ frame sampling and the Qwen-VL resize rule are reimplemented below.
 """
 from __future__ import annotations
 
+import contextvars
 import glob
 import json
 import math
 import os
+import types
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -33,6 +35,9 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..models import functional as Fn
+from ..ops import SequencePack
 
 REWARD_TOKENS = ("<|VQ_reward|>", "<|MQ_reward|>", "<|TA_reward|>")
 DIMENSIONS = ("VQ", "MQ", "TA")
@@ -298,8 +303,60 @@ def merge_training_state(model_sd: Dict[str, torch.Tensor], tensors: Dict[str, t
     return out
 
 
+# ---------------------------------------------------------------------------- kernels of the backbone
+
+ATTENTION_NAME = "osp_packed"          # the packed kernel's name among transformers' attention functions
+_PACK: contextvars.ContextVar = contextvars.ContextVar("videoalign_pack", default=None)
+
+
+def _packed_attention(module, query, key, value, attention_mask=None, scaling=None, **kw):
+    """transformers' attention function: query [B, heads, L, D], key and value [B, key heads, L, D] ->
+    ([B, L, heads, D], None), causal, over the rows of the current batch's pack."""
+    B, H, L, D = query.shape
+    if key.shape[2] != L or attention_mask is not None or kw.get("sliding_window"):
+        raise ValueError("packed attention of a whole prompt: no cache, mask or window")
+    pack = _PACK.get()
+    if pack is None or pack.rows > B * L or pack.device != query.device:
+        pack = SequencePack.padded([L] * B, L, device=query.device)
+
+    def rows(t):
+        return t.transpose(1, 2).reshape(B * L, t.shape[1], D)
+    o = Fn.packed_attention(rows(query), rows(key), rows(value), pack, causal=True, scale=scaling)
+    return o.view(B, L, H, D).to(query.dtype), None
+
+
+def _gated_mlp(self, x):
+    """A SiLU-gated MLP's forward on the gated feed-forward kernels."""
+    return Fn.gated_ffn(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, "silu").to(x.dtype)
+
+
+def _silu_types():
+    from transformers.activations import ACT2FN
+    return (nn.SiLU, type(ACT2FN["silu"]))
+
+
+def _kernels_fit(config) -> bool:
+    """Whether the packed kernel takes the text layers' heads."""
+    c = getattr(config, "text_config", config)
+    dim = getattr(c, "head_dim", None) or c.hidden_size // c.num_attention_heads
+    return dim % 8 == 0 and dim <= 128
+
+
+def _mask_runs(attention_mask):
+    """(first, length) of each row's tokens, or None where some row's are not one run."""
+    m = attention_mask.bool().cpu()
+    n = m.sum(1)
+    first = torch.where(n > 0, m.int().argmax(1), 0)
+    at = torch.arange(m.shape[1])[None]
+    whole = torch.equal(m, (at >= first[:, None]) & (at < (first + n)[:, None]))
+    return (first.tolist(), n.tolist()) if whole else None
+
+
 class VideoAlignRewardModel(nn.Module):
-    """Qwen2-VL backbone + ``rm_head``; ``forward`` returns pooled reward logits [B, n]."""
+    """Qwen2-VL backbone + ``rm_head``; ``forward`` returns pooled reward logits [B, n].
+
+    :meth:`use_kernels` runs the text layers' attention and MLPs on this framework's kernels (bf16 on
+    the GPU); the scorer does so by itself there."""
 
     def __init__(self, vl_model: nn.Module, output_dim: int = 3, reward_token: str = "special",
                  special_token_ids: Optional[Sequence[int]] = None, pad_token_id: Optional[int] = None):
@@ -312,6 +369,41 @@ class VideoAlignRewardModel(nn.Module):
         self.special_token_ids = list(special_token_ids) if special_token_ids else None
         self.reward_token = "special" if self.special_token_ids else reward_token
         self.pad_token_id = pad_token_id
+        self._library_attention = None          # what the text layers ran before use_kernels
+
+    def use_kernels(self):
+        """Text attention on the packed kernel (padding costs nothing: rows are packed by the mask) and
+        SiLU-gated MLPs without biases on the gated feed-forward kernels."""
+        from transformers import AttentionInterface
+        AttentionInterface.register(ATTENTION_NAME, _packed_attention)
+        if self._library_attention is None:
+            self._library_attention = self.vl.config.text_config._attn_implementation
+        self.vl.set_attn_implementation({"text_config": ATTENTION_NAME})
+        for m in self.vl.model.language_model.modules():
+            parts = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+            if all(type(p) is nn.Linear and p.bias is None for p in parts) and isinstance(
+                    getattr(m, "act_fn", None), _silu_types()):
+                m.forward = types.MethodType(_gated_mlp, m)
+        return self
+
+    def _hidden(self, input_ids, attention_mask, **kw):
+        """Last hidden states; with the kernels, each row's tokens as one packed sequence."""
+        if self._library_attention is None:
+            return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
+        B, L = input_ids.shape
+        runs = ([0] * B, [L] * B) if attention_mask is None else _mask_runs(attention_mask)
+        if runs is None:                        # tokens with holes between them: the library's masks
+            self.vl.set_attn_implementation({"text_config": self._library_attention})
+            try:
+                return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
+            finally:
+                self.vl.set_attn_implementation({"text_config": ATTENTION_NAME})
+        pack = SequencePack(runs[1], starts=[i * L + f for i, f in enumerate(runs[0])], device=input_ids.device)
+        token = _PACK.set(pack)
+        try:
+            return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
+        finally:
+            _PACK.reset(token)
 
     def state_dict_for_checkpoint(self) -> Dict[str, torch.Tensor]:
         sd = {k[len("vl."):]: v for k, v in self.state_dict().items() if k.startswith("vl.")}
@@ -326,9 +418,8 @@ class VideoAlignRewardModel(nn.Module):
                 self.rm_head.weight.copy_(head)
 
     def forward(self, input_ids, attention_mask=None, pixel_values_videos=None, video_grid_thw=None, **kw):
-        h = self.vl.model(input_ids=input_ids, attention_mask=attention_mask,
-                          pixel_values_videos=pixel_values_videos, video_grid_thw=video_grid_thw,
-                          **kw).last_hidden_state
+        h = self._hidden(input_ids, attention_mask, pixel_values_videos=pixel_values_videos,
+                         video_grid_thw=video_grid_thw, **kw)
         logits = self.rm_head(h)                                    # [B, L, out]
         B = input_ids.shape[0]
         if self.reward_token == "special":
@@ -396,6 +487,8 @@ class VideoAlignScorer:
         scale = a / math.sqrt(r) if self.cfg.use_rslora else a / r
         model.load_checkpoint_tensors(merge_training_state(model.state_dict_for_checkpoint(), tensors, scale))
         self.model = model.to(device=device, dtype=dtype).eval()
+        if torch.device(device).type == "cuda" and dtype == torch.bfloat16 and _kernels_fit(vl_model.config):
+            self.model.use_kernels()
 
     def normalise(self, scores: Dict[str, float]) -> Dict[str, float]:
         if self.use_norm and self.cfg.norm:
