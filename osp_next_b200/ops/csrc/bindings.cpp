@@ -45,9 +45,9 @@ void attention_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
                    at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta, double scale, int64_t max_q,
                    int64_t max_k);
 std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                        const at::Tensor& items, const at::Tensor& joins, int64_t slots, bool causal,
-                                        double scale, const c10::optional<at::Tensor>& rel_bias, bool want_lse,
-                                        bool fill);
+                                        const at::Tensor& items, const at::Tensor& joins, int64_t slots,
+                                        int64_t positions, int64_t tiles, bool causal, double scale,
+                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, bool fill);
 std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                         const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,

@@ -367,25 +367,26 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   }
 }
 
-// dV and dK of key tiles whose queries were split: parts added in their order.  A warp per row.
-__global__ void packed_join_kernel(const int* joins, int Hkv, int Dr, const float* part, __nv_bfloat16* dk,
-                                   __nv_bfloat16* dv) {
+// dV and dK of key tiles whose queries were split: parts added in their order.  A warp per row, 8 rows
+// a block.
+__global__ void __launch_bounds__(256)
+packed_join_kernel(const int* joins, int Hkv, int Dr, const float* part, __nv_bfloat16* dk, __nv_bfloat16* dv) {
   const int4 j = reinterpret_cast<const int4*>(joins)[blockIdx.x];   // k_row, n_k, first slot, parts
-  const int kvh = blockIdx.y, which = blockIdx.z, c = (threadIdx.x % 32) * 4;
-  if (c >= Dr) return;
+  const int kvh = blockIdx.y, which = blockIdx.z & 1, c = (threadIdx.x % 32) * 4;
+  const int r = (blockIdx.z >> 1) * 8 + threadIdx.x / 32;
+  if (c >= Dr || r >= j.y) return;
   const long stride = (long)Hkv * 2 * kT * Dr;
-  for (int r = threadIdx.x / 32; r < j.y; r += blockDim.x / 32) {
-    const float* src = part + (((long)j.z * Hkv + kvh) * 2 * kT + which * kT + r) * Dr + c;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < j.w; ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(src + s * stride);
-      acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
-    }
-    uint2 w;
-    w.x = pack_bf16x2(acc[0], acc[1]);
-    w.y = pack_bf16x2(acc[2], acc[3]);
-    *reinterpret_cast<uint2*>((which ? dk : dv) + ((long)(j.x + r) * Hkv + kvh) * Dr + c) = w;
+  const float* src = part + (((long)j.z * Hkv + kvh) * 2 * kT + which * kT + r) * Dr + c;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < j.w; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(src + s * stride);
+    acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
   }
+  uint2 w;
+  w.x = pack_bf16x2(acc[0], acc[1]);
+  w.y = pack_bf16x2(acc[2], acc[3]);
+  *reinterpret_cast<uint2*>((which ? dk : dv) + ((long)(j.x + r) * Hkv + kvh) * Dr + c) = w;
 }
 
 // ---------------------------------------------------------------------------- dQ
@@ -693,7 +694,7 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k
   else launch_packed_bwd<64>(tq, tk, tv, tdo, a, rows, keys, stream);
   if (joins.size(0) > 0) {
     TORCH_CHECK(slots > 0, "packed_attention: joins without slots");
-    packed_join_kernel<<<dim3((unsigned)joins.size(0), (unsigned)s.Hkv, 2), 256, 0, stream>>>(
+    packed_join_kernel<<<dim3((unsigned)joins.size(0), (unsigned)s.Hkv, 2 * kT / 8), 256, 0, stream>>>(
         joins.data_ptr<int>(), s.Hkv, s.D, a.part, a.dk, a.dv);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }

@@ -3,10 +3,10 @@
 //
 //   S = scale q k^T + bias;  o = softmax(S) v over the keys that a query sees;  lse = log sum exp S
 //
-// A CTA computes two row tiles (packed_attn.cuh) that pass over the same key tiles, as the kernel in
-// attention_fwd.cuh does: warps 0-3 and 4-7 the softmax of tile 0 and 1 (a thread per row, running
-// maximum and sum in fp32, O rescaled only when the maximum grows by more than 2^8), warp 8 the
-// TMA loads, warp 9 the MMAs; P goes to bf16 in tensor memory, over S.  Under a causal mask tile 0
+// A CTA computes one or two row tiles (packed_attn.cuh) that pass over the same key tiles, as the
+// kernel in attention_fwd.cuh does: four warps a tile for the softmax (a thread per row, running
+// maximum and sum in fp32, O rescaled only when the maximum grows by more than 2^8), one warp for the
+// TMA loads and one for the MMAs; P goes to bf16 in tensor memory, over S.  Under a causal mask tile 0
 // needs up to one key tile less than tile 1 and leaves the rest out.  A row's keys are those below
 // a limit, so the mask costs one comparison per score, in tiles that hold such a limit only.
 //
@@ -28,95 +28,143 @@ namespace osp {
 
 struct PackedFwdArgs {
   const int* items;
-  int G, P, Hq, Hkv, Dr;    // heads per key head, positions per tile, query and key heads, head dim
+  int units;                // items x heads that they are run for
+  int heads;                // key heads, or query heads where a tile holds one head (bias)
+  int kv_ratio;             // of those to one key head
+  int G, P, Hq, Dr;         // heads and positions of a tile, query heads, head dim
   int causal;
+  int q_box;                // bytes of a query box in shared memory (G * P rows, to 1024 bytes)
+  int slots;                // of the K / V ring
   __nv_bfloat16* out;       // [Nq, Hq, Dr]
   float* lse;               // [Nq, Hq] or null
   float scale_log2;
   const float* bias;        // [Hq, 2 M - 1] or null
   int bias_m;               // M
-  float* part_o;            // [slots, Hkv, 2 * 128, Dr]
-  float* part_l;            // [slots, Hkv, 2 * 128], log2 domain
+  float* part_o;            // [slots, heads, kTiles * 128, Dr]
+  float* part_l;            // [slots, heads, kTiles * 128], log2 domain
   int* err;
 };
 
-template <int D>
+// kTiles row tiles in a CTA.  Two share the key tiles that they pass over and take turns on the tensor
+// core; one leaves room for a second CTA on the SM (256 columns of tensor memory, at most 113 KB).
+template <int D, int kTiles, bool kBias>
 struct PackedFwdCfg {
-  static constexpr int kProdWarp = 8, kMmaWarp = 9, kThreads = 320;
+  static constexpr int kProdWarp = 4 * kTiles, kMmaWarp = kProdWarp + 1, kThreads = 32 * (kProdWarp + 2);
+  static constexpr int kCtas = kTiles == 2 ? 1 : 2;            // per SM
   static constexpr int BOX = pa::kRows * 128;
   static constexpr int DB = D / 64;
   static constexpr int TILE = DB * BOX;
-  static constexpr int kSlots = 5;
-  static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_BAR = OFF_KV + kSlots * TILE;
-  static constexpr int USED = OFF_BAR + 256;
-  static constexpr int kMaxSmem = 232448;
-  static constexpr int SLACK = (kMaxSmem - USED) < 1008 ? (kMaxSmem - USED) : 1008;
-  static constexpr int BYTES = USED + SLACK;
+  static constexpr int kMaxSlots = 5;
+  static constexpr int kPiece = kTiles == 2 ? 128 : 64;        // bytes of a row of results that leave at once
+  static constexpr int kOut = 32 * kPiece;                     // of a warp's 32 rows
+  static constexpr int kBiasBytes = kBias ? 2 * 2 * 2 * pa::kRows * 4 : 0;   // of a row tile: 2 x 2 x 256 entries
+  static constexpr int kRoom = kTiles == 2 ? 232448 : 115712;  // dynamic shared memory of a CTA
+  // barriers, bias and results lie in front, at fixed places: pointers cost the softmax no registers
+  static constexpr int OFF_OUT = 1024;
+  static constexpr int OFF_BIAS = OFF_OUT + 4 * kTiles * kOut;
+  static constexpr int OFF_Q = OFF_BIAS + kTiles * kBiasBytes;
+  static_assert(OFF_Q % 1024 == 0, "swizzled tiles");
+  static constexpr int kExtra = OFF_Q + 1024;                  // + alignment of the base
+  static constexpr uint32_t kCols = kTiles == 2 ? 512 : 256;
 };
 
-// S values of a row (raw) -> scaled scores in the log2 domain with the bias added.
-template <bool kFull>
-__device__ __forceinline__ void add_bias(uint32_t* sr, float sl2, const float* brow, int n_valid) {
+// Work of a CTA: an item of the list for one head.
+template <int kTiles>
+struct FwdUnit {
+  pa::FwdItem it;
+  int head, kvh;
+  int n_t[kTiles];          // key tiles of each row tile: those below the limit of its last query
+  int c_t[kTiles];          // columns of the last of them that any row sees
+  int n_kv, last_rows;      // key tiles loaded, keys of the sequence in the last one
+  bool has_tail;
+
+  __device__ FwdUnit(const PackedFwdArgs& args, const pa::FwdItem& item) : it(item) {
+    constexpr int kT = pa::kRows;
+    head = blockIdx.x % args.heads;
+    kvh = head / args.kv_ratio;
+    n_kv = 0;
 #pragma unroll
-  for (int c = 0; c < pa::kRows; ++c) {
-    const float b = (kFull || c < n_valid) ? __ldg(brow + c) : 0.f;
-    sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), sl2, b * pa::kLog2e));
+    for (int t = 0; t < kTiles; ++t) {
+      const int nq = min(args.P, it.n_q - t * args.P);
+      const int lim = max(0, args.causal ? min(it.n_keys, it.limit + t * args.P + nq - 1) : it.n_keys);
+      n_t[t] = nq > 0 ? max(0, min(it.kt1, (lim + kT - 1) / kT) - it.kt0) : 0;
+      c_t[t] = min(kT, lim - (it.kt0 + n_t[t] - 1) * kT);
+      n_kv = max(n_kv, n_t[t]);
+    }
+    last_rows = it.n_keys - (it.kt0 + n_kv - 1) * kT;
+    has_tail = n_kv > 0 && last_rows < kT;
   }
+};
+
+// Row maximum over the columns below `cols` (the warp's) and n_valid (the row's).
+__device__ __forceinline__ float masked_max(const uint32_t* sr, int cols, int n_valid) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < pa::kRows / 16; ++g) {
+    if (g * 16 >= cols) break;
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = g * 16 + i;
+      m4[i & 3] = fmaxf(m4[i & 3], c < n_valid ? __uint_as_float(sr[c]) : -INFINITY);
+    }
+    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+  }
+  return mx;
 }
 
-template <int D, bool kBias>
-__global__ void __launch_bounds__(PackedFwdCfg<D>::kThreads, 1)
+// 16 bytes of a warp's 32 rows x kPiece bytes in shared memory, swizzled by the row: eight rows' pieces
+// lie in different banks, and so do the pieces of a row.
+template <int kPiece>
+__device__ __forceinline__ uint4* out_piece(uint8_t* buf, int row, int piece) {
+  const int x = kPiece == 128 ? row & 7 : (row >> 1) & 3;
+  return reinterpret_cast<uint4*>(buf + row * kPiece + ((piece ^ x) << 4));
+}
+
+template <int D, bool kBias, int kTiles>
+__global__ void __launch_bounds__(PackedFwdCfg<D, kTiles, kBias>::kThreads, PackedFwdCfg<D, kTiles, kBias>::kCtas)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, PackedFwdArgs args) {
-  using L = PackedFwdCfg<D>;
-  constexpr int kT = pa::kRows, kSlots = L::kSlots;
-  const pa::FwdItem it = pa::load_fwd_item(args.items, blockIdx.x / args.Hkv);
-  const int kvh = blockIdx.x % args.Hkv;
-  const int G = args.G, P = args.P;
+  using L = PackedFwdCfg<D, kTiles, kBias>;
+  using Unit = FwdUnit<kTiles>;
+  constexpr int kT = pa::kRows, kMaxSlots = L::kMaxSlots;
+  constexpr uint32_t kO = 128u * kTiles;                       // tensor memory: S tiles, then O tiles
+  const int G = args.G, P = args.P, slots = args.slots;
 
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
-  if (pad > (uint32_t)L::SLACK) {                              // CTA-uniform: report, do nothing
-    if (threadIdx.x == 0) record_error(args.err, kErrAttnLayout);
-    return;
-  }
-  uint8_t* smem = smem_raw + pad;
-  uint8_t* sQ = smem;
-  uint8_t* sKV = smem + L::OFF_KV;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+  uint8_t* sQ = smem + L::OFF_Q;
+  uint8_t* sKV = sQ + kTiles * L::DB * args.q_box;
   uint64_t* q_full = bars + 0;
   uint64_t* tail = bars + 1;                       // the V tile that reaches over the sequence's end
-  uint64_t* kv_full = bars + 2;                    // [kSlots]
-  uint64_t* kv_empty = kv_full + kSlots;           // [kSlots]
-  uint64_t* s_full = kv_empty + kSlots;            // [2]
-  uint64_t* p_half = s_full + 2;                   // [2]
-  uint64_t* p_full = p_half + 2;                   // [2]
-  uint64_t* o_done = p_full + 2;                   // [2]
-  uint64_t* done = o_done + 2;
+  uint64_t* kv_full = bars + 2;                    // [slots]
+  uint64_t* kv_empty = kv_full + kMaxSlots;        // [slots]
+  uint64_t* s_full = kv_empty + kMaxSlots;         // [kTiles]
+  uint64_t* p_half = s_full + kTiles;              // [kTiles]
+  uint64_t* p_full = p_half + kTiles;              // [kTiles]
+  uint64_t* o_done = p_full + kTiles;              // [kTiles]
+  uint64_t* done = o_done + kTiles;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(done + 2);
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
 
-  // key tiles of each row tile: those below the limit of its last query
-  int n_t[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int nq = min(P, it.n_q - t * P);
-    const int lim = args.causal ? min(it.n_keys, it.limit + t * P + nq - 1) : it.n_keys;
-    n_t[t] = nq > 0 ? max(0, min(it.kt1, (max(lim, 0) + kT - 1) / kT) - it.kt0) : 0;
+  // the item's fetch and the tensor maps' run under the set-up; the copy is for the way out
+  const pa::FwdItem item = pa::load_fwd_item(args.items, blockIdx.x / args.heads);
+  pa::FwdItem* item_copy = reinterpret_cast<pa::FwdItem*>(smem + 512);
+  if (warp == L::kProdWarp && lane == 0) {
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+    *item_copy = item;
   }
-  const int n0 = n_t[0], n1 = n_t[1], n_kv = max(n0, n1);
-  const int last_rows = it.n_keys - (it.kt0 + n_kv - 1) * kT;  // keys of the last tile
-  const bool has_tail = n_kv > 0 && last_rows < kT;
-
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(tail, 1);
-    for (int i = 0; i < kSlots; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
-    for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < slots; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
+    for (int t = 0; t < kTiles; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
@@ -125,12 +173,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&tmQ);
-    prefetch_tmap(&tmK);
-    prefetch_tmap(&tmV);
   }
   if (warp == L::kMmaWarp) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, L::kCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -140,101 +185,114 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (warp == L::kProdWarp) {
     // ------------------------------------------------------------------ producer
-    const int krow0 = it.k_row + it.kt0 * kT;
-    auto load_kv = [&](int u, uint64_t* bar) {
-      const int slot = u % kSlots;
-      mbar_expect_tx(bar, L::TILE);
-      const CUtensorMap* tm = (u & 1) ? &tmV : &tmK;
-      for (int db = 0; db < L::DB; ++db)
-        tma_load_3d(tm, bar, sKV + slot * L::TILE + db * L::BOX, db * 64, kvh, krow0 + (u >> 1) * kT);
-    };
-    const int units = 2 * n_kv;
-    const int plain = has_tail ? units - 1 : units;
     bool ok = true;
-    if (lane == 0 && n_kv > 0) {
-      const int tiles = (n0 > 0) + (n1 > 0);
-      mbar_expect_tx(q_full, tiles * L::DB * G * P * 128);
-      for (int t = 0; t < 2; ++t)
-        for (int db = 0; db < L::DB && n_t[t] > 0; ++db)
-          tma_load_3d(&tmQ, q_full, sQ + t * L::TILE + db * L::BOX, db * 64, kvh * G, it.q_row + t * P);
-      for (int u = 0; u < units && !*abort_flag; ++u) {
-        if (!(ok = mbar_wait(&kv_empty[u % kSlots], ((u / kSlots) & 1) ^ 1, args.err, kErrAttnProducer))) break;
-        load_kv(u, u < plain ? &kv_full[u % kSlots] : tail);
+    int slot = 0;
+    uint32_t phase = 1;
+    {
+      const Unit un(args, item);
+      const int krow0 = un.it.k_row + un.it.kt0 * kT;
+      const int units = 2 * un.n_kv;
+      if (lane == 0 && un.n_kv > 0) {
+        {
+          int tiles = 0;
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) tiles += un.n_t[t] > 0;
+          mbar_expect_tx(q_full, tiles * L::DB * G * P * 128);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            for (int db = 0; db < L::DB && un.n_t[t] > 0; ++db)
+              tma_load_3d(&tmQ, q_full, sQ + (t * L::DB + db) * args.q_box, db * 64, un.head * G, un.it.q_row + t * P);
+        }
+        for (int i = 0; i < units && ok; ++i) {
+          if (*abort_flag || !mbar_wait(&kv_empty[slot], phase, args.err, kErrAttnProducer)) { ok = false; break; }
+          uint64_t* bar = un.has_tail && i == units - 1 ? tail : &kv_full[slot];
+          mbar_expect_tx(bar, L::TILE);
+          const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
+          for (int db = 0; db < L::DB; ++db)
+            tma_load_3d(tm, bar, sKV + slot * L::TILE + db * L::BOX, db * 64, un.kvh, krow0 + (i >> 1) * kT);
+          if (++slot == slots) { slot = 0; phase ^= 1; }
+        }
       }
-    }
-    __syncwarp();
-    if (has_tail) {
-      ok = __shfl_sync(0xffffffffu, ok && !*abort_flag, 0);
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(tail, 0, args.err, kErrAttnProducer));
-      if (ok) {
-        const int slot = (units - 1) % kSlots;
-        pa::zero_rows(sKV + slot * L::TILE, L::DB, last_rows, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[slot]);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (ok && un.has_tail) {
+        ok = __all_sync(0xffffffffu, mbar_wait(tail, 0, args.err, kErrAttnProducer));
+        if (ok) {
+          const int at = __shfl_sync(0xffffffffu, slot == 0 ? slots - 1 : slot - 1, 0);
+          pa::zero_rows(sKV + at * L::TILE, L::DB, un.last_rows, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[at]);
+        }
       }
     }
     if (!ok) *abort_flag = 1;
   } else if (warp == L::kMmaWarp) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n_kv > 0) {
+    if (lane == 0) {
       constexpr uint32_t ID_S = idesc_bf16(128, kT);
       constexpr uint32_t ID_PV = idesc_bf16(128, D, /*b_mn_major=*/true);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, args.err, kErrAttnMma); };
       auto issue_s = [&](int t, int slot) {
-        const uint32_t qa = smem_u32(sQ + t * L::TILE);
+        const uint32_t qa = smem_u32(sQ + t * L::DB * args.q_box);
         const uint32_t ka = smem_u32(sKV + slot * L::TILE);
         const uint32_t d = tmem + 128u * t;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * L::BOX + (k % 4) * 32;
-          umma_bf16(d, sdesc_sw128(qa + off, 16, 1024), sdesc_sw128(ka + off, 16, 1024), ID_S, k > 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(d, sdesc_sw128(qa + (k / 4) * args.q_box + (k % 4) * 32, 16, 1024),
+                    sdesc_sw128(ka + (k / 4) * L::BOX + (k % 4) * 32, 16, 1024), ID_S, k > 0 ? 1u : 0u);
         umma_commit(&s_full[t]);
       };
-      auto issue_pv = [&](int t, int slot, int k0, int k1, bool acc) {
+      // P V over the keys of this tile: its last one may have fewer
+      auto pv = [&](int t, const Unit& un, int j, int slot) -> bool {
         const uint32_t va = smem_u32(sKV + slot * L::TILE);
-        const uint32_t d = tmem + 256u + (uint32_t)D * t;
+        const uint32_t d = tmem + kO + (uint32_t)D * t;
         const uint32_t pr = tmem + 128u * t;
-#pragma unroll
-        for (int k = k0; k < k1; ++k)
-          umma_bf16_ts(d, pr + 8u * k, sdesc_sw128(va + k * 2048, L::BOX, 1024), ID_PV, (acc || k > 0) ? 1u : 0u);
-      };
-      auto pv = [&](int t, int j, int slot) -> bool {
+        const int steps = j + 1 == un.n_t[t] ? (un.c_t[t] + 15) / 16 : kT / 16;
         if (!wait(&p_half[t], j & 1)) return false;
         tc_fence_after();
-        issue_pv(t, slot, 0, kT / 32, j > 0);
+        for (int k = 0; k < min(steps, kT / 32); ++k)
+          umma_bf16_ts(d, pr + 8u * k, sdesc_sw128(va + k * 2048, L::BOX, 1024), ID_PV, (j > 0 || k > 0) ? 1u : 0u);
         if (!wait(&p_full[t], j & 1)) return false;
         tc_fence_after();
-        issue_pv(t, slot, kT / 32, kT / 16, j > 0);
+        for (int k = kT / 32; k < steps; ++k)
+          umma_bf16_ts(d, pr + 8u * k, sdesc_sw128(va + k * 2048, L::BOX, 1024), ID_PV, 1u);
+        if (j + 1 == un.n_t[t]) umma_commit(&o_done[t]);
         return true;
       };
-      bool ok = wait(q_full, 0) && wait(&kv_full[0], 0);
-      if (ok) {
+      bool ok = true;
+      int slot = 0;
+      uint32_t phase = 0;
+      auto next = [&] { if (++slot == slots) { slot = 0; phase ^= 1; } };
+      const Unit un(args, item);
+      const int n_kv = un.n_kv, n0 = un.n_t[0], n1 = un.n_t[kTiles - 1];
+      if (n_kv > 0) ok = wait(q_full, 0) && wait(&kv_full[slot], phase);
+      if (n_kv > 0 && ok) {
         tc_fence_after();
-        if (n0 > 0) issue_s(0, 0);
-        if (n1 > 0) issue_s(1, 0);
-        umma_commit(&kv_empty[0]);
-      }
-      for (int j = 0; j < n_kv && ok; ++j) {
-        const int uV = 2 * j + 1, uK = 2 * j + 2;
-        const int sV = uV % kSlots, sK = uK % kSlots;
-        if (!(ok = wait(&kv_full[sV], (uV / kSlots) & 1))) break;
-        tc_fence_after();
-        if (j < n0) {
-          if (!(ok = pv(0, j, sV))) break;
-          if (j + 1 == n0) umma_commit(&o_done[0]);
+        if (n0 > 0) issue_s(0, slot);
+        if (kTiles == 2 && n1 > 0) issue_s(1, slot);
+        umma_commit(&kv_empty[slot]);
+        next();
+        for (int j = 0; j < n_kv; ++j) {
+          const int sV = slot;
+          if (!(ok = wait(&kv_full[sV], phase))) break;
+          next();
+          tc_fence_after();
+          if (j < n0 && !(ok = pv(0, un, j, sV))) break;
+          if (kTiles == 1) umma_commit(&kv_empty[sV]);
+          const int sK = slot;
+          if (j + 1 < n_kv) {
+            if (!(ok = wait(&kv_full[sK], phase))) break;
+            next();
+            tc_fence_after();
+            if (j + 1 < n0) issue_s(0, sK);
+          }
+          if (kTiles == 2) {
+            if (j < n1 && !(ok = pv(1, un, j, sV))) break;
+            umma_commit(&kv_empty[sV]);
+            if (j + 1 < n1) issue_s(1, sK);
+          }
+          if (j + 1 < n_kv) umma_commit(&kv_empty[sK]);
         }
-        if (j + 1 < n_kv && !(ok = wait(&kv_full[sK], (uK / kSlots) & 1))) break;
-        tc_fence_after();
-        if (j + 1 < n0) issue_s(0, sK);
-        if (j < n1) {
-          if (!(ok = pv(1, j, sV))) break;
-          if (j + 1 == n1) umma_commit(&o_done[1]);
-        }
-        umma_commit(&kv_empty[sV]);
-        if (j + 1 < n1) issue_s(1, sK);
-        if (j + 1 < n_kv) umma_commit(&kv_empty[sK]);
       }
       if (!ok) *abort_flag = 1;
       umma_commit(done);
@@ -247,161 +305,267 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int r = quarter * 32 + lane;                // row of the tile
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + 128u * t + lane_off;
-    const uint32_t tO = tmem + 256u + (uint32_t)D * t + lane_off;
-    const int nq = min(P, it.n_q - t * P);            // queries of the tile (<= 0: it has none)
-    const int pos = min(r / G, max(nq, 1) - 1);       // rows behind the last query repeat its mask
-    const int head = kvh * G + r % G;
-    const bool in = r < G * P && r / G < nq;
-    const int limit = args.causal ? min(it.n_keys, it.limit + t * P + pos) : it.n_keys;
+    const uint32_t tO = tmem + kO + (uint32_t)D * t + lane_off;
     const float sl2 = args.scale_log2;
-    const float* brow = nullptr;
-    if (kBias)                                        // entry of key 0 for this query
-      brow = args.bias + (long)(in ? head : kvh * G) * (2 * args.bias_m - 1) + args.bias_m -
-             (it.limit + t * P + pos);
-    float m_ref = -INFINITY, l = 0.f;
+    uint8_t* buf = smem + L::OFF_OUT + warp * L::kOut;
+    float* bias_buf = reinterpret_cast<float*>(smem + L::OFF_BIAS + t * L::kBiasBytes);
     bool ok = true;
-    const int n = t == 0 ? n0 : n1;
-    for (int j = 0; j < n; ++j) {
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, args.err, kErrAttnSoftmax)))) break;
-      tc_fence_after();
-      const int key0 = (it.kt0 + j) * kT;
-      const int n_valid = limit - key0;
-      const bool full = __all_sync(0xffffffffu, n_valid >= kT);
-      uint32_t sr[kT];
+    do {
+      // what the passes over the keys need; the rest of the unit is read again behind them, as the
+      // scores of a row take 128 of a thread's 168 registers
+      int n, last_cols, limit, bias_at, bias_row, bias_off;
+      bool idle;
+      {
+        const Unit un(args, item);
+        const int nq = min(P, un.it.n_q - t * P);       // queries of the tile (<= 0: it has none)
+        if (nq <= 0) break;                             // uniform for the tile's warps
+        const int pos = min(r / G, nq - 1);             // rows behind the last query repeat its mask
+        idle = !__any_sync(0xffffffffu, r / G < nq && r < G * P);   // a warp without rows keeps step, no more
+        const int first = un.it.limit + t * P;          // 1 + position of the tile's first query
+        limit = args.causal ? min(un.it.n_keys, first + pos) : un.it.n_keys;
+        n = t == 0 ? un.n_t[0] : un.n_t[kTiles - 1];
+        last_cols = t == 0 ? un.c_t[0] : un.c_t[kTiles - 1];
+        const int key0 = un.it.kt0 * kT;
+        // entry e of a key tile's stretch of the bias: key - position = key0 + e - (P - 1) - (first - 1)
+        bias_at = key0 + r - P - first + 1 + args.bias_m;
+        bias_row = un.head;
+        limit -= key0;
+        bias_off = P - 1 - pos;                         // even, or odd and one further on in the second copy
+        bias_off += bias_off & 1 ? 2 * kT + 1 : 0;
+      }
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j) {
+        if (kBias) {
+          const float* row = args.bias + (long)bias_row * (2 * args.bias_m - 1);
+          // twice, the second time one place further on, so that every row reads aligned pairs
+          float* dst = bias_buf + (j & 1) * 4 * kT;
 #pragma unroll
-      for (int c = 0; c < kT / 32; ++c) tmem_ld32(tS + c * 32, sr + c * 32);
-      tmem_ld_wait();
-      if (kBias) {
-        if (full) add_bias<true>(sr, sl2, brow + key0, kT);
-        else add_bias<false>(sr, sl2, brow + key0, n_valid);
-      }
-      const float mul = kBias ? 1.0f : sl2;
-      float mx = full ? attn_row_max<kT, true>(sr, kT) : attn_row_max<kT, false>(sr, n_valid);
-      mx *= mul;
-      const bool need = mx > m_ref + 8.0f;
-      const float m_new = need ? mx : m_ref;
-      // O is stable here: the PV of step j - 1 was issued before S(j), whose completion we waited for
-      if (j > 0 && __any_sync(0xffffffffu, need)) {
-        const float alpha = need ? ex2(m_ref - m_new) : 1.0f;
-        l *= alpha;
-        attn_rescale_o(tO, D, alpha);
-      }
-      m_ref = m_new;
-      if (full) l += attn_exp_store<64, true, 0u, 0>(sr, mul, m_ref, 64, tS);
-      else l += attn_exp_store<64, false, 0u, 0>(sr, mul, m_ref, n_valid, tS);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_half[t]);
-      if (full) l += attn_exp_store<64, true, 0u, 4>(sr + 64, mul, m_ref, 64, tS + 32);
-      else l += attn_exp_store<64, false, 0u, 4>(sr + 64, mul, m_ref, n_valid - 64, tS + 32);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
-    }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], 0, args.err, kErrAttnSoftmax));
-    if (!ok) *abort_flag = 1;
-    tc_fence_after();
-    const bool write = ok && in;
-    const float inv_l = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);   // no key seen: 0; NaN stays
-    const float lse2 = m_ref + __log2f(l);
-    const long row = (long)(it.q_row + t * P + r / G) * args.Hq + head;
-    const long prow = it.slot < 0 ? 0 : ((long)it.slot * args.Hkv + kvh) * (2 * kT) + t * kT + r;
-    if (nq > 0) {
-#pragma unroll 1
-      for (int c = 0; c < args.Dr; c += 32) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_ld32(tO + c, o);
+          for (int e = 0; e < 2 * kT; e += kT) {
+            const int at = bias_at + j * kT + e;
+            const float b = at >= 0 && at < 2 * args.bias_m - 1 ? row[at] * pa::kLog2e : 0.f;
+            dst[r + e] = b;
+            dst[2 * kT + ((r + e + 1) & (2 * kT - 1))] = b;
+          }
+          named_bar_sync(1 + t, 4 * 32);
+        }
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, args.err, kErrAttnSoftmax)))) break;
+        tc_fence_after();
+        const int n_valid = limit - j * kT;
+        const int cols = j + 1 == n ? last_cols : kT;   // columns that any row of the tile sees
+        const bool full = __all_sync(0xffffffffu, n_valid >= kT);
+        if (!idle) {
+          uint32_t sr[kT];
+#pragma unroll
+          for (int c = 0; c < kT / 32; ++c)
+            if (c * 32 < cols) tmem_ld32(tS + c * 32, sr + c * 32);
           tmem_ld_wait();
-        } else {
+          if (kBias) {
+            const float* brow = bias_buf + (j & 1) * 4 * kT + bias_off;
+            const uint64_t sl2x2 = pk2(sl2, sl2);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
-        }
-        if (!write) continue;
-        if (it.slot < 0) {
+            for (int g = 0; g < kT / 32; ++g) {
+              if (g * 32 >= cols) break;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c + 8 * i < args.Dr)
-              *reinterpret_cast<uint4*>(args.out + row * args.Dr + c + 8 * i) = pa::pack8(o + 8 * i, inv_l);
-        } else {
+              for (int c = g * 32; c < g * 32 + 32; c += 2) {
+                const float2 b = *reinterpret_cast<const float2*>(brow + c);
+                float x, y;
+                upk2(ffma2(pk2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sl2x2, pk2(b.x, b.y)), x, y);
+                sr[c] = __float_as_uint(x);
+                sr[c + 1] = __float_as_uint(y);
+              }
+            }
+          }
+          const float mul = kBias ? 1.0f : sl2;
+          float mx = full ? attn_row_max<kT, true>(sr, kT) : masked_max(sr, cols, n_valid);
+          mx *= mul;
+          const bool need = mx > m_ref + 8.0f;
+          const float m_new = need ? mx : m_ref;
+          // O is stable here: the PV of step j - 1 was issued before S(j), whose completion we waited for
+          if (j > 0 && __any_sync(0xffffffffu, need)) {
+            const float alpha = need ? ex2(m_ref - m_new) : 1.0f;
+            l *= alpha;
+            attn_rescale_o(tO, D, alpha);
+          }
+          m_ref = m_new;
+          if (full) {
+            l += attn_exp_store<64, true, 0u, 0>(sr, mul, m_ref, 64, tS);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + 4 * i < args.Dr)
-              *reinterpret_cast<float4*>(args.part_o + prow * args.Dr + c + 4 * i) =
-                  make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
-                              __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
+            for (int g = 0; g < 4; ++g)
+              if (g * 16 < cols)
+                l += attn_exp_store<16, false, 0u, 0>(sr + g * 16, mul, m_ref, n_valid - g * 16, tS + g * 8);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[t]);
+          if (full) {
+            l += attn_exp_store<64, true, 0u, 4>(sr + 64, mul, m_ref, 64, tS + 32);
+          } else {
+#pragma unroll
+            for (int g = 4; g < 8; ++g)
+              if (g * 16 < cols)
+                l += attn_exp_store<16, false, 0u, 0>(sr + g * 16, mul, m_ref, n_valid - g * 16, tS + g * 8);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+        } else if (lane == 0) {
+          mbar_arrive(&p_half[t]);
+          mbar_arrive(&p_full[t]);
         }
       }
-      if (write) {
+      if (ok && n > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], 0, args.err, kErrAttnSoftmax));
+      }
+      if (!ok) break;
+      if (idle) break;
+      tc_fence_after();
+      const float inv_l = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);   // no key seen: 0; NaN stays
+      const float lse2 = m_ref + __log2f(l);
+      const pa::FwdItem it = *item_copy;
+      const int unit_head = blockIdx.x % args.heads;
+      const int rp = r / G, rh = r - rp * G;            // position and head of the row
+      const bool in = rp < min(P, it.n_q - t * P) && r < G * P;
+      const long row = (long)(it.q_row + t * P + rp) * args.Hq + unit_head * G + rh;
+      const long prow = ((long)it.slot * args.heads + unit_head) * (kTiles * kT) + t * kT + r;
+      if (in) {
         if (it.slot >= 0) args.part_l[prow] = lse2;
         else if (args.lse) args.lse[row] = lse2 * 0.69314718055994531f;
       }
-    }
+      // kPiece bytes of each row at a time through shared memory, so that kPiece / 16 lanes write a
+      // row's piece; the row's place comes from the lane that owns it
+      constexpr int kLanes = L::kPiece / 16;
+      const int size = it.slot < 0 ? 2 : 4;             // bytes per value
+      const int per = L::kPiece / size;                 // values of a row per pass: 64, 32 or 16
+      const long at = in ? (it.slot < 0 ? row : prow) * args.Dr * size : -1;
+      uint8_t* base = it.slot < 0 ? reinterpret_cast<uint8_t*>(args.out) : reinterpret_cast<uint8_t*>(args.part_o);
+      const int piece = lane % kLanes;
+      uint32_t o[32];
+#pragma unroll 1
+      for (int c0 = 0; c0 < args.Dr; c0 += 16) {        // 16 columns at a time
+        if (c0 % 32 == 0) {
+          if (n > 0) {
+            tmem_ld32(tO + c0, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = o[i + 16];
+        }
+        const int first = c0 % per * size / 16;         // the first piece that these columns fill
+        if (size == 2) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) *out_piece<L::kPiece>(buf, lane, first + i) = pa::pack8(o + 8 * i, inv_l);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(out_piece<L::kPiece>(buf, lane, first + i)) =
+                make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
+                            __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
+        }
+        if ((c0 + 16) % per != 0 && c0 + 16 < args.Dr) continue;
+        __syncwarp();
+        const int b0 = c0 / per * L::kPiece + piece * 16;   // byte of the row
+#pragma unroll
+        for (int i = 0; i < 32 / (32 / kLanes); ++i) {
+          const int rr = i * (32 / kLanes) + lane / kLanes;
+          const long to = __shfl_sync(0xffffffffu, at, rr);
+          if (to >= 0 && b0 < args.Dr * size)
+            *reinterpret_cast<uint4*>(base + to + b0) = *out_piece<L::kPiece>(buf, rr, piece);
+        }
+        __syncwarp();
+      }
+    } while (false);
+    if (!ok) *abort_flag = 1;
   }
 
   tc_fence_before();
   __syncthreads();
   if (warp == L::kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, L::kCols);
   }
 }
 
-// o = sum_i 2^(l_i - l) o_i over the parts of one item, 2^l = sum_i 2^(l_i).  A warp per row.
-__global__ void packed_combine_kernel(const int* joins, int G, int P, int Hq, int Dr, const float* part_o,
-                                      const float* part_l, __nv_bfloat16* out, float* lse) {
+// o = sum_i 2^(l_i - l) o_i over the parts of one item, 2^l = sum_i 2^(l_i).  A warp per row; block
+// (join, key head, 8 rows).  The parts' weights are read by the lanes at once, 32 parts at a time.
+__global__ void __launch_bounds__(256)
+packed_combine_kernel(const int* joins, int G, int P, int tiles, int Hq, int Dr, const float* part_o,
+                      const float* part_l, __nv_bfloat16* out, float* lse) {
   const int4 j = reinterpret_cast<const int4*>(joins)[blockIdx.x];   // q_row, n_q, first slot, parts
   const int kvh = blockIdx.y, lane = threadIdx.x % 32;
-  for (int i = threadIdx.x / 32; i < j.y * G; i += blockDim.x / 32) {
-    const int p = i / G, g = i % G;
-    const int t = p / P;
-    const long r = t * pa::kRows + (p - t * P) * G + g;
-    const long stride = (long)gridDim.y * 2 * pa::kRows;
-    const long first = (long)j.z * stride + (long)kvh * 2 * pa::kRows + r;
-    float top = -INFINITY;
-    for (int s = 0; s < j.w; ++s) {
-      const float v = part_l[first + s * stride];
-      top = v != v ? v : fmaxf(top, v);
-    }
-    float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int s = 0; s < j.w; ++s) {
-      const float w = exp2f(part_l[first + s * stride] - base);
+  const int i = blockIdx.z * 8 + threadIdx.x / 32;
+  if (i >= j.y * G) return;
+  const int p = i / G, g = i % G, t = p / P;
+  const long stride = (long)gridDim.y * tiles * pa::kRows;
+  const long first = (long)j.z * stride + (long)kvh * tiles * pa::kRows + t * pa::kRows + (p - t * P) * G + g;
+  float top = -INFINITY;
+  for (int s = lane; s < j.w; s += 32) {
+    const float v = part_l[first + s * stride];
+    top = v != v || top != top ? NAN : fmaxf(top, v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float v = __shfl_xor_sync(0xffffffffu, top, o);
+    top = v != v || top != top ? NAN : fmaxf(top, v);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < j.w; s0 += 32) {
+    const float mine = s0 + lane < j.w ? exp2f(part_l[first + (s0 + lane) * stride] - base) : 0.f;
+    const int n = min(32, j.w - s0);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float w = __shfl_sync(0xffffffffu, mine, s);
       sum += w;
-      if (lane * 4 < Dr && w != 0.f) {
-        const float4 v = *reinterpret_cast<const float4*>(part_o + (first + s * stride) * Dr + lane * 4);
+      if (lane * 4 < Dr) {                     // a part without keys has zeros and weight 0
+        const float4 v = *reinterpret_cast<const float4*>(part_o + (first + (s0 + s) * stride) * Dr + lane * 4);
         acc[0] += w * v.x; acc[1] += w * v.y; acc[2] += w * v.z; acc[3] += w * v.w;
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const long row = (long)(j.x + p) * Hq + kvh * G + g;
-    if (lane * 4 < Dr) {
-      uint2 w;
-      w.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-      w.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<uint2*>(out + row * Dr + lane * 4) = w;
-    }
-    if (lane == 0 && lse) lse[row] = (base + log2f(sum)) * 0.69314718055994531f;
   }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const long row = (long)(j.x + p) * Hq + kvh * G + g;
+  if (lane * 4 < Dr) {
+    uint2 w;
+    w.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    w.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>(out + row * Dr + lane * 4) = w;
+  }
+  if (lane == 0 && lse) lse[row] = (base + log2f(sum)) * 0.69314718055994531f;
+}
+
+template <int D, bool kBias, int kTiles>
+static void launch_packed_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, PackedFwdArgs a,
+                              cudaStream_t stream) {
+  using L = PackedFwdCfg<D, kTiles, kBias>;
+  a.q_box = (a.G * a.P * 128 + 1023) / 1024 * 1024;
+  const int q_bytes = kTiles * L::DB * a.q_box;
+  a.slots = std::min(L::kMaxSlots, (L::kRoom - L::kExtra - q_bytes) / L::TILE);
+  auto kern = packed_fwd_kernel<D, kBias, kTiles>;
+  smem_opt_in(reinterpret_cast<const void*>(kern), L::kRoom);
+  kern<<<a.units, L::kThreads, q_bytes + a.slots * L::TILE + L::kExtra, stream>>>(tq, tk, tv, a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 template <int D, bool kBias>
-static void launch_packed_fwd(dim3 grid, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+static void launch_packed_fwd(int64_t tiles, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const PackedFwdArgs& a, cudaStream_t stream) {
-  auto kern = packed_fwd_kernel<D, kBias>;
-  smem_opt_in(reinterpret_cast<const void*>(kern), PackedFwdCfg<D>::BYTES);
-  kern<<<grid, PackedFwdCfg<D>::kThreads, PackedFwdCfg<D>::BYTES, stream>>>(tq, tk, tv, a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (tiles == 1) launch_packed_fwd<D, kBias, 1>(tq, tk, tv, a, stream);
+  else launch_packed_fwd<D, kBias, 2>(tq, tk, tv, a, stream);
 }
 
 // (o [Nq, Hq, D] bf16, lse [Nq, Hq] fp32 or empty).  `items` / `joins` are int32 lists on the device,
 // laid out by ops.SequencePack for this group size; rows of no sequence are zeros (`fill`).
 std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                        const at::Tensor& items, const at::Tensor& joins, int64_t slots, bool causal,
-                                        double scale, const c10::optional<at::Tensor>& rel_bias, bool want_lse,
-                                        bool fill) {
+                                        const at::Tensor& items, const at::Tensor& joins, int64_t slots,
+                                        int64_t positions, int64_t tiles, bool causal, double scale,
+                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, bool fill) {
   const pa::Shape s = pa::check_shapes(q, k, v, "packed_attention");
   pa::check_list(items, 8, q, "packed_attention: items");
   pa::check_list(joins, 4, q, "packed_attention: joins");
@@ -417,10 +581,16 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k
   if (n == 0 || s.Hq == 0 || s.D == 0) return {out, lse};
   PackedFwdArgs a{};
   a.items = items.data_ptr<int>();
-  a.G = s.G;
-  a.P = pa::kRows / s.G;
+  // with a bias a tile holds one query head: its rows then read one stretch of the bias
+  const int group = rel_bias.has_value() ? 1 : s.G;
+  a.G = group;
+  a.heads = s.Hq / group;
+  a.kv_ratio = a.heads / s.Hkv;
+  TORCH_CHECK(n * a.heads < (1ll << 30), "packed_attention: too much work for one call");
+  a.units = (int)(n * a.heads);
+  a.P = (int)positions;
+  TORCH_CHECK(a.P >= 1 && a.P * group <= pa::kRows && (tiles == 1 || tiles == 2), "packed_attention: row tiles");
   a.Hq = s.Hq;
-  a.Hkv = s.Hkv;
   a.Dr = s.D;
   a.causal = causal ? 1 : 0;
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
@@ -436,26 +606,26 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k
   a.err = error_word(q.get_device());
   at::Tensor part_o, part_l;
   if (slots > 0) {
-    part_o = at::empty({slots, s.Hkv, 2 * pa::kRows, s.D}, opt.dtype(at::kFloat));
-    part_l = at::empty({slots, s.Hkv, 2 * pa::kRows}, opt.dtype(at::kFloat));
+    part_o = at::empty({slots, a.heads, tiles * pa::kRows, s.D}, opt.dtype(at::kFloat));
+    part_l = at::empty({slots, a.heads, tiles * pa::kRows}, opt.dtype(at::kFloat));
     a.part_o = part_o.data_ptr<float>();
     a.part_l = part_l.data_ptr<float>();
   }
-  const CUtensorMap tq = pa::tile_map(q, q, s.D, s.G, a.P);
+  const CUtensorMap tq = pa::tile_map(q, q, s.D, group, a.P);
   const CUtensorMap tk = pa::tile_map(k, q, s.D, 1, pa::kRows), tv = pa::tile_map(v, q, s.D, 1, pa::kRows);
-  dim3 grid((unsigned)(n * s.Hkv));
   auto stream = c10::cuda::getCurrentCUDAStream();
   if (s.D > 64) {
-    if (a.bias) launch_packed_fwd<128, true>(grid, tq, tk, tv, a, stream);
-    else launch_packed_fwd<128, false>(grid, tq, tk, tv, a, stream);
+    if (a.bias) launch_packed_fwd<128, true>(tiles, tq, tk, tv, a, stream);
+    else launch_packed_fwd<128, false>(tiles, tq, tk, tv, a, stream);
   } else {
-    if (a.bias) launch_packed_fwd<64, true>(grid, tq, tk, tv, a, stream);
-    else launch_packed_fwd<64, false>(grid, tq, tk, tv, a, stream);
+    if (a.bias) launch_packed_fwd<64, true>(tiles, tq, tk, tv, a, stream);
+    else launch_packed_fwd<64, false>(tiles, tq, tk, tv, a, stream);
   }
   if (joins.size(0) > 0) {
     TORCH_CHECK(slots > 0, "packed_attention: joins without slots");
-    packed_combine_kernel<<<dim3((unsigned)joins.size(0), (unsigned)s.Hkv), 256, 0, stream>>>(
-        joins.data_ptr<int>(), s.G, a.P, s.Hq, s.D, a.part_o, a.part_l, a.out, a.lse);
+    const unsigned rows = (unsigned)(a.P * tiles * group);
+    packed_combine_kernel<<<dim3((unsigned)joins.size(0), (unsigned)a.heads, (rows + 7) / 8), 256, 0, stream>>>(
+        joins.data_ptr<int>(), group, a.P, (int)tiles, s.Hq, s.D, a.part_o, a.part_l, a.out, a.lse);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   return {out, lse};

@@ -19,6 +19,7 @@ from . import reference as ref
 from ._ext import ext
 
 TILE = 128             # rows of a tensor-core tile: group heads x positions, or keys
+_LONG_STEPS = 8        # mean key tiles of an item from which a forward CTA takes two row tiles
 _MIN_FWD_STEPS = 4     # key tiles below which splitting an item further costs more than it gives
 _MIN_KEY_STEPS = 8     # the same for the row tiles of a key tile's gradient
 
@@ -117,33 +118,45 @@ class SequencePack:
     def _sms(self):
         return torch.cuda.get_device_properties(self.device).multi_processor_count
 
-    def _get(self, key, make):
+    def forward_lists(self, group: int, heads: int, causal: bool):
+        """(items, joins, slots, positions per row tile, row tiles per CTA) of the forward kernel for
+        ``heads`` groups of ``group`` query heads; lists on the device."""
+        key = ("fwd", group, heads, causal)
         hit = self._lists.get(key)
         if hit is None:
-            arrays, slots = make()
-            hit = self._lists[key] = (*self._upload(*arrays), slots)
+            tiles = row_tiles(self, group, causal)
+            (items, joins), slots = forward_items(self, group, heads, causal, self._sms(), tiles)
+            hit = self._lists[key] = (*self._upload(items, joins), slots, positions(self, group), tiles)
         return hit
-
-    def forward_lists(self, group: int, kv_heads: int, causal: bool):
-        """(items, joins, slots) of the forward kernel on the device."""
-        return self._get(("fwd", group, kv_heads, causal),
-                         lambda: forward_items(self, group, kv_heads, causal, self._sms()))
 
     def backward_lists(self, group: int, kv_heads: int, causal: bool):
         """(rows, keys, joins, slots) of the backward kernels on the device."""
-        def make():
+        key = ("bwd", group, kv_heads, causal)
+        hit = self._lists.get(key)
+        if hit is None:
             keys, joins, slots = key_items(self, group, kv_heads, causal, self._sms())
-            return (row_items(self, group, causal), keys, joins), slots
-        return self._get(("bwd", group, kv_heads, causal), make)
+            hit = self._lists[key] = (*self._upload(row_items(self, group, causal), keys, joins), slots)
+        return hit
 
 
 def _tiles(n):
     return -(-n // TILE)
 
 
-def _row_items(pack, group, causal, tiles):
-    """Items of ``tiles`` row tiles each, without splits: int64 [n, 8] and their key tiles."""
-    per = TILE // group * tiles
+def positions(pack, group):
+    """Positions of a forward row tile: as many as its 128 rows take, no more than any sequence has."""
+    return max(1, min(TILE // group, int(pack.lengths.max(initial=0))))
+
+
+def row_tiles(pack, group, causal):
+    """Row tiles of a forward CTA: two share the key tiles that they read, one leaves room for a second
+    CTA on the SM, which covers the latency of short passes."""
+    _, steps = _row_items(pack, group, causal, 2 * positions(pack, group))
+    return 1 if len(steps) and steps.mean() < _LONG_STEPS else 2
+
+
+def _row_items(pack, group, causal, per):
+    """Items of ``per`` queries each, without splits: int64 [n, 8] and their key tiles."""
     count = -(-pack.lengths // per)
     seq = np.repeat(np.arange(len(pack)), count)
     first = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * per
@@ -163,7 +176,7 @@ def _longest_first(items, steps):
 
 def row_items(pack, group, causal):
     """Items of the dQ kernel: one row tile each, over the keys that its last query sees."""
-    return _longest_first(*_row_items(pack, group, causal, 1))
+    return _longest_first(*_row_items(pack, group, causal, TILE // group))
 
 
 def _split(steps, kv_heads, sms, least):
@@ -173,11 +186,11 @@ def _split(steps, kv_heads, sms, least):
     return np.maximum(1, -(-steps // share))
 
 
-def forward_items(pack, group, kv_heads, causal, sms):
-    """((items, joins), slots) of the forward kernel: two row tiles each, longest first; items with
-    many keys are split, and joined in the order of their parts."""
-    items, steps = _row_items(pack, group, causal, 2)
-    parts = _split(steps, kv_heads, sms, _MIN_FWD_STEPS)
+def forward_items(pack, group, kv_heads, causal, sms, tiles):
+    """((items, joins), slots) of the forward kernel: ``tiles`` row tiles each, longest first; items
+    with many keys are split, and joined in the order of their parts."""
+    items, steps = _row_items(pack, group, causal, tiles * positions(pack, group))
+    parts = _split(steps, kv_heads, sms * (2 if tiles == 1 else 1), _MIN_FWD_STEPS)
     size = -(-steps // parts)
     parts = np.maximum(1, -(-steps // np.maximum(size, 1)))         # no empty part
     cut = parts > 1
@@ -293,10 +306,11 @@ def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
     if rel_bias is not None:
         rel_bias = rel_bias.float().contiguous()
     Hkv = k.shape[1]
-    items, joins, slots = pack.forward_lists(q.shape[1] // Hkv, Hkv, bool(causal))
+    group = 1 if rel_bias is not None else q.shape[1] // Hkv      # heads of a row tile (one with a bias)
+    items, joins, slots, per, tiles = pack.forward_lists(group, q.shape[1] // group, bool(causal))
     fill = not (pack.dense and q.shape[0] == pack.rows)
-    o, lse = ext().packed_attn_fwd(tma_rows(q), tma_rows(k), tma_rows(v), items, joins, slots, bool(causal), scale,
-                                   rel_bias, bool(return_lse), fill)
+    o, lse = ext().packed_attn_fwd(tma_rows(q), tma_rows(k), tma_rows(v), items, joins, slots, per, tiles,
+                                   bool(causal), scale, rel_bias, bool(return_lse), fill)
     return (o, lse) if return_lse else o
 
 

@@ -121,12 +121,12 @@ def test_work_lists_cover_every_pair_once(lengths, keys, group, kv, causal):
             cols = np.arange(kt0 * T, min(kt1 * T, max(lim, 0)))
             seen[row + i, k_row + cols] += 1
 
-    for sms in (1, 4, 148, 4000):
-        (items, joins), slots = packed.forward_items(pack, group, kv, causal, sms)
+    for sms, tiles in ((1, 2), (4, 1), (148, 2), (148, 1), (4000, 2), (4000, 1)):
+        (items, joins), slots = packed.forward_items(pack, group, kv, causal, sms, tiles)
         seen, written = np.zeros_like(want), np.zeros(pack.rows, dtype=int)
         used = []
         for row, n_q, limit, k_row, n_keys, kt0, kt1, slot in items:
-            assert 0 < n_q <= 2 * per and (kt1 > kt0 or kt0 == 0 == kt1) and kt1 <= -(-n_keys // T)
+            assert 0 < n_q <= tiles * packed.positions(pack, group) <= tiles * per and (kt1 > kt0 or kt0 == 0 == kt1) and kt1 <= -(-n_keys // T)
             assert len(set(seq_of[row:row + n_q])) == 1
             mark(seen, row, n_q, limit, k_row, n_keys, kt0, kt1)
             if slot < 0:
@@ -257,6 +257,12 @@ gpu = pytest.mark.gpu
 HEADS = [(4, 4, 64), (7, 1, 128), (6, 2, 80), (16, 2, 128), (40, 1, 40), (5, 1, 96), (2, 2, 8), (128, 1, 64)]
 
 
+@pytest.fixture(params=[1, 2], ids=["one_tile", "two_tiles"])
+def tiles(request, monkeypatch):
+    """Both forms of the forward kernel at every size."""
+    monkeypatch.setattr(packed, "row_tiles", lambda *a: request.param)
+
+
 def _pass(pack, heads, kv, dim, causal, seed=0, bias=None, train=True, scale=None, std=1.0):
     q, k, v, do = tensors(pack, heads, kv, dim, "cuda", seed, std=std)
     scale = dim ** -0.5 if scale is None else scale
@@ -276,7 +282,7 @@ def _pass(pack, heads, kv, dim, causal, seed=0, bias=None, train=True, scale=Non
 @gpu
 @pytest.mark.parametrize("lengths,keys", PACKS)
 @pytest.mark.parametrize("causal", [True, False])
-def test_gpu_lengths(lengths, keys, causal):
+def test_gpu_lengths(lengths, keys, causal, tiles):
     for heads, kv, dim in ((4, 2, 64), (6, 2, 128)):
         _pass(ops.SequencePack(lengths, keys), heads, kv, dim, causal)
 
@@ -284,12 +290,12 @@ def test_gpu_lengths(lengths, keys, causal):
 @gpu
 @pytest.mark.parametrize("heads,kv,dim", HEADS)
 @pytest.mark.parametrize("causal", [True, False])
-def test_gpu_heads(heads, kv, dim, causal):
+def test_gpu_heads(heads, kv, dim, causal, tiles):
     _pass(ops.SequencePack([1, 150, 33, 0, 260]), heads, kv, dim, causal)
 
 
 @gpu
-def test_gpu_long_and_split():
+def test_gpu_long_and_split(tiles):
     _pass(ops.SequencePack([2111, 5, 640]), 8, 2, 128, True)
     _pass(ops.SequencePack([1, 2, 40], [5003, 1200, 6001]), 8, 1, 128, True)
     _pass(ops.SequencePack([1], [9001]), 4, 4, 64, False)
@@ -298,7 +304,7 @@ def test_gpu_long_and_split():
 
 @gpu
 @pytest.mark.parametrize("lengths", [[1], [77, 3], [128, 129, 1, 512], [20, 200]])
-def test_gpu_relative_bias(lengths):
+def test_gpu_relative_bias(lengths, tiles):
     pack = ops.SequencePack(lengths)
     for extra in (0, 13):
         m = pack.longest + extra
@@ -309,13 +315,13 @@ def test_gpu_relative_bias(lengths):
 
 
 @gpu
-def test_gpu_large_scores():
+def test_gpu_large_scores(tiles):
     """Scores to some 500: the running maximum moves, weights are nearly one-hot."""
     _pass(ops.SequencePack([300, 41]), 4, 2, 64, True, std=6.0)
 
 
 @gpu
-def test_gpu_neighbours_and_gaps():
+def test_gpu_neighbours_and_gaps(tiles):
     """NaN and infinities in other sequences and in rows of none reach nobody."""
     pack = ops.SequencePack([70, 130, 5], starts=[3, 100, 240])
     q, k, v, do = tensors(pack, 6, 2, 64, "cuda", spare=4)
