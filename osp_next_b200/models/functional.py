@@ -427,13 +427,18 @@ class _GatedFFNFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, wg, wu, wd, act):
-        x2 = ops.gated.matrix(x.reshape(x.shape[:-1].numel(), x.shape[-1]))
-        g, u, d = ops.gated.hidden_rows(wg), ops.gated.hidden_rows(wu), ops.gated.hidden_rows(wd)
-        h, gu = ops.ext().gated_linear_fwd(x2, g, u, ops.gated.ACTS[act], True)
-        y = ops.ext().ffn_product(h, d, None, None, False, False, False)
+        code = ops.gated.ACTS[act]
+        g, u, d = wg, wu, wd
+        out = ops.ext().gated_ffn_fwd(x, g, u, d, code, True)
+        if not out:                                       # copies that the kernels can read
+            x2 = ops.gated.matrix(x.reshape(x.shape[:-1].numel(), x.shape[-1]))
+            g, u, d = ops.gated.hidden_rows(wg), ops.gated.hidden_rows(wu), ops.gated.hidden_rows(wd)
+            out = ops.ext().gated_ffn_fwd(x2, g, u, d, code, True)
+            out[0] = out[0][:, :wd.shape[0]].reshape(*x.shape[:-1], wd.shape[0])
+        y, x2, gu = out
         ctx.save_for_backward(x2, g, u, d, gu)
-        ctx.meta = (x.shape, x.dtype, wg.shape, wg.dtype, wu.dtype, wd.shape, wd.dtype, ops.gated.ACTS[act])
-        return y[:, :wd.shape[0]].reshape(*x.shape[:-1], wd.shape[0])
+        ctx.meta = (x.shape, x.dtype, wg.shape, wg.dtype, wu.dtype, wd.shape, wd.dtype, code)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -447,17 +452,17 @@ class _GatedFFNFn(torch.autograd.Function):
         fp, (f, k) = wg.shape[0], wshape
         dx = dwg = dwu = dwd = None
         if need_x:
-            dx = product(dgu[:, :fp], wg, dgu[:, fp:], wu, False, True, xdt != _BF16)
+            dx = product(dgu[:, :fp], wg, dgu[:, fp:], wu, False, True, xdt != _BF16, False)
             dx = dx[:, :k].reshape(xshape).to(xdt)
         if need_g or need_u:
             part = dgu if need_g and need_u else dgu[:, :fp] if need_g else dgu[:, fp:]
-            dw = product(part, x2, None, None, True, True, gdt != _BF16 or udt != _BF16)
+            dw = product(part, x2, None, None, True, True, gdt != _BF16 or udt != _BF16, False)
             if need_g:
                 dwg = dw[:f, :k].to(gdt)
             if need_u:
                 dwu = dw[-fp:][:f, :k].to(udt)
         if need_d:
-            dwd = product(dy, h, None, None, True, True, ddt != _BF16)[:dshape[0], :f].to(ddt)
+            dwd = product(dy, h, None, None, True, True, ddt != _BF16, False)[:dshape[0], :f].to(ddt)
         return dx, dwg, dwu, dwd, None
 
 
@@ -470,6 +475,6 @@ def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
     if _fused(x, w_gate, w_up, w_down):
         return ops.gated_ffn(x, w_gate, w_up, w_down, act)
     ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
-    if 0 in w_gate.shape or 0 in w_down.shape:                # empty sums
+    if 0 in w_gate.shape or 0 in w_down.shape or 0 in x.shape:         # empty sums
         return ref.gated_ffn(x.to(_BF16), w_gate, w_up, w_down, act)
     return _GatedFFNFn.apply(x, w_gate, w_up, w_down, act)

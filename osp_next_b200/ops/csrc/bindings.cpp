@@ -46,8 +46,9 @@ void attention_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
                    int64_t max_k);
 std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                         const at::Tensor& items, const at::Tensor& joins, int64_t slots,
-                                        int64_t positions, int64_t tiles, bool causal, double scale,
-                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, bool fill);
+                                        int64_t positions, int64_t tiles, bool causal, double scale, bool own_scale,
+                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, int64_t rows,
+                                        int64_t key_rows, int64_t longest, bool dense);
 std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                         const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
@@ -56,9 +57,12 @@ std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& 
                                          bool keep);
 std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor& wd, const at::Tensor& gu, int64_t act);
 at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& a2,
-                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32);
+                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32, bool ahead);
+std::vector<at::Tensor> gated_ffn_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                                      const at::Tensor& wd, int64_t act, bool keep);
 std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos,
-                                     const at::Tensor& table, std::vector<int64_t> sections, bool half, bool inverse);
+                                     const at::Tensor& table, const std::vector<int64_t>& sections, bool half,
+                                     bool inverse);
 void cfg_euler(const at::Tensor& lat, const at::Tensor& cond, const at::Tensor& unc, at::Tensor& out, double g,
                double dt);
 void hif8_round(const at::Tensor& x, at::Tensor& out, double s);
@@ -181,6 +185,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("packed_attn_bwd", &osp::packed_attn_bwd);
   m.def("gated_linear_fwd", &osp::gated_linear_fwd);
   m.def("gated_linear_bwd", &osp::gated_linear_bwd);
+  m.def("gated_ffn_fwd", &osp::gated_ffn_fwd);
   m.def("ffn_product", &osp::ffn_product);
   m.def("rotary_apply", &osp::rotary_apply);
   m.def("cfg_euler", &osp::cfg_euler);

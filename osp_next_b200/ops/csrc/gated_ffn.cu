@@ -22,6 +22,8 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include "common.cuh"
+#include "launch.h"
+#include <algorithm>
 #include <string>
 
 #include "tma_host.h"
@@ -326,6 +328,223 @@ gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMa
   }
 }
 
+// ---------------------------------------------------------------------------- few rows
+// Up to kFewRows rows of x: what takes time is reading the weights once.  The product is formed as
+// W x^T, so that 128 weight rows fill the tensor core's M and the rows of x (padded to 16) its N; a
+// CTA holds 128 rows of Wg and the same of Wu (two accumulators, so a thread owns g and u of its
+// weight row), or 128 rows of Wd.  Two CTAs share an SM where their accumulators take 256 columns of
+// tensor memory.  Tiles that are too few to fill the SMs split K over a cluster of up to 8 CTAs,
+// whose parts are added through distributed shared memory in rank order: no workspace, and results do
+// not depend on timing.  The down projection starts while the gate kernel runs and loads its first
+// weights before it waits for it.  192 threads: warp 0 loads, warp 1 MMAs, warps 2..5 results.
+struct FewArgs {
+  int M, N, KB;                // rows of x, weight rows, blocks of 64 along K
+  int bnx;                     // rows of x that a CTA takes (blockIdx.y: which), a multiple of 16
+  int stages;                  // of the ring
+  int splits;
+  int chunk;                   // rows of x whose sums fit the ring, a multiple of 16
+  int cols;                    // tensor-memory columns
+  int act;
+  int ahead;                   // load weights before the wait for the kernel in front
+  __nv_bfloat16* out;          // [M, N]
+  int* err;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {   // every warp of every CTA arrives converged
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 load_from_cta(const float* p, uint32_t rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+constexpr int kFewRows = 256;
+constexpr int kFewThreads = 192;
+constexpr int kFewMaxStages = 12;
+constexpr uint32_t kWTile = 128 * kBK * 2;
+
+template <bool kGateForm>
+__global__ void __launch_bounds__(kFewThreads)
+few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+           const __grid_constant__ CUtensorMap tmW2, const FewArgs args) {
+  constexpr int kAcc = kGateForm ? 2 : 1;
+  const uint32_t x_bytes = args.bnx * kBK * 2;
+  const uint32_t stage_bytes = kAcc * kWTile + x_bytes;
+  const int stages = args.stages;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty = full + kFewMaxStages;
+  uint64_t* tfull = empty + kFewMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  uint8_t* ring = smem + 1024;
+  float* part = reinterpret_cast<float*>(ring);            // [kAcc][chunk][128] over the ring when it is done with
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int split = args.splits > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / args.splits;
+  const int x0 = blockIdx.y * args.bnx, my_rows = min(args.bnx, args.M - x0);
+  const int kb0 = (int)((long)args.KB * split / args.splits), kb1 = (int)((long)args.KB * (split + 1) / args.splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(tfull, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmW);
+    if (kGateForm) prefetch_tmap(&tmW2);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, args.cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (warp != 0 || !args.ahead) {
+    grid_dependency_wait();
+    allow_dependents();
+  }
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load_w = [&](int kb, int stage) {
+        uint8_t* dst = ring + stage * stage_bytes;
+        mbar_expect_tx(&full[stage], stage_bytes);
+        tma_load_2d(&tmW, &full[stage], dst, kb * kBK, tile * 128);
+        if (kGateForm) tma_load_2d(&tmW2, &full[stage], dst + kWTile, kb * kBK, tile * 128);
+      };
+      auto load_x = [&](int kb, int stage) {
+        tma_load_2d(&tmX, &full[stage], ring + stage * stage_bytes + kAcc * kWTile, kb * kBK, x0);
+      };
+      const int n = min(stages, kb1 - kb0);
+      for (int i = 0; i < n; ++i) load_w(kb0 + i, i);
+      if (args.ahead) grid_dependency_wait();
+      for (int i = 0; i < n; ++i) load_x(kb0 + i, i);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0 + n; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase, args.err, kErrGemmProducer)) break;
+        load_w(kb, stage);
+        load_x(kb, stage);
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      // the last loads have landed before the ring is reused and the block ends
+      for (int s = 0; s < n; ++s) mbar_wait(&full[s], s < stage ? phase ^ 1 : phase, args.err, kErrGemmTeardown);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_bf16(128, args.bnx);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, args.err, kErrGemmMma)) break;
+        tc_fence_after();
+        const uint32_t w = smem_u32(ring + stage * stage_bytes), x = w + kAcc * kWTile;
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a)
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            umma_bf16(tmem + a * args.bnx, sdesc_sw128(w + a * kWTile + k * 32, 16, 1024),
+                      sdesc_sw128(x + k * 32, 16, 1024), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      umma_commit(tfull);
+    }
+    __syncwarp();
+  }
+
+  // Sums leave tensor memory (a lane per weight row) for shared memory, [row of x][128], and from there
+  // a warp per row of x adds the parts of all CTAs and writes 128 results in one piece; as many rows
+  // of x at a time as the ring has room for.
+  const int quarter = warp & 3;
+  const int n0 = tile * 128 + lane * 4;
+  bool ok = true;
+  if (warp >= 2) {
+    ok = __all_sync(0xffffffffu, mbar_wait(tfull, 0, args.err, kErrGemmEpilogue));
+    tc_fence_after();
+  }
+  for (int c0 = 0; c0 < my_rows; c0 += args.chunk) {
+    const int rows = min(args.chunk, my_rows - c0);
+    if (warp >= 2 && ok) {
+      const uint32_t t_row = tmem + ((uint32_t)(quarter * 32) << 16) + c0;
+      float* mine = part + quarter * 32 + lane;
+      for (int m0 = 0; m0 < rows; m0 += 16) {              // rows of x from M on are zeros of the tile
+        uint32_t r[kAcc][16];
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a) tmem_ld16(t_row + a * args.bnx + m0, r[a]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) mine[(a * args.chunk + m0 + j) * 128] = __uint_as_float(r[a][j]);
+      }
+    }
+    if (args.splits > 1) cluster_sync();
+    else __syncthreads();
+    if (warp >= 2 && ok && n0 < args.N) {
+#pragma unroll 2
+      for (int m = split + (warp - 2) * args.splits; m < rows; m += 4 * args.splits) {
+        float4 v[kAcc];
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a) {
+          const float* src = part + (a * args.chunk + m) * 128 + lane * 4;
+          if (args.splits == 1) {
+            v[a] = *reinterpret_cast<const float4*>(src);
+          } else {
+            float4 p[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+              if (s < args.splits) p[s] = load_from_cta(src, s);
+            v[a] = p[0];
+#pragma unroll
+            for (int s = 1; s < 8; ++s)
+              if (s < args.splits) { v[a].x += p[s].x; v[a].y += p[s].y; v[a].z += p[s].z; v[a].w += p[s].w; }
+          }
+        }
+        if constexpr (kGateForm) {
+          float d;
+          v[0].x = act_f<false>(args.act, v[0].x, d) * v[1].x;
+          v[0].y = act_f<false>(args.act, v[0].y, d) * v[1].y;
+          v[0].z = act_f<false>(args.act, v[0].z, d) * v[1].z;
+          v[0].w = act_f<false>(args.act, v[0].w, d) * v[1].w;
+        }
+        *reinterpret_cast<uint2*>(args.out + (long)(x0 + c0 + m) * args.N + n0) =
+            make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
+      }
+    }
+    if (args.splits > 1) cluster_sync();                   // no CTA goes on while its part may be read
+    else __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, args.cols);
+  }
+}
+
 template <int BN>
 constexpr int smem_bytes() {
   constexpr int stage = kBM * kBK * 2 + BN * kBK * 2;
@@ -352,6 +571,47 @@ static void launch(const at::Tensor& a, const at::Tensor& b, const at::Tensor* a
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// Whether the form for few rows takes a product: up to kFewRows of them (154 x 4096 -> 10240 -> 4096: 65 us
+// against 124), and more where the tiles of the other form leave SMs idle.
+static bool few_rows(int64_t M, int64_t N, int out_n, int sms) {
+  return M <= kFewRows || (M + kBM - 1) / kBM * ((N + out_n - 1) / out_n) < sms;
+}
+
+// out [M, N] = act(x W^T) o (x W2^T), or x W^T without W2.
+static void launch_few(const at::Tensor& x, const at::Tensor& w, const at::Tensor* w2, at::Tensor& out, int64_t act,
+                       bool ahead, cudaStream_t stream) {
+  const int sms = num_sms(x.get_device());
+  const int acc = w2 ? 2 : 1;
+  FewArgs a{};
+  a.M = (int)x.size(0);
+  a.N = (int)w.size(0);
+  a.KB = (int)((x.size(1) + kBK - 1) / kBK);
+  const int blocks = (a.M + kFewRows - 1) / kFewRows;
+  a.bnx = ((a.M + blocks - 1) / blocks + 15) / 16 * 16;
+  a.cols = 32;
+  while (a.cols < acc * a.bnx) a.cols *= 2;
+  const int stage = acc * (int)kWTile + a.bnx * kBK * 2;
+  const bool two = a.cols <= 256 && 111 * 1024 / stage >= 3;     // CTAs per SM
+  a.stages = std::min(kFewMaxStages, (two ? 111 : 224) * 1024 / stage);
+  const int tiles = (a.N + 127) / 128;
+  // as many parts of K as there is room for, of at least 4 blocks
+  a.splits = std::max(1, std::min({8, (two ? 2 : 1) * sms / (tiles * blocks), a.KB / 4}));
+  a.chunk = std::min(a.bnx, a.stages * stage / (acc * 512) / 16 * 16);
+  a.act = (int)act;
+  a.ahead = ahead ? 1 : 0;
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.err = error_word(x.get_device());
+  const CUtensorMap mx = map_of(x, false, a.bnx), mw = map_of(w, false, 128), mw2 = w2 ? map_of(*w2, false, 128) : mw;
+  const int smem = 2048 + a.stages * stage;
+  if (w2) {
+    smem_opt_in(reinterpret_cast<const void*>(few_kernel<true>), 227 * 1024);
+    launch_kernel(few_kernel<true>, dim3(tiles * a.splits, blocks), kFewThreads, smem, a.splits, stream, mx, mw, mw2, a);
+  } else {
+    smem_opt_in(reinterpret_cast<const void*>(few_kernel<false>), 227 * 1024);
+    launch_kernel(few_kernel<false>, dim3(tiles * a.splits, blocks), kFewThreads, smem, a.splits, stream, mx, mw, mw2, a);
+  }
+}
+
 static void check(const at::Tensor& t, const at::Tensor& x, int64_t rows, int64_t cols, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 &&
               t.size(0) == rows && t.size(1) == cols, "gated_ffn: ", what, " bf16 [", std::to_string(rows), ", ", std::to_string(cols), "]");
@@ -373,6 +633,9 @@ static Args make_args(const at::Tensor& x, int64_t M, int64_t N, int64_t K, int6
 
 }  // namespace ffn
 
+at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& a2,
+                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32, bool ahead);
+
 // {h [M, F]} or, with `keep`, {h, gu [M, 2 F]}: h = act(x wg^T) (x wu^T).
 std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act,
                                          bool keep) {
@@ -390,9 +653,35 @@ std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& 
     Args a = make_args(x, M, F, K, act);
     a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
     a.gu = keep ? reinterpret_cast<__nv_bfloat16*>(gu.data_ptr()) : nullptr;
-    launch<256, kGate, false, false>(x, wg, nullptr, &wu, a, c10::cuda::getCurrentCUDAStream());
+    if (!keep && few_rows(M, F, 128, num_sms(x.get_device()))) launch_few(x, wg, &wu, h, act, false, c10::cuda::getCurrentCUDAStream());
+    else launch<256, kGate, false, false>(x, wg, nullptr, &wu, a, c10::cuda::getCurrentCUDAStream());
   }
   return {h, gu};
+}
+
+// {y [..., C], x as a matrix, gu} of the whole block, gu with `keep` alone; nothing where an operand is not as the
+// kernels read it (bf16, sizes multiples of 8, rows at multiples of 16 bytes): the caller then makes copies.
+std::vector<at::Tensor> gated_ffn_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+                                      const at::Tensor& wd, int64_t act, bool keep) {
+  auto fits = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.device() == x.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 &&
+           t.size(0) > 0 && t.size(1) > 0 && t.size(1) % 8 == 0 && t.stride(1) == 1 && t.stride(0) % 8 == 0 &&
+           t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  };
+  if (x.dim() < 1 || x.size(-1) == 0) return {};
+  const int64_t K = x.size(-1);
+  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({x.numel() / K, K});
+  if (!fits(x2) || !fits(wg) || !fits(wu) || !fits(wd) || wg.size(1) != K || wu.sizes() != wg.sizes() ||
+      wd.size(1) != wg.size(0) || wd.size(0) % 8 != 0 || act < 0 || act > 1)
+    return {};
+  auto h = gated_linear_fwd(x2, wg, wu, act, keep);
+  at::Tensor y = ffn_product(h[0], wd, c10::nullopt, c10::nullopt, false, false, false, !keep);
+  if (x.dim() != 2) {
+    auto sizes = x.sizes().vec();
+    sizes.back() = wd.size(0);
+    y = y.view(sizes);
+  }
+  return {y, x2, h[1]};
 }
 
 // {h [M, F], dgu [M, 2 F]} of dy [M, C], wd [C, F] and the kept gu [M, 2 F].
@@ -416,9 +705,10 @@ std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor&
   return {h, dgu};
 }
 
+// `ahead`: the kernel in front on this stream is the gate kernel that wrote `a`.
 // A B^T (+ A2 B2^T) in bf16 or fp32.  a [M, K] or, with a_mn, [K, M]; b [N, K] or, with b_mn, [K, N].
 at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& a2,
-                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32) {
+                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32, bool ahead) {
   using namespace ffn;
   TORCH_CHECK(a.dim() == 2 && b.dim() == 2, "gated_ffn: matrices");
   const int64_t M = a.size(a_mn ? 1 : 0), K = a.size(a_mn ? 0 : 1), N = b.size(b_mn ? 1 : 0);
@@ -441,7 +731,9 @@ at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::opti
   const at::Tensor* pb = b2.has_value() ? &*b2 : nullptr;
   auto stream = c10::cuda::getCurrentCUDAStream();
   TORCH_CHECK(b_mn || !a_mn, "gated_ffn: operand order");
-  if (a_mn) launch<256, kPlain, true, true>(a, b, pa, pb, args, stream);
+  if (!a_mn && !b_mn && !pa && !f32 && few_rows(M, N, 256, num_sms(a.get_device())))
+    launch_few(a, b, nullptr, out, 0, ahead, stream);
+  else if (a_mn) launch<256, kPlain, true, true>(a, b, pa, pb, args, stream);
   else if (b_mn) launch<256, kPlain, false, true>(a, b, pa, pb, args, stream);
   else launch<256, kPlain, false, false>(a, b, pa, pb, args, stream);
   return out;

@@ -640,10 +640,13 @@ static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, cons
 }
 
 // (dq, dk, dv) bf16.  `rows`, `keys`, `joins`: work lists of ops.SequencePack on the device.
-std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                        const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse,
+std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                                        const at::Tensor& o_, const at::Tensor& dout_, const at::Tensor& lse_,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, bool causal, double scale, bool fill) {
+  const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
+  const at::Tensor o = pa::tma_rows(o_.contiguous()), lse = lse_.contiguous();
+  const at::Tensor dout = pa::tma_rows(dout_.to(at::kBFloat16).contiguous());
   const pa::Shape s = pa::check_shapes(q, k, v, "packed_attention");
   pa::check_operand(dout, q, "packed_attention: gradient");
   TORCH_CHECK(dout.is_contiguous() && o.is_contiguous() && dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&

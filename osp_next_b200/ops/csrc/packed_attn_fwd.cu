@@ -20,6 +20,9 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "attention_fwd.cuh"
 #include "packed_attn.cuh"
 #include "packed_attn_host.h"
@@ -561,14 +564,22 @@ static void launch_packed_fwd(int64_t tiles, const CUtensorMap& tq, const CUtens
 }
 
 // (o [Nq, Hq, D] bf16, lse [Nq, Hq] fp32 or empty).  `items` / `joins` are int32 lists on the device,
-// laid out by ops.SequencePack for this group size; rows of no sequence are zeros (`fill`).
-std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+// laid out by ops.SequencePack for this group size; the pack needs `rows` and `key_rows`, its longest
+// sequence has `longest` rows.  Rows of no sequence are zeros.
+std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                         const at::Tensor& items, const at::Tensor& joins, int64_t slots,
-                                        int64_t positions, int64_t tiles, bool causal, double scale,
-                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, bool fill) {
+                                        int64_t positions, int64_t tiles, bool causal, double scale, bool own_scale,
+                                        const c10::optional<at::Tensor>& rel_bias_, bool want_lse, int64_t rows,
+                                        int64_t key_rows, int64_t longest, bool dense) {
+  const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
   const pa::Shape s = pa::check_shapes(q, k, v, "packed_attention");
+  TORCH_CHECK(s.Nq >= rows && s.Nk >= key_rows, "packed_attention: fewer rows than the pack's");
   pa::check_list(items, 8, q, "packed_attention: items");
   pa::check_list(joins, 4, q, "packed_attention: joins");
+  if (own_scale) scale = 1.0 / std::sqrt((double)std::max(1, s.D));
+  const bool fill = !(dense && s.Nq == rows);
+  c10::optional<at::Tensor> rel_bias;
+  if (rel_bias_.has_value()) rel_bias = rel_bias_->to(at::kFloat).contiguous();
   c10::cuda::CUDAGuard guard(q.device());
   auto opt = q.options();
   at::Tensor out = fill ? at::zeros({s.Nq, s.Hq, s.D}, opt) : at::empty({s.Nq, s.Hq, s.D}, opt);
@@ -599,7 +610,8 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k
   if (rel_bias.has_value()) {
     TORCH_CHECK(rel_bias->is_cuda() && rel_bias->device() == q.device() && rel_bias->scalar_type() == at::kFloat &&
                 rel_bias->is_contiguous() && rel_bias->dim() == 2 && rel_bias->size(0) == s.Hq &&
-                rel_bias->size(1) % 2 == 1, "packed_attention: rel_bias fp32 [heads, 2 M - 1]");
+                rel_bias->size(1) % 2 == 1 && rel_bias->size(1) >= 2 * longest - 1,
+                "packed_attention: rel_bias fp32 [heads, 2 M - 1], M at least the longest sequence");
     a.bias = rel_bias->data_ptr<float>();
     a.bias_m = (int)((rel_bias->size(1) + 1) / 2);
   }

@@ -12,6 +12,16 @@ struct Shape {
   int Nq, Nk, Hq, Hkv, D, G;
 };
 
+// `t` [N, H, D] as TMA can read it: itself where its last dim is contiguous and rows and heads lie at
+// multiples of 16 bytes (none of them broadcast), else a copy.
+static inline at::Tensor tma_rows(const at::Tensor& t) {
+  if (t.dim() != 3 || t.numel() == 0) return t;
+  const bool fits = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                    (t.size(1) == 1 || (t.stride(1) > 0 && t.stride(1) % 8 == 0)) &&
+                    (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % 8 == 0));
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // A [N, H, D] tensor that TMA can read as it lies.
 static inline void check_operand(const at::Tensor& x, const at::Tensor& q, const char* what) {
   TORCH_CHECK(x.is_cuda() && x.device() == q.device(), what, ": CUDA tensors on one device");

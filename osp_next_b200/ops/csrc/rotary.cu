@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
+#include <algorithm>
 #include <string>
 
 #include "common.cuh"
@@ -165,76 +166,89 @@ static void launch_type(const Args& a, bool half, int vec, cudaStream_t stream) 
 
 }  // namespace rotary
 
-// Rotated copies of q [n, Hq, D] and, if given, k [n, Hk, D].  pos int32 [n, axes]; table fp32
-// [positions, R / 2, 2]; sections: pairs of each axis (their sum R / 2).
-std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos,
-                                     const at::Tensor& table, std::vector<int64_t> sections, bool half, bool inverse) {
+// Rotated copies of q [..., n, Hq, D] and, if given, k [..., n, Hk, D].  pos [n] or [n, axes]; table fp32
+// [positions, R / 2, 2]; sections: pairs of each axis (their sum R / 2), or empty for one axis.
+std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos_,
+                                     const at::Tensor& table_, const std::vector<int64_t>& sections, bool half,
+                                     bool inverse) {
   using namespace rotary;
   const char* what = "rotary: ";
-  TORCH_CHECK(q.is_cuda() && q.dim() == 3, what, "CUDA q [tokens, heads, head_dim]");
-  const int64_t n = q.size(0), D = q.size(2), R = 2 * table.size(1);
-  TORCH_CHECK(pos.device() == q.device() && pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.dim() == 2 &&
-              pos.size(0) == n && pos.size(1) == (int64_t)sections.size() && pos.size(1) >= 1 && pos.size(1) <= 4,
-              what, "positions int32 [tokens, axes], 1 to 4 axes");
-  TORCH_CHECK(table.device() == q.device() && table.scalar_type() == at::kFloat && table.is_contiguous() &&
-              table.dim() == 3 && table.size(2) == 2 && table.size(0) < (1ll << 31), what,
-              "table fp32 [positions, pairs, 2]");
-  TORCH_CHECK(R <= D && D <= 256 && D % 2 == 0, what, "table of ", std::to_string(R / 2), " pairs for a head dim of ", std::to_string(D),
-              " (even, at most 256)");
+  TORCH_CHECK(q.is_cuda() && q.dim() >= 3 && table_.dim() == 3, what, "CUDA q [..., tokens, heads, head_dim]");
+  const int64_t tokens = q.size(-3), D = q.size(-1), R = 2 * table_.size(1);
+  int64_t lead = 1;
+  for (int64_t i = 0; i + 3 < q.dim(); ++i) lead *= q.size(i);
+  const int64_t n = lead * tokens, axes = std::max<int64_t>(1, (int64_t)sections.size());
+  TORCH_CHECK(pos_.device() == q.device() && at::isIntegralType(pos_.scalar_type(), false) &&
+              (pos_.dim() == 1 || pos_.dim() == 2) && pos_.size(0) == tokens &&
+              (pos_.dim() == 1 ? axes == 1 : pos_.size(1) == axes) && axes <= 4,
+              what, "whole positions [tokens] or [tokens, axes], 1 to 4 axes");
+  TORCH_CHECK(table_.device() == q.device() && table_.scalar_type() == at::kFloat && table_.size(2) == 2 &&
+              table_.size(0) < (1ll << 31), what, "table fp32 [positions, pairs, 2]");
+  TORCH_CHECK(R <= D && D <= 256 && D % 2 == 0, what, "table of ", std::to_string(R / 2), " pairs for a head dim of ",
+              std::to_string(D), " (even, at most 256)");
+  TORCH_CHECK(n < (1ll << 31), what, "too many tokens");
   c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor pos = pos_.to(at::kInt).contiguous();
+  if (lead > 1) pos = pos.view({tokens, axes}).repeat({lead, 1});
+  const at::Tensor table = table_.contiguous();
   Args a{};
-  std::vector<at::Tensor> out;
-  const int size = (int)q.element_size();
-  int vec = 16 / size;
-  const at::Tensor* in[2] = {&q, k.has_value() ? &*k : nullptr};
-  for (int i = 0; i < 2 && in[i]; ++i) {
-    const at::Tensor& x = *in[i];
-    TORCH_CHECK(x.device() == q.device() && x.scalar_type() == q.scalar_type() && x.dim() == 3 && x.size(0) == n &&
-                x.size(2) == D && (D == 0 || x.stride(2) == 1), what, "q and k [tokens, heads, head_dim] of one type");
-    out.push_back(at::empty({n, x.size(1), D}, x.options()));
-    a.t[i] = {x.data_ptr(), out.back().data_ptr(), x.stride(0), x.stride(1), (int)x.size(1)};
-    auto fits = [&](int v) {
-      return reinterpret_cast<uintptr_t>(x.data_ptr()) % (v * size) == 0 && x.stride(0) % v == 0 && x.stride(1) % v == 0;
+  std::vector<at::Tensor> in, out;
+  const int size = (int)q.element_size(), wide = 16 / size;
+  in.push_back(q);
+  if (k.has_value()) in.push_back(*k);
+  // every piece lies in the turned or in the copied part
+  int fit = wide;
+  while (fit > 1 && ((half ? R / 2 : R) % fit || (D - R) % fit)) fit >>= 1;
+  int vec = fit;
+  for (size_t i = 0; i < in.size(); ++i) {
+    const at::Tensor& x = in[i];
+    TORCH_CHECK(x.device() == q.device() && x.scalar_type() == q.scalar_type() && x.dim() == q.dim() &&
+                x.size(-1) == D, what, "q and k [..., tokens, heads, head_dim] of one type");
+    for (int64_t j = 0; j + 2 < q.dim(); ++j)
+      TORCH_CHECK(x.size(j) == q.size(j), what, "q and k of as many tokens");
+    out.push_back(at::empty(x.sizes(), x.options()));
+    if (x.dim() != 3) in[i] = x.reshape({n, x.size(-2), D});
+    auto fits = [&](const at::Tensor& t, int v) {
+      return t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % (v * size) == 0 && t.stride(0) % v == 0 &&
+             t.stride(1) % v == 0;
     };
-    while (vec > 1 && !fits(vec)) vec >>= 1;
+    if (in[i].numel() > 0) {
+      if (in[i].stride(2) != 1) in[i] = in[i].contiguous();
+      // pairs at odd addresses: one aligned copy
+      if (!half && !fits(in[i], 2)) in[i] = in[i].clone(at::MemoryFormat::Contiguous);
+      while (vec > 1 && !fits(in[i], vec)) vec >>= 1;
+    }
+    a.t[i] = {in[i].data_ptr(), out[i].data_ptr(), in[i].stride(0), in[i].stride(1), (int)in[i].size(1)};
   }
+  int64_t end = 0;
+  for (int64_t i = 0; i < axes; ++i) {
+    const int64_t pairs = sections.empty() ? R / 2 : sections[i];
+    TORCH_CHECK(pairs >= 0, what, "sections from 0 on");
+    a.end[i] = (int)(end += pairs);
+  }
+  TORCH_CHECK(end == R / 2, what, "sections of ", std::to_string(end), " pairs, table of ", std::to_string(R / 2));
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat, what,
+              "bf16, fp16 or fp32");
   if (n == 0 || D == 0 || R == 0) {
-    for (int i = 0; i < 2 && in[i]; ++i) out[i].copy_(*in[i]);
+    for (size_t i = 0; i < in.size(); ++i) out[i].copy_(q.dim() == 3 ? in[i] : in[i].view(out[i].sizes()));
     return out;
   }
-  // every piece lies in the turned or in the copied part
-  while (vec > 1 && ((half ? R / 2 : R) % vec || (D - R) % vec)) vec >>= 1;
-  const int wide = 16 / size;
   vec = vec == wide ? wide : vec >= 2 ? 2 : 1;
-  if (!half && vec == 1) {       // pairs at odd addresses: one aligned copy, then as usual
-    std::vector<at::Tensor> c;
-    for (int i = 0; i < 2 && in[i]; ++i) c.push_back(in[i]->clone(at::MemoryFormat::Contiguous));
-    return rotary_apply(c[0], c.size() > 1 ? c10::optional<at::Tensor>(c[1]) : c10::nullopt, pos, table, sections,
-                        half, inverse);
-  }
   a.pos = pos.data_ptr<int>();
   a.table = reinterpret_cast<const float2*>(table.data_ptr<float>());
   TORCH_CHECK(reinterpret_cast<uintptr_t>(a.table) % 8 == 0, what, "table at a multiple of 8 bytes");
   a.n = n;
-  a.axes = (int)sections.size();
+  a.axes = (int)axes;
   a.positions = (int)table.size(0);
   a.D = (int)D;
   a.R = (int)R;
-  int64_t end = 0;
-  for (size_t i = 0; i < sections.size(); ++i) {
-    TORCH_CHECK(sections[i] >= 0, what, "sections from 0 on");
-    a.end[i] = (int)(end += sections[i]);
-  }
-  TORCH_CHECK(end == R / 2, what, "sections of ", std::to_string(end), " pairs, table of ",
-              std::to_string(R / 2));
   a.sign = inverse ? -1.0f : 1.0f;
   a.err = error_word(q.get_device());
   auto stream = c10::cuda::getCurrentCUDAStream();
   switch (q.scalar_type()) {
     case at::kBFloat16: launch_type<__nv_bfloat16>(a, half, vec, stream); break;
     case at::kHalf: launch_type<__half>(a, half, vec, stream); break;
-    case at::kFloat: launch_type<float>(a, half, vec, stream); break;
-    default: TORCH_CHECK(false, what, "bf16, fp16 or fp32");
+    default: launch_type<float>(a, half, vec, stream);
   }
   return out;
 }

@@ -70,17 +70,21 @@ def gated_linear(x, w_gate, w_up, act: str = "silu"):
 def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
     """``(act(x W_gate^T) * (x W_up^T)) W_down^T``: x [..., K], W_gate and W_up [F, K], W_down [C, F] ->
     [..., C] (bf16 on the GPU).  It records no graph (see :func:`gated_linear`)."""
-    check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
         raise RuntimeError("gated_ffn has no gradient here: use models.functional.gated_ffn, or torch.no_grad()")
+    if x.is_cuda and act in ACTS:
+        out = ext().gated_ffn_fwd(x, w_gate, w_up, w_down, ACTS[act], False)
+        if out:
+            return out[0]
+    check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
     if not x.is_cuda:
         return ref.gated_ffn(x, w_gate, w_up, w_down, act)
     C, F = w_down.shape
     K = x.shape[-1]
     lead = x.shape[:-1]
-    if K == 0 or F == 0 or C == 0:
+    if 0 in (K, F, C, lead.numel()):
         return x.new_zeros(*lead, C, dtype=torch.bfloat16)
-    h = ext().gated_linear_fwd(matrix(x.reshape(lead.numel(), K)), hidden_rows(w_gate), hidden_rows(w_up), ACTS[act],
-                               False)[0]
-    y = ext().ffn_product(h, hidden_rows(w_down), None, None, False, False, False)
-    return y[:, :C].reshape(*lead, C)
+    # copies that fit; the down weight's too before the gate kernel, which the product starts behind
+    parts = [matrix(x.reshape(lead.numel(), K)), hidden_rows(w_gate), hidden_rows(w_up), hidden_rows(w_down)]
+    return ext().gated_ffn_fwd(*parts, ACTS[act], False)[0][:, :C].reshape(*lead, C)

@@ -19,7 +19,7 @@ from . import reference as ref
 from ._ext import ext
 
 TILE = 128             # rows of a tensor-core tile: group heads x positions, or keys
-_LONG_STEPS = 8        # mean key tiles of an item from which a forward CTA takes two row tiles
+_LONG_STEPS = 6        # mean key tiles of an item from which a forward CTA takes two row tiles
 _MIN_FWD_STEPS = 4     # key tiles below which splitting an item further costs more than it gives
 _MIN_KEY_STEPS = 8     # the same for the row tiles of a key tile's gradient
 
@@ -150,9 +150,14 @@ def positions(pack, group):
 
 def row_tiles(pack, group, causal):
     """Row tiles of a forward CTA: two share the key tiles that they read, one leaves room for a second
-    CTA on the SM, which covers the latency of short passes."""
-    _, steps = _row_items(pack, group, causal, 2 * positions(pack, group))
-    return 1 if len(steps) and steps.mean() < _LONG_STEPS else 2
+    CTA on the SM, which covers the latency of short passes and of tiles of few rows (one token each over
+    up to 8192 keys: 127 us in ones, 155 in twos; 8 prompts of 512 tokens 46 and 48; one of 8192: 555
+    and 474).  Sequences that fit one tile have no use for two."""
+    per = positions(pack, group)
+    if pack.lengths.max(initial=0) <= per:
+        return 1
+    _, steps = _row_items(pack, group, causal, 2 * per)
+    return 1 if steps.mean() < _LONG_STEPS else 2
 
 
 def _row_items(pack, group, causal, per):
@@ -268,15 +273,6 @@ def check_packed(q, k, v, pack, rel_bias=None, what="packed_attention"):
             raise TypeError(f"{what}: rel_bias on {rel_bias.device}, q on {q.device}")
 
 
-def tma_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [N, H, D] with a contiguous last dimension, rows and heads at multiples of 16 bytes and no
-    broadcast ones: itself where it lies that way, else a copy."""
-    n, h, _ = t.shape
-    fits = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (h == 1 or (t.stride(1) > 0 and t.stride(1) % 8 == 0))
-            and (n == 1 or (t.stride(0) > 0 and t.stride(0) % 8 == 0)))
-    return t if fits else t.clone(memory_format=torch.contiguous_format)
-
-
 def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Optional[float] = None, rel_bias=None,
                      return_lse: bool = False):
     """softmax(scale q k^T + bias) v inside each sequence of ``pack``: o [Nq, heads, D] like q
@@ -293,24 +289,29 @@ def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
     among them.
 
     It records no graph: ``models.functional.packed_attention`` is the form under autograd."""
-    check_packed(q, k, v, pack, rel_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, rel_bias)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (rel_bias is not None and rel_bias.requires_grad)):
+        check_packed(q, k, v, pack, rel_bias)
         raise RuntimeError("packed_attention has no gradient: use models.functional.packed_attention, or "
                            "torch.no_grad()")
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not q.is_cuda:
+        check_packed(q, k, v, pack, rel_bias)
+        scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
         o, lse = ref.packed_attention(q, k, v, pack, causal, scale, rel_bias)
         return (o, lse) if return_lse else o
-    if q.dtype != torch.bfloat16:
-        raise TypeError(f"packed_attention: bf16 on the GPU, got {q.dtype}")
-    if rel_bias is not None:
-        rel_bias = rel_bias.float().contiguous()
-    Hkv = k.shape[1]
-    group = 1 if rel_bias is not None else q.shape[1] // Hkv      # heads of a row tile (one with a bias)
-    items, joins, slots, per, tiles = pack.forward_lists(group, q.shape[1] // group, bool(causal))
-    fill = not (pack.dense and q.shape[0] == pack.rows)
-    o, lse = ext().packed_attn_fwd(tma_rows(q), tma_rows(k), tma_rows(v), items, joins, slots, per, tiles,
-                                   bool(causal), scale, rel_bias, bool(return_lse), fill)
+    try:
+        # the kernel's own checks come first: a call of a few microseconds has no time for both
+        Hkv = k.shape[1]
+        group = 1 if rel_bias is not None else q.shape[1] // Hkv  # heads of a row tile (one with a bias)
+        items, joins, slots, per, tiles = pack.forward_lists(group, q.shape[1] // group, bool(causal))
+        o, lse = ext().packed_attn_fwd(q, k, v, items, joins, slots, per, tiles, bool(causal),
+                                       -1.0 if scale is None else float(scale), scale is None, rel_bias,
+                                       bool(return_lse), pack.rows, pack.key_rows, pack.longest, pack.dense)
+    except (AttributeError, IndexError, RuntimeError, TypeError, ValueError, ZeroDivisionError):
+        check_packed(q, k, v, pack, rel_bias)
+        if q.dtype != torch.bfloat16:
+            raise TypeError(f"packed_attention: bf16 on the GPU, got {q.dtype}") from None
+        raise
     return (o, lse) if return_lse else o
 
 
@@ -328,7 +329,4 @@ def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool
     Hkv = k.shape[1]
     rows, keys, joins, slots = pack.backward_lists(q.shape[1] // Hkv, Hkv, bool(causal))
     fill = not (pack.dense and pack.key_dense and q.shape[0] == pack.rows and k.shape[0] == pack.key_rows)
-    dout = dout.to(torch.bfloat16).contiguous()
-    dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
-    return ext().packed_attn_bwd(tma_rows(q), tma_rows(k), tma_rows(v), o.contiguous(), dout, lse.contiguous(), rows,
-                                 keys, joins, slots, bool(causal), scale, fill)
+    return ext().packed_attn_bwd(q, k, v, o, dout, lse, rows, keys, joins, slots, bool(causal), scale, fill)

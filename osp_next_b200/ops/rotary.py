@@ -89,6 +89,25 @@ def rotary(q, k, pos, table, layout: str = "half", sections: Optional[Sequence[i
     and is reported by ``check_device_errors`` on the GPU, and raises on the CPU.
 
     It records no graph: ``models.functional.rotary`` is the form under autograd."""
+    if q.is_cuda and not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        try:
+            # the kernel's own checks come first: a call of a few microseconds has no time for both
+            if layout == "half" or layout == "interleaved":
+                out = ext().rotary_apply(q, k, pos, table, () if sections is None else sections, layout == "half",
+                                         inverse)
+                return out[0], out[1] if k is not None else None
+        except (RuntimeError, TypeError):
+            _check(q, k, pos, table, layout, sections)
+            raise
+    ts, pos, sections = _check(q, k, pos, table, layout, sections)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError("rotary has no gradient here: use models.functional.rotary, or torch.no_grad()")
+    out = [ref.rotary(t, pos, table, layout, sections, inverse) for t in ts]
+    return out[0], out[1] if k is not None else None
+
+
+def _check(q, k, pos, table, layout, sections):
+    """Raise for arguments that do not fit each other; (tensors, pos [n, axes], sections)."""
     ts = [t for t in (q, k) if t is not None]
     if layout not in LAYOUTS:
         raise ValueError(f"rotary: layout one of {LAYOUTS}, got {layout!r}")
@@ -113,16 +132,4 @@ def rotary(q, k, pos, table, layout: str = "half", sections: Optional[Sequence[i
         pos = pos[:, None]
     if pos.shape != (n, axes):
         raise ValueError(f"rotary: pos [{n}] or [{n}, {axes}], got {tuple(pos.shape)}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError("rotary has no gradient here: use models.functional.rotary, or torch.no_grad()")
-    if not q.is_cuda:
-        out = [ref.rotary(t, pos, table, layout, sections, inverse) for t in ts]
-    else:
-        lead = q.shape[:-3].numel()
-        p = pos.to(torch.int32).contiguous() if lead == 1 else pos.to(torch.int32).repeat(lead, 1)
-        flat = [t.reshape(lead * n, t.shape[-2], D) for t in ts]
-        flat = [t if t.stride(-1) == 1 or D == 0 else t.contiguous() for t in flat]
-        out = ext().rotary_apply(flat[0], flat[1] if k is not None else None, p, table.contiguous(), sections,
-                                 layout == "half", bool(inverse))
-        out = [o.view(t.shape) for o, t in zip(out, ts)]
-    return out[0], out[1] if k is not None else None
+    return ts, pos, sections
