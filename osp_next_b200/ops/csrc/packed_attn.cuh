@@ -57,6 +57,16 @@ __device__ __forceinline__ KeyItem load_key_item(const int* list, int i) {
   return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 
+// Item and head of this CTA.  Items are sorted longest first; `at_once` heads are run together, the next
+// ones behind them, so that the CTAs that run at a time share keys in L2.
+__device__ __forceinline__ void unit_of(int units, int heads, int at_once, int& item, int& head) {
+  const int u = blockIdx.x, n = units / heads;
+  const int group = u / (n * at_once), in = u - group * n * at_once;
+  const int wide = min(at_once, heads - group * at_once);
+  item = in / wide;
+  head = group * at_once + in - item * wide;
+}
+
 // Zeros into rows [row0, 128) of `boxes` boxes of 128 rows x 128 bytes, by one warp.  Whole rows, so
 // the swizzle inside a row does not matter.  The caller fences towards the async proxy.
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int boxes, int row0, int lane) {
@@ -75,6 +85,72 @@ __device__ __forceinline__ uint4 pack8(const uint32_t* v, float mul) {
   w.z = pack_bf16x2(__uint_as_float(v[4]) * mul, __uint_as_float(v[5]) * mul);
   w.w = pack_bf16x2(__uint_as_float(v[6]) * mul, __uint_as_float(v[7]) * mul);
   return w;
+}
+
+// 16 bytes of a warp's 32 rows x kPiece bytes in shared memory, swizzled by the row: eight rows' pieces
+// lie in different banks, and so do the pieces of a row.
+template <int kPiece>
+__device__ __forceinline__ uint4* out_piece(uint8_t* buf, int row, int piece) {
+  const int x = kPiece == 128 ? row & 7 : (row >> 1) & 3;
+  return reinterpret_cast<uint4*>(buf + row * kPiece + ((piece ^ x) << 4));
+}
+
+// kCols (32 or 64) columns of a warp's 32 rows of tensor memory, scaled, to bf16 rows in global memory:
+// through `buf` (4 KB of the warp's own), so that 4 or 8 lanes write a row's piece.  `at`: place of this
+// lane's row and first column in `base`, or -1; `have`: the accumulator was written (else zeros).
+template <int kCols>
+__device__ __forceinline__ void store_rows(uint8_t* buf, uint32_t taddr, bool have, float mul, __nv_bfloat16* base,
+                                           long at, int valid, int lane) {
+  constexpr int kLanes = kCols / 8;
+#pragma unroll
+  for (int h = 0; h < kCols / 32; ++h) {
+    uint32_t o[32];
+    if (have) {
+      tmem_ld32(taddr + h * 32, o);
+      tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *out_piece<kCols * 2>(buf, lane, h * 4 + i) = pack8(o + 8 * i, mul);
+  }
+  __syncwarp();
+  const int piece = lane % kLanes;
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i) {
+    const int rr = i * (32 / kLanes) + lane / kLanes;
+    const long to = __shfl_sync(0xffffffffu, at, rr);
+    if (to >= 0 && piece * 8 < valid)
+      *reinterpret_cast<uint4*>(base + to + piece * 8) = *out_piece<kCols * 2>(buf, rr, piece);
+  }
+  __syncwarp();
+}
+// The same in fp32 (parts of a sum), 32 columns at a time.
+template <int kCols>
+__device__ __forceinline__ void store_rows32(uint8_t* buf, uint32_t taddr, float mul, float* base, long at, int valid,
+                                             int lane) {
+#pragma unroll
+  for (int h = 0; h < kCols / 32; ++h) {
+    uint32_t o[32];
+    tmem_ld32(taddr + h * 32, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<float4*>(out_piece<128>(buf, lane, i)) =
+          make_float4(__uint_as_float(o[4 * i]) * mul, __uint_as_float(o[4 * i + 1]) * mul,
+                      __uint_as_float(o[4 * i + 2]) * mul, __uint_as_float(o[4 * i + 3]) * mul);
+    __syncwarp();
+    const int piece = lane % 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int rr = i * 4 + lane / 8;
+      const long to = __shfl_sync(0xffffffffu, at, rr);
+      if (to >= 0 && h * 32 + piece * 4 < valid)
+        *reinterpret_cast<uint4*>(base + to + h * 32 + piece * 4) = *out_piece<128>(buf, rr, piece);
+    }
+    __syncwarp();
+  }
 }
 
 }  // namespace pa

@@ -22,6 +22,8 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
+
 #include "packed_attn.cuh"
 #include "packed_attn_host.h"
 
@@ -35,6 +37,7 @@ constexpr int kBwdThreads = 384;
 struct PackedBwdArgs {
   const int* items;
   int G, P, Hq, Hkv, Dr;
+  int units, at_once;      // items x key heads, heads run together (pa::unit_of)
   int causal;
   const float* lse;        // [Nq, Hq] natural log
   const float* delta;      // [Nq, Hq]
@@ -78,21 +81,6 @@ __device__ __forceinline__ void store_pairs(uint32_t taddr, const float* v) {
   tmem_st4(taddr, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// 32 columns of a gradient row, scaled, to bf16 (columns from Dr on do not exist).
-__device__ __forceinline__ void store_grad(__nv_bfloat16* row, int c, int Dr, const uint32_t* v, float mul) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (c + 8 * i < Dr) *reinterpret_cast<uint4*>(row + c + 8 * i) = pa::pack8(v + 8 * i, mul);
-}
-__device__ __forceinline__ void store_part(float* row, int c, int Dr, const uint32_t* v, float mul) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c + 4 * i < Dr)
-      *reinterpret_cast<float4*>(row + c + 4 * i) =
-          make_float4(__uint_as_float(v[4 * i]) * mul, __uint_as_float(v[4 * i + 1]) * mul,
-                      __uint_as_float(v[4 * i + 2]) * mul, __uint_as_float(v[4 * i + 3]) * mul);
-}
-
 // ---------------------------------------------------------------------------- dK, dV
 template <int D>
 struct KeySmem {
@@ -111,8 +99,9 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                    PackedBwdArgs args) {
   using L = KeySmem<D>;
-  const pa::KeyItem it = pa::load_key_item(args.items, blockIdx.x / args.Hkv);
-  const int kvh = blockIdx.x % args.Hkv;
+  int item_no, kvh;
+  pa::unit_of(args.units, args.Hkv, args.at_once, item_no, kvh);
+  const pa::KeyItem it = pa::load_key_item(args.items, item_no);
   const int G = args.G, P = args.P;
   const int n_q = (it.n_q + P - 1) / P;                   // row tiles
   const int used = G * P;
@@ -177,6 +166,27 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         tma_load_3d(&tmV, kv_full, sV + db * L::BOX, db * 64, kvh, it.k_row);
       }
     }
+    // this lane's four columns of a row tile: log-sum-exp and delta, fetched a tile ahead
+    int col[4];
+    float vl[4], vd[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = lane + 32 * e;
+      col[e] = c / G * args.Hq + c % G;
+    }
+    const float* lse0 = args.lse + (long)it.q_row * args.Hq + kvh * G;
+    const float* del0 = args.delta + (long)it.q_row * args.Hq + kvh * G;
+    auto fetch = [&](int i) {
+      const int rows = min(P, it.n_q - i * P) * G;
+      const long at = (long)i * P * args.Hq;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = lane + 32 * e < rows;
+        vl[e] = in ? lse0[at + col[e]] : 0.f;
+        vd[e] = in ? del0[at + col[e]] : 0.f;
+      }
+    };
+    if (n_q > 0) fetch(0);
     for (int i = 0; i < n_q && !*abort_flag; ++i) {
       const int st = i & 1;
       const int rows = min(P, it.n_q - i * P) * G;             // rows of the sequence in this tile
@@ -197,11 +207,11 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       float* v = sVec + st * 2 * kT;
 #pragma unroll
-      for (int c = lane; c < kT; c += 32) {
-        const long row = (long)(it.q_row + i * P + c / G) * args.Hq + kvh * G + c % G;
-        v[c] = c < rows ? args.lse[row] * pa::kLog2e : 0.f;
-        v[kT + c] = c < rows ? args.delta[row] : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        v[lane + 32 * e] = vl[e] * pa::kLog2e;
+        v[kT + lane + 32 * e] = vd[e];
       }
+      if (i + 1 < n_q) fetch(i + 1);
       if (cut) {
         ok = __all_sync(0xffffffffu, mbar_wait(tail, 0, args.err, kErrAttnProducer));
         if (!ok) { *abort_flag = 1; break; }
@@ -335,28 +345,18 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(done, 0, args.err, kErrAttnTeardown)))) *abort_flag = 1;
       tc_fence_after();
     }
+    // K and V have been read for the last time: their place stages the results
+    uint8_t* buf = smem + (warp - 4) * 4096;
+    const int c0 = half * (D / 2), left = args.Dr - c0;
     const bool valid = ok && r < it.n_k;
-    const long row = ((long)(it.k_row + r) * args.Hkv + kvh) * args.Dr;
-    const long prow = it.slot < 0 ? 0 : (((long)it.slot * args.Hkv + kvh) * 2 * kT + r) * args.Dr;
-#pragma unroll 1
-    for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-      uint32_t a[32], g[32];
-      if (n_q > 0) {
-        tmem_ld32(tDV + lane_off + c, a);
-        tmem_ld32(tDK + lane_off + c, g);
-        tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) a[e] = g[e] = 0u;
-      }
-      if (!valid) continue;
-      if (it.slot < 0) {
-        store_grad(args.dv + row, c, args.Dr, a, 1.0f);
-        store_grad(args.dk + row, c, args.Dr, g, args.scale);
-      } else {
-        store_part(args.part + prow, c, args.Dr, a, 1.0f);
-        store_part(args.part + prow + (long)kT * args.Dr, c, args.Dr, g, args.scale);
-      }
+    if (it.slot < 0) {
+      const long at = valid ? ((long)(it.k_row + r) * args.Hkv + kvh) * args.Dr + c0 : -1;
+      pa::store_rows<D / 2>(buf, tDV + lane_off + c0, n_q > 0, 1.0f, args.dv, at, left, lane);
+      pa::store_rows<D / 2>(buf, tDK + lane_off + c0, n_q > 0, args.scale, args.dk, at, left, lane);
+    } else {
+      const long at = valid ? (((long)it.slot * args.Hkv + kvh) * 2 * kT + r) * args.Dr + c0 : -1;
+      pa::store_rows32<D / 2>(buf, tDV + lane_off + c0, 1.0f, args.part, at, left, lane);
+      pa::store_rows32<D / 2>(buf, tDK + lane_off + c0, args.scale, args.part + (long)kT * args.Dr, at, left, lane);
     }
   }
   tc_fence_before();
@@ -406,8 +406,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                  PackedBwdArgs args) {
   using L = RowSmem<D>;
-  const pa::FwdItem it = pa::load_fwd_item(args.items, blockIdx.x / args.Hkv);
-  const int kvh = blockIdx.x % args.Hkv;
+  int item_no, kvh;
+  pa::unit_of(args.units, args.Hkv, args.at_once, item_no, kvh);
+  const pa::FwdItem it = pa::load_fwd_item(args.items, item_no);
   const int G = args.G, P = args.P;
   const int n_kv = it.kt1;
   const int last_rows = it.n_keys - (n_kv - 1) * kT;
@@ -596,19 +597,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(done, 0, args.err, kErrAttnTeardown)))) *abort_flag = 1;
       tc_fence_after();
     }
-    const bool valid = ok && in;
-#pragma unroll 1
-    for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-      uint32_t a[32];
-      if (n_kv > 0) {
-        tmem_ld32(tDQ + lane_off + c, a);
-        tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) a[e] = 0u;
-      }
-      if (valid) store_grad(args.dq + row * args.Dr, c, args.Dr, a, args.scale);
-    }
+    // Q and dO have been read for the last time: their place stages the results
+    const int c0 = half * (D / 2);
+    pa::store_rows<D / 2>(smem + (warp - 4) * 4096, tDQ + lane_off + c0, n_kv > 0, args.scale, args.dq,
+                          ok && in ? row * args.Dr + c0 : -1, args.Dr - c0, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -622,19 +614,23 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 template <int D>
 static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const CUtensorMap& tdo, PackedBwdArgs a, const at::Tensor& rows, const at::Tensor& keys,
-                              cudaStream_t stream) {
+                              int64_t row_heads, int64_t key_heads, cudaStream_t stream) {
   if (keys.size(0) > 0) {
     auto kern = packed_dkdv_kernel<D>;
     smem_opt_in(reinterpret_cast<const void*>(kern), KeySmem<D>::BYTES);
     a.items = keys.data_ptr<int>();
-    kern<<<(unsigned)(keys.size(0) * a.Hkv), kBwdThreads, KeySmem<D>::BYTES, stream>>>(tq, tk, tv, tdo, a);
+    a.units = (int)(keys.size(0) * a.Hkv);
+    a.at_once = (int)std::clamp<int64_t>(key_heads, 1, a.Hkv);
+    kern<<<(unsigned)a.units, kBwdThreads, KeySmem<D>::BYTES, stream>>>(tq, tk, tv, tdo, a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   if (rows.size(0) > 0) {
     auto kern = packed_dq_kernel<D>;
     smem_opt_in(reinterpret_cast<const void*>(kern), RowSmem<D>::BYTES);
     a.items = rows.data_ptr<int>();
-    kern<<<(unsigned)(rows.size(0) * a.Hkv), kBwdThreads, RowSmem<D>::BYTES, stream>>>(tq, tk, tv, tdo, a);
+    a.units = (int)(rows.size(0) * a.Hkv);
+    a.at_once = (int)std::clamp<int64_t>(row_heads, 1, a.Hkv);
+    kern<<<(unsigned)a.units, kBwdThreads, RowSmem<D>::BYTES, stream>>>(tq, tk, tv, tdo, a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
 }
@@ -643,7 +639,8 @@ static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, cons
 std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                         const at::Tensor& o_, const at::Tensor& dout_, const at::Tensor& lse_,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
-                                        int64_t slots, bool causal, double scale, bool fill) {
+                                        int64_t slots, int64_t row_heads, int64_t key_heads, bool causal, double scale,
+                                        bool fill) {
   const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
   const at::Tensor o = pa::tma_rows(o_.contiguous()), lse = lse_.contiguous();
   const at::Tensor dout = pa::tma_rows(dout_.to(at::kBFloat16).contiguous());
@@ -657,6 +654,7 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& 
   pa::check_list(rows, 8, q, "packed_attention: rows");
   pa::check_list(keys, 8, q, "packed_attention: keys");
   pa::check_list(joins, 4, q, "packed_attention: joins");
+  TORCH_CHECK(std::max(rows.size(0), keys.size(0)) * s.Hkv < (1ll << 30), "packed_attention: too much work for one call");
   c10::cuda::CUDAGuard guard(q.device());
   auto opt = q.options();
   auto make = [&](at::IntArrayRef sizes) { return fill ? at::zeros(sizes, opt) : at::empty(sizes, opt); };
@@ -693,8 +691,8 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& 
   }
   const CUtensorMap tq = pa::tile_map(q, q, s.D, s.G, a.P), tdo = pa::tile_map(dout, q, s.D, s.G, a.P);
   const CUtensorMap tk = pa::tile_map(k, q, s.D, 1, pa::kRows), tv = pa::tile_map(v, q, s.D, 1, pa::kRows);
-  if (s.D > 64) launch_packed_bwd<128>(tq, tk, tv, tdo, a, rows, keys, stream);
-  else launch_packed_bwd<64>(tq, tk, tv, tdo, a, rows, keys, stream);
+  if (s.D > 64) launch_packed_bwd<128>(tq, tk, tv, tdo, a, rows, keys, row_heads, key_heads, stream);
+  else launch_packed_bwd<64>(tq, tk, tv, tdo, a, rows, keys, row_heads, key_heads, stream);
   if (joins.size(0) > 0) {
     TORCH_CHECK(slots > 0, "packed_attention: joins without slots");
     packed_join_kernel<<<dim3((unsigned)joins.size(0), (unsigned)s.Hkv, 2 * kT / 8), 256, 0, stream>>>(

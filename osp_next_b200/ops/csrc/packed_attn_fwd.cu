@@ -33,6 +33,7 @@ struct PackedFwdArgs {
   const int* items;
   int units;                // items x heads that they are run for
   int heads;                // key heads, or query heads where a tile holds one head (bias)
+  int at_once;              // heads run together (pa::unit_of)
   int kv_ratio;             // of those to one key head
   int G, P, Hq, Dr;         // heads and positions of a tile, query heads, head dim
   int causal;
@@ -81,9 +82,8 @@ struct FwdUnit {
   int n_kv, last_rows;      // key tiles loaded, keys of the sequence in the last one
   bool has_tail;
 
-  __device__ FwdUnit(const PackedFwdArgs& args, const pa::FwdItem& item) : it(item) {
+  __device__ FwdUnit(const PackedFwdArgs& args, const pa::FwdItem& item, int h) : it(item), head(h) {
     constexpr int kT = pa::kRows;
-    head = blockIdx.x % args.heads;
     kvh = head / args.kv_ratio;
     n_kv = 0;
 #pragma unroll
@@ -114,14 +114,6 @@ __device__ __forceinline__ float masked_max(const uint32_t* sr, int cols, int n_
     mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
   }
   return mx;
-}
-
-// 16 bytes of a warp's 32 rows x kPiece bytes in shared memory, swizzled by the row: eight rows' pieces
-// lie in different banks, and so do the pieces of a row.
-template <int kPiece>
-__device__ __forceinline__ uint4* out_piece(uint8_t* buf, int row, int piece) {
-  const int x = kPiece == 128 ? row & 7 : (row >> 1) & 3;
-  return reinterpret_cast<uint4*>(buf + row * kPiece + ((piece ^ x) << 4));
 }
 
 template <int D, bool kBias, int kTiles>
@@ -155,7 +147,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int lane = threadIdx.x % 32;
 
   // the item's fetch and the tensor maps' run under the set-up; the copy is for the way out
-  const pa::FwdItem item = pa::load_fwd_item(args.items, blockIdx.x / args.heads);
+  int item_no, unit_head;
+  pa::unit_of(args.units, args.heads, args.at_once, item_no, unit_head);
+  const pa::FwdItem item = pa::load_fwd_item(args.items, item_no);
   pa::FwdItem* item_copy = reinterpret_cast<pa::FwdItem*>(smem + 512);
   if (warp == L::kProdWarp && lane == 0) {
     prefetch_tmap(&tmQ);
@@ -192,7 +186,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     int slot = 0;
     uint32_t phase = 1;
     {
-      const Unit un(args, item);
+      const Unit un(args, item, unit_head);
       const int krow0 = un.it.k_row + un.it.kt0 * kT;
       const int units = 2 * un.n_kv;
       if (lane == 0 && un.n_kv > 0) {
@@ -250,15 +244,26 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t va = smem_u32(sKV + slot * L::TILE);
         const uint32_t d = tmem + kO + (uint32_t)D * t;
         const uint32_t pr = tmem + 128u * t;
+        auto mma = [&](int k, bool acc) {
+          umma_bf16_ts(d, pr + 8u * k, sdesc_sw128(va + k * 2048, L::BOX, 1024), ID_PV, acc ? 1u : 0u);
+        };
         const int steps = j + 1 == un.n_t[t] ? (un.c_t[t] + 15) / 16 : kT / 16;
         if (!wait(&p_half[t], j & 1)) return false;
         tc_fence_after();
-        for (int k = 0; k < min(steps, kT / 32); ++k)
-          umma_bf16_ts(d, pr + 8u * k, sdesc_sw128(va + k * 2048, L::BOX, 1024), ID_PV, (j > 0 || k > 0) ? 1u : 0u);
+        if (steps == kT / 16) {                    // a rolled loop issues too slowly for whole tiles
+#pragma unroll
+          for (int k = 0; k < kT / 32; ++k) mma(k, j > 0 || k > 0);
+        } else {
+          for (int k = 0; k < min(steps, kT / 32); ++k) mma(k, j > 0 || k > 0);
+        }
         if (!wait(&p_full[t], j & 1)) return false;
         tc_fence_after();
-        for (int k = kT / 32; k < steps; ++k)
-          umma_bf16_ts(d, pr + 8u * k, sdesc_sw128(va + k * 2048, L::BOX, 1024), ID_PV, 1u);
+        if (steps == kT / 16) {
+#pragma unroll
+          for (int k = kT / 32; k < kT / 16; ++k) mma(k, true);
+        } else {
+          for (int k = kT / 32; k < steps; ++k) mma(k, true);
+        }
         if (j + 1 == un.n_t[t]) umma_commit(&o_done[t]);
         return true;
       };
@@ -266,7 +271,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       int slot = 0;
       uint32_t phase = 0;
       auto next = [&] { if (++slot == slots) { slot = 0; phase ^= 1; } };
-      const Unit un(args, item);
+      const Unit un(args, item, unit_head);
       const int n_kv = un.n_kv, n0 = un.n_t[0], n1 = un.n_t[kTiles - 1];
       if (n_kv > 0) ok = wait(q_full, 0) && wait(&kv_full[slot], phase);
       if (n_kv > 0 && ok) {
@@ -319,7 +324,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       int n, last_cols, limit, bias_at, bias_row, bias_off;
       bool idle;
       {
-        const Unit un(args, item);
+        const Unit un(args, item, unit_head);
         const int nq = min(P, un.it.n_q - t * P);       // queries of the tile (<= 0: it has none)
         if (nq <= 0) break;                             // uniform for the tile's warps
         const int pos = min(r / G, nq - 1);             // rows behind the last query repeat its mask
@@ -428,7 +433,6 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const float inv_l = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);   // no key seen: 0; NaN stays
       const float lse2 = m_ref + __log2f(l);
       const pa::FwdItem it = *item_copy;
-      const int unit_head = blockIdx.x % args.heads;
       const int rp = r / G, rh = r - rp * G;            // position and head of the row
       const bool in = rp < min(P, it.n_q - t * P) && r < G * P;
       const long row = (long)(it.q_row + t * P + rp) * args.Hq + unit_head * G + rh;
@@ -463,11 +467,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int first = c0 % per * size / 16;         // the first piece that these columns fill
         if (size == 2) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) *out_piece<L::kPiece>(buf, lane, first + i) = pa::pack8(o + 8 * i, inv_l);
+          for (int i = 0; i < 2; ++i) *pa::out_piece<L::kPiece>(buf, lane, first + i) = pa::pack8(o + 8 * i, inv_l);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(out_piece<L::kPiece>(buf, lane, first + i)) =
+            *reinterpret_cast<float4*>(pa::out_piece<L::kPiece>(buf, lane, first + i)) =
                 make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
                             __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
         }
@@ -479,7 +483,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const int rr = i * (32 / kLanes) + lane / kLanes;
           const long to = __shfl_sync(0xffffffffu, at, rr);
           if (to >= 0 && b0 < args.Dr * size)
-            *reinterpret_cast<uint4*>(base + to + b0) = *out_piece<L::kPiece>(buf, rr, piece);
+            *reinterpret_cast<uint4*>(base + to + b0) = *pa::out_piece<L::kPiece>(buf, rr, piece);
         }
         __syncwarp();
       }
@@ -568,7 +572,8 @@ static void launch_packed_fwd(int64_t tiles, const CUtensorMap& tq, const CUtens
 // sequence has `longest` rows.  Rows of no sequence are zeros.
 std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                         const at::Tensor& items, const at::Tensor& joins, int64_t slots,
-                                        int64_t positions, int64_t tiles, bool causal, double scale, bool own_scale,
+                                        int64_t positions, int64_t tiles, int64_t at_once, bool causal, double scale,
+                                        bool own_scale,
                                         const c10::optional<at::Tensor>& rel_bias_, bool want_lse, int64_t rows,
                                         int64_t key_rows, int64_t longest, bool dense) {
   const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
@@ -599,6 +604,7 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& 
   a.kv_ratio = a.heads / s.Hkv;
   TORCH_CHECK(n * a.heads < (1ll << 30), "packed_attention: too much work for one call");
   a.units = (int)(n * a.heads);
+  a.at_once = (int)std::clamp<int64_t>(at_once, 1, a.heads);
   a.P = (int)positions;
   TORCH_CHECK(a.P >= 1 && a.P * group <= pa::kRows && (tiles == 1 || tiles == 2), "packed_attention: row tiles");
   a.Hq = s.Hq;
