@@ -99,6 +99,12 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                    PackedBwdArgs args) {
   using L = KeySmem<D>;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+    prefetch_tmap(&tmDO);
+  }
   int item_no, kvh;
   pa::unit_of(args.units, args.Hkv, args.at_once, item_no, kvh);
   const pa::KeyItem it = pa::load_key_item(args.items, item_no);
@@ -138,10 +144,6 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     mbar_init(tail, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&tmQ);
-    prefetch_tmap(&tmK);
-    prefetch_tmap(&tmV);
-    prefetch_tmap(&tmDO);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -406,6 +408,12 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                  PackedBwdArgs args) {
   using L = RowSmem<D>;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+    prefetch_tmap(&tmDO);
+  }
   int item_no, kvh;
   pa::unit_of(args.units, args.Hkv, args.at_once, item_no, kvh);
   const pa::FwdItem it = pa::load_fwd_item(args.items, item_no);
@@ -445,10 +453,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     mbar_init(tail, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&tmQ);
-    prefetch_tmap(&tmK);
-    prefetch_tmap(&tmV);
-    prefetch_tmap(&tmDO);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);

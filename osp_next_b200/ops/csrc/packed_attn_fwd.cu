@@ -38,6 +38,7 @@ struct PackedFwdArgs {
   int G, P, Hq, Dr;         // heads and positions of a tile, query heads, head dim
   int causal;
   int q_box;                // bytes of a query box in shared memory (G * P rows, to 1024 bytes)
+  int q_tile;               // of a row tile's queries, whose place its results take on their way out
   int slots;                // of the K / V ring
   __nv_bfloat16* out;       // [Nq, Hq, Dr]
   float* lse;               // [Nq, Hq] or null
@@ -63,9 +64,8 @@ struct PackedFwdCfg {
   static constexpr int kOut = 32 * kPiece;                     // of a warp's 32 rows
   static constexpr int kBiasBytes = kBias ? 2 * 2 * 2 * pa::kRows * 4 : 0;   // of a row tile: 2 x 2 x 256 entries
   static constexpr int kRoom = kTiles == 2 ? 232448 : 115712;  // dynamic shared memory of a CTA
-  // barriers, bias and results lie in front, at fixed places: pointers cost the softmax no registers
-  static constexpr int OFF_OUT = 1024;
-  static constexpr int OFF_BIAS = OFF_OUT + 4 * kTiles * kOut;
+  // barriers and bias lie in front, at fixed places: pointers cost the softmax no registers
+  static constexpr int OFF_BIAS = 1024;
   static constexpr int OFF_Q = OFF_BIAS + kTiles * kBiasBytes;
   static_assert(OFF_Q % 1024 == 0, "swizzled tiles");
   static constexpr int kExtra = OFF_Q + 1024;                  // + alignment of the base
@@ -130,7 +130,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
   uint8_t* sQ = smem + L::OFF_Q;
-  uint8_t* sKV = sQ + kTiles * L::DB * args.q_box;
+  uint8_t* sKV = sQ + kTiles * args.q_tile;
   uint64_t* q_full = bars + 0;
   uint64_t* tail = bars + 1;                       // the V tile that reaches over the sequence's end
   uint64_t* kv_full = bars + 2;                    // [slots]
@@ -198,7 +198,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
             for (int db = 0; db < L::DB && un.n_t[t] > 0; ++db)
-              tma_load_3d(&tmQ, q_full, sQ + (t * L::DB + db) * args.q_box, db * 64, un.head * G, un.it.q_row + t * P);
+              tma_load_3d(&tmQ, q_full, sQ + t * args.q_tile + db * args.q_box, db * 64, un.head * G, un.it.q_row + t * P);
         }
         for (int i = 0; i < units && ok; ++i) {
           if (*abort_flag || !mbar_wait(&kv_empty[slot], phase, args.err, kErrAttnProducer)) { ok = false; break; }
@@ -230,7 +230,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       constexpr uint32_t ID_PV = idesc_bf16(128, D, /*b_mn_major=*/true);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, args.err, kErrAttnMma); };
       auto issue_s = [&](int t, int slot) {
-        const uint32_t qa = smem_u32(sQ + t * L::DB * args.q_box);
+        const uint32_t qa = smem_u32(sQ + t * args.q_tile);
         const uint32_t ka = smem_u32(sKV + slot * L::TILE);
         const uint32_t d = tmem + 128u * t;
 #pragma unroll
@@ -315,7 +315,6 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t tS = tmem + 128u * t + lane_off;
     const uint32_t tO = tmem + kO + (uint32_t)D * t + lane_off;
     const float sl2 = args.scale_log2;
-    uint8_t* buf = smem + L::OFF_OUT + warp * L::kOut;
     float* bias_buf = reinterpret_cast<float*>(smem + L::OFF_BIAS + t * L::kBiasBytes);
     bool ok = true;
     do {
@@ -444,6 +443,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // kPiece bytes of each row at a time through shared memory, so that kPiece / 16 lanes write a
       // row's piece; the row's place comes from the lane that owns it
       constexpr int kLanes = L::kPiece / 16;
+      uint8_t* buf = sQ + t * args.q_tile + quarter * L::kOut;   // the last S has been formed
       const int size = it.slot < 0 ? 2 : 4;             // bytes per value
       const int per = L::kPiece / size;                 // values of a row per pass: 64, 32 or 16
       const long at = in ? (it.slot < 0 ? row : prow) * args.Dr * size : -1;
@@ -552,7 +552,8 @@ static void launch_packed_fwd(const CUtensorMap& tq, const CUtensorMap& tk, cons
                               cudaStream_t stream) {
   using L = PackedFwdCfg<D, kTiles, kBias>;
   a.q_box = (a.G * a.P * 128 + 1023) / 1024 * 1024;
-  const int q_bytes = kTiles * L::DB * a.q_box;
+  a.q_tile = std::max(L::DB * a.q_box, 4 * L::kOut);
+  const int q_bytes = kTiles * a.q_tile;
   a.slots = std::min(L::kMaxSlots, (L::kRoom - L::kExtra - q_bytes) / L::TILE);
   auto kern = packed_fwd_kernel<D, kBias, kTiles>;
   smem_opt_in(reinterpret_cast<const void*>(kern), L::kRoom);
