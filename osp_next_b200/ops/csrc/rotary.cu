@@ -45,16 +45,102 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
-
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec { T v[V]; };
+
+// V values and their fp32 form; 16-bit ones two at a time (one conversion instruction each way).
+template <int V>
+__device__ __forceinline__ void widen(const Vec<float, V>& x, float* f) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = x.v[j];
+}
+template <int V>
+__device__ __forceinline__ void widen(const Vec<__half, V>& x, float* f) {
+  if constexpr (V == 1) {
+    f[0] = __half2float(x.v[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&x.v[j]));
+      f[j] = p.x;
+      f[j + 1] = p.y;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void widen(const Vec<__nv_bfloat16, V>& x, float* f) {
+  if constexpr (V == 1) {
+    f[0] = __bfloat162float(x.v[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x.v[j]));
+      f[j] = p.x;
+      f[j + 1] = p.y;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void narrow(Vec<float, V>& x, const float* f) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) x.v[j] = f[j];
+}
+template <int V>
+__device__ __forceinline__ void narrow(Vec<__half, V>& x, const float* f) {
+  if constexpr (V == 1) {
+    x.v[0] = __float2half_rn(f[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) *reinterpret_cast<__half2*>(&x.v[j]) = __floats2half2_rn(f[j], f[j + 1]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void narrow(Vec<__nv_bfloat16, V>& x, const float* f) {
+  if constexpr (V == 1) {
+    x.v[0] = __float2bfloat16(f[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) *reinterpret_cast<__nv_bfloat162*>(&x.v[j]) = __floats2bfloat162_rn(f[j], f[j + 1]);
+  }
+}
+
+// kHeads pieces (and, in the half layout, their partners `far` elements on), `step` elements apart,
+// all loads in flight before the first is used.
+template <typename T, int V, bool kHalf, int kHeads>
+__device__ __forceinline__ void turn_pieces(const T* src, T* dst, long in_step, int out_step, int far, bool turn,
+                                            const float2* cs) {
+  Vec<T, V> a[kHeads], b[kHeads];
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {
+    a[u] = *reinterpret_cast<const Vec<T, V>*>(src + u * in_step);
+    if (kHalf && turn) b[u] = *reinterpret_cast<const Vec<T, V>*>(src + u * in_step + far);
+  }
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {
+    if (turn) {
+      float fa[V], fb[V], x[V], y[V];
+      widen<V>(a[u], fa);
+      if constexpr (kHalf) {
+        widen<V>(b[u], fb);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          x[j] = fa[j] * cs[j].x - fb[j] * cs[j].y;
+          y[j] = fa[j] * cs[j].y + fb[j] * cs[j].x;
+        }
+        narrow<V>(b[u], y);
+        *reinterpret_cast<Vec<T, V>*>(dst + u * out_step + far) = b[u];
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          x[j] = fa[j] * cs[j / 2].x - fa[j + 1] * cs[j / 2].y;
+          x[j + 1] = fa[j] * cs[j / 2].y + fa[j + 1] * cs[j / 2].x;
+        }
+      }
+      narrow<V>(a[u], x);
+    }
+    *reinterpret_cast<Vec<T, V>*>(dst + u * out_step) = a[u];
+  }
+}
 
 __device__ __forceinline__ float2 pair_of(const Args& a, long token, int i, int first_pos, bool& bad) {
   int axis = 0;
@@ -71,7 +157,7 @@ __device__ __forceinline__ float2 pair_of(const Args& a, long token, int i, int 
 // One piece = V elements of a pair's first half and V of its second (half layout), or V elements
 // (V / 2 pairs, interleaved; also the copied elements).  Pieces of a head: half layout R / 2 / V and
 // (D - R) / V to copy, interleaved D / V.
-template <typename T, int V, bool kHalf, int kPieces>
+template <typename T, int V, bool kHalf, int kPieces, int kHeads>
 __global__ void __launch_bounds__(256)
 rotate(const Args args) {
   const long token = (long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
@@ -99,41 +185,26 @@ rotate(const Args args) {
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const Tensor& t = args.t[w];
-    const T* in = reinterpret_cast<const T*>(t.in) + token * t.row;
-    T* out = reinterpret_cast<T*>(t.out) + token * t.heads * D;
-    for (int h = group; h < t.heads; h += groups) {
 #pragma unroll
-      for (int k = 0; k < kPieces; ++k) {
-        const int p = sub + k * per;
-        if (p >= pieces) continue;
-        const T* src = in + h * t.head;
-        T* dst = out + (long)h * D;
-        if (p >= turned) {
-          const int o = R + (p - turned) * V;
-          *reinterpret_cast<Vec<T, V>*>(dst + o) = *reinterpret_cast<const Vec<T, V>*>(src + o);
-        } else if (kHalf) {
-          const Vec<T, V> a = *reinterpret_cast<const Vec<T, V>*>(src + p * V);
-          const Vec<T, V> b = *reinterpret_cast<const Vec<T, V>*>(src + R / 2 + p * V);
-          Vec<T, V> x, y;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float fa = to_f(a.v[j]), fb = to_f(b.v[j]);
-            x.v[j] = from_f<T>(fa * cs[k][j].x - fb * cs[k][j].y);
-            y.v[j] = from_f<T>(fa * cs[k][j].y + fb * cs[k][j].x);
-          }
-          *reinterpret_cast<Vec<T, V>*>(dst + p * V) = x;
-          *reinterpret_cast<Vec<T, V>*>(dst + R / 2 + p * V) = y;
-        } else {
-          const Vec<T, V> a = *reinterpret_cast<const Vec<T, V>*>(src + p * V);
-          Vec<T, V> x;
-#pragma unroll
-          for (int j = 0; j < V / 2; ++j) {
-            const float fa = to_f(a.v[2 * j]), fb = to_f(a.v[2 * j + 1]);
-            x.v[2 * j] = from_f<T>(fa * cs[k][j].x - fb * cs[k][j].y);
-            x.v[2 * j + 1] = from_f<T>(fa * cs[k][j].y + fb * cs[k][j].x);
-          }
-          *reinterpret_cast<Vec<T, V>*>(dst + p * V) = x;
-        }
+    for (int k = 0; k < kPieces; ++k) {
+      const int p = sub + k * per;
+      if (p >= pieces) continue;
+      const bool turn = p < turned;
+      const int o = turn ? p * V : R + (p - turned) * V;     // this piece's place in the head
+      const T* src = reinterpret_cast<const T*>(t.in) + token * t.row + group * t.head + o;
+      T* dst = reinterpret_cast<T*>(t.out) + (token * t.heads + group) * D + o;
+      const long in_step = groups * t.head;
+      const int out_step = groups * D;
+      int h = group;
+      for (; h + (kHeads - 1) * groups < t.heads; h += kHeads * groups) {
+        turn_pieces<T, V, kHalf, kHeads>(src, dst, in_step, out_step, R / 2, turn, cs[k]);
+        src += kHeads * in_step;
+        dst += kHeads * out_step;
+      }
+      for (; h < t.heads; h += groups) {
+        turn_pieces<T, V, kHalf, 1>(src, dst, in_step, out_step, R / 2, turn, cs[k]);
+        src += in_step;
+        dst += out_step;
       }
     }
   }
@@ -145,9 +216,9 @@ static void launch(const Args& a, cudaStream_t stream) {
   const unsigned blocks = (unsigned)((a.n + 7) / 8);
   const int turned = kHalf ? a.R / 2 / V : a.R / V;
   const int pieces = turned + (a.D - a.R) / V;
-  if (pieces <= 32) rotate<T, V, kHalf, 1><<<blocks, 256, 0, stream>>>(a);
-  else if (pieces <= 64) rotate<T, V, kHalf, 2><<<blocks, 256, 0, stream>>>(a);
-  else rotate<T, V, kHalf, 8><<<blocks, 256, 0, stream>>>(a);
+  if (pieces <= 32) rotate<T, V, kHalf, 1, 4><<<blocks, 256, 0, stream>>>(a);
+  else if (pieces <= 64) rotate<T, V, kHalf, 2, 2><<<blocks, 256, 0, stream>>>(a);
+  else rotate<T, V, kHalf, 8, 1><<<blocks, 256, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
