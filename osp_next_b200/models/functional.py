@@ -384,22 +384,22 @@ def attention(q, k, v, seg_q, seg_k, scale=None):
 
 class _PackedAttnFn(torch.autograd.Function):
     """Attention over packed sequences with both passes on the tcgen05 kernels; keeps
-    (q, k, v, o, log-sum-exp) and recomputes P."""
+    (q, k, v, o, log-sum-exp, a byte per value of what o's rounding left) and recomputes P."""
 
     @staticmethod
     def forward(ctx, q, k, v, pack, causal, scale):
         qb, kb, vb = q.to(_BF16), k.to(_BF16), v.to(_BF16)
-        o, lse = ops.packed_attention(qb, kb, vb, pack, causal, scale, return_lse=True)
-        ctx.save_for_backward(qb, kb, vb, o, lse)
+        o, lse, rest = ops.packed.packed_attention_for_grad(qb, kb, vb, pack, causal, scale)
+        ctx.save_for_backward(qb, kb, vb, o, lse, rest)
         ctx.meta = (pack, causal, scale, (q.dtype, k.dtype, v.dtype))
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, lse, rest = ctx.saved_tensors
         pack, causal, scale, dtypes = ctx.meta
-        grads = ops.packed_attention_bwd(q, k, v, o, go, lse, pack, causal, scale)
+        grads = ops.packed_attention_bwd(q, k, v, o, go, lse, pack, causal, scale, rest)
         return (*(g.to(t) for g, t in zip(grads, dtypes)), None, None, None)
 
 

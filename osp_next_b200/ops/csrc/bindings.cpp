@@ -48,11 +48,13 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q, const at::Tensor& k
                                         const at::Tensor& items, const at::Tensor& joins, int64_t slots,
                                         int64_t positions, int64_t tiles, int64_t at_once, bool causal, double scale,
                                         bool own_scale,
-                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, int64_t rows,
+                                        const c10::optional<at::Tensor>& rel_bias, bool want_lse, bool want_low,
+                                        int64_t rows,
                                         int64_t key_rows, int64_t longest, bool dense);
 std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                         const at::Tensor& o, const at::Tensor& dout, const at::Tensor& lse,
-                                        const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
+                                        const c10::optional<at::Tensor>& low, const at::Tensor& rows,
+                                        const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, int64_t row_heads, int64_t key_heads, bool causal, double scale,
                                         bool fill);
 std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act,

@@ -12,7 +12,7 @@
 // issues tcgen05.mma into one of two accumulators, warps 2..9 are two groups of epilogue warps that take
 // half of the tile's columns each.  Operands lie K-major or MN-major as the tensors are; results leave
 // through shared memory as whole 64-byte row segments.  Sums are fp32 in tensor memory; g, u, dg, du and
-// h are rounded to bf16 once, as operands of the next product have to be.
+// h are rounded to bf16 once, as operands of the next product have to be (dg, du, h; g and u: keep16).
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
@@ -44,7 +44,7 @@ struct Args {
   int act;
   __nv_bfloat16* out;          // kPlain: [M, N]; kGate: h [M, N]; kGateBwd: h [M, N]
   float* out32;                // kPlain: the result in fp32 instead (gradients of fp32 weights), or null
-  __nv_bfloat16* gu;           // [M, 2 N]: g | u written (kGate, or null), read (kGateBwd)
+  uint16_t* gu;                // [M, 2 N]: g | u (keep16) written (kGate, or null), read (kGateBwd)
   __nv_bfloat16* dgu;          // [M, 2 N]: dg | du written (kGateBwd)
   int* err;
 };
@@ -67,6 +67,33 @@ __device__ __forceinline__ float act_f(int act, float g, float& d) {
   return g * s;
 }
 
+// Projections kept for the backward pass: 16 bits, 1 sign, 6 exponent, 9 mantissa (values 2^-31 to 2^32, zero
+// below, the largest above, all ones for NaN and infinity).  As bf16 their rounding, 2^-9 of the value in
+// the mean of a step's ends, would be as large as that of dg and du themselves and show in every
+// gradient (weight gradients 3.5e-3 from 64 bits against 2.4e-3); projections span no 2^63.
+__device__ __forceinline__ uint32_t keep16(float v) {
+  const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
+  int t = (int)((m + 0x1fffu + ((m >> 14) & 1u)) >> 14) - (96 << 9);
+  t = min(max(t, 0), 0x7ffe);
+  t = m >= 0x7f800000u ? 0x7fff : t;
+  return ((b >> 16) & 0x8000u) | (uint32_t)t;
+}
+__device__ __forceinline__ float kept(uint32_t c) {       // 16 bits
+  const uint32_t t = c & 0x7fffu;
+  const uint32_t m = t == 0 ? 0u : t == 0x7fffu ? 0x7fc00000u : (t + (96u << 9)) << 14;
+  return __uint_as_float(m | ((c & 0x8000u) << 16));
+}
+struct AsBf16 {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+struct AsKept {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return keep16(a) | keep16(b) << 16; }
+  static __device__ __forceinline__ float low(uint32_t w) { return kept(w & 0xffffu); }
+  static __device__ __forceinline__ float high(uint32_t w) { return kept(w >> 16); }
+};
+
 __device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int& mb, int& nb) {
   const int per_group = kGroupM * num_n;
   const int g = t / per_group;
@@ -77,24 +104,26 @@ __device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int& mb
   nb = r / gsize;
 }
 
+template <typename As>
 __device__ __forceinline__ uint4 pack8(const float* v) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  return make_uint4(As::pack(v[0], v[1]), As::pack(v[2], v[3]), As::pack(v[4], v[5]), As::pack(v[6], v[7]));
 }
+template <typename As>
 __device__ __forceinline__ void unpack8(const uint4& w, float* v) {
   const uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    v[2 * i] = As::low(r[i]);
+    v[2 * i + 1] = As::high(r[i]);
   }
 }
 
 // A warp's 32 rows x 32 columns (a row per lane) to dst [rows of `pitch`], in 64-byte row segments.
-__device__ __forceinline__ void store_tile(const float* v, uint8_t* stg, __nv_bfloat16* dst, long pitch, long row0,
+template <typename As = AsBf16, typename T>
+__device__ __forceinline__ void store_tile(const float* v, uint8_t* stg, T* dst, long pitch, long row0,
                                            int rows, int col0, int cols, int lane) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stg + lane * kStageRow + j * 16) = pack8(v + 8 * j);
+  for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stg + lane * kStageRow + j * 16) = pack8<As>(v + 8 * j);
   __syncwarp();
   const int q = lane >> 2, cc = lane & 3;
   if (col0 + cc * 8 < cols) {
@@ -109,7 +138,8 @@ __device__ __forceinline__ void store_tile(const float* v, uint8_t* stg, __nv_bf
   __syncwarp();
 }
 // The same way in: 32 columns of this lane's row, zeros outside.
-__device__ __forceinline__ void load_tile(float* v, uint8_t* stg, const __nv_bfloat16* src, long pitch, long row0,
+template <typename As, typename T>
+__device__ __forceinline__ void load_tile(float* v, uint8_t* stg, const T* src, long pitch, long row0,
                                           int rows, int col0, int cols, int lane) {
   const int q = lane >> 2, cc = lane & 3;
 #pragma unroll
@@ -122,7 +152,7 @@ __device__ __forceinline__ void load_tile(float* v, uint8_t* stg, const __nv_bfl
   }
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) unpack8(*reinterpret_cast<const uint4*>(stg + lane * kStageRow + j * 16), v + 8 * j);
+  for (int j = 0; j < 4; ++j) unpack8<As>(*reinterpret_cast<const uint4*>(stg + lane * kStageRow + j * 16), v + 8 * j);
   __syncwarp();
 }
 
@@ -274,8 +304,8 @@ gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMa
 #pragma unroll
           for (int j = 0; j < 32; ++j) { v[j] = __uint_as_float(r[j]); u[j] = __uint_as_float(ru[j]); }
           if (args.gu) {
-            store_tile(v, stg, args.gu, 2l * args.N, row0, args.M, col0, args.N, lane);
-            store_tile(u, stg, args.gu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
+            store_tile<AsKept>(v, stg, args.gu, 2l * args.N, row0, args.M, col0, args.N, lane);
+            store_tile<AsKept>(u, stg, args.gu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -284,8 +314,8 @@ gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMa
           }
         } else if constexpr (MODE == kGateBwd) {
           float g[32], u[32];
-          load_tile(g, stg, args.gu, 2l * args.N, row0, args.M, col0, args.N, lane);
-          load_tile(u, stg, args.gu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
+          load_tile<AsKept>(g, stg, args.gu, 2l * args.N, row0, args.M, col0, args.N, lane);
+          load_tile<AsKept>(u, stg, args.gu + args.N, 2l * args.N, row0, args.M, col0, args.N, lane);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -648,11 +678,11 @@ std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& 
   TORCH_CHECK(F % 8 == 0 && K > 0, "gated_ffn: F a multiple of 8");
   c10::cuda::CUDAGuard guard(x.device());
   at::Tensor h = at::empty({M, F}, x.options()), gu;
-  if (keep) gu = at::empty({M, 2 * F}, x.options());
+  if (keep) gu = at::empty({M, 2 * F}, x.options().dtype(at::kShort));
   if (M > 0 && F > 0) {
     Args a = make_args(x, M, F, K, act);
     a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
-    a.gu = keep ? reinterpret_cast<__nv_bfloat16*>(gu.data_ptr()) : nullptr;
+    a.gu = keep ? reinterpret_cast<uint16_t*>(gu.data_ptr()) : nullptr;
     if (!keep && few_rows(M, F, 128, num_sms(x.get_device()))) launch_few(x, wg, &wu, h, act, false, c10::cuda::getCurrentCUDAStream());
     else launch<256, kGate, false, false>(x, wg, nullptr, &wu, a, c10::cuda::getCurrentCUDAStream());
   }
@@ -691,14 +721,14 @@ std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor&
   const int64_t M = dy.size(0), C = dy.size(1), F = wd.size(1);
   check(dy, dy, M, C, "output gradient");
   check(wd, dy, C, F, "down weight");
-  check(gu, dy, M, 2 * F, "kept projections");
-  TORCH_CHECK(gu.is_contiguous() && F % 8 == 0 && C > 0, "gated_ffn: contiguous kept projections, F a multiple of 8");
+  TORCH_CHECK(gu.device() == dy.device() && gu.scalar_type() == at::kShort && gu.dim() == 2 && gu.size(0) == M &&
+              gu.size(1) == 2 * F && gu.is_contiguous() && F % 8 == 0 && C > 0, "gated_ffn: contiguous kept projections, F a multiple of 8");
   c10::cuda::CUDAGuard guard(dy.device());
   at::Tensor h = at::empty({M, F}, dy.options()), dgu = at::empty({M, 2 * F}, dy.options());
   if (M > 0 && F > 0) {
     Args a = make_args(dy, M, F, C, act);
     a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
-    a.gu = reinterpret_cast<__nv_bfloat16*>(gu.data_ptr());
+    a.gu = reinterpret_cast<uint16_t*>(gu.data_ptr());
     a.dgu = reinterpret_cast<__nv_bfloat16*>(dgu.data_ptr());
     launch<256, kGateBwd, false, true>(dy, wd, nullptr, nullptr, a, c10::cuda::getCurrentCUDAStream());
   }

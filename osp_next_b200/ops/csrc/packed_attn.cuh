@@ -15,6 +15,8 @@
 // 0 * NaN is NaN in a product that sums over those rows, so the producer warp overwrites the rows
 // behind the end with zeros in shared memory before it hands the tile on.
 #pragma once
+#include <cuda_fp8.h>
+
 #include "common.cuh"
 #include "attn_math.cuh"
 
@@ -55,6 +57,27 @@ __device__ __forceinline__ FwdItem load_fwd_item(const int* list, int i) {
 __device__ __forceinline__ KeyItem load_key_item(const int* list, int i) {
   const int4 a = item_ptr(list, i)[0], b = item_ptr(list, i)[1];
   return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+// What rounding o to bf16 left, times 2^8, in e5m2: kept for the gradient alone.  delta = rowsum(dO o O)
+// takes it in; from the rounded o, dS of short rows is off by as much as by its own rounding (dQ
+// 2.6e-3 from 64 bits, 2.4e-3 with it).
+constexpr float kLowScale = 256.0f;
+__device__ __forceinline__ uint32_t low_pair(float a, float b) {
+  const float2 r = make_float2((a - bf16_round(a)) * kLowScale, (b - bf16_round(b)) * kLowScale);
+  return __nv_cvt_float2_to_fp8x2(r, __NV_SATFINITE, __NV_E5M2);
+}
+__device__ __forceinline__ uint32_t low_bits4(const float* v, float mul) {
+  return low_pair(v[0] * mul, v[1] * mul) | low_pair(v[2] * mul, v[3] * mul) << 16;
+}
+__device__ __forceinline__ uint2 low_bits8(const uint32_t* v, float mul) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i]);
+  return make_uint2(low_bits4(f, mul), low_bits4(f + 4, mul));
+}
+__device__ __forceinline__ float low_value(uint32_t byte) {       // e5m2 is the top byte of a half
+  return __half2float(__ushort_as_half((unsigned short)(byte << 8))) * (1.0f / kLowScale);
 }
 
 // Item and head of this CTA.  Items are sorted longest first; `at_once` heads are run together, the next

@@ -50,8 +50,9 @@ struct PackedBwdArgs {
 };
 
 // delta of each (token, head) row: 16 lanes x 8 elements, two rows per warp.
-__global__ void packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout,
-                                    float* __restrict__ delta, long rows, int Dr) {
+__global__ void packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const uint8_t* __restrict__ low,
+                                    const __nv_bfloat16* __restrict__ dout, float* __restrict__ delta, long rows,
+                                    int Dr) {
   const long row = ((long)blockIdx.x * blockDim.x + threadIdx.x) / 16;
   const int c = (threadIdx.x % 16) * 8;
   float acc = 0.f;
@@ -59,12 +60,14 @@ __global__ void packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const _
     const uint4 a = *reinterpret_cast<const uint4*>(o + row * Dr + c);
     const uint4 g = *reinterpret_cast<const uint4*>(dout + row * Dr + c);
     const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+    const uint2 l = low ? *reinterpret_cast<const uint2*>(low + row * Dr + c) : make_uint2(0u, 0u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&aw[i]));
       const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gw[i]));
-      acc = fmaf(x.x, y.x, acc);
-      acc = fmaf(x.y, y.y, acc);
+      const uint32_t lw = (i < 2 ? l.x : l.y) >> (16 * (i & 1));
+      acc = fmaf(x.x + pa::low_value(lw & 0xffu), y.x, acc);
+      acc = fmaf(x.y + pa::low_value(lw >> 8 & 0xffu), y.y, acc);
     }
   }
 #pragma unroll
@@ -642,6 +645,7 @@ static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, cons
 // (dq, dk, dv) bf16.  `rows`, `keys`, `joins`: work lists of ops.SequencePack on the device.
 std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                         const at::Tensor& o_, const at::Tensor& dout_, const at::Tensor& lse_,
+                                        const c10::optional<at::Tensor>& low,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, int64_t row_heads, int64_t key_heads, bool causal, double scale,
                                         bool fill) {
@@ -655,6 +659,9 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& 
               "packed_attention: contiguous output and gradient shaped like q");
   TORCH_CHECK(lse.is_contiguous() && lse.scalar_type() == at::kFloat && lse.device() == q.device() &&
               lse.numel() == (int64_t)s.Nq * s.Hq, "packed_attention: fp32 log-sum-exp [tokens, heads]");
+  if (low.has_value())
+    TORCH_CHECK(low->device() == q.device() && low->scalar_type() == at::kByte && low->is_contiguous() &&
+                low->numel() == q.numel(), "packed_attention: remainder of the output [tokens, heads, head_dim]");
   pa::check_list(rows, 8, q, "packed_attention: rows");
   pa::check_list(keys, 8, q, "packed_attention: keys");
   pa::check_list(joins, 4, q, "packed_attention: joins");
@@ -670,8 +677,8 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& 
   const long n = (long)s.Nq * s.Hq;
   if (n > 0) {
     packed_delta_kernel<<<(unsigned)((n * 16 + 255) / 256), 256, 0, stream>>>(
-        reinterpret_cast<const __nv_bfloat16*>(o.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr()),
-        delta.data_ptr<float>(), n, s.D);
+        reinterpret_cast<const __nv_bfloat16*>(o.data_ptr()), low.has_value() ? low->data_ptr<uint8_t>() : nullptr,
+        reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr()), delta.data_ptr<float>(), n, s.D);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   PackedBwdArgs a{};

@@ -42,6 +42,7 @@ struct PackedFwdArgs {
   int slots;                // of the K / V ring
   __nv_bfloat16* out;       // [Nq, Hq, Dr]
   float* lse;               // [Nq, Hq] or null
+  uint8_t* low;             // [Nq, Hq, Dr] what o's rounding left (pa::low_bits), or null
   float scale_log2;
   const float* bias;        // [Hq, 2 M - 1] or null
   int bias_m;               // M
@@ -465,6 +466,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int i = 0; i < 16; ++i) o[i] = o[i + 16];
         }
         const int first = c0 % per * size / 16;         // the first piece that these columns fill
+        if (args.low && size == 2 && in) {              // for the gradient: 16 bytes of this lane's own row
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (c0 + 8 * h < args.Dr)
+              *reinterpret_cast<uint2*>(args.low + row * args.Dr + c0 + 8 * h) = pa::low_bits8(o + 8 * h, inv_l);
+        }
         if (size == 2) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) *pa::out_piece<L::kPiece>(buf, lane, first + i) = pa::pack8(o + 8 * i, inv_l);
@@ -503,7 +510,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 // (join, key head, 8 rows).  The parts' weights are read by the lanes at once, 32 parts at a time.
 __global__ void __launch_bounds__(256)
 packed_combine_kernel(const int* joins, int G, int P, int tiles, int Hq, int Dr, const float* part_o,
-                      const float* part_l, __nv_bfloat16* out, float* lse) {
+                      const float* part_l, __nv_bfloat16* out, float* lse, uint8_t* low) {
   const int4 j = reinterpret_cast<const int4*>(joins)[blockIdx.x];   // q_row, n_q, first slot, parts
   const int kvh = blockIdx.y, lane = threadIdx.x % 32;
   const int i = blockIdx.z * 8 + threadIdx.x / 32;
@@ -543,6 +550,7 @@ packed_combine_kernel(const int* joins, int G, int P, int tiles, int Hq, int Dr,
     w.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
     w.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
     *reinterpret_cast<uint2*>(out + row * Dr + lane * 4) = w;
+    if (low) *reinterpret_cast<uint32_t*>(low + row * Dr + lane * 4) = pa::low_bits4(acc, inv);
   }
   if (lane == 0 && lse) lse[row] = (base + log2f(sum)) * 0.69314718055994531f;
 }
@@ -568,14 +576,15 @@ static void launch_packed_fwd(int64_t tiles, const CUtensorMap& tq, const CUtens
   else launch_packed_fwd<D, kBias, 2>(tq, tk, tv, a, stream);
 }
 
-// (o [Nq, Hq, D] bf16, lse [Nq, Hq] fp32 or empty).  `items` / `joins` are int32 lists on the device,
+// (o [Nq, Hq, D] bf16, lse [Nq, Hq] fp32 or empty, what o's rounding left or empty).  `items` / `joins` are int32 lists on the device,
 // laid out by ops.SequencePack for this group size; the pack needs `rows` and `key_rows`, its longest
 // sequence has `longest` rows.  Rows of no sequence are zeros.
 std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                         const at::Tensor& items, const at::Tensor& joins, int64_t slots,
                                         int64_t positions, int64_t tiles, int64_t at_once, bool causal, double scale,
                                         bool own_scale,
-                                        const c10::optional<at::Tensor>& rel_bias_, bool want_lse, int64_t rows,
+                                        const c10::optional<at::Tensor>& rel_bias_, bool want_lse, bool want_low,
+                                        int64_t rows,
                                         int64_t key_rows, int64_t longest, bool dense) {
   const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
   const pa::Shape s = pa::check_shapes(q, k, v, "packed_attention");
@@ -594,8 +603,11 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& 
     lse = at::empty({s.Nq, s.Hq}, opt.dtype(at::kFloat));
     if (fill) lse.fill_(-INFINITY);
   }
+  at::Tensor low;
+  if (want_low) low = at::empty({s.Nq, s.Hq, s.D}, opt.dtype(at::kByte));
+  if (want_low && fill) low.zero_();
   const int64_t n = items.size(0);
-  if (n == 0 || s.Hq == 0 || s.D == 0) return {out, lse};
+  if (n == 0 || s.Hq == 0 || s.D == 0) return {out, lse, low};
   PackedFwdArgs a{};
   a.items = items.data_ptr<int>();
   // with a bias a tile holds one query head: its rows then read one stretch of the bias
@@ -613,6 +625,7 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& 
   a.causal = causal ? 1 : 0;
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  a.low = want_low ? low.data_ptr<uint8_t>() : nullptr;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   if (rel_bias.has_value()) {
     TORCH_CHECK(rel_bias->is_cuda() && rel_bias->device() == q.device() && rel_bias->scalar_type() == at::kFloat &&
@@ -644,10 +657,10 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& 
     TORCH_CHECK(slots > 0, "packed_attention: joins without slots");
     const unsigned rows = (unsigned)(a.P * tiles * group);
     packed_combine_kernel<<<dim3((unsigned)joins.size(0), (unsigned)a.heads, (rows + 7) / 8), 256, 0, stream>>>(
-        joins.data_ptr<int>(), group, a.P, (int)tiles, s.Hq, s.D, a.part_o, a.part_l, a.out, a.lse);
+        joins.data_ptr<int>(), group, a.P, (int)tiles, s.Hq, s.D, a.part_o, a.part_l, a.out, a.lse, a.low);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
-  return {out, lse};
+  return {out, lse, low};
 }
 
 }  // namespace osp

@@ -315,25 +315,37 @@ def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
         scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
         o, lse = ref.packed_attention(q, k, v, pack, causal, scale, rel_bias)
         return (o, lse) if return_lse else o
+    o, lse, _ = _forward(q, k, v, pack, causal, scale, rel_bias, bool(return_lse), False)
+    return (o, lse) if return_lse else o
+
+
+def _forward(q, k, v, pack, causal, scale, rel_bias, want_lse, want_low):
+    """(o, log-sum-exp, what o's rounding left) on the GPU; the last two None where not asked for."""
     try:
         # the kernel's own checks come first: a call of a few microseconds has no time for both
         Hkv = k.shape[1]
         group = 1 if rel_bias is not None else q.shape[1] // Hkv  # heads of a row tile (one with a bias)
         items, joins, slots, per, tiles, together = pack.forward_lists(group, q.shape[1] // group, bool(causal))
-        o, lse = ext().packed_attn_fwd(q, k, v, items, joins, slots, per, tiles, together, bool(causal),
-                                       -1.0 if scale is None else float(scale), scale is None, rel_bias,
-                                       bool(return_lse), pack.rows, pack.key_rows, pack.longest, pack.dense)
+        return ext().packed_attn_fwd(q, k, v, items, joins, slots, per, tiles, together, bool(causal),
+                                     -1.0 if scale is None else float(scale), scale is None, rel_bias, want_lse,
+                                     want_low, pack.rows, pack.key_rows, pack.longest, pack.dense)
     except (AttributeError, IndexError, RuntimeError, TypeError, ValueError, ZeroDivisionError):
         check_packed(q, k, v, pack, rel_bias)
         if q.dtype != torch.bfloat16:
             raise TypeError(f"packed_attention: bf16 on the GPU, got {q.dtype}") from None
         raise
-    return (o, lse) if return_lse else o
 
 
-def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool = True, scale: Optional[float] = None):
+def packed_attention_for_grad(q, k, v, pack: SequencePack, causal: bool = True, scale: Optional[float] = None):
+    """(o, log-sum-exp, remainder) for :func:`packed_attention_bwd` on the GPU: the remainder, a byte per
+    value, is what the rounding of o to bf16 left."""
+    return _forward(q, k, v, pack, causal, scale, None, True, True)
+
+
+def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool = True, scale: Optional[float] = None,
+                         remainder=None):
     """Gradients (dq, dk, dv) of :func:`packed_attention` without a bias, from its output and
-    log-sum-exp; rows of no sequence get zeros."""
+    log-sum-exp (and the remainder of :func:`packed_attention_for_grad`); rows of no sequence get zeros."""
     check_packed(q, k, v, pack, what="packed_attention_bwd")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not q.is_cuda:
@@ -345,5 +357,5 @@ def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool
     Hkv = k.shape[1]
     rows, keys, joins, slots, row_heads, key_heads = pack.backward_lists(q.shape[1] // Hkv, Hkv, bool(causal))
     fill = not (pack.dense and pack.key_dense and q.shape[0] == pack.rows and k.shape[0] == pack.key_rows)
-    return ext().packed_attn_bwd(q, k, v, o, dout, lse, rows, keys, joins, slots, row_heads, key_heads,
+    return ext().packed_attn_bwd(q, k, v, o, dout, lse, remainder, rows, keys, joins, slots, row_heads, key_heads,
                                  bool(causal), scale, fill)

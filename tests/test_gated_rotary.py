@@ -46,8 +46,8 @@ def ffn_oracle(x, wg, wu, wd, act, dy=None):
     C = wd.shape[0]
     dh = dy @ wd
     edh = C * F32 * (dy.abs() @ wd.abs())
-    # kept projections are rounded: g and u are off by half a step
-    kg, ku = eg + HALF * g.abs(), eu + HALF * u.abs()
+    # kept projections have 9 bits of mantissa: off by half a step, 2^-10; zero below 2^-31
+    kg, ku = eg + 2.0 ** -10 * g.abs() + 2.0 ** -31, eu + 2.0 ** -10 * u.abs() + 2.0 ** -31
     da = 1.13 * kg + fast * (a.abs() + 1)
     h2 = (h, (da * u.abs() + (a.abs() + da) * ku) * (1 + HALF) + HALF * h.abs())
     dg, du = dh * u * d, dh * a
