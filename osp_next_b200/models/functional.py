@@ -445,24 +445,16 @@ class _GatedFFNFn(torch.autograd.Function):
     def backward(ctx, gy):
         x2, wg, wu, wd, gu = ctx.saved_tensors
         xshape, xdt, wshape, gdt, udt, dshape, ddt, act = ctx.meta
-        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
-        dy = ops.gated.matrix(gy.reshape(gy.shape[:-1].numel(), gy.shape[-1]))
-        product = ops.ext().ffn_product
-        h, dgu = ops.ext().gated_linear_bwd(dy, wd, gu, act)
-        fp, (f, k) = wg.shape[0], wshape
-        dx = dwg = dwu = dwd = None
-        if need_x:
-            dx = product(dgu[:, :fp], wg, dgu[:, fp:], wu, False, True, xdt != _BF16, False)
+        f, k = wshape
+        c = dshape[0]
+        if wd.shape[0] != c:                              # sizes padded to multiples of 8
+            gy = F.pad(gy, (0, wd.shape[0] - c))
+        dx, dwg, dwu, dwd = ops.ext().gated_ffn_bwd(gy, x2, wg, wu, wd, gu, act, *ctx.needs_input_grad[:4],
+                                                    xdt != _BF16, gdt != _BF16 or udt != _BF16, ddt != _BF16)
+        if dx is not None:
             dx = dx[:, :k].reshape(xshape).to(xdt)
-        if need_g or need_u:
-            part = dgu if need_g and need_u else dgu[:, :fp] if need_g else dgu[:, fp:]
-            dw = product(part, x2, None, None, True, True, gdt != _BF16 or udt != _BF16, False)
-            if need_g:
-                dwg = dw[:f, :k].to(gdt)
-            if need_u:
-                dwu = dw[-fp:][:f, :k].to(udt)
-        if need_d:
-            dwd = product(dy, h, None, None, True, True, ddt != _BF16, False)[:dshape[0], :f].to(ddt)
+        dwg, dwu, dwd = (None if t is None else t[:r, :q].to(dt) for t, r, q, dt in (
+            (dwg, f, k, gdt), (dwu, f, k, udt), (dwd, c, f, ddt)))
         return dx, dwg, dwu, dwd, None
 
 

@@ -59,11 +59,11 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k
                                         bool fill);
 std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act,
                                          bool keep);
-std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor& wd, const at::Tensor& gu, int64_t act);
-at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& a2,
-                       const c10::optional<at::Tensor>& b2, bool a_mn, bool b_mn, bool f32, bool ahead);
 std::vector<at::Tensor> gated_ffn_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                                       const at::Tensor& wd, int64_t act, bool keep);
+std::vector<at::Tensor> gated_ffn_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& wg,
+                                      const at::Tensor& wu, const at::Tensor& wd, const at::Tensor& gu, int64_t act,
+                                      bool need_x, bool need_g, bool need_u, bool need_d, bool x32, bool w32, bool d32);
 std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos,
                                      const at::Tensor& table, const std::vector<int64_t>& sections, bool half,
                                      bool inverse);
@@ -188,9 +188,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("packed_attn_fwd", &osp::packed_attn_fwd);
   m.def("packed_attn_bwd", &osp::packed_attn_bwd);
   m.def("gated_linear_fwd", &osp::gated_linear_fwd);
-  m.def("gated_linear_bwd", &osp::gated_linear_bwd);
   m.def("gated_ffn_fwd", &osp::gated_ffn_fwd);
-  m.def("ffn_product", &osp::ffn_product);
+  m.def("gated_ffn_bwd", &osp::gated_ffn_bwd);
   m.def("rotary_apply", &osp::rotary_apply);
   m.def("cfg_euler", &osp::cfg_euler);
   m.def("hif8_round", &osp::hif8_round);

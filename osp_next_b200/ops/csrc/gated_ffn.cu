@@ -769,4 +769,33 @@ at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::opti
   return out;
 }
 
+// Gradients {dx, dwg, dwu, dwd} of the block for dy [M, C], those that are asked for; in fp32 where `*32`.
+// x, weights and gu as gated_ffn_fwd left them.
+std::vector<at::Tensor> gated_ffn_bwd(const at::Tensor& dy_, const at::Tensor& x, const at::Tensor& wg,
+                                      const at::Tensor& wu, const at::Tensor& wd, const at::Tensor& gu, int64_t act,
+                                      bool need_x, bool need_g, bool need_u, bool need_d, bool x32, bool w32, bool d32) {
+  const int64_t M = x.size(0), F = wg.size(0), C = wd.size(0);
+  at::Tensor dy = dy_.to(at::kBFloat16);
+  if (dy.dim() != 2) dy = dy.reshape({M, dy.size(-1)});
+  TORCH_CHECK(dy.dim() == 2 && dy.size(0) == M && dy.size(1) == C, "gated_ffn: gradient of the output");
+  if (dy.stride(1) != 1 || dy.stride(0) % 8 != 0 || dy.stride(0) < C ||
+      reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 != 0)
+    dy = dy.clone(at::MemoryFormat::Contiguous);
+  auto hd = gated_linear_bwd(dy, wd, gu, act);
+  const at::Tensor dg = hd[1].narrow(1, 0, F), du = hd[1].narrow(1, F, F);
+  at::Tensor dx, dwg, dwu, dwd;
+  if (need_x) dx = ffn_product(dg, wg, du, wu, false, true, x32, false);
+  if (need_g && need_u) {
+    const at::Tensor both = ffn_product(hd[1], x, c10::nullopt, c10::nullopt, true, true, w32, false);
+    dwg = both.narrow(0, 0, F);
+    dwu = both.narrow(0, F, F);
+  } else if (need_g) {
+    dwg = ffn_product(dg, x, c10::nullopt, c10::nullopt, true, true, w32, false);
+  } else if (need_u) {
+    dwu = ffn_product(du, x, c10::nullopt, c10::nullopt, true, true, w32, false);
+  }
+  if (need_d) dwd = ffn_product(dy, hd[0], c10::nullopt, c10::nullopt, true, true, d32, false);
+  return {dx, dwg, dwu, dwd};
+}
+
 }  // namespace osp
