@@ -1,6 +1,7 @@
 // Host checks and tensor maps of the packed attention launchers.
 #pragma once
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAStream.h>
 
 #include "packed_attn.cuh"
 #include "tma_host.h"
@@ -51,9 +52,11 @@ static inline Shape check_shapes(const at::Tensor& q, const at::Tensor& k, const
   return s;
 }
 
+// A work list; its memory is not given away before the work that is now on this stream is done.
 static inline void check_list(const at::Tensor& t, int width, const at::Tensor& q, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == q.device() && t.scalar_type() == at::kInt && t.is_contiguous() &&
               t.dim() == 2 && t.size(1) == width, what);
+  if (t.numel() > 0) t.record_stream(c10::cuda::getCurrentCUDAStream(q.get_device()).unwrap());
 }
 
 // [N, H, D] as a 3-D tensor (D, H, N) with boxes of 64 elements x heads x positions (128B swizzle);

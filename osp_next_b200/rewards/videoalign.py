@@ -339,7 +339,7 @@ def _kernels_fit(config) -> bool:
     """Whether the packed kernel takes the text layers' heads."""
     c = getattr(config, "text_config", config)
     dim = getattr(c, "head_dim", None) or c.hidden_size // c.num_attention_heads
-    return dim % 8 == 0 and dim <= 128
+    return dim % 8 == 0 and dim <= 128 and not getattr(c, "use_sliding_window", False)
 
 
 def _mask_runs(attention_mask):

@@ -97,7 +97,7 @@ def tensors(pack, heads, kv_heads, dim, device, seed=0, dtype=torch.bfloat16, sp
 # ---------------------------------------------------------------------------- CPU
 
 PACKS = [([1], None), ([1, 1, 1], None), ([128], None), ([127, 1, 129], None), ([5, 0, 300, 77], None),
-         ([1, 3, 130], [700, 3, 131]), ([9, 4, 200], [2, 0, 130]), ([0, 0], None), ([1], [3000])]
+         ([1, 3, 130], [700, 3, 131]), ([9, 4, 200], [2, 0, 130]), ([0, 0], None), ([], None), ([1], [3000])]
 
 
 @pytest.mark.parametrize("lengths,keys", PACKS)
@@ -376,6 +376,25 @@ def test_gpu_views_copies_and_devices():
     bias = torch.zeros(4, 179, device="cuda")
     with pytest.raises(RuntimeError, match="no gradient with rel_bias"):
         Fn.packed_attention(q.detach().requires_grad_(), k, v, pack, rel_bias=bias)
+
+
+@gpu
+def test_gpu_two_streams_share_a_pack():
+    """Calls of one pack on two streams at once, the pack dropped while they run."""
+    packs = [ops.SequencePack([500, 1, 300]) for _ in range(2)]
+    q, k, v, do = tensors(packs[0], 16, 4, 128, "cuda")
+    want = ops.packed_attention(q, k, v, packs[0])
+    ops.packed_attention(q, k, v, packs[1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(ops.packed_attention(q, k, v, packs[1]))
+    del packs[1]
+    junk = [torch.full((64, 8), -1, dtype=torch.int32, device="cuda") for _ in range(50)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got) and len(junk) == 50
 
 
 @gpu
