@@ -367,8 +367,11 @@ gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMa
 // whose parts are added through distributed shared memory in rank order: no workspace, and results do
 // not depend on timing.  The down projection starts while the gate kernel runs and loads its first
 // weights before it waits for it.  192 threads: warp 0 loads, warp 1 MMAs, warps 2..5 results.
+// The same form serves the backward pass: dh = dy Wd with its epilogue and dx = dg Wg + du Wu read the
+// weights as they lie, MN-major (kWMn).
 struct FewArgs {
-  int M, N, KB;                // rows of x, weight rows, blocks of 64 along K
+  int M, N, KB;                // rows of x, result columns, blocks of 64 along K (of both operand pairs)
+  int KB1;                     // of the first pair
   int bnx;                     // rows of x that a CTA takes (blockIdx.y: which), a multiple of 16
   int stages;                  // of the ring
   int splits;
@@ -376,7 +379,10 @@ struct FewArgs {
   int cols;                    // tensor-memory columns
   int act;
   int ahead;                   // load weights before the wait for the kernel in front
-  __nv_bfloat16* out;          // [M, N]
+  __nv_bfloat16* out;          // [M, N] (kPlain, or null; kGate, kGateBwd: h)
+  float* out32;                // kPlain: the result in fp32 instead, or null
+  uint16_t* gu;                // as in Args
+  __nv_bfloat16* dgu;
   int* err;
 };
 
@@ -410,11 +416,12 @@ constexpr int kFewThreads = 192;
 constexpr int kFewMaxStages = 12;
 constexpr uint32_t kWTile = 128 * kBK * 2;
 
-template <bool kGateForm>
+template <int MODE, bool kWMn>
 __global__ void __launch_bounds__(kFewThreads)
 few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-           const __grid_constant__ CUtensorMap tmW2, const FewArgs args) {
-  constexpr int kAcc = kGateForm ? 2 : 1;
+           const __grid_constant__ CUtensorMap tmX2, const __grid_constant__ CUtensorMap tmW2, const FewArgs args) {
+  constexpr int kAcc = MODE == kGate ? 2 : 1;
+  constexpr uint32_t MN_BOX = 64 * kBK * 2;
   const uint32_t x_bytes = args.bnx * kBK * 2;
   const uint32_t stage_bytes = kAcc * kWTile + x_bytes;
   const int stages = args.stages;
@@ -440,7 +447,8 @@ few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUte
     fence_mbar_init();
     prefetch_tmap(&tmX);
     prefetch_tmap(&tmW);
-    if (kGateForm) prefetch_tmap(&tmW2);
+    if (MODE == kGate || args.KB > args.KB1) prefetch_tmap(&tmW2);
+    if (args.KB > args.KB1) prefetch_tmap(&tmX2);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, args.cols);
@@ -460,11 +468,25 @@ few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUte
       auto load_w = [&](int kb, int stage) {
         uint8_t* dst = ring + stage * stage_bytes;
         mbar_expect_tx(&full[stage], stage_bytes);
-        tma_load_2d(&tmW, &full[stage], dst, kb * kBK, tile * 128);
-        if (kGateForm) tma_load_2d(&tmW2, &full[stage], dst + kWTile, kb * kBK, tile * 128);
+        if constexpr (MODE == kGate) {
+          tma_load_2d(&tmW, &full[stage], dst, kb * kBK, tile * 128);
+          tma_load_2d(&tmW2, &full[stage], dst + kWTile, kb * kBK, tile * 128);
+        } else {
+          const bool second = kb >= args.KB1;
+          const CUtensorMap* tm = second ? &tmW2 : &tmW;
+          const int kc = (second ? kb - args.KB1 : kb) * kBK;
+          if constexpr (kWMn) {
+            tma_load_2d(tm, &full[stage], dst, tile * 128, kc);
+            tma_load_2d(tm, &full[stage], dst + MN_BOX, tile * 128 + 64, kc);
+          } else {
+            tma_load_2d(tm, &full[stage], dst, kc, tile * 128);
+          }
+        }
       };
       auto load_x = [&](int kb, int stage) {
-        tma_load_2d(&tmX, &full[stage], ring + stage * stage_bytes + kAcc * kWTile, kb * kBK, x0);
+        const bool second = MODE != kGate && kb >= args.KB1;
+        tma_load_2d(second ? &tmX2 : &tmX, &full[stage], ring + stage * stage_bytes + kAcc * kWTile,
+                    (second ? kb - args.KB1 : kb) * kBK, x0);
       };
       const int n = min(stages, kb1 - kb0);
       for (int i = 0; i < n; ++i) load_w(kb0 + i, i);
@@ -484,7 +506,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUte
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = idesc_bf16(128, args.bnx);
+      const uint32_t idesc = idesc_bf16(128, args.bnx, false, kWMn);
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -495,7 +517,8 @@ few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUte
         for (int a = 0; a < kAcc; ++a)
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k)
-            umma_bf16(tmem + a * args.bnx, sdesc_sw128(w + a * kWTile + k * 32, 16, 1024),
+            umma_bf16(tmem + a * args.bnx,
+                      kWMn ? sdesc_sw128(w + k * 2048, MN_BOX, 1024) : sdesc_sw128(w + a * kWTile + k * 32, 16, 1024),
                       sdesc_sw128(x + k * 32, 16, 1024), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
         umma_commit(&empty[stage]);
         if (++stage == stages) { stage = 0; phase ^= 1; }
@@ -553,15 +576,38 @@ few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUte
               if (s < args.splits) { v[a].x += p[s].x; v[a].y += p[s].y; v[a].z += p[s].z; v[a].w += p[s].w; }
           }
         }
-        if constexpr (kGateForm) {
-          float d;
-          v[0].x = act_f<false>(args.act, v[0].x, d) * v[1].x;
-          v[0].y = act_f<false>(args.act, v[0].y, d) * v[1].y;
-          v[0].z = act_f<false>(args.act, v[0].z, d) * v[1].z;
-          v[0].w = act_f<false>(args.act, v[0].w, d) * v[1].w;
+        const long at = (long)(x0 + c0 + m) * args.N + n0, at2 = (long)(x0 + c0 + m) * 2 * args.N + n0;
+        float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, d;
+        if constexpr (MODE == kGate) {
+          const float u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+          if (args.gu) {
+            *reinterpret_cast<uint2*>(args.gu + at2) = make_uint2(AsKept::pack(f[0], f[1]), AsKept::pack(f[2], f[3]));
+            *reinterpret_cast<uint2*>(args.gu + at2 + args.N) =
+                make_uint2(AsKept::pack(u[0], u[1]), AsKept::pack(u[2], u[3]));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = act_f<false>(args.act, f[e], d) * u[e];
+        } else if constexpr (MODE == kGateBwd) {
+          const uint2 wg = *reinterpret_cast<const uint2*>(args.gu + at2);
+          const uint2 wu = *reinterpret_cast<const uint2*>(args.gu + at2 + args.N);
+          const float g[4] = {AsKept::low(wg.x), AsKept::high(wg.x), AsKept::low(wg.y), AsKept::high(wg.y)};
+          const float u[4] = {AsKept::low(wu.x), AsKept::high(wu.x), AsKept::low(wu.y), AsKept::high(wu.y)};
+          float dg[4], du[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = act_f<true>(args.act, g[e], d);
+            dg[e] = f[e] * u[e] * d;
+            du[e] = f[e] * a;
+            f[e] = a * u[e];
+          }
+          *reinterpret_cast<uint2*>(args.dgu + at2) = make_uint2(pack_bf16x2(dg[0], dg[1]), pack_bf16x2(dg[2], dg[3]));
+          *reinterpret_cast<uint2*>(args.dgu + at2 + args.N) =
+              make_uint2(pack_bf16x2(du[0], du[1]), pack_bf16x2(du[2], du[3]));
         }
-        *reinterpret_cast<uint2*>(args.out + (long)(x0 + c0 + m) * args.N + n0) =
-            make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
+        if (MODE == kPlain && args.out32)
+          *reinterpret_cast<float4*>(args.out32 + at) = make_float4(f[0], f[1], f[2], f[3]);
+        else
+          *reinterpret_cast<uint2*>(args.out + at) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
       }
     }
     if (args.splits > 1) cluster_sync();                   // no CTA goes on while its part may be read
@@ -607,15 +653,17 @@ static bool few_rows(int64_t M, int64_t N, int out_n, int sms) {
   return M <= kFewRows || (M + kBM - 1) / kBM * ((N + out_n - 1) / out_n) < sms;
 }
 
-// out [M, N] = act(x W^T) o (x W2^T), or x W^T without W2.
-static void launch_few(const at::Tensor& x, const at::Tensor& w, const at::Tensor* w2, at::Tensor& out, int64_t act,
-                       bool ahead, cudaStream_t stream) {
+// The product of `args` (its sizes and pointers) in the form for few rows; weights [N, K], or [K, N] with kWMn.
+template <int MODE, bool kWMn>
+static void launch_few(const at::Tensor& x, const at::Tensor& w, const at::Tensor* x2, const at::Tensor* w2,
+                       const Args& args, bool ahead, cudaStream_t stream) {
   const int sms = num_sms(x.get_device());
-  const int acc = w2 ? 2 : 1;
+  constexpr int acc = MODE == kGate ? 2 : 1;
   FewArgs a{};
-  a.M = (int)x.size(0);
-  a.N = (int)w.size(0);
-  a.KB = (int)((x.size(1) + kBK - 1) / kBK);
+  a.M = args.M;
+  a.N = args.N;
+  a.KB1 = (args.K + kBK - 1) / kBK;
+  a.KB = a.KB1 + (args.K2 + kBK - 1) / kBK;
   const int blocks = (a.M + kFewRows - 1) / kFewRows;
   a.bnx = ((a.M + blocks - 1) / blocks + 15) / 16 * 16;
   a.cols = 32;
@@ -627,19 +675,19 @@ static void launch_few(const at::Tensor& x, const at::Tensor& w, const at::Tenso
   // as many parts of K as there is room for, of at least 4 blocks
   a.splits = std::max(1, std::min({8, (two ? 2 : 1) * sms / (tiles * blocks), a.KB / 4}));
   a.chunk = std::min(a.bnx, a.stages * stage / (acc * 512) / 16 * 16);
-  a.act = (int)act;
+  a.act = args.act;
   a.ahead = ahead ? 1 : 0;
-  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
-  a.err = error_word(x.get_device());
-  const CUtensorMap mx = map_of(x, false, a.bnx), mw = map_of(w, false, 128), mw2 = w2 ? map_of(*w2, false, 128) : mw;
-  const int smem = 2048 + a.stages * stage;
-  if (w2) {
-    smem_opt_in(reinterpret_cast<const void*>(few_kernel<true>), 227 * 1024);
-    launch_kernel(few_kernel<true>, dim3(tiles * a.splits, blocks), kFewThreads, smem, a.splits, stream, mx, mw, mw2, a);
-  } else {
-    smem_opt_in(reinterpret_cast<const void*>(few_kernel<false>), 227 * 1024);
-    launch_kernel(few_kernel<false>, dim3(tiles * a.splits, blocks), kFewThreads, smem, a.splits, stream, mx, mw, mw2, a);
-  }
+  a.out = args.out;
+  a.out32 = args.out32;
+  a.gu = args.gu;
+  a.dgu = args.dgu;
+  a.err = args.err;
+  const CUtensorMap mx = map_of(x, false, a.bnx), mw = map_of(w, kWMn, 128);
+  const CUtensorMap mx2 = x2 ? map_of(*x2, false, a.bnx) : mx, mw2 = w2 ? map_of(*w2, kWMn, 128) : mw;
+  auto kern = few_kernel<MODE, kWMn>;
+  smem_opt_in(reinterpret_cast<const void*>(kern), 227 * 1024);
+  launch_kernel(kern, dim3(tiles * a.splits, blocks), kFewThreads, 2048 + a.stages * stage, a.splits, stream, mx, mw,
+                mx2, mw2, a);
 }
 
 static void check(const at::Tensor& t, const at::Tensor& x, int64_t rows, int64_t cols, const char* what) {
@@ -683,8 +731,9 @@ std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& 
     Args a = make_args(x, M, F, K, act);
     a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
     a.gu = keep ? reinterpret_cast<uint16_t*>(gu.data_ptr()) : nullptr;
-    if (!keep && few_rows(M, F, 128, num_sms(x.get_device()))) launch_few(x, wg, &wu, h, act, false, c10::cuda::getCurrentCUDAStream());
-    else launch<256, kGate, false, false>(x, wg, nullptr, &wu, a, c10::cuda::getCurrentCUDAStream());
+    auto stream = c10::cuda::getCurrentCUDAStream();
+    if (few_rows(M, F, 128, num_sms(x.get_device()))) launch_few<kGate, false>(x, wg, nullptr, &wu, a, false, stream);
+    else launch<256, kGate, false, false>(x, wg, nullptr, &wu, a, stream);
   }
   return {h, gu};
 }
@@ -705,7 +754,7 @@ std::vector<at::Tensor> gated_ffn_fwd(const at::Tensor& x, const at::Tensor& wg,
       wd.size(1) != wg.size(0) || wd.size(0) % 8 != 0 || act < 0 || act > 1)
     return {};
   auto h = gated_linear_fwd(x2, wg, wu, act, keep);
-  at::Tensor y = ffn_product(h[0], wd, c10::nullopt, c10::nullopt, false, false, false, !keep);
+  at::Tensor y = ffn_product(h[0], wd, c10::nullopt, c10::nullopt, false, false, false, true);
   if (x.dim() != 2) {
     auto sizes = x.sizes().vec();
     sizes.back() = wd.size(0);
@@ -730,7 +779,11 @@ std::vector<at::Tensor> gated_linear_bwd(const at::Tensor& dy, const at::Tensor&
     a.out = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
     a.gu = reinterpret_cast<uint16_t*>(gu.data_ptr());
     a.dgu = reinterpret_cast<__nv_bfloat16*>(dgu.data_ptr());
-    launch<256, kGateBwd, false, true>(dy, wd, nullptr, nullptr, a, c10::cuda::getCurrentCUDAStream());
+    auto stream = c10::cuda::getCurrentCUDAStream();
+    if (few_rows(M, F, 256, num_sms(dy.get_device())))
+      launch_few<kGateBwd, true>(dy, wd, nullptr, nullptr, a, false, stream);
+    else
+      launch<256, kGateBwd, false, true>(dy, wd, nullptr, nullptr, a, stream);
   }
   return {h, dgu};
 }
@@ -761,8 +814,9 @@ at::Tensor ffn_product(const at::Tensor& a, const at::Tensor& b, const c10::opti
   const at::Tensor* pb = b2.has_value() ? &*b2 : nullptr;
   auto stream = c10::cuda::getCurrentCUDAStream();
   TORCH_CHECK(b_mn || !a_mn, "gated_ffn: operand order");
-  if (!a_mn && !b_mn && !pa && !f32 && few_rows(M, N, 256, num_sms(a.get_device())))
-    launch_few(a, b, nullptr, out, 0, ahead, stream);
+  const bool few = !a_mn && few_rows(M, N, 256, num_sms(a.get_device()));
+  if (few && b_mn) launch_few<kPlain, true>(a, b, pa, pb, args, ahead, stream);
+  else if (few) launch_few<kPlain, false>(a, b, pa, pb, args, ahead, stream);
   else if (a_mn) launch<256, kPlain, true, true>(a, b, pa, pb, args, stream);
   else if (b_mn) launch<256, kPlain, false, true>(a, b, pa, pb, args, stream);
   else launch<256, kPlain, false, false>(a, b, pa, pb, args, stream);
