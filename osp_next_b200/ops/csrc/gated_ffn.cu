@@ -13,6 +13,10 @@
 // half of the tile's columns each.  Operands lie K-major or MN-major as the tensors are; results leave
 // through shared memory as whole 64-byte row segments.  Sums are fp32 in tensor memory; g, u, dg, du and
 // h are rounded to bf16 once, as operands of the next product have to be (dg, du, h; g and u: keep16).
+//
+// What bounds it: large blocks the power cap (20160 x 5120 -> 13824, training step: 20.4 ms, 1260 TFLOP/s; the
+// gate kernel 1220, dx and the weight gradients 1320); few rows reading the weights (1 x 4096 -> 10240 ->
+// 4096: 44 us, 0.87 of the copy rate; 154 rows 67 us).
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
