@@ -321,7 +321,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int r = quarter * 32 + lane;                // row of the tile
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + 128u * t + lane_off;
-    const uint32_t tO = tmem + kO + (uint32_t)D * t + lane_off;
+    const uint32_t tO = tS + kO + (uint32_t)(D - 128) * t;
     const float sl2 = args.scale_log2;
     float* bias_buf = reinterpret_cast<float*>(smem + L::OFF_BIAS + t * L::kBiasBytes);
     bool ok = true;
@@ -371,8 +371,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!idle) {
           uint32_t sr[kT];
 #pragma unroll
-          for (int c = 0; c < kT / 32; ++c)
-            if (c * 32 < cols) tmem_ld32(tS + c * 32, sr + c * 32);
+          for (int c = 0; c < kT / 32; ++c) tmem_ld32(tS + c * 32, sr + c * 32);
           tmem_ld_wait();
           if (kBias) {
             const float* brow = bias_buf + (j & 1) * 4 * kT + bias_off;
