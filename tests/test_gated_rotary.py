@@ -351,6 +351,30 @@ def test_gpu_rotary_addresses_batches_and_bad_positions():
         ops.rotary(q.double(), None, pos[:25], table)
 
 
+@gpu
+def test_gpu_offsets_past_32_bits():
+    """Rows beyond 2^31 elements of the kept projections, and of a rotated tensor."""
+    M, K, F = 90000, 64, 12296
+    x, wg, wu, wd, dy = ffn_tensors(M, K, F)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = Fn.gated_ffn(*leaves)
+    dx, = torch.autograd.grad(y, leaves[0], dy)
+    assert 2 * M * F > 1 << 31
+    at = torch.tensor([0, 1, M // 2, M - 130, M - 1], device="cuda")
+    want = ffn_oracle(x.detach()[at], *[t.detach() for t in leaves[1:]], "silu", dy[at])
+    close(y.detach()[at], want["y"], "y")
+    close(dx[at], want["dx"], "dx")
+    n = 140000
+    q = torch.zeros(n, 64, 256, device="cuda", dtype=torch.bfloat16)
+    q[-3:] = torch.randn(3, 64, 256, device="cuda")
+    table = ops.rotary_table(256, 16)
+    pos = torch.arange(n, device="cuda") % 16
+    got = ops.rotary(q, None, pos, table)[0]
+    assert q.numel() > 1 << 31
+    close(got[-3:], turned(q[-3:], pos[-3:, None], table, "half", [128]), "far rows")
+    assert not got[:-3].any()
+
+
 def _layer(x, ws, pos, table, pack, heads, kv, dim, rotary, attend, ffn, rnd):
     """A causal layer: projections, rotary positions, attention, gated feed-forward, both residuals."""
     qkv = rnd(x @ ws[0].t())

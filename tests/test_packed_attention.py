@@ -379,6 +379,30 @@ def test_gpu_views_copies_and_devices():
 
 
 @gpu
+def test_gpu_offsets_past_32_bits():
+    """Rows whose elements lie beyond 2^31 of their tensors: the same values as in a tensor of their own."""
+    rows, heads, dim = 280000, 64, 128
+    small = ops.SequencePack([130, 7])
+    q, k, v, do = tensors(small, heads, 2, dim, "cuda")
+    far = ops.SequencePack([130, 7], [130, 7], starts=[rows - 200, rows - 40], key_starts=[0, 130])
+    big = []
+    for t in (q, do):
+        b = torch.zeros(rows, heads, dim, device="cuda", dtype=torch.bfloat16)
+        b[rows - 200:rows - 70], b[rows - 40:rows - 33] = t[:130], t[130:]
+        big.append(b)
+    assert big[0].numel() > 1 << 31
+    def run(q, k, v, do, pack):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = Fn.packed_attention(*leaves, pack)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    want, got = run(q, k, v, do, small), run(big[0], k, v, big[1], far)
+    for w, g in ((want[0], got[0]), (want[1], got[1])):
+        assert torch.equal(g[rows - 200:rows - 70], w[:130]) and torch.equal(g[rows - 40:rows - 33], w[130:])
+        assert not g[:1000].any() and not g[rows - 70:rows - 40].any()
+    assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+
+
+@gpu
 def test_gpu_two_streams_share_a_pack():
     """Calls of one pack on two streams at once, the pack dropped while they run."""
     packs = [ops.SequencePack([500, 1, 300]) for _ in range(2)]
