@@ -431,6 +431,7 @@ class _GatedFFNFn(torch.autograd.Function):
         g, u, d = wg, wu, wd
         out = ops.ext().gated_ffn_fwd(x, g, u, d, code, True)
         if not out:                                       # copies that the kernels can read
+            ops.gated.check_gated(x, wg, wu, act, wd, "gated_ffn")
             x2 = ops.gated.matrix(x.reshape(x.shape[:-1].numel(), x.shape[-1]))
             g, u, d = ops.gated.hidden_rows(wg), ops.gated.hidden_rows(wu), ops.gated.hidden_rows(wd)
             out = ops.ext().gated_ffn_fwd(x2, g, u, d, code, True)
@@ -466,7 +467,8 @@ def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
         return ref.gated_ffn(x, w_gate, w_up, w_down, act)
     if _fused(x, w_gate, w_up, w_down):
         return ops.gated_ffn(x, w_gate, w_up, w_down, act)
-    ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
+    if act not in ops.gated.ACTS or w_gate.dim() != 2 or w_down.dim() != 2 or x.dim() == 0:
+        ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
     if 0 in w_gate.shape or 0 in w_down.shape or 0 in x.shape:         # empty sums
         return ref.gated_ffn(x.to(_BF16), w_gate, w_up, w_down, act)
     return _GatedFFNFn.apply(x, w_gate, w_up, w_down, act)

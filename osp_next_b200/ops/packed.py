@@ -346,16 +346,20 @@ def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool
                          remainder=None):
     """Gradients (dq, dk, dv) of :func:`packed_attention` without a bias, from its output and
     log-sum-exp (and the remainder of :func:`packed_attention_for_grad`); rows of no sequence get zeros."""
-    check_packed(q, k, v, pack, what="packed_attention_bwd")
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not q.is_cuda:
-        return ref.packed_attention_bwd(q, k, v, dout, pack, causal, scale)
-    if q.dtype != torch.bfloat16:
-        raise TypeError(f"packed_attention_bwd: bf16 on the GPU, got {q.dtype}")
-    if dout.shape != q.shape or o.shape != q.shape or lse.shape != q.shape[:2]:
-        raise ValueError("packed_attention_bwd: o and dout like q, lse [tokens, heads]")
-    Hkv = k.shape[1]
-    rows, keys, joins, slots, row_heads, key_heads = pack.backward_lists(q.shape[1] // Hkv, Hkv, bool(causal))
-    fill = not (pack.dense and pack.key_dense and q.shape[0] == pack.rows and k.shape[0] == pack.key_rows)
-    return ext().packed_attn_bwd(q, k, v, o, dout, lse, remainder, rows, keys, joins, slots, row_heads, key_heads,
-                                 bool(causal), scale, fill)
+        check_packed(q, k, v, pack, what="packed_attention_bwd")
+        return ref.packed_attention_bwd(q, k, v, dout, pack, causal,
+                                        1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale))
+    try:
+        Hkv = k.shape[1]
+        rows, keys, joins, slots, row_heads, key_heads = pack.backward_lists(q.shape[1] // Hkv, Hkv, bool(causal))
+        fill = not (pack.dense and pack.key_dense and q.shape[0] == pack.rows and k.shape[0] == pack.key_rows)
+        if q.shape[0] < pack.rows or k.shape[0] < pack.key_rows:
+            raise ValueError("packed_attention_bwd: fewer rows than the pack's")
+        return ext().packed_attn_bwd(q, k, v, o, dout, lse, remainder, rows, keys, joins, slots, row_heads, key_heads,
+                                     bool(causal), 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), fill)
+    except (AttributeError, IndexError, RuntimeError, TypeError, ValueError, ZeroDivisionError):
+        check_packed(q, k, v, pack, what="packed_attention_bwd")
+        if q.dtype != torch.bfloat16:
+            raise TypeError(f"packed_attention_bwd: bf16 on the GPU, got {q.dtype}") from None
+        raise
