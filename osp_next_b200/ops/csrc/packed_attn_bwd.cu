@@ -16,8 +16,8 @@
 // are added in a fixed order by packed_join_kernel.
 //
 // What bounds it: products and elementwise work in turn; 16 heads of 128 over 8192 tokens, all pairs: dK, dV
-// 904 us and dQ 704 (1.9 and 1.4 PFLOP/s of products); 12 causal samples of 5 to 4096 tokens, 16 heads to 4:
-// 195 and 165 us, tensor pipe 50 % and 43 % active.
+// 860 us and dQ 673 (1.28 and 1.23 PFLOP/s of products); 12 causal samples of 5 to 4096 tokens, 16 heads to 4:
+// 186 and 161 us, tensor pipe 50 % and 43 % active.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>

@@ -17,7 +17,7 @@
 // to 4, causal: 2.6 to 2.9 ms, 1000 to 1100 TFLOP/s); one query each over long keys memory (48 x 1024 to
 // 8192 keys, 8 key heads: 127 to 138 us, 0.75 of the copy rate); short sequences the latency of a CTA's chain of
 // load, product, softmax, product and store, some 9000 cycles beside 5000 a key tile (32 prompts of 20
-// to 512 tokens, 64 heads of 64, bias: 139 us).  The bias is staged in shared memory, twice, one place
+// to 512 tokens, 64 heads of 64, bias: 136 us).  The bias is staged in shared memory, twice, one place
 // apart, so that rows read aligned pairs (from global memory: 162 us there).
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>

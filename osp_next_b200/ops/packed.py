@@ -198,7 +198,7 @@ def _split(steps, kv_heads, sms, least):
 
 def heads_together(steps, heads, slots):
     """Heads whose items run side by side, longest first: as few as fill the ``slots`` CTAs that run at
-    a time, so that these share keys in L2 (gradients over 16 heads of 8192 keys: dK and dV 904 us five
+    a time, so that these share keys in L2 (gradients over 16 heads of 8192 keys: dK and dV 904 us six
     at a time, 943 all together), but enough for the last ones to take twice their longest item."""
     total = int(steps.sum())
     if not total:
