@@ -22,7 +22,6 @@ frame sampling and the Qwen-VL resize rule are reimplemented below.
 """
 from __future__ import annotations
 
-import contextvars
 import glob
 import json
 import math
@@ -306,22 +305,48 @@ def merge_training_state(model_sd: Dict[str, torch.Tensor], tensors: Dict[str, t
 # ---------------------------------------------------------------------------- kernels of the backbone
 
 ATTENTION_NAME = "osp_packed"          # the packed kernel's name among transformers' attention functions
-_PACK: contextvars.ContextVar = contextvars.ContextVar("videoalign_pack", default=None)
+
+
+class _PackedMask:
+    """What the text layers get in the place of a mask tensor: each row's tokens as one packed sequence.  It
+    is an argument of every layer, so that a layer recomputed in the backward pass sees the same one."""
+
+    def __init__(self, first, lengths, width: int):
+        self._rows = (lengths, [i * width + f for i, f in enumerate(first)])
+        self._packs = {}
+
+    def pack(self, device) -> SequencePack:
+        """On the device of a layer (layers may lie on several)."""
+        if device not in self._packs:
+            self._packs[device] = SequencePack(self._rows[0], starts=self._rows[1], device=device)
+        return self._packs[device]
+
+
+def _packed_mask(**args):
+    """transformers' mask function, called once a forward: a :class:`_PackedMask` for a whole causal prompt
+    whose rows are one run of tokens each; the library's mask with a cache, a window or holes."""
+    from transformers.masking_utils import causal_mask_function, sdpa_mask
+    B, L, m = args["batch_size"], args["q_length"], args.get("attention_mask")
+    whole = args["kv_length"] == L and all(int(args.get(n, 0)) == 0 for n in ("q_offset", "kv_offset"))
+    if whole and args.get("mask_function", causal_mask_function) is causal_mask_function:
+        runs = ([0] * B, [L] * B) if m is None else _mask_runs(m)
+        if runs is not None:
+            return _PackedMask(*runs, L)
+    return sdpa_mask(**args)
 
 
 def _packed_attention(module, query, key, value, attention_mask=None, scaling=None, **kw):
     """transformers' attention function: query [B, heads, L, D], key and value [B, key heads, L, D] ->
-    ([B, L, heads, D], None), causal, over the rows of the current batch's pack."""
+    ([B, L, heads, D], None).  Masks that are no :class:`_PackedMask` go to the library's attention."""
+    if not isinstance(attention_mask, _PackedMask):
+        from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+        return ALL_ATTENTION_FUNCTIONS["sdpa"](module, query, key, value, attention_mask, scaling=scaling, **kw)
     B, H, L, D = query.shape
-    if key.shape[2] != L or attention_mask is not None or kw.get("sliding_window"):
-        raise ValueError("packed attention of a whole prompt: no cache, mask or window")
-    pack = _PACK.get()
-    if pack is None or pack.rows > B * L or pack.device != query.device:
-        pack = SequencePack.padded([L] * B, L, device=query.device)
 
     def rows(t):
         return t.transpose(1, 2).reshape(B * L, t.shape[1], D)
-    o = Fn.packed_attention(rows(query), rows(key), rows(value), pack, causal=True, scale=scaling)
+    o = Fn.packed_attention(rows(query), rows(key), rows(value), attention_mask.pack(query.device), causal=True,
+                            scale=scaling)
     return o.view(B, L, H, D).to(query.dtype), None
 
 
@@ -369,15 +394,13 @@ class VideoAlignRewardModel(nn.Module):
         self.special_token_ids = list(special_token_ids) if special_token_ids else None
         self.reward_token = "special" if self.special_token_ids else reward_token
         self.pad_token_id = pad_token_id
-        self._library_attention = None          # what the text layers ran before use_kernels
 
     def use_kernels(self):
         """Text attention on the packed kernel (padding costs nothing: rows are packed by the mask) and
         SiLU-gated MLPs without biases on the gated feed-forward kernels."""
-        from transformers import AttentionInterface
+        from transformers import AttentionInterface, AttentionMaskInterface
         AttentionInterface.register(ATTENTION_NAME, _packed_attention)
-        if self._library_attention is None:
-            self._library_attention = self.vl.config.text_config._attn_implementation
+        AttentionMaskInterface.register(ATTENTION_NAME, _packed_mask)
         self.vl.set_attn_implementation({"text_config": ATTENTION_NAME})
         for m in self.vl.model.language_model.modules():
             parts = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
@@ -387,23 +410,8 @@ class VideoAlignRewardModel(nn.Module):
         return self
 
     def _hidden(self, input_ids, attention_mask, **kw):
-        """Last hidden states; with the kernels, each row's tokens as one packed sequence."""
-        if self._library_attention is None:
-            return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
-        B, L = input_ids.shape
-        runs = ([0] * B, [L] * B) if attention_mask is None else _mask_runs(attention_mask)
-        if runs is None:                        # tokens with holes between them: the library's masks
-            self.vl.set_attn_implementation({"text_config": self._library_attention})
-            try:
-                return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
-            finally:
-                self.vl.set_attn_implementation({"text_config": ATTENTION_NAME})
-        pack = SequencePack(runs[1], starts=[i * L + f for i, f in enumerate(runs[0])], device=input_ids.device)
-        token = _PACK.set(pack)
-        try:
-            return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
-        finally:
-            _PACK.reset(token)
+        """Last hidden states."""
+        return self.vl.model(input_ids=input_ids, attention_mask=attention_mask, **kw).last_hidden_state
 
     def state_dict_for_checkpoint(self) -> Dict[str, torch.Tensor]:
         sd = {k[len("vl."):]: v for k, v in self.state_dict().items() if k.startswith("vl.")}

@@ -1,0 +1,106 @@
+"""Calls around the umT5 encoder and the reward backbone that reach their kernels by another way than the
+scorer and the prompt encoder: the backbone called directly, recomputed in the backward pass, generating;
+layers replaced, wrapped or watched after the model was made."""
+import threading
+
+import pytest
+import torch
+
+from osp_next_b200 import ops
+from osp_next_b200.rewards import videoalign as va
+from test_videoalign import _tiny_vl
+
+gpu = pytest.mark.gpu
+
+
+def _batch(side, B=3, L=24, seed=1):
+    ids = torch.randint(3, 280, (B, L), generator=torch.Generator().manual_seed(seed))
+    mask = torch.ones_like(ids)
+    if side == "right":
+        mask[1, 15:], mask[2, 1:] = 0, 0
+    elif side == "left":
+        mask[1, :9], mask[2, :L - 1] = 0, 0
+    elif side == "holes":
+        mask[1, 5:9] = 0
+    return ids, mask
+
+
+def _backbones():
+    """The same random backbone without and with the kernels."""
+    return _tiny_vl(), va.VideoAlignRewardModel(_tiny_vl(), output_dim=1, reward_token="last").use_kernels().vl
+
+
+@pytest.mark.parametrize("side", ["right", "left", "none", "holes"])
+def test_backbone_called_directly_keeps_its_mask(side):
+    ids, mask = _batch(side)
+    plain, kernels = _backbones()
+    with torch.no_grad():
+        want, got = (m.model(input_ids=ids, attention_mask=mask).last_hidden_state for m in (plain, kernels))
+    assert torch.allclose(got[mask > 0], want[mask > 0], atol=1e-5)
+
+
+@pytest.mark.parametrize("side", ["right", "left", "holes"])
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_backbone_recomputed_in_the_backward_pass(side, reentrant):
+    ids, mask = _batch(side)
+    grads = []
+    for m, recompute in zip(_backbones(), (False, True)):
+        if recompute:
+            m.gradient_checkpointing_enable({"use_reentrant": reentrant})
+            m.train()
+        x = m.get_input_embeddings()(ids).detach().requires_grad_(True)
+        h = m.model(inputs_embeds=x, attention_mask=mask, use_cache=False,
+                    position_ids=torch.arange(ids.shape[1]).expand(3, *ids.shape)).last_hidden_state
+        h[mask > 0].square().sum().backward()
+        grads.append({"x": x.grad, **{n: p.grad for n, p in m.named_parameters() if p.grad is not None}})
+    assert "x" in grads[1]
+    for n, g in grads[1].items():
+        want = grads[0][n]
+        assert torch.allclose(g, want, atol=1e-4 * max(1.0, float(want.abs().max()))), n
+
+
+@pytest.mark.parametrize("side", ["left", "none"])
+def test_backbone_generates(side):
+    """A prompt at once, then single tokens over a cache."""
+    ids, mask = _batch(side)
+    plain, kernels = _backbones()
+    want, got = (m.generate(input_ids=ids, attention_mask=mask, max_new_tokens=4, do_sample=False, pad_token_id=0)
+                 for m in (plain, kernels))
+    assert torch.equal(got, want)
+
+
+def test_backbone_with_a_mask_of_its_callers():
+    """A mask [B, 1, L, L] made by the caller."""
+    ids, _ = _batch("none")
+    m4 = torch.ones(24, 24, dtype=torch.bool).tril().triu(-5)[None, None].expand(3, 1, 24, 24)
+    with torch.no_grad():
+        want, got = (m.model(input_ids=ids, attention_mask=m4).last_hidden_state for m in _backbones())
+    assert torch.allclose(got, want, atol=1e-5)
+
+
+def test_backbone_config_stays_during_a_call():
+    """Batches with holes in their masks in one thread, others in a second one, on the same model."""
+    model = va.VideoAlignRewardModel(_tiny_vl(), output_dim=1, reward_token="last")
+    batches = [_batch("holes"), _batch("left", seed=2)]
+    with torch.no_grad():
+        want = [model._hidden(*b) for b in batches]
+    model.use_kernels()
+
+    def refuse(*a, **k):
+        raise AssertionError("the shared configuration is switched during a call")
+    model.vl.set_attn_implementation = refuse
+    got = [[], []]
+
+    def work(i):
+        with torch.no_grad():
+            for _ in range(5):
+                got[i].append(model._hidden(*batches[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i, (_, mask) in enumerate(batches):
+        assert len(got[i]) == 5
+        for h in got[i]:
+            assert torch.allclose(h[mask > 0], want[i][mask > 0], atol=1e-5)
