@@ -309,11 +309,13 @@ ATTENTION_NAME = "osp_packed"          # the packed kernel's name among transfor
 
 class _PackedMask:
     """What the text layers get in the place of a mask tensor: each row's tokens as one packed sequence.  It
-    is an argument of every layer, so that a layer recomputed in the backward pass sees the same one."""
+    is an argument of every layer, so that a layer recomputed in the backward pass sees the same one.  ``library``: makes
+    the mask of a layer that the packed kernel does not take."""
 
-    def __init__(self, first, lengths, width: int):
+    def __init__(self, first, lengths, width: int, library):
         self._rows = (lengths, [i * width + f for i, f in enumerate(first)])
         self._packs = {}
+        self.library = library
 
     def pack(self, device) -> SequencePack:
         """On the device of a layer (layers may lie on several)."""
@@ -331,16 +333,25 @@ def _packed_mask(**args):
     if whole and args.get("mask_function", causal_mask_function) is causal_mask_function:
         runs = ([0] * B, [L] * B) if m is None else _mask_runs(m)
         if runs is not None:
-            return _PackedMask(*runs, L)
+            return _PackedMask(*runs, L, lambda: sdpa_mask(**args))
     return sdpa_mask(**args)
 
 
-def _packed_attention(module, query, key, value, attention_mask=None, scaling=None, **kw):
+def _takes(query, key) -> bool:
+    D = query.shape[-1]
+    return (not query.is_cuda or query.dtype == torch.bfloat16) and D % 8 == 0 and D <= 128 and (
+        query.shape[1] <= 128 * key.shape[1])
+
+
+def _packed_attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, **kw):
     """transformers' attention function: query [B, heads, L, D], key and value [B, key heads, L, D] ->
-    ([B, L, heads, D], None).  Masks that are no :class:`_PackedMask` go to the library's attention."""
-    if not isinstance(attention_mask, _PackedMask):
+    ([B, L, heads, D], None).  What the packed kernel does not do goes to the library's attention: masks that
+    are no :class:`_PackedMask`, dropout, other types than bf16 on the GPU, other heads."""
+    packed = isinstance(attention_mask, _PackedMask)
+    if not packed or dropout or not _takes(query, key):
         from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
-        return ALL_ATTENTION_FUNCTIONS["sdpa"](module, query, key, value, attention_mask, scaling=scaling, **kw)
+        mask = attention_mask.library() if packed else attention_mask
+        return ALL_ATTENTION_FUNCTIONS["sdpa"](module, query, key, value, mask, scaling=scaling, dropout=dropout, **kw)
     B, H, L, D = query.shape
 
     def rows(t):

@@ -104,3 +104,17 @@ def test_backbone_config_stays_during_a_call():
         assert len(got[i]) == 5
         for h in got[i]:
             assert torch.allclose(h[mask > 0], want[i][mask > 0], atol=1e-5)
+
+
+def test_backbone_in_training_drops_attention_weights(monkeypatch):
+    """attention_dropout of a backbone in training: every weight dropped leaves the layers without attention."""
+    ids, mask = _batch("left")
+    plain, kernels = _backbones()
+    out = []
+    for m in (plain, kernels):
+        m.train()
+        for layer in m.model.language_model.layers:
+            layer.self_attn.attention_dropout = 1.0
+        with torch.no_grad():
+            out.append(m.model(input_ids=ids, attention_mask=mask).last_hidden_state)
+    assert torch.allclose(out[0], out[1], atol=1e-5)
