@@ -421,6 +421,18 @@ def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=No
 
 # ----------------------------------------------------------------------------- gated feed-forward
 
+def as_made(m, cls) -> bool:
+    """Whether a layer computes what its class does: that class itself (no adapter, no quantised or
+    parametrised form), no hooks, no forward of its own.  Its parameters may then stand for it."""
+    return (type(m) is cls and "forward" not in m.__dict__ and not m._forward_hooks and not m._forward_pre_hooks
+            and not m._backward_hooks and not m._backward_pre_hooks)
+
+
+def plain_linears(*ms) -> bool:
+    """Whether all are plain ``nn.Linear`` layers without a bias (see :func:`as_made`) and with a plain weight."""
+    return all(as_made(m, torch.nn.Linear) and m.bias is None and type(m.weight) is torch.nn.Parameter for m in ms)
+
+
 class _GatedFFNFn(torch.autograd.Function):
     """Gated feed-forward block on the kernels of ops/csrc/gated_ffn.cu.  Keeps x, the weights and both
     projections; h comes back from them in the epilogue of dh = dy W_down."""

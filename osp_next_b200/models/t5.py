@@ -114,11 +114,16 @@ class T5FeedForward(nn.Module):
         self.fc2 = nn.Linear(dim_ffn, dim, bias=False)
         self.dropout = nn.Dropout(dropout)
 
+    def _plain(self) -> bool:
+        """Whether the layers are those of __init__: adapters, quantised layers and hooks run as modules."""
+        return (Fn.as_made(self.gate, nn.Sequential) and len(self.gate) == 2 and Fn.as_made(self.gate[1], nn.GELU)
+                and self.gate[1].approximate == "tanh" and Fn.plain_linears(self.gate[0], self.fc1, self.fc2))
+
     def forward(self, x):
-        ws = (self.gate[0].weight, self.fc1.weight, self.fc2.weight)
-        if (x.is_cuda and x.dtype == torch.bfloat16 and all(w.dtype == torch.bfloat16 for w in ws)
-                and not (self.training and self.dropout.p > 0)):
-            return Fn.gated_ffn(x, *ws, act="gelu_tanh")        # one kernel up to the product, one down
+        if (x.is_cuda and x.dtype == torch.bfloat16 and not (self.training and self.dropout.p > 0) and self._plain()):
+            ws = (self.gate[0].weight, self.fc1.weight, self.fc2.weight)
+            if all(w.dtype == torch.bfloat16 for w in ws):
+                return Fn.gated_ffn(x, *ws, act="gelu_tanh")    # one kernel up to the product, one down
         return self.dropout(self.fc2(self.dropout(self.fc1(x) * self.gate(x))))
 
 

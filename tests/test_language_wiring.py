@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from osp_next_b200 import ops
+from osp_next_b200.models import t5
 from osp_next_b200.rewards import videoalign as va
 from test_videoalign import _tiny_vl
 
@@ -118,3 +119,71 @@ def test_backbone_in_training_drops_attention_weights(monkeypatch):
         with torch.no_grad():
             out.append(m.model(input_ids=ids, attention_mask=mask).last_hidden_state)
     assert torch.allclose(out[0], out[1], atol=1e-5)
+
+
+def _touch(block, names, how):
+    """Adapters, quantisation, hooks or another forward on the layers ``names`` of a gated block."""
+    torch.manual_seed(5)
+    if how == "lora":
+        from osp_next_b200.models.lora import LoraLinear, inject_lora
+        assert len(inject_lora(block, 8, 16.0, names)) == len(names)
+        for m in block.modules():
+            if isinstance(m, LoraLinear):
+                for part in (m.lora_A, m.lora_B):
+                    torch.nn.init.normal_(part["default"].weight)
+    elif how == "quantised":
+        from osp_next_b200.quant.fp8 import FP8Linear
+        for n in names:
+            old = block.get_submodule(n)
+            new = FP8Linear(old.in_features, old.out_features, bias=False)
+            new.weight = old.weight
+            parent, _, leaf = n.rpartition(".")
+            setattr(block.get_submodule(parent), leaf, new)
+    elif how == "bias":
+        for n in names:
+            m = block.get_submodule(n)
+            m.bias = torch.nn.Parameter(torch.randn(m.out_features, dtype=m.weight.dtype, device=m.weight.device))
+    elif how == "forward":
+        m = block.get_submodule(names[0])
+        plain = m.forward
+        m.forward = lambda x: 2 * plain(x)
+    else:
+        hook = {"hook": "register_forward_hook", "pre": "register_forward_pre_hook",
+                "backward": "register_full_backward_hook"}[how]
+        getattr(block.get_submodule(names[-1]), hook)(
+            {"hook": lambda m, a, y: 2 * y, "pre": lambda m, a: (2 * a[0],), "backward": lambda m, a, g: None}[how])
+
+
+TOUCHES = ["lora", "quantised", "bias", "forward", "hook", "pre", "backward"]
+
+
+def test_t5_feed_forward_knows_its_layers():
+    names = ["gate.0", "fc1", "fc2"]
+    ffn = t5.T5FeedForward(16, 40, 0.0)
+    assert ffn._plain()
+    for how in TOUCHES:
+        ffn = t5.T5FeedForward(16, 40, 0.0)
+        _touch(ffn, names, how)
+        assert not ffn._plain(), how
+    ffn = t5.T5FeedForward(16, 40, 0.0)
+    ffn.gate[1] = torch.nn.GELU()
+    assert not ffn._plain()
+    ffn = t5.T5FeedForward(16, 40, 0.0)
+    ffn.gate.register_forward_hook(lambda m, a, y: 2 * y)
+    assert not ffn._plain()
+
+
+@gpu
+@pytest.mark.parametrize("how", TOUCHES)
+def test_gpu_t5_feed_forward_runs_its_layers(how):
+    """The module gives what its layers give one after another, whatever they are."""
+    torch.manual_seed(0)
+    ffn = t5.T5FeedForward(64, 136, 0.0).eval().to("cuda", torch.bfloat16)
+    x = torch.randn(5, 64, device="cuda").bfloat16()
+    with torch.no_grad():
+        before = ffn(x)
+        _touch(ffn, ["gate.0", "fc1", "fc2"], how)
+        want = ffn.cuda().fc2(ffn.fc1(x) * ffn.gate(x))
+        got = ffn(x)
+    assert torch.equal(got, want)
+    assert how == "backward" or not torch.equal(got, before)
