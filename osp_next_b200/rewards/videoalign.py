@@ -22,6 +22,7 @@ frame sampling and the Qwen-VL resize rule are reimplemented below.
 """
 from __future__ import annotations
 
+import functools
 import glob
 import json
 import math
@@ -362,10 +363,20 @@ def _packed_attention(module, query, key, value, attention_mask=None, scaling=No
 
 
 def _gated_mlp(self, x):
-    """A SiLU-gated MLP's forward on the gated feed-forward kernels."""
-    return Fn.gated_ffn(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, "silu").to(x.dtype)
+    """A SiLU-gated MLP's forward on the gated feed-forward kernels; adapters, quantised layers and hooks that
+    the layers got since, and other types than bf16 on the GPU, run as the module's own forward."""
+    parts = (self.gate_proj, self.up_proj, self.down_proj)
+    if not _plain_mlp(self) or any(p.weight.dtype != x.dtype for p in parts) or (x.is_cuda and x.dtype != torch.bfloat16):
+        return type(self).forward(self, x)
+    return Fn.gated_ffn(x, *(p.weight for p in parts), "silu").to(x.dtype)
 
 
+def _plain_mlp(m) -> bool:
+    parts = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+    return Fn.plain_linears(*parts) and any(Fn.as_made(getattr(m, "act_fn", None), t) for t in _silu_types())
+
+
+@functools.lru_cache(maxsize=None)
 def _silu_types():
     from transformers.activations import ACT2FN
     return (nn.SiLU, type(ACT2FN["silu"]))
@@ -408,15 +419,14 @@ class VideoAlignRewardModel(nn.Module):
 
     def use_kernels(self):
         """Text attention on the packed kernel (padding costs nothing: rows are packed by the mask) and
-        SiLU-gated MLPs without biases on the gated feed-forward kernels."""
+        SiLU-gated MLPs without biases on the gated feed-forward kernels, for models in bf16 on the GPU; what
+        these do not take runs as before."""
         from transformers import AttentionInterface, AttentionMaskInterface
         AttentionInterface.register(ATTENTION_NAME, _packed_attention)
         AttentionMaskInterface.register(ATTENTION_NAME, _packed_mask)
         self.vl.set_attn_implementation({"text_config": ATTENTION_NAME})
         for m in self.vl.model.language_model.modules():
-            parts = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
-            if all(type(p) is nn.Linear and p.bias is None for p in parts) and isinstance(
-                    getattr(m, "act_fn", None), _silu_types()):
+            if _plain_mlp(m):
                 m.forward = types.MethodType(_gated_mlp, m)
         return self
 

@@ -187,3 +187,33 @@ def test_gpu_t5_feed_forward_runs_its_layers(how):
         got = ffn(x)
     assert torch.equal(got, want)
     assert how == "backward" or not torch.equal(got, before)
+
+
+@pytest.mark.parametrize("how", TOUCHES)
+def test_backbone_mlp_runs_its_layers(how):
+    """Layers replaced, wrapped or watched after use_kernels."""
+    torch.manual_seed(0)
+    plain, kernels = (m.model.language_model.layers[0].mlp for m in _backbones())
+    x = torch.randn(5, 64)
+    with torch.no_grad():
+        before = kernels(x)
+        assert torch.allclose(before, plain(x), atol=1e-5)
+        for m in (plain, kernels):
+            _touch(m, ["gate_proj", "up_proj", "down_proj"], how)
+        want, got = plain(x), kernels(x)
+    assert torch.equal(got, want)
+    assert how == "backward" or not torch.equal(got, before)
+
+
+@gpu
+def test_gpu_backbone_in_other_types_and_heads():
+    """fp32, and heads that the packed kernel does not take: the library's attention.  fp32 sums of some 200
+    terms a layer on both sides, 2^-24 each."""
+    ids, mask = _batch("left")
+    with torch.no_grad():
+        want = _tiny_vl().model(input_ids=ids, attention_mask=mask).last_hidden_state
+        m = va.VideoAlignRewardModel(_tiny_vl(), output_dim=1, reward_token="last").cuda().use_kernels().vl
+        n0 = ops._ext.launch_count()
+        got = m.model(input_ids=ids.cuda(), attention_mask=mask.cuda()).last_hidden_state.cpu()
+        assert ops._ext.launch_count() == n0
+    assert (got - want)[mask > 0].norm() <= 2 * 200 * 2.0 ** -24 * want[mask > 0].norm()
