@@ -410,7 +410,7 @@ def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=No
     none: with it, call without autograd.  First derivatives only."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if not q.is_cuda:
-        ops.packed.check_packed(q, k, v, pack, rel_bias)
+        ops.packed.check_packed(q, k, v, pack, rel_bias, scale=scale)
         return ref.packed_attention(q, k, v, pack, causal, scale, rel_bias)[0]
     if _fused(q, k, v, rel_bias):
         return ops.packed_attention(q.to(_BF16), k.to(_BF16), v.to(_BF16), pack, causal, scale, rel_bias)

@@ -27,6 +27,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "packed_attn.cuh"
@@ -663,6 +664,7 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& 
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, int64_t row_heads, int64_t key_heads, bool causal, double scale,
                                         bool fill) {
+  TORCH_CHECK(std::abs(scale) < 1e38, "packed_attention: a finite scale");
   const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
   const at::Tensor o = pa::tma_rows(o_.contiguous()), lse = lse_.contiguous();
   const at::Tensor dout = pa::tma_rows(dout_.to(at::kBFloat16).contiguous());

@@ -592,7 +592,11 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& 
                                         const c10::optional<at::Tensor>& rel_bias_, bool want_lse, bool want_low,
                                         int64_t rows,
                                         int64_t key_rows, int64_t longest, bool dense) {
-  const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
+  TORCH_CHECK(own_scale || std::abs(scale) < 1e38, "packed_attention: a finite scale");
+  // a row's maximum is taken before the scale, which has to be positive: (-q) k (-scale) otherwise
+  const bool flip = !own_scale && scale < 0;
+  if (flip) scale = -scale;
+  const at::Tensor q = pa::tma_rows(flip ? q_.neg() : q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
   const pa::Shape s = pa::check_shapes(q, k, v, "packed_attention");
   TORCH_CHECK(s.Nq >= rows && s.Nk >= key_rows, "packed_attention: fewer rows than the pack's");
   pa::check_list(items, 8, q, "packed_attention: items");

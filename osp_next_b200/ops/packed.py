@@ -255,8 +255,10 @@ def key_items(pack, group, kv_heads, causal, sms):
 
 # ---------------------------------------------------------------------------- calls
 
-def check_packed(q, k, v, pack, rel_bias=None, what="packed_attention"):
+def check_packed(q, k, v, pack, rel_bias=None, what="packed_attention", scale=None):
     """Raise for operands that do not fit each other or the pack."""
+    if scale is not None and not abs(float(scale)) < 1e38:         # in fp32, times log2 e
+        raise ValueError(f"{what}: a finite scale, got {scale}")
     if not isinstance(pack, SequencePack):
         raise TypeError(f"{what}: pack has to be a SequencePack")
     for n, t in (("q", q), ("k", k), ("v", v)):
@@ -296,7 +298,7 @@ def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
 
     q [Nq, heads, D], k and v [Nk, key heads, D] (bf16 on the GPU; rows of any stride, views of a
     fused projection among them).  Heads h G .. (h + 1) G - 1 of q read key head h, G = heads / key
-    heads.  D: multiples of 8 up to 128.  Query i of a sequence with lq queries and lk keys stands at
+    heads.  D: multiples of 8 up to 128.  ``scale``: any finite number.  Query i of a sequence with lq queries and lk keys stands at
     position i + lk - lq; ``causal`` queries see the keys up to their position.  ``rel_bias`` fp32
     [heads, 2 M - 1] adds ``rel_bias[h, key position - query position + M - 1]``, finite values.
     A query that sees no key gives zeros and a log-sum-exp of -inf; so do rows of no sequence.
@@ -307,11 +309,11 @@ def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
     It records no graph: ``models.functional.packed_attention`` is the form under autograd."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (rel_bias is not None and rel_bias.requires_grad)):
-        check_packed(q, k, v, pack, rel_bias)
+        check_packed(q, k, v, pack, rel_bias, scale=scale)
         raise RuntimeError("packed_attention has no gradient: use models.functional.packed_attention, or "
                            "torch.no_grad()")
     if not q.is_cuda:
-        check_packed(q, k, v, pack, rel_bias)
+        check_packed(q, k, v, pack, rel_bias, scale=scale)
         scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
         o, lse = ref.packed_attention(q, k, v, pack, causal, scale, rel_bias)
         return (o, lse) if return_lse else o
@@ -330,7 +332,7 @@ def _forward(q, k, v, pack, causal, scale, rel_bias, want_lse, want_low):
                                      -1.0 if scale is None else float(scale), scale is None, rel_bias, want_lse,
                                      want_low, pack.rows, pack.key_rows, pack.longest, pack.dense)
     except (AttributeError, IndexError, RuntimeError, TypeError, ValueError, ZeroDivisionError):
-        check_packed(q, k, v, pack, rel_bias)
+        check_packed(q, k, v, pack, rel_bias, scale=scale)
         if q.dtype != torch.bfloat16:
             raise TypeError(f"packed_attention: bf16 on the GPU, got {q.dtype}") from None
         raise
@@ -347,7 +349,7 @@ def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool
     """Gradients (dq, dk, dv) of :func:`packed_attention` without a bias, from its output and
     log-sum-exp (and the remainder of :func:`packed_attention_for_grad`); rows of no sequence get zeros."""
     if not q.is_cuda:
-        check_packed(q, k, v, pack, what="packed_attention_bwd")
+        check_packed(q, k, v, pack, what="packed_attention_bwd", scale=scale)
         return ref.packed_attention_bwd(q, k, v, dout, pack, causal,
                                         1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale))
     try:
@@ -359,7 +361,7 @@ def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool
         return ext().packed_attn_bwd(q, k, v, o, dout, lse, remainder, rows, keys, joins, slots, row_heads, key_heads,
                                      bool(causal), 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), fill)
     except (AttributeError, IndexError, RuntimeError, TypeError, ValueError, ZeroDivisionError):
-        check_packed(q, k, v, pack, what="packed_attention_bwd")
+        check_packed(q, k, v, pack, what="packed_attention_bwd", scale=scale)
         if q.dtype != torch.bfloat16:
             raise TypeError(f"packed_attention_bwd: bf16 on the GPU, got {q.dtype}") from None
         raise
