@@ -37,7 +37,8 @@ struct Tensor {
 
 struct Args {
   Tensor t[2];
-  const int* pos;              // [n, axes]
+  const void* pos;             // [n, axes], int32 or int64
+  int pos64;
   const float2* table;         // [positions, R / 2]
   long n;
   int axes, positions;
@@ -144,11 +145,17 @@ __device__ __forceinline__ void turn_pieces(const T* src, T* dst, long in_step, 
   }
 }
 
+// Entry i of the positions, -1 where it lies outside the table; 64-bit ones are compared as they are.
+__device__ __forceinline__ int position(const Args& a, long i) {
+  const long long p = a.pos64 ? static_cast<const long long*>(a.pos)[i] : static_cast<const int*>(a.pos)[i];
+  return p >= 0 && p < a.positions ? (int)p : -1;
+}
+
 __device__ __forceinline__ float2 pair_of(const Args& a, long token, int i, int first_pos, bool& bad) {
   int axis = 0;
   while (axis + 1 < a.axes && i >= a.end[axis]) ++axis;
-  const int p = a.axes == 1 ? first_pos : a.pos[token * a.axes + axis];
-  if (p < 0 || p >= a.positions) {          // no such position: NaN results and an error for the host
+  const int p = a.axes == 1 ? first_pos : position(a, token * a.axes + axis);
+  if (p < 0) {                              // no such position: NaN results and an error for the host
     bad = true;
     return make_float2(NAN, NAN);
   }
@@ -168,7 +175,7 @@ rotate(const Args args) {
   const int R = args.R, D = args.D;
   const int turned = kHalf ? R / 2 / V : R / V;
   const int pieces = turned + (D - R) / V;
-  const int first_pos = args.axes == 1 ? args.pos[token] : 0;
+  const int first_pos = args.axes == 1 ? position(args, token) : 0;
   bool bad = false;
   // heads are dealt so that a warp is full: `per` lanes to a head, 32 / per heads at a time
   int per = 1;
@@ -261,7 +268,10 @@ std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at
               std::to_string(D), " (even, at most 256)");
   TORCH_CHECK(n < (1ll << 31), what, "too many tokens");
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor pos = pos_.to(at::kInt).contiguous();
+  // types whose values fit 32 bits are read as int32
+  const at::ScalarType pt = pos_.scalar_type();
+  const bool narrow = pt == at::kInt || pt == at::kShort || pt == at::kChar || pt == at::kByte || pt == at::kUInt16;
+  at::Tensor pos = pos_.to(narrow ? at::kInt : at::kLong).contiguous();
   if (lead > 1) pos = pos.view({tokens, axes}).repeat({lead, 1});
   const at::Tensor table = table_.contiguous();
   Args a{};
@@ -307,7 +317,8 @@ std::vector<at::Tensor> rotary_apply(const at::Tensor& q, const c10::optional<at
     return out;
   }
   vec = vec == wide ? wide : vec >= 2 ? 2 : 1;
-  a.pos = pos.data_ptr<int>();
+  a.pos = pos.data_ptr();
+  a.pos64 = narrow ? 0 : 1;
   a.table = reinterpret_cast<const float2*>(table.data_ptr<float>());
   TORCH_CHECK(reinterpret_cast<uintptr_t>(a.table) % 8 == 0, what, "table at a multiple of 8 bytes");
   a.n = n;
