@@ -40,3 +40,31 @@ def test_gpu_types_of_positions(dtype):
     close(ops.rotary(q, None, two.to(dtype), table, "interleaved", [20, 12])[0][1],
           turned(q[1], two, table, "interleaved", [20, 12]), str(dtype))
     ops.check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rot,sections", [(32, None), (64, [10, 12, 10]), (24, [12, 0]), (0, None), (2, [0, 1])])
+def test_gpu_a_bad_position_makes_its_whole_token_nan(layout, dtype, rot, sections):
+    """The copied elements, the pairs of the other axes and heads of k too, from any axis, also one without pairs."""
+    table = ops.rotary_table(rot, 100) if rot else torch.zeros(100, 0, 2, device="cuda")
+    g = torch.Generator("cuda").manual_seed(1)
+    q, k = (torch.randn(9, h, 64, generator=g, device="cuda").to(dtype) for h in (5, 2))
+    axes = 1 if sections is None else len(sections)
+    pos = torch.randint(0, 100, (9, axes), generator=g, device="cuda")
+    kw = dict(layout=layout, sections=sections)
+    want = ops.rotary(q, k, pos, table, **kw)
+    ops.check_device_errors()
+    for axis in range(axes):
+        for value in (100, -1):
+            bad = pos.clone()
+            bad[4, axis] = value
+            got = ops.rotary(q, k, bad, table, **kw)
+            with pytest.raises(ops.DeviceWaitError, match="rotary position"):
+                ops.check_device_errors()
+            rest = torch.arange(9, device="cuda") != 4
+            for a, b in zip(got, want):
+                assert torch.isnan(a[4]).all() and torch.equal(a[rest], b[rest])
+            with pytest.raises(IndexError, match="positions 0 to 99"):
+                ops.rotary(q.cpu(), k.cpu(), bad.cpu(), table.cpu(), **kw)
