@@ -309,20 +309,20 @@ def apply_rope(x, pos, freqs):
 
 
 class _RotaryFn(torch.autograd.Function):
-    """Rotation of q and k in one launch; the gradient is the rotation back."""
+    """Rotation of q and k in one launch; the gradient is the rotation the other way."""
 
     @staticmethod
-    def forward(ctx, q, k, pos, table, layout, sections):
+    def forward(ctx, q, k, pos, table, layout, sections, inverse):
         ctx.save_for_backward(pos, table)
-        ctx.meta = (layout, sections)
-        return ops.rotary(q, k, pos, table, layout, sections)
+        ctx.meta = (layout, sections, inverse)
+        return ops.rotary(q, k, pos, table, layout, sections, inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
         pos, table = ctx.saved_tensors
-        layout, sections = ctx.meta
-        gq, gk = rotary(gq, gk, pos, table, layout, sections, inverse=True)
-        return gq, gk, None, None, None, None
+        layout, sections, inverse = ctx.meta
+        gq, gk = rotary(gq, gk, pos, table, layout, sections, not inverse)
+        return gq, gk, None, None, None, None, None
 
 
 def rotary(q, k, pos, table, layout: str = "half", sections=None, inverse: bool = False):
@@ -330,8 +330,7 @@ def rotary(q, k, pos, table, layout: str = "half", sections=None, inverse: bool 
     if _fused(q, k) or not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k))):
         return ops.rotary(q, k, pos, table, layout, sections, inverse)
     if q.is_cuda:
-        t = table if not inverse else table * table.new_tensor([1.0, -1.0])
-        return _RotaryFn.apply(q, k, pos, t, layout, sections)
+        return _RotaryFn.apply(q, k, pos, table, layout, sections, inverse)
     with torch.no_grad():
         ops.rotary(q, k, pos, table, layout, sections)                # the same refusals
     p = pos[:, None] if pos.dim() == 1 else pos

@@ -68,3 +68,31 @@ def test_gpu_a_bad_position_makes_its_whole_token_nan(layout, dtype, rot, sectio
                 assert torch.isnan(a[4]).all() and torch.equal(a[rest], b[rest])
             with pytest.raises(IndexError, match="positions 0 to 99"):
                 ops.rotary(q.cpu(), k.cpu(), bad.cpu(), table.cpu(), **kw)
+
+
+@gpu
+def test_gpu_inverse_and_second_derivatives_are_captured():
+    """The inverse under autograd, its gradient and the gradient of that, in a graph: no copy from the host."""
+    table = ops.rotary_table(64, 100)
+    pos = torch.arange(20, device="cuda")
+    g = torch.Generator("cuda").manual_seed(1)
+    static = [torch.randn(20, 3, 64, generator=g, device="cuda") for _ in range(3)]
+
+    def step(x, do, dd):
+        x, do = x.detach().requires_grad_(True), do.detach().requires_grad_(True)
+        y = Fn.rotary(x, None, pos, table, inverse=True)[0]
+        gx, = torch.autograd.grad(y, x, do, create_graph=True)
+        gdo, = torch.autograd.grad(gx, do, dd)
+        return y.detach(), gx.detach(), gdo
+    want = step(*static)
+    for i, back in ((0, True), (1, False), (2, True)):
+        close(want[i], turned(static[i], pos[:, None], table, "half", [32], back), str(i))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step(*static)
+    for t in static:
+        t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, step(*static)))
