@@ -326,10 +326,11 @@ class _RotaryFn(torch.autograd.Function):
 
 
 def rotary(q, k, pos, table, layout: str = "half", sections=None, inverse: bool = False):
-    """Rotary positions of q and k (k may be None; see :func:`ops.rotary`), under autograd too."""
-    if _fused(q, k) or not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k))):
+    """Rotary positions of q and k (k may be None; see :func:`ops.rotary`), under autograd too (a table with a
+    gradient takes elementary operations)."""
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, table))):
         return ops.rotary(q, k, pos, table, layout, sections, inverse)
-    if q.is_cuda:
+    if q.is_cuda and not table.requires_grad:
         return _RotaryFn.apply(q, k, pos, table, layout, sections, inverse)
     with torch.no_grad():
         ops.rotary(q, k, pos, table, layout, sections)                # the same refusals

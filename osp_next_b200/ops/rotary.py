@@ -89,7 +89,8 @@ def rotary(q, k, pos, table, layout: str = "half", sections: Optional[Sequence[i
     and is reported by ``check_device_errors`` on the GPU, and raises on the CPU.
 
     It records no graph: ``models.functional.rotary`` is the form under autograd."""
-    if q.is_cuda and not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+    if q.is_cuda and not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
+                                                       or table.requires_grad)):
         try:
             # the kernel's own checks come first: a call of a few microseconds has no time for both
             if layout == "half" or layout == "interleaved":
@@ -100,7 +101,7 @@ def rotary(q, k, pos, table, layout: str = "half", sections: Optional[Sequence[i
             _check(q, k, pos, table, layout, sections)
             raise
     ts, pos, sections = _check(q, k, pos, table, layout, sections)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (*ts, table)):
         raise RuntimeError("rotary has no gradient here: use models.functional.rotary, or torch.no_grad()")
     out = [ref.rotary(t, pos, table, layout, sections, inverse) for t in ts]
     return out[0], out[1] if k is not None else None

@@ -70,6 +70,30 @@ def test_gpu_a_bad_position_makes_its_whole_token_nan(layout, dtype, rot, sectio
                 ops.rotary(q.cpu(), k.cpu(), bad.cpu(), table.cpu(), **kw)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("layout,inverse", [("half", False), ("interleaved", True)])
+def test_gradient_of_the_table(device, layout, inverse):
+    """No call drops it: against differences, alone and beside that of q, and refused where nothing is recorded."""
+    g = torch.Generator().manual_seed(1)
+    table = torch.randn(10, 4, 2, generator=g).to(device)
+    q, do = (torch.randn(3, 2, 8, generator=g).to(device) for _ in range(2))
+    pos = torch.tensor([2, 9, 2], device=device)
+    leaf = table.clone().requires_grad_()
+    for x in (q, q.clone().requires_grad_()):
+        got, = torch.autograd.grad(Fn.rotary(x, None, pos, leaf, layout, inverse=inverse)[0], leaf, do)
+        for at in ((2, 0, 0), (2, 3, 1), (9, 1, 1), (4, 0, 0)):
+            step = torch.zeros_like(table)
+            step[at] = 0.5                                              # the rotation is linear in the table
+            want = sum(s * (ref.rotary(q.double(), pos[:, None], table + s * step, layout, [4], inverse) * do).sum()
+                       for s in (1, -1))
+            # cosines and sines of some 3 as fp32, 2^-23 each, times 3 x 2 x 8 products of some 1
+            assert abs(got[at] - want) <= 48 * 3 * 2.0 ** -23 * 4, at
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.rotary(q, None, pos, leaf)
+    with torch.no_grad():
+        assert not ops.rotary(q, None, pos, leaf)[0].requires_grad
+
+
 @gpu
 def test_gpu_inverse_and_second_derivatives_are_captured():
     """The inverse under autograd, its gradient and the gradient of that, in a graph: no copy from the host."""
