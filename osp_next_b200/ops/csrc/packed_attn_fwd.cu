@@ -11,7 +11,7 @@
 // a limit, so the mask costs one comparison per score, in tiles that hold such a limit only.
 //
 // Items with many keys and few rows are split along the keys: each part leaves its normalised fp32
-// output and log-sum-exp in a workspace and packed_combine_kernel joins them.
+// output, maximum and sum in a workspace and packed_combine_kernel joins them.
 //
 // What bounds it: long sequences the tensor pipe and the softmax in turn (20161 tokens, 28 heads of 128
 // to 4, causal: 2.6 to 2.9 ms, 1000 to 1100 TFLOP/s); one query each over long keys memory (48 x 1024 to
@@ -54,7 +54,7 @@ struct PackedFwdArgs {
   const float* bias;        // [Hq, 2 M - 1] or null
   int bias_m;               // M
   float* part_o;            // [slots, heads, kTiles * 128, Dr]
-  float* part_l;            // [slots, heads, kTiles * 128], log2 domain
+  float2* part_l;           // [slots, heads, kTiles * 128] (maximum, sum of 2^(S - maximum)), log2 domain
   int* err;
 };
 
@@ -106,6 +106,14 @@ struct FwdUnit {
     has_tail = n_kv > 0 && last_rows < kT;
   }
 };
+
+// A bias times log2 e, to +-1e38: the type's lowest value hides a key, and a tile that it fills keeps a finite
+// maximum (-inf - -inf is NaN), which the first key that is not hidden replaces.  A NaN stays one.
+__device__ __forceinline__ float finite_bias(float b) {
+  b *= pa::kLog2e;
+  b = b < -1e38f ? -1e38f : b;
+  return b > 1e38f ? 1e38f : b;
+}
 
 // Row maximum over the columns below `cols` (the warp's) and n_valid (the row's).
 __device__ __forceinline__ float masked_max(const uint32_t* sr, int cols, int n_valid) {
@@ -357,7 +365,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 2 * kT; e += kT) {
             const int at = bias_at + j * kT + e;
-            const float b = at >= 0 && at < 2 * args.bias_m - 1 ? row[at] * pa::kLog2e : 0.f;
+            const float b = at >= 0 && at < 2 * args.bias_m - 1 ? finite_bias(row[at]) : 0.f;
             dst[r + e] = b;
             dst[2 * kT + ((r + e + 1) & (2 * kT - 1))] = b;
           }
@@ -444,7 +452,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const long row = (long)(it.q_row + t * P + rp) * args.Hq + unit_head * G + rh;
       const long prow = ((long)it.slot * args.heads + unit_head) * (kTiles * kT) + t * kT + r;
       if (in) {
-        if (it.slot >= 0) args.part_l[prow] = lse2;
+        if (it.slot >= 0) args.part_l[prow] = make_float2(m_ref, l);
         else if (args.lse) args.lse[row] = lse2 * 0.69314718055994531f;
       }
       // kPiece bytes of each row at a time through shared memory, so that kPiece / 16 lanes write a
@@ -512,11 +520,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// o = sum_i 2^(l_i - l) o_i over the parts of one item, 2^l = sum_i 2^(l_i).  A warp per row; block
-// (join, key head, 8 rows).  The parts' weights are read by the lanes at once, 32 parts at a time.
+// o = sum_i w_i o_i / sum_i w_i over the parts of one item, w_i = l_i 2^(m_i - m) from their maxima and sums
+// (apart: next to a maximum of 1e38 the logarithm of a sum would be lost).  A warp per row; block (join, key
+// head, 8 rows).  The parts' weights are read by the lanes at once, 32 parts at a time.
 __global__ void __launch_bounds__(256)
 packed_combine_kernel(const int* joins, int G, int P, int tiles, int Hq, int Dr, const float* part_o,
-                      const float* part_l, __nv_bfloat16* out, float* lse, uint8_t* low) {
+                      const float2* part_l, __nv_bfloat16* out, float* lse, uint8_t* low) {
   const int4 j = reinterpret_cast<const int4*>(joins)[blockIdx.x];   // q_row, n_q, first slot, parts
   const int kvh = blockIdx.y, lane = threadIdx.x % 32;
   const int i = blockIdx.z * 8 + threadIdx.x / 32;
@@ -525,19 +534,17 @@ packed_combine_kernel(const int* joins, int G, int P, int tiles, int Hq, int Dr,
   const long stride = (long)gridDim.y * tiles * pa::kRows;
   const long first = (long)j.z * stride + (long)kvh * tiles * pa::kRows + t * pa::kRows + (p - t * P) * G + g;
   float top = -INFINITY;
-  for (int s = lane; s < j.w; s += 32) {
-    const float v = part_l[first + s * stride];
-    top = v != v || top != top ? NAN : fmaxf(top, v);
-  }
+  for (int s = lane; s < j.w; s += 32) top = fmaxf(top, part_l[first + s * stride].x);   // NaN is in the sums
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float v = __shfl_xor_sync(0xffffffffu, top, o);
-    top = v != v || top != top ? NAN : fmaxf(top, v);
-  }
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float base = top == -INFINITY ? 0.f : top;
   float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < j.w; s0 += 32) {
-    const float mine = s0 + lane < j.w ? exp2f(part_l[first + (s0 + lane) * stride] - base) : 0.f;
+    float mine = 0.f;
+    if (s0 + lane < j.w) {
+      const float2 ml = part_l[first + (s0 + lane) * stride];
+      mine = exp2f(ml.x - base) * ml.y;
+    }
     const int n = min(32, j.w - s0);
 #pragma unroll 4
     for (int s = 0; s < n; ++s) {
@@ -649,9 +656,9 @@ std::vector<at::Tensor> packed_attn_fwd(const at::Tensor& q_, const at::Tensor& 
   at::Tensor part_o, part_l;
   if (slots > 0) {
     part_o = at::empty({slots, a.heads, tiles * pa::kRows, s.D}, opt.dtype(at::kFloat));
-    part_l = at::empty({slots, a.heads, tiles * pa::kRows}, opt.dtype(at::kFloat));
+    part_l = at::empty({slots, a.heads, tiles * pa::kRows, 2}, opt.dtype(at::kFloat));
     a.part_o = part_o.data_ptr<float>();
-    a.part_l = part_l.data_ptr<float>();
+    a.part_l = reinterpret_cast<float2*>(part_l.data_ptr<float>());
   }
   const CUtensorMap tq = pa::tile_map(q, q, s.D, group, a.P);
   const CUtensorMap tk = pa::tile_map(k, q, s.D, 1, pa::kRows), tv = pa::tile_map(v, q, s.D, 1, pa::kRows);

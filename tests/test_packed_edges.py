@@ -64,3 +64,65 @@ def test_gpu_scale_of_zero_and_refusals(tiles):  # noqa: F811
                 call(q, k, v, pack, scale=scale)
         with pytest.raises(ValueError, match="finite scale"):
             ops.packed_attention_bwd(q, k, v, q, do, torch.zeros(103, 6, device="cuda"), pack, scale=scale)
+
+
+def _masking_bias(pack, heads, low):
+    """Each head hides another stretch of relative positions by the lowest value of the type: near keys, far
+    keys, those behind, those ahead, all of them; the rest is some +-1."""
+    m = pack.longest
+    d = torch.arange(1 - m, m, device="cuda")
+    hide = [d.abs() < 140, d.abs() > 130, d < 0, d > 0, d == d, d == 3][:heads]
+    b = torch.randn(heads, 2 * m - 1, generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+    return torch.where(torch.stack(hide), low, b)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,keys,dim", [([300, 77], None, 64), ([1, 20], [2500, 1300], 64), ([300], [700], 128)])
+def test_gpu_bias_of_the_lowest_value(lengths, keys, dim, causal, tiles):  # noqa: F811
+    """Hidden keys have no weight, also where they fill the first key tiles of a row; a row all of whose keys are
+    hidden weighs them alike, as scores that such a value swallows do (split along the keys or not)."""
+    pack = ops.SequencePack(lengths, keys)
+    q, k, v, _ = tensors(pack, 6, 3, dim, "cuda")
+    low = torch.finfo(torch.float32).min
+    bias = _masking_bias(pack, 6, low)
+    o, lse = ops.packed_attention(q, k, v, pack, causal=causal, scale=0.1, rel_bias=bias, return_lse=True)
+    ops.check_device_errors()
+    HALF, F32 = 2.0 ** -8, 2.0 ** -23
+    for a0, a, b0, b in zip(pack.starts, pack.lengths, pack.key_starts, pack.key_lengths):
+        place, key = torch.arange(b - a, b, device="cuda")[:, None], torch.arange(b, device="cuda")[None]
+        for h in range(6):
+            qs, ks, vs = q[a0:a0 + a, h].double(), k[b0:b0 + b, h // 2].double(), v[b0:b0 + b, h // 2].double()
+            add = bias[h][key - place + pack.longest - 1].double()
+            seen = key <= place if causal else torch.ones(a, b, dtype=torch.bool, device="cuda")
+            open_ = seen & (add > low)
+            none = seen.any(1) & ~open_.any(1)
+            s = qs @ ks.t() * 0.1
+            es = (dim + 2) * F32 * 0.1 * (qs.abs() @ ks.abs().t()) + 8 * F32 * (s.abs() + 4)
+            s = torch.where(none[:, None], 0.0, s + add).masked_fill(~torch.where(none[:, None], seen, open_), -math.inf)
+            want = torch.logsumexp(s, 1)
+            p = torch.where(torch.isinf(want)[:, None], 0.0, torch.exp(s - want[:, None]))
+            off = (2 * es.masked_fill(~open_, 0.0).amax(1, keepdim=True) + 16 * F32 + F32 * b ** 0.5 * 4).expm1()
+            ov = p @ vs
+            close(o[a0:a0 + a, h], ov, HALF * ov.abs() + (1 + HALF) * (HALF + off + b * F32) * (p @ vs.abs()), f"o {h}")
+            got = lse[a0:a0 + a, h].double()
+            assert torch.isfinite(got[none]).all() and (got[none] < -6e37).all()
+            close(got[~none], want[~none], (es.masked_fill(~open_, 0.0).amax(1) + 64 * F32 * (1 + s.masked_fill(
+                torch.isinf(s), 0.0).abs().amax(1)))[~none], f"lse {h}")
+
+
+@gpu
+def test_gpu_bias_of_the_largest_value(tiles):  # noqa: F811
+    """A row's keys of the largest value share its weight alike; a NaN stays one."""
+    pack = ops.SequencePack([200])
+    q, k, v, _ = tensors(pack, 2, 2, 64, "cuda")
+    bias = torch.zeros(2, 399, device="cuda")
+    bias[:, 199 - 4:199 + 1] = torch.finfo(torch.float32).max          # the last five positions
+    o = ops.packed_attention(q, k, v, pack, scale=0.1, rel_bias=bias)
+    want = torch.stack([v[max(0, i - 4):i + 1].double().mean(0) for i in range(200)])
+    size = torch.stack([v[max(0, i - 4):i + 1].double().abs().mean(0) for i in range(200)])
+    close(o, want, 2.0 ** -8 * want.abs() + 1.01 * 2.0 ** -8 * size, "o")
+    bias[1, 199 - 150] = math.nan
+    o = ops.packed_attention(q, k, v, pack, scale=0.1, rel_bias=bias)
+    assert torch.isnan(o[150:, 1]).all() and torch.isfinite(o[:, 0]).all() and torch.isfinite(o[:150, 1]).all()
+    ops.check_device_errors()
