@@ -155,7 +155,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* p_half = s_full + kTiles;              // [kTiles]
   uint64_t* p_full = p_half + kTiles;              // [kTiles]
   uint64_t* o_done = p_full + kTiles;              // [kTiles]
-  uint64_t* done = o_done + kTiles;
+  uint64_t* bias_full = o_done + kTiles;           // [kTiles] a key tile's stretch of the bias, by the tile's four warps
+  uint64_t* done = bias_full + kTiles;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(done + 2);
 
@@ -182,6 +183,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
+      mbar_init(&bias_full[t], 4);
     }
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -369,7 +371,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             dst[r + e] = b;
             dst[2 * kT + ((r + e + 1) & (2 * kT - 1))] = b;
           }
-          named_bar_sync(1 + t, 4 * 32);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bias_full[t]);
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bias_full[t], j & 1, args.err, kErrAttnSoftmax)))) break;
         }
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, args.err, kErrAttnSoftmax)))) break;
         tc_fence_after();

@@ -126,3 +126,14 @@ def test_gpu_bias_of_the_largest_value(tiles):  # noqa: F811
     o = ops.packed_attention(q, k, v, pack, scale=0.1, rel_bias=bias)
     assert torch.isnan(o[150:, 1]).all() and torch.isfinite(o[:, 0]).all() and torch.isfinite(o[:150, 1]).all()
     ops.check_device_errors()
+
+
+def test_waits_of_the_forward_kernel_are_bounded():
+    """Warps that may give up at a bounded wait meet others only at waits that are bounded too, and once, all
+    of them, before the block ends."""
+    src = (pathlib.Path(ops.__file__).parent / "csrc" / "packed_attn_fwd.cu").read_text()
+    kernel = src[src.index("packed_fwd_kernel(const __grid_constant__"):src.index("packed_combine_kernel(const int* joins")]
+    assert "named_bar_sync" not in kernel and "bar.sync" not in kernel
+    assert kernel.count("__syncthreads()") == 2
+    roles = kernel[kernel.index("if (warp == L::kProdWarp) {\n    // ---"):kernel.rindex("__syncthreads()")]
+    assert "__syncthreads" not in roles and "return;" not in roles
