@@ -473,7 +473,8 @@ class _GatedFFNFn(torch.autograd.Function):
 
 def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
     """``(act(x W_gate^T) * (x W_up^T)) W_down^T`` (see :func:`ops.gated_ffn`), under autograd too; bf16 on
-    the GPU, where gradients come in their tensor's type.  First derivatives only."""
+    the GPU, where gradients come in their tensor's type.  First derivatives only.  The projections are kept
+    for them in 16 bits, within 2^-10 of values from 2^-20 to 2^16 and 2^-7 of smaller and larger ones."""
     if not x.is_cuda:
         ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
         return ref.gated_ffn(x, w_gate, w_up, w_down, act)

@@ -63,28 +63,33 @@ __device__ __forceinline__ float act_f(int act, float g, float& d) {
     const float k = 1.5957691216057308f;      // 2 sqrt(2 / pi)
     const float g2 = g * g;
     z = k * g * fmaf(0.044715f, g2, 1.0f);
-    if (kGrad) dz = k * fmaf(3.0f * 0.044715f, g2, 1.0f);
+    if (kGrad) dz = k * fmaf(3.0f * 0.044715f, fminf(g2, 1e30f), 1.0f);   // finite: 0 times it stays 0
   }
   const float s = sigmoid_f(z);
-  // act' = s + g s (1 - s) z'; far from 0 (1 - s) s underflows before z' overflows
+  // act' = s + g s (1 - s) z'; far from 0 (1 - s) or s is 0
   if (kGrad) d = s + (g * s) * ((1.0f - s) * dz);
   return g * s;
 }
 
-// Projections kept for the backward pass: 16 bits, 1 sign, 6 exponent, 9 mantissa (values 2^-31 to 2^32, zero
-// below, the largest above, all ones for NaN and infinity).  As bf16 their rounding, 2^-9 of the value in
-// the mean of a step's ends, would be as large as that of dg and du themselves and show in every
-// gradient (weight gradients 3.5e-3 from 64 bits against 2.4e-3); projections span no 2^63.
+// Projections kept for the backward pass in 16 bits: a sign and the place of the value among those with 9 bits of
+// mantissa from 2^-20 to 2^16 and 6 bits below and above, over the whole range of fp32 (all ones for NaN and
+// infinity).  As bf16 their rounding, 2^-9 of the value in the mean of a step's ends, would be as large as that of
+// dg and du themselves and show in every gradient (weight gradients 3.5e-3 from 64 bits against 2.4e-3).
+constexpr uint32_t kFine0 = 107u << 23, kFine1 = 143u << 23;      // 2^-20 and 2^16 as bits
+constexpr uint32_t kCode0 = kFine0 >> 17, kCode1 = kCode0 + ((kFine1 - kFine0) >> 14);   // their codes
+constexpr uint32_t kLow = (kFine0 >> 14) - kCode0, kHigh = kCode1 - (kFine1 >> 17);      // codes are cut bits -+ these
 __device__ __forceinline__ uint32_t keep16(float v) {
   const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
-  int t = (int)((m + 0x1fffu + ((m >> 14) & 1u)) >> 14) - (96 << 9);
-  t = min(max(t, 0), 0x7ffe);
-  t = m >= 0x7f800000u ? 0x7fff : t;
-  return ((b >> 16) & 0x8000u) | (uint32_t)t;
+  const bool fine = m - kFine0 < kFine1 - kFine0;
+  const uint32_t near = (m + 0x1fffu + ((m >> 14) & 1u)) >> 14, far = (m + 0xffffu + ((m >> 17) & 1u)) >> 17;
+  uint32_t t = fine ? near - kLow : far + (m >= kFine1 ? kHigh : 0u);
+  t = m >= 0x7f800000u ? 0x7fffu : min(t, (0x7f800000u >> 17) + kHigh - 1u);   // the largest stay finite
+  return ((b >> 16) & 0x8000u) | t;
 }
 __device__ __forceinline__ float kept(uint32_t c) {       // 16 bits
   const uint32_t t = c & 0x7fffu;
-  const uint32_t m = t == 0 ? 0u : t == 0x7fffu ? 0x7fc00000u : (t + (96u << 9)) << 14;
+  uint32_t m = t < kCode0 ? t << 17 : t < kCode1 ? (t + kLow) << 14 : (t - kHigh) << 17;
+  m = t == 0x7fffu ? 0x7fc00000u : m;
   return __uint_as_float(m | ((c & 0x8000u) << 16));
 }
 struct AsBf16 {
