@@ -20,6 +20,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import ops
@@ -36,6 +37,20 @@ def _fused(*ts) -> bool:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         return False
     return True
+
+
+def transformed(*ts) -> bool:
+    """Whether a forward-mode derivative or a torch.func transform runs: the kernels know neither, so such calls
+    take elementary operations."""
+    if torch._C._functorch.peek_interpreter_stack() is not None:
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
+def fused(*ts) -> bool:
+    """:func:`_fused` calls that no transform of torch's watches either."""
+    return _fused(*ts) and not transformed(*ts)
 
 
 def _grad_cuda(*ts) -> bool:
@@ -299,10 +314,14 @@ def qk_norm_rope_packed(qkv, wq, wk, pos, freqs, num_heads: int, eps: float):
     return q.reshape(B, n, num_heads, D), k.reshape(B, n, num_heads, D), v.reshape(B, n, num_heads, D)
 
 
+def _rope_kernel(*ts) -> bool:
+    return all(t.is_cuda and t.dtype in (_BF16, torch.float16, torch.float32) for t in ts) and not transformed(*ts)
+
+
 def apply_rope(x, pos, freqs):
     """x [B,n,H,D] rotated at (t, h, w) positions [n,3]: fp32 on the CPU, on the rotary kernel in x's own
     type on the GPU (heads without q/k norm, forward and backward)."""
-    if not x.is_cuda or x.dtype not in (_BF16, torch.float16, torch.float32):
+    if not _rope_kernel(x):
         return ref.apply_rope(x, pos, freqs)
     return rotary(x, None, pos.to(x.device), ops.rope_cos_sin(freqs, x.device), "interleaved",
                   ref.rope_split(x.shape[-1]))[0]
@@ -328,14 +347,12 @@ class _RotaryFn(torch.autograd.Function):
 def rotary(q, k, pos, table, layout: str = "half", sections=None, inverse: bool = False):
     """Rotary positions of q and k (k may be None; see :func:`ops.rotary`), under autograd too (a table with a
     gradient takes elementary operations)."""
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, table))):
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, table))) and not (
+            transformed(q, k, table)):
         return ops.rotary(q, k, pos, table, layout, sections, inverse)
-    if q.is_cuda and not table.requires_grad:
+    if q.is_cuda and not table.requires_grad and not transformed(q, k):
         return _RotaryFn.apply(q, k, pos, table, layout, sections, inverse)
-    with torch.no_grad():
-        ops.rotary(q, k, pos, table, layout, sections)                # the same refusals
-    p = pos[:, None] if pos.dim() == 1 else pos
-    s = [table.shape[1]] if sections is None else list(sections)
+    _, p, s = ops.check_rotary(q, k, pos, table, layout, sections)
     return tuple(None if t is None else ref.rotary(t, p, table, layout, s, inverse) for t in (q, k))
 
 
@@ -409,7 +426,7 @@ def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=No
     of a shared key head is the sum over its query heads.  ``rel_bias`` has no gradient and allows
     none: with it, call without autograd.  First derivatives only."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    if not q.is_cuda:
+    if not q.is_cuda or transformed(q, k, v, rel_bias):
         ops.packed.check_packed(q, k, v, pack, rel_bias, scale=scale)
         return ref.packed_attention(q, k, v, pack, causal, scale, rel_bias)[0]
     if _fused(q, k, v, rel_bias):
@@ -475,7 +492,7 @@ def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
     """``(act(x W_gate^T) * (x W_up^T)) W_down^T`` (see :func:`ops.gated_ffn`), under autograd too; bf16 on
     the GPU, where gradients come in their tensor's type.  First derivatives only.  The projections are kept
     for them in 16 bits, within 2^-10 of values from 2^-20 to 2^16 and 2^-7 of smaller and larger ones."""
-    if not x.is_cuda:
+    if not x.is_cuda or transformed(x, w_gate, w_up, w_down):
         ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
         return ref.gated_ffn(x, w_gate, w_up, w_down, act)
     if _fused(x, w_gate, w_up, w_down):

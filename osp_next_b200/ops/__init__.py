@@ -18,7 +18,7 @@ from .fp8 import (Fp8Tensor, adamw8_decode, adamw8_state, adamw_multi_, fp8_matm
                   fp8_quantize_with_sums)
 from .gated import gated_ffn, gated_linear  # noqa: F401
 from .packed import SequencePack, packed_attention, packed_attention_bwd  # noqa: F401
-from .rotary import rotary, rotary_angles, rotary_table  # noqa: F401
+from .rotary import check_rotary, rotary, rotary_angles, rotary_table  # noqa: F401
 
 _BF16 = torch.bfloat16
 

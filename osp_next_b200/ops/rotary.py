@@ -98,16 +98,16 @@ def rotary(q, k, pos, table, layout: str = "half", sections: Optional[Sequence[i
                                          inverse)
                 return out[0], out[1] if k is not None else None
         except (RuntimeError, TypeError):
-            _check(q, k, pos, table, layout, sections)
+            check_rotary(q, k, pos, table, layout, sections)
             raise
-    ts, pos, sections = _check(q, k, pos, table, layout, sections)
+    ts, pos, sections = check_rotary(q, k, pos, table, layout, sections)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (*ts, table)):
         raise RuntimeError("rotary has no gradient here: use models.functional.rotary, or torch.no_grad()")
     out = [ref.rotary(t, pos, table, layout, sections, inverse) for t in ts]
     return out[0], out[1] if k is not None else None
 
 
-def _check(q, k, pos, table, layout, sections):
+def check_rotary(q, k, pos, table, layout, sections):
     """Raise for arguments that do not fit each other; (tensors, pos [n, axes], sections)."""
     ts = [t for t in (q, k) if t is not None]
     if layout not in LAYOUTS:

@@ -217,3 +217,50 @@ def test_gpu_backbone_in_other_types_and_heads():
         got = m.model(input_ids=ids.cuda(), attention_mask=mask.cuda()).last_hidden_state.cpu()
         assert ops._ext.launch_count() == n0
     assert (got - want)[mask > 0].norm() <= 2 * 200 * 2.0 ** -24 * want[mask > 0].norm()
+
+
+def _tangents(f, x, t):
+    from torch.autograd import forward_ad as fw
+    with torch.no_grad(), fw.dual_level():
+        return fw.unpack_dual(f(fw.make_dual(x, t))).tangent
+
+
+@gpu
+@pytest.mark.parametrize("how", ["forward_mode", "jvp", "vmap"])
+def test_gpu_transforms_of_t5_feed_forward(how):
+    """What torch does with the modules one by one it does with the block: derivatives forward, over a batch of
+    calls and of derivatives.  bf16: some four roundings a value on either side."""
+    torch.manual_seed(0)
+    ffn = t5.T5FeedForward(64, 136, 0.0).eval().requires_grad_(False).to("cuda", torch.bfloat16)
+    x, t = (torch.randn(5, 64, device="cuda").bfloat16() for _ in range(2))
+
+    def parts(z):
+        return ffn.fc2(ffn.fc1(z) * ffn.gate(z))
+
+    def result(f):
+        if how == "forward_mode":
+            return _tangents(f, x, t)
+        if how == "jvp":
+            return torch.func.jvp(f, (x,), (t,))[1]
+        if how == "vmap":
+            return torch.func.vmap(f)(x)
+        leaf = x.clone().requires_grad_(True)
+        g, = torch.autograd.grad(f(leaf), leaf, t, create_graph=True)
+        return torch.autograd.grad(g, leaf, x)[0]
+    got, want = result(ffn), result(parts)
+    assert got is not None and (got.float() - want.float()).norm() <= 8 * 2.0 ** -8 * want.float().norm()
+
+
+@gpu
+def test_gpu_operators_under_transforms():
+    """No tangent is dropped by the operators of the language models."""
+    from osp_next_b200.models import functional as Fn
+    pack, table = ops.SequencePack([3, 17]), ops.rotary_table(16, 20)
+    pos = torch.arange(20, device="cuda")
+    g = torch.Generator("cuda").manual_seed(1)
+    x, t = (torch.randn(20, 2, 16, generator=g, device="cuda") for _ in range(2))
+    w = [torch.randn(*s, generator=g, device="cuda") for s in ((40, 16), (40, 16), (16, 40))]
+    for f in (lambda z: Fn.rotary(z, None, pos, table)[0], lambda z: Fn.packed_attention(z, z, z, pack),
+              lambda z: Fn.gated_ffn(z, *w)):
+        got = _tangents(f, x, t)
+        assert got is not None and torch.allclose(torch.func.jvp(f, (x,), (t,))[1], got, atol=1e-4)
