@@ -319,12 +319,19 @@ def _rope_kernel(*ts) -> bool:
 
 
 def apply_rope(x, pos, freqs):
-    """x [B,n,H,D] rotated at (t, h, w) positions [n,3]: fp32 on the CPU, on the rotary kernel in x's own
-    type on the GPU (heads without q/k norm, forward and backward)."""
+    """x [B,n,H,D] rotated at (t, h, w) positions [n,3], in fp32 (on the rotary kernel on the GPU)."""
     if not _rope_kernel(x):
         return ref.apply_rope(x, pos, freqs)
-    return rotary(x, None, pos.to(x.device), ops.rope_cos_sin(freqs, x.device), "interleaved",
+    return rotary(x.float(), None, pos.to(x.device), ops.rope_cos_sin(freqs, x.device), "interleaved",
                   ref.rope_split(x.shape[-1]))[0]
+
+
+def apply_rope_qk(q, k, pos, freqs):
+    """:func:`apply_rope` of heads without q/k norm in one launch, forward and backward; in q's own type on the
+    GPU, which spares the rounding of fp32 results."""
+    if not _rope_kernel(q, k) or q.dtype != k.dtype:
+        return apply_rope(q, pos, freqs), apply_rope(k, pos, freqs)
+    return rotary(q, k, pos.to(q.device), ops.rope_cos_sin(freqs, q.device), "interleaved", ref.rope_split(q.shape[-1]))
 
 
 class _RotaryFn(torch.autograd.Function):

@@ -168,8 +168,7 @@ class OSPNextSelfAttention(nn.Module):
         q = self.norm_q(_lin(self.q, x)).view(B, n, H, D)
         k = self.norm_k(_lin(self.k, x)).view(B, n, H, D)
         v = _lin(self.v, x).view(B, n, H, D)
-        q = Fn.apply_rope(q, ctx.pos, ctx.freqs)
-        k = Fn.apply_rope(k, ctx.pos, ctx.freqs)
+        q, k = Fn.apply_rope_qk(q, k, ctx.pos, ctx.freqs)
         dt = torch.bfloat16 if x.is_cuda else v.dtype
         return q.to(dt), k.to(dt), v.to(dt)
 

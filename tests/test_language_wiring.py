@@ -252,6 +252,25 @@ def test_gpu_transforms_of_t5_feed_forward(how):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gpu_apply_rope_is_fp32(dtype):
+    """The DiT's rotation gives fp32 whatever x is, on both devices, and takes part in torch's transforms."""
+    from osp_next_b200.models import functional as Fn
+    from osp_next_b200.ops import reference as ref
+    pos, freqs = torch.randint(0, 60, (50, 3), device="cuda"), ref.rope_freqs(64).cuda()
+    x, t = (torch.randn(2, 50, 3, 64, device="cuda").to(dtype) for _ in range(2))
+    want = ref.apply_rope(x, pos, freqs)
+    got = Fn.apply_rope(x, pos, freqs)
+    # angles to 60 in fp32 on one side: half a step of 2^-18 each
+    assert got.dtype == want.dtype == torch.float32 and torch.allclose(got, want, atol=5e-5)
+
+    def f(z):
+        return Fn.apply_rope(z, pos, freqs)
+    assert torch.allclose(_tangents(f, x, t), ref.apply_rope(t, pos, freqs), atol=5e-5)
+    assert torch.allclose(torch.func.vmap(f)(x[:, None])[:, 0], want, atol=5e-5)
+
+
+@gpu
 def test_gpu_operators_under_transforms():
     """No tangent is dropped by the operators of the language models."""
     from osp_next_b200.models import functional as Fn
