@@ -23,6 +23,7 @@ import torch.nn.functional as F
 
 from . import functional as Fn
 from ..ops import SequencePack
+from ..ops import reference as ref
 
 
 class T5LayerNorm(nn.Module):
@@ -74,6 +75,10 @@ class T5RelativeEmbedding(nn.Module):
         return self.embedding(b).t().float().contiguous()
 
 
+def _kernel_heads(dim: int) -> bool:
+    return dim % 8 == 0 and dim <= 128
+
+
 class T5Attention(nn.Module):
     def __init__(self, dim, dim_attn, num_heads, dropout=0.1):
         super().__init__()
@@ -87,7 +92,13 @@ class T5Attention(nn.Module):
     def forward(self, x, context=None, mask=None, pos_bias=None, pack=None):
         if pack is not None:        # packed rows [N, dim], pos_bias [heads, 2 M - 1] by relative position
             q, k, v = (m(x).unflatten(-1, (self.num_heads, self.head_dim)) for m in (self.q, self.k, self.v))
-            o = Fn.packed_attention(q, k, v, pack, causal=False, scale=1.0, rel_bias=pos_bias)
+            # the kernel for bf16 without a gradient; elementary operations in the model's own type otherwise
+            if Fn.fused(q, k, v, pos_bias) and q.dtype == torch.bfloat16 and _kernel_heads(self.head_dim):
+                o = Fn.packed_attention(q, k, v, pack, causal=False, scale=1.0, rel_bias=pos_bias)
+            else:
+                if q.shape[0] < pack.rows:
+                    raise ValueError(f"T5Attention: the pack needs {pack.rows} rows, got {q.shape[0]}")
+                o = ref.packed_attention(q, k, v, pack, False, 1.0, pos_bias)[0]
             return self.dropout(self.o(o.to(x.dtype).flatten(1)))
         ctx = x if context is None else context
         b, n, c = x.size(0), self.num_heads, self.head_dim
@@ -267,7 +278,7 @@ class T5EncoderModel:
     def _packs(self) -> bool:
         """Whether the packed kernels take this encoder: bf16, heads of a multiple of 8 up to 128."""
         attn = next((m for m in self.model.modules() if isinstance(m, T5Attention)), None)
-        return (attn is not None and attn.head_dim % 8 == 0 and attn.head_dim <= 128
+        return (attn is not None and _kernel_heads(attn.head_dim)
                 and self.model.token_embedding.weight.dtype == torch.bfloat16)
 
     def _encode_packed(self, ids, real, lengths):

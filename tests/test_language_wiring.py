@@ -219,6 +219,45 @@ def test_gpu_backbone_in_other_types_and_heads():
     assert (got - want)[mask > 0].norm() <= 2 * 200 * 2.0 ** -24 * want[mask > 0].norm()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype,dim,grad", [(torch.float32, 64, False), (torch.float32, 64, True), (torch.bfloat16, 64, True),
+                                            (torch.float32, 48, False)])
+def test_t5_packed_in_other_types_and_under_autograd(device, dtype, dim, grad):
+    """Packed prompts in a type, with heads or gradients that the packed kernel does not take: elementary
+    operations in the model's type, here against 64 bits.  Bounds: two layers of some ten roundings on a path, half
+    a step each, were none to cancel, with sums of some 100 terms in fp32 (2^-24 each) in the place of bf16's
+    steps for fp32."""
+    cfg = dict(vocab=100, dim=dim, dim_attn=dim, dim_ffn=136, num_heads=4, num_layers=2, num_buckets=32, dropout=0.0,
+               shared_pos=True)
+    torch.manual_seed(0)
+    enc = t5.T5Encoder(**cfg).eval().to(dtype)
+    plain = t5.T5Encoder(**cfg).eval()
+    plain.load_state_dict({k: v.float() for k, v in enc.state_dict().items()})
+    enc, plain = enc.to(device), plain.double().to(device)
+    lengths = [20, 1, 33, 0]
+    ids = torch.randint(1, 100, (sum(lengths),), generator=torch.Generator().manual_seed(3)).to(device)
+    pack = ops.SequencePack(lengths, device=device)
+    out = []
+    for m in (enc, plain):
+        with torch.set_grad_enabled(grad):
+            y, at = [], 0
+            if m is enc:
+                y = m(ids, pack=pack)
+            else:
+                for n in lengths[:3]:
+                    y.append(m(ids[None, at:at + n], torch.ones(1, n, device=device))[0])
+                    at += n
+                y = torch.cat(y)
+            out.append([y.detach().double()])
+            if grad:
+                # squares would cancel: rows leave a norm with the same sum of them
+                (y * torch.linspace(-1, 1, y.numel(), device=device).view(y.shape).to(y.dtype)).sum().backward()
+                out[-1] += [p.grad.double() for p in m.parameters()]
+    bound = 2 * 10 * (2.0 ** -8 if dtype == torch.bfloat16 else 100 * 2.0 ** -24) * (4 if grad else 1)
+    for a, b in zip(*out):
+        assert (a - b).norm() <= bound * b.norm()
+
+
 def _tangents(f, x, t):
     from torch.autograd import forward_ad as fw
     with torch.no_grad(), fw.dual_level():
