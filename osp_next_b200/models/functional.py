@@ -473,14 +473,19 @@ class _GatedFFNFn(torch.autograd.Function):
             out = ops.ext().gated_ffn_fwd(x2, g, u, d, code, True)
             out[0] = out[0][:, :wd.shape[0]].reshape(*x.shape[:-1], wd.shape[0])
         y, x2, gu = out
-        ctx.save_for_backward(x2, g, u, d, gu)
+        ctx.save_for_backward(x2, g, u, d, gu, x, wg, wu, wd)
         ctx.meta = (x.shape, x.dtype, wg.shape, wg.dtype, wu.dtype, wd.shape, wd.dtype, code)
+        ctx.act = act
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gy):
-        x2, wg, wu, wd, gu = ctx.saved_tensors
+        x2, wg, wu, wd, gu, *own = ctx.saved_tensors
+        if torch.is_grad_enabled():                       # for second derivatives: elementary operations in fp32
+            ask = [t for t, need in zip(own, ctx.needs_input_grad) if need]
+            y = ref.gated_ffn(own[0].float(), *own[1:], ctx.act)
+            grads = iter(torch.autograd.grad(y, ask, gy.float(), create_graph=True))
+            return (*(next(grads) if need else None for need in ctx.needs_input_grad[:4]), None)
         xshape, xdt, wshape, gdt, udt, dshape, ddt, act = ctx.meta
         f, k = wshape
         c = dshape[0]
@@ -497,7 +502,7 @@ class _GatedFFNFn(torch.autograd.Function):
 
 def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
     """``(act(x W_gate^T) * (x W_up^T)) W_down^T`` (see :func:`ops.gated_ffn`), under autograd too; bf16 on
-    the GPU, where gradients come in their tensor's type.  First derivatives only.  The projections are kept
+    the GPU, where gradients come in their tensor's type (second derivatives by elementary operations).  The projections are kept
     for them in 16 bits, within 2^-10 of values from 2^-20 to 2^16 and 2^-7 of smaller and larger ones."""
     if not x.is_cuda or transformed(x, w_gate, w_up, w_down):
         ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")

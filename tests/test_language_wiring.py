@@ -265,7 +265,7 @@ def _tangents(f, x, t):
 
 
 @gpu
-@pytest.mark.parametrize("how", ["forward_mode", "jvp", "vmap"])
+@pytest.mark.parametrize("how", ["forward_mode", "jvp", "vmap", "double"])
 def test_gpu_transforms_of_t5_feed_forward(how):
     """What torch does with the modules one by one it does with the block: derivatives forward, over a batch of
     calls and of derivatives.  bf16: some four roundings a value on either side."""
