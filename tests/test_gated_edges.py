@@ -87,3 +87,39 @@ def test_gpu_kept_projections_at_their_ends():
         close(dwd.diagonal(), (a, err + 2.0 ** -126), "h")
         close(dwg[:, 0], (d, torch.where(g.abs() > 200, 0.0, CURVE * kept(g)) + 2.0 ** -16 + HALF * d.abs()), "act'")
     ops.check_device_errors()
+
+
+def _kernels(f):
+    """Names of the block's kernels that a call launches."""
+    from torch.profiler import ProfilerActivity, profile
+    f()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        f()
+        torch.cuda.synchronize()
+    return [e.name for e in p.events() if "osp::ffn::" in e.name]
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("M,K,F,C", [(2499, 2056, 2312, 2064), (5003, 776, 1032, 1160)])
+def test_gpu_tiled_form(act, M, K, F, C):
+    """Every product in whole tiles, with several blocks along K and ragged last tiles: values, all gradients,
+    and gradients of fp32 leaves."""
+    from test_gated_rotary import ffn_oracle
+    x, wg, wu, wd, dy = ffn_tensors(M, K, F, C)
+    want = ffn_oracle(x, wg, wu, wd, act, dy)
+    close(ops.gated_linear(x, wg, wu, act), want["h"], "h")
+    close(ops.gated_ffn(x, wg, wu, wd, act), want["y"], "y")
+    for dtype in (torch.bfloat16, torch.float32):
+        leaves = [t.to(dtype).requires_grad_(True) for t in (x, wg, wu, wd)]
+
+        def step():
+            return torch.autograd.grad(Fn.gated_ffn(*leaves, act=act), leaves, dy)
+        if torch.cuda.get_device_properties(0).multi_processor_count <= 148:
+            names = _kernels(step)
+            assert len(names) == 6 and all("::gemm<" in n for n in names), names
+        for got, n in zip(step(), ("dx", "dwg", "dwu", "dwd")):
+            assert got.dtype == dtype
+            close(got, want[n], n)
+    ops.check_device_errors()

@@ -137,3 +137,13 @@ def test_waits_of_the_forward_kernel_are_bounded():
     assert kernel.count("__syncthreads()") == 2
     roles = kernel[kernel.index("if (warp == L::kProdWarp) {\n    // ---"):kernel.rindex("__syncthreads()")]
     assert "__syncthreads" not in roles and "return;" not in roles
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 128), (6, 2, 80), (3, 1, 72), (2, 2, 120), (4, 2, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_gpu_bias_with_other_heads(heads, kv, dim, causal, tiles):  # noqa: F811
+    for lengths, keys in (([77, 1, 300], None), ([3, 130], [700, 131]), ([2], [3000])):
+        pack = ops.SequencePack(lengths, keys)
+        bias = torch.randn(heads, 2 * pack.longest + 5, generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+        _pass(pack, heads, kv, dim, causal, bias=bias, train=False, scale=0.05)
