@@ -276,7 +276,10 @@ class T5EncoderModel:
         return out
 
     def _packs(self) -> bool:
-        """Whether the packed kernels take this encoder: bf16, heads of a multiple of 8 up to 128."""
+        """Whether the packed kernels take this encoder: a T5Encoder (no wrapper or encoder of the caller's, which may
+        know ids and mask alone) in bf16 with heads of a multiple of 8 up to 128."""
+        if not isinstance(self.model, T5Encoder):
+            return False
         attn = next((m for m in self.model.modules() if isinstance(m, T5Attention)), None)
         return (attn is not None and _kernel_heads(attn.head_dim)
                 and self.model.token_embedding.weight.dtype == torch.bfloat16)

@@ -322,3 +322,38 @@ def test_gpu_operators_under_transforms():
               lambda z: Fn.gated_ffn(z, *w)):
         got = _tangents(f, x, t)
         assert got is not None and torch.allclose(torch.func.jvp(f, (x,), (t,))[1], got, atol=1e-4)
+
+
+class _Wrapped(torch.nn.Module):
+    """What a caller's shard function or another encoder may be: ids and mask in, [B, L, dim] out."""
+
+    def __init__(self, encoder):
+        super().__init__()
+        self.module = encoder
+
+    def forward(self, ids, mask):
+        return self.module(ids, mask)
+
+
+def _wraps(device, dtype):
+    torch.manual_seed(0)
+    cfg = dict(vocab=100, dim=64, dim_attn=64, dim_ffn=136, num_heads=4, num_layers=1, num_buckets=32, dropout=0.0)
+    enc = t5.T5Encoder(**cfg)
+    ids = torch.randint(1, 100, (2, 20), generator=torch.Generator().manual_seed(3))
+    mask = (torch.arange(20)[None] < torch.tensor([20, 3])[:, None]).long()
+    out = [t5.T5EncoderModel(text_len=24, dtype=dtype, device=device, encoder=enc, shard_fn=f)
+           for f in (None, lambda m: _Wrapped(m).to(device, dtype))]
+    assert not out[1]._packs()
+    return [m(ids, mask).float() for m in out]
+
+
+def test_prompt_encoder_with_a_wrapped_encoder():
+    a, b = _wraps("cpu", torch.float32)
+    assert torch.allclose(a, b, atol=1e-6)
+
+
+@gpu
+def test_gpu_prompt_encoder_with_a_wrapped_encoder():
+    """Packed and padded: one layer of some ten roundings to bf16, none cancelled."""
+    a, b = _wraps("cuda", torch.bfloat16)
+    assert (a - b).norm() <= 10 * 2.0 ** -8 * b.norm()
