@@ -382,9 +382,12 @@ def _silu_types():
     return (nn.SiLU, type(ACT2FN["silu"]))
 
 
-def _kernels_fit(config) -> bool:
-    """Whether the packed kernel takes the text layers' heads."""
-    c = getattr(config, "text_config", config)
+def _kernels_fit(vl) -> bool:
+    """Whether a backbone has text layers where :meth:`VideoAlignRewardModel.use_kernels` looks for them, with heads
+    that the packed kernel takes."""
+    c = getattr(vl.config, "text_config", None)
+    if c is None or not hasattr(getattr(vl, "model", None), "language_model"):
+        return False
     dim = getattr(c, "head_dim", None) or c.hidden_size // c.num_attention_heads
     return dim % 8 == 0 and dim <= 128 and not getattr(c, "use_sliding_window", False)
 
@@ -420,7 +423,7 @@ class VideoAlignRewardModel(nn.Module):
     def use_kernels(self):
         """Text attention on the packed kernel (padding costs nothing: rows are packed by the mask) and
         SiLU-gated MLPs without biases on the gated feed-forward kernels, for models in bf16 on the GPU; what
-        these do not take runs as before."""
+        these do not take runs as before.  Hidden states of padding are other values than the library's."""
         from transformers import AttentionInterface, AttentionMaskInterface
         AttentionInterface.register(ATTENTION_NAME, _packed_attention)
         AttentionMaskInterface.register(ATTENTION_NAME, _packed_mask)
@@ -516,7 +519,7 @@ class VideoAlignScorer:
         scale = a / math.sqrt(r) if self.cfg.use_rslora else a / r
         model.load_checkpoint_tensors(merge_training_state(model.state_dict_for_checkpoint(), tensors, scale))
         self.model = model.to(device=device, dtype=dtype).eval()
-        if torch.device(device).type == "cuda" and dtype == torch.bfloat16 and _kernels_fit(vl_model.config):
+        if torch.device(device).type == "cuda" and dtype == torch.bfloat16 and _kernels_fit(vl_model):
             self.model.use_kernels()
 
     def normalise(self, scores: Dict[str, float]) -> Dict[str, float]:

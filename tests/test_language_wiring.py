@@ -357,3 +357,42 @@ def test_gpu_prompt_encoder_with_a_wrapped_encoder():
     """Packed and padded: one layer of some ten roundings to bf16, none cancelled."""
     a, b = _wraps("cuda", torch.bfloat16)
     assert (a - b).norm() <= 10 * 2.0 ** -8 * b.norm()
+
+
+def test_kernels_fit_the_backbones_that_have_their_layers():
+    import types
+    vl = _tiny_vl()
+    assert va._kernels_fit(vl)
+    text = vl.config.text_config
+    for other in (types.SimpleNamespace(config=vl.config),                                  # no text layers found
+                  types.SimpleNamespace(config=vl.config, model=types.SimpleNamespace()),
+                  types.SimpleNamespace(config=text, model=vl.model),                       # no text config
+                  types.SimpleNamespace(config=types.SimpleNamespace(), model=vl.model)):
+        assert not va._kernels_fit(other)
+    text.use_sliding_window = True
+    assert not va._kernels_fit(vl)
+    text.use_sliding_window, text.head_dim = False, 12
+    assert not va._kernels_fit(vl)
+
+
+@gpu
+@pytest.mark.parametrize("side", ["left", "holes"])
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_gpu_backbone_recomputed_in_the_backward_pass(side, reentrant):
+    """The same gradients with and without recomputation: kernels and library repeat themselves."""
+    ids, mask = (t.cuda() for t in _batch(side))
+    grads = []
+    for recompute in (False, True):
+        m = va.VideoAlignRewardModel(_tiny_vl().bfloat16(), output_dim=1, reward_token="last").cuda().use_kernels().vl
+        if recompute:
+            m.gradient_checkpointing_enable({"use_reentrant": reentrant})
+            m.train()
+        x = m.get_input_embeddings()(ids).detach().requires_grad_(True)
+        h = m.model(inputs_embeds=x, attention_mask=mask, use_cache=False,
+                    position_ids=torch.arange(ids.shape[1], device="cuda").expand(3, *ids.shape)).last_hidden_state
+        (h[mask > 0] * torch.linspace(-1, 1, 64, device="cuda").bfloat16()).sum().backward()
+        grads.append([x.grad, *(p.grad for p in m.parameters() if p.grad is not None)])
+    assert len(grads[0]) == len(grads[1]) and torch.isfinite(grads[0][0]).all() and grads[0][0].any()
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+    ops.check_device_errors()
