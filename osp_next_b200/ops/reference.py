@@ -417,11 +417,12 @@ def gated_ffn(x, w_gate, w_up, w_down, act: str):
 
 def rotary(x, pos, table, layout: str, sections, inverse: bool = False):
     """x [..., n, H, D] rotated by table [positions, pairs, 2] at pos [n, axes]; differentiable."""
+    pos = pos.long()
     if pos.numel() and (int(pos.min()) < 0 or int(pos.max()) >= table.shape[0]):
         raise IndexError(f"rotary: positions 0 to {table.shape[0] - 1}, got {int(pos.min())} to {int(pos.max())}")
     axis = torch.repeat_interleave(torch.tensor(sections, device=pos.device))
     pair = torch.arange(table.shape[1], device=pos.device)
-    cs = table[pos.long()[:, axis], pair[None]]                                     # [n, pairs, 2]
+    cs = table[pos[:, axis], pair[None]]                                     # [n, pairs, 2]
     acc = torch.float64 if x.dtype == torch.float64 else torch.float32
     c, s = cs[:, None, :, 0].to(acc), cs[:, None, :, 1].to(acc)
     s = -s if inverse else s

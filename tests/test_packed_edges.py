@@ -147,3 +147,20 @@ def test_gpu_bias_with_other_heads(heads, kv, dim, causal, tiles):  # noqa: F811
         pack = ops.SequencePack(lengths, keys)
         bias = torch.randn(heads, 2 * pack.longest + 5, generator=torch.Generator("cuda").manual_seed(3), device="cuda")
         _pass(pack, heads, kv, dim, causal, bias=bias, train=False, scale=0.05)
+
+
+@gpu
+def test_gpu_pack_first_used_in_inference_mode():
+    """Work lists laid out in inference mode serve calls under autograd and captured ones."""
+    with torch.inference_mode():
+        pack = ops.SequencePack([100, 7])
+        q, k, v, do = tensors(pack, 4, 2, 64, "cuda")
+        want = ops.packed_attention(q, k, v, pack)
+        ops.packed_attention_bwd(q, k, v, want, do, torch.zeros(107, 4, device="cuda"), pack)
+    q, k, v, do = (t.clone() for t in (q, k, v, do))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = Fn.packed_attention(*leaves, pack)
+    grads = torch.autograd.grad(out, leaves, do)
+    fresh = ops.SequencePack([100, 7])
+    again = torch.autograd.grad(Fn.packed_attention(*leaves, fresh), leaves, do)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, again))

@@ -120,3 +120,16 @@ def test_gpu_inverse_and_second_derivatives_are_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, step(*static)))
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.uint16, torch.uint32,
+                                   torch.uint64])
+def test_types_of_positions(dtype):
+    table = ops.rotary_table(8, 100, device="cpu")
+    q, pos = torch.randn(3, 2, 8), torch.tensor([0, 99, 3])
+    assert torch.equal(ops.rotary(q, None, pos.to(dtype), table)[0], ops.rotary(q, None, pos, table)[0])
+    if dtype.is_signed:
+        with pytest.raises(IndexError, match="positions 0 to 99"):
+            ops.rotary(q, None, torch.tensor([0, -1, 3], dtype=dtype), table)
+    with pytest.raises(IndexError, match="positions 0 to 99"):
+        ops.rotary(q, None, torch.tensor([0, 100, 3], dtype=dtype), table)
