@@ -39,10 +39,15 @@ def _fused(*ts) -> bool:
     return True
 
 
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
 def transformed(*ts) -> bool:
-    """Whether a forward-mode derivative or a torch.func transform runs: the kernels know neither, so such calls
-    take elementary operations."""
-    if torch._C._functorch.peek_interpreter_stack() is not None:
+    """Whether a forward-mode derivative, a torch.func transform or a trace runs, or a tensor is of a class of its
+    own (without data, distributed): the kernels know none of these, so such calls take elementary operations."""
+    if torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None:
+        return True
+    if any(t is not None and type(t) not in _TENSORS for t in ts):
         return True
     return forward_ad._current_level >= 0 and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
@@ -445,10 +450,16 @@ def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=No
 
 # ----------------------------------------------------------------------------- gated feed-forward
 
+def computes_bf16(x) -> bool:
+    """Whether a Linear layer with weights in bf16 would compute x in bf16 on the GPU (autocast may say otherwise)."""
+    return x.is_cuda and x.dtype == _BF16 and not (
+        torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != _BF16)
+
+
 def as_made(m, cls) -> bool:
     """Whether a layer computes what its class does: that class itself (no adapter, no quantised or
     parametrised form), no hooks, no forward of its own.  Its parameters may then stand for it."""
-    return (type(m) is cls and "forward" not in m.__dict__ and not m._forward_hooks and not m._forward_pre_hooks
+    return (type(m) is cls and not torch.nn.modules.module._has_any_global_hook() and "forward" not in m.__dict__ and not m._forward_hooks and not m._forward_pre_hooks
             and not m._backward_hooks and not m._backward_pre_hooks)
 
 

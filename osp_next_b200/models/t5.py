@@ -131,7 +131,7 @@ class T5FeedForward(nn.Module):
                 and self.gate[1].approximate == "tanh" and Fn.plain_linears(self.gate[0], self.fc1, self.fc2))
 
     def forward(self, x):
-        if (x.is_cuda and x.dtype == torch.bfloat16 and not (self.training and self.dropout.p > 0) and self._plain()
+        if (Fn.computes_bf16(x) and not (self.training and self.dropout.p > 0) and self._plain()
                 and not Fn.transformed(x)):
             ws = (self.gate[0].weight, self.fc1.weight, self.fc2.weight)
             if all(w.dtype == torch.bfloat16 for w in ws):

@@ -329,6 +329,8 @@ def _packed_mask(**args):
     """transformers' mask function, called once a forward: a :class:`_PackedMask` for a whole causal prompt
     whose rows are one run of tokens each; the library's mask with a cache, a window or holes."""
     from transformers.masking_utils import causal_mask_function, sdpa_mask
+    if "q_length" not in args:
+        return sdpa_mask(**args)
     B, L, m = args["batch_size"], args["q_length"], args.get("attention_mask")
     whole = args["kv_length"] == L and all(int(args.get(n, 0)) == 0 for n in ("q_offset", "kv_offset"))
     if whole and args.get("mask_function", causal_mask_function) is causal_mask_function:
@@ -366,7 +368,8 @@ def _gated_mlp(self, x):
     """A SiLU-gated MLP's forward on the gated feed-forward kernels; adapters, quantised layers and hooks that
     the layers got since, and other types than bf16 on the GPU, run as the module's own forward."""
     parts = (self.gate_proj, self.up_proj, self.down_proj)
-    if not _plain_mlp(self) or any(p.weight.dtype != x.dtype for p in parts) or (x.is_cuda and x.dtype != torch.bfloat16):
+    if (not _plain_mlp(self) or any(p.weight.dtype != x.dtype for p in parts)
+            or (x.is_cuda and not Fn.computes_bf16(x)) or Fn.transformed(x)):
         return type(self).forward(self, x)
     return Fn.gated_ffn(x, *(p.weight for p in parts), "silu").to(x.dtype)
 

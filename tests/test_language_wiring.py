@@ -396,3 +396,35 @@ def test_gpu_backbone_recomputed_in_the_backward_pass(side, reentrant):
     for a, b in zip(*grads):
         assert torch.equal(a, b)
     ops.check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("how", ["global_hook", "compiled", "fake", "autocast"])
+def test_gpu_t5_feed_forward_as_its_layers_would(how):
+    """Hooks on every module, tracing, tensors without data, and autocast to another type: what the layers do one
+    after another."""
+    torch.manual_seed(0)
+    ffn = t5.T5FeedForward(64, 136, 0.0).eval().requires_grad_(False).to("cuda", torch.bfloat16)
+    x = torch.randn(5, 64, device="cuda").bfloat16()
+    want = ffn.fc2(ffn.fc1(x) * ffn.gate(x))
+    if how == "global_hook":
+        seen = []
+        hook = torch.nn.modules.module.register_module_forward_hook(lambda m, a, y: seen.append(m))
+        try:
+            assert torch.equal(ffn(x), want)
+        finally:
+            hook.remove()
+        assert all(any(m is s for s in seen) for m in (ffn.gate[0], ffn.fc1, ffn.fc2))
+    elif how == "compiled":
+        assert torch.equal(torch.compile(ffn, backend="eager", fullgraph=True)(x), want)
+    elif how == "fake":
+        from torch._subclasses.fake_tensor import FakeTensorMode
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            y = ffn(mode.from_tensor(x))
+        assert y.shape == want.shape and y.dtype == want.dtype and y.device.type == "cuda"
+    else:
+        with torch.autocast("cuda", torch.float16):
+            got, want = ffn(x), ffn.fc2(ffn.fc1(x) * ffn.gate(x))
+        assert got.dtype == want.dtype == torch.float16 and torch.equal(got, want)
+        with torch.autocast("cuda", torch.bfloat16):
+            assert ffn(x).dtype == torch.bfloat16
