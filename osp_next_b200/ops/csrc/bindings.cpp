@@ -56,7 +56,7 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q, const at::Tensor& k
                                         const c10::optional<at::Tensor>& low, const at::Tensor& rows,
                                         const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, int64_t row_heads, int64_t key_heads, bool causal, double scale,
-                                        bool fill);
+                                        bool fill, bool two);
 std::vector<at::Tensor> gated_linear_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, int64_t act,
                                          bool keep);
 std::vector<at::Tensor> gated_ffn_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,

@@ -90,6 +90,18 @@ __device__ __forceinline__ void store_pairs(uint32_t taddr, const float* v) {
   tmem_st4(taddr, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
+// What rounding those values to bf16 left, rounded in turn (kTwo).  Packs of sequences of up to 32 rows multiply dS
+// as two bf16 numbers: their dQ and dK are then off by little more than the rounding of the result, 1.8e-3 to 1.9e-3
+// from 64 bits.  With one number it is 2.5e-3, up to 2.9e-3 in a batch of few rows; longer sequences, where the
+// second product would take its time, stay at 2.4e-3 (400 samples of 16 tokens, 16 heads of 64 to 4: dK, dV 77 and
+// with two 84 us, dQ 55 and 59; with the choice made inside the kernels dK, dV over 4096 tokens took 159 for 154).
+__device__ __forceinline__ void store_rest(uint32_t taddr, const float* v) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i] - bf16_round(v[i]);
+  store_pairs(taddr, r);
+}
+
 // ---------------------------------------------------------------------------- dK, dV
 template <int D>
 struct KeySmem {
@@ -102,7 +114,7 @@ struct KeySmem {
   static constexpr int BYTES = OFF_BAR + 256 + 1024;
 };
 
-template <int D>
+template <int D, bool kTwo>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
@@ -250,6 +262,10 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           umma_bf16_ts(d, a_tmem + pair_col(k), sdesc_sw128(ya + k * 2048, L::BOX, 1024), ID_G,
                        (acc || k > 0) ? 1u : 0u);
       };
+      auto mma_rest = [&](uint32_t d, uint32_t a_tmem, uint32_t ya, int steps) {
+        for (int k = 0; k < steps; ++k)
+          umma_bf16_ts(d, a_tmem + 32u + pair_col(k), sdesc_sw128(ya + k * 2048, L::BOX, 1024), ID_G, 1u);
+      };
       auto qa = [&](int i) { return smem_u32(sStage + (i & 1) * L::STAGE); };
       auto da = [&](int i) { return smem_u32(sStage + (i & 1) * L::STAGE + L::TILE); };
       bool ok = mbar_wait(kv_full, 0, args.err, kErrAttnMma) && mbar_wait(&q_full[0], 0, args.err, kErrAttnMma);
@@ -274,6 +290,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (!(ok = mbar_wait(ds_full, i & 1, args.err, kErrAttnMma))) break;
         tc_fence_after();
         mma_ts(tDK, tDP, qa(i), i > 0);
+        if (kTwo) mma_rest(tDK, tDP, qa(i), (min(P, it.n_q - i * P) * G + 15) / 16);
         umma_commit(&q_empty[i & 1]);
         if (more) {
           mma_nt(tDP, va, da(i + 1));
@@ -332,6 +349,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       tmem_ld32(tDP + lane_off + half * 64, sr);
       tmem_ld32(tDP + lane_off + half * 64 + 32, sr + 32);
       tmem_ld_wait();
+      const int rest = (hi + 15) / 16 * 16;                           // columns with a second number
       // a masked place is cleared by its own select: its P is 0, but 0 * NaN is not
       auto ds = [&](auto masked) {
 #pragma unroll
@@ -347,6 +365,7 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (decltype(masked)::value) g[e] = (c >= lo && c < hi) ? g[e] : 0.f;
           }
           store_pairs(tDP + lane_off + half * 64 + c8 * 4, g);
+          if (kTwo && 8 * c8 < rest) store_rest(tDP + lane_off + half * 64 + 32 + c8 * 4, g);
         }
       };
       if (full) ds(std::false_type{});
@@ -416,7 +435,7 @@ struct RowSmem {
   static constexpr int BYTES = OFF_BAR + 256 + 1024;
 };
 
-template <int D>
+template <int D, bool kTwo>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
@@ -550,6 +569,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int k = 0; k < kT / 16; ++k)
           umma_bf16_ts(tDQ, tDP + pair_col(k), sdesc_sw128(ka(j) + k * 2048, L::BOX, 1024), ID_G,
                        (j > 0 || k > 0) ? 1u : 0u);
+        if (kTwo) {
+          for (int k = 0; k < (it.n_keys + 15) / 16; ++k)
+            umma_bf16_ts(tDQ, tDP + 32u + pair_col(k), sdesc_sw128(ka(j) + k * 2048, L::BOX, 1024), ID_G, 1u);
+        }
         umma_commit(&kv_empty[j & 1]);
         if (more) {
           mma_nt(tDP, doa, va(j + 1));
@@ -573,6 +596,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const long row = (long)(it.q_row + r / G) * args.Hq + kvh * G + r % G;
     const float lse2 = in ? args.lse[row] * pa::kLog2e : 0.f;
     const float dlt = in ? args.delta[row] : 0.f;
+    const int rest = (it.n_keys + 15) / 16 * 16 - half * 64;      // columns with a second number
     bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
       const int nv = limit - j * kT - half * 64;
@@ -605,6 +629,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (decltype(masked)::value) g[e] = c < nv ? g[e] : 0.f;
           }
           store_pairs(tDP + lane_off + half * 64 + c8 * 4, g);
+          if (kTwo && 8 * c8 < rest) store_rest(tDP + lane_off + half * 64 + 32 + c8 * 4, g);
         }
       };
       if (full) ds(std::false_type{});
@@ -633,12 +658,12 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------- host
-template <int D>
+template <int D, bool kTwo>
 static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const CUtensorMap& tdo, PackedBwdArgs a, const at::Tensor& rows, const at::Tensor& keys,
                               int64_t row_heads, int64_t key_heads, cudaStream_t stream) {
   if (keys.size(0) > 0) {
-    auto kern = packed_dkdv_kernel<D>;
+    auto kern = packed_dkdv_kernel<D, kTwo>;
     smem_opt_in(reinterpret_cast<const void*>(kern), KeySmem<D>::BYTES);
     a.items = keys.data_ptr<int>();
     a.units = (int)(keys.size(0) * a.Hkv);
@@ -647,7 +672,7 @@ static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, cons
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   if (rows.size(0) > 0) {
-    auto kern = packed_dq_kernel<D>;
+    auto kern = packed_dq_kernel<D, kTwo>;
     smem_opt_in(reinterpret_cast<const void*>(kern), RowSmem<D>::BYTES);
     a.items = rows.data_ptr<int>();
     a.units = (int)(rows.size(0) * a.Hkv);
@@ -657,13 +682,14 @@ static void launch_packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, cons
   }
 }
 
-// (dq, dk, dv) bf16.  `rows`, `keys`, `joins`: work lists of ops.SequencePack on the device.
+// (dq, dk, dv) bf16.  `rows`, `keys`, `joins`: work lists of ops.SequencePack on the device; `two`: dS as two
+// numbers, for sequences of up to 32 rows.
 std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
                                         const at::Tensor& o_, const at::Tensor& dout_, const at::Tensor& lse_,
                                         const c10::optional<at::Tensor>& low,
                                         const at::Tensor& rows, const at::Tensor& keys, const at::Tensor& joins,
                                         int64_t slots, int64_t row_heads, int64_t key_heads, bool causal, double scale,
-                                        bool fill) {
+                                        bool fill, bool two) {
   TORCH_CHECK(std::abs(scale) < 1e38, "packed_attention: a finite scale");
   const at::Tensor q = pa::tma_rows(q_), k = pa::tma_rows(k_), v = pa::tma_rows(v_);
   const at::Tensor o = pa::tma_rows(o_.contiguous()), lse = lse_.contiguous();
@@ -718,8 +744,9 @@ std::vector<at::Tensor> packed_attn_bwd(const at::Tensor& q_, const at::Tensor& 
   }
   const CUtensorMap tq = pa::tile_map(q, q, s.D, s.G, a.P), tdo = pa::tile_map(dout, q, s.D, s.G, a.P);
   const CUtensorMap tk = pa::tile_map(k, q, s.D, 1, pa::kRows), tv = pa::tile_map(v, q, s.D, 1, pa::kRows);
-  if (s.D > 64) launch_packed_bwd<128>(tq, tk, tv, tdo, a, rows, keys, row_heads, key_heads, stream);
-  else launch_packed_bwd<64>(tq, tk, tv, tdo, a, rows, keys, row_heads, key_heads, stream);
+  auto launch = two ? (s.D > 64 ? launch_packed_bwd<128, true> : launch_packed_bwd<64, true>)
+                    : (s.D > 64 ? launch_packed_bwd<128, false> : launch_packed_bwd<64, false>);
+  launch(tq, tk, tv, tdo, a, rows, keys, row_heads, key_heads, stream);
   if (joins.size(0) > 0) {
     TORCH_CHECK(slots > 0, "packed_attention: joins without slots");
     packed_join_kernel<<<dim3((unsigned)joins.size(0), (unsigned)s.Hkv, 2 * kT / 8), 256, 0, stream>>>(

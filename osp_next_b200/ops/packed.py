@@ -22,6 +22,7 @@ TILE = 128             # rows of a tensor-core tile: group heads x positions, or
 _LONG_STEPS = 6        # mean key tiles of an item from which a forward CTA takes two row tiles
 _MIN_FWD_STEPS = 4     # key tiles below which splitting an item further costs more than it gives
 _MIN_KEY_STEPS = 8     # the same for the row tiles of a key tile's gradient
+_SHORT = 32            # longest sequence of a pack whose gradients' kernels multiply dS as two bf16 numbers
 
 
 def _whole(v, what: str) -> np.ndarray:
@@ -360,7 +361,8 @@ def packed_attention_bwd(q, k, v, o, dout, lse, pack: SequencePack, causal: bool
         if q.shape[0] < pack.rows or k.shape[0] < pack.key_rows:
             raise ValueError("packed_attention_bwd: fewer rows than the pack's")
         return ext().packed_attn_bwd(q, k, v, o, dout, lse, remainder, rows, keys, joins, slots, row_heads, key_heads,
-                                     bool(causal), 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), fill)
+                                     bool(causal), 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), fill,
+                                     pack.longest <= _SHORT)
     except (AttributeError, IndexError, RuntimeError, TypeError, ValueError, ZeroDivisionError):
         check_packed(q, k, v, pack, what="packed_attention_bwd", scale=scale)
         if q.dtype != torch.bfloat16:
