@@ -44,7 +44,7 @@ struct KeyItem {       // dK, dV of one tile of 128 keys
   int n_q;             // queries from there on
   int lead;            // key 0 is seen by query max(0, lead) of those, key i by query lead + i
   int slot;            // place of its partial result, or -1
-  int pad;
+  int n_keys;          // keys of the sequence
 };
 
 __device__ __forceinline__ const int4* item_ptr(const int* list, int i) {

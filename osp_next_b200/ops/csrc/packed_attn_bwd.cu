@@ -383,15 +383,15 @@ packed_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // K and V have been read for the last time: their place stages the results
     uint8_t* buf = smem + (warp - 4) * 4096;
     const int c0 = half * (D / 2), left = args.Dr - c0;
-    const bool valid = ok && r < it.n_k;
+    const bool valid = ok && r < it.n_k, one = it.n_keys == 1;   // one key: dS is 0, not what dP - delta leaves
     if (it.slot < 0) {
       const long at = valid ? ((long)(it.k_row + r) * args.Hkv + kvh) * args.Dr + c0 : -1;
       pa::store_rows<D / 2>(buf, tDV + lane_off + c0, n_q > 0, 1.0f, args.dv, at, left, lane);
-      pa::store_rows<D / 2>(buf, tDK + lane_off + c0, n_q > 0, args.scale, args.dk, at, left, lane);
+      pa::store_rows<D / 2>(buf, tDK + lane_off + c0, n_q > 0 && !one, args.scale, args.dk, at, left, lane);
     } else {
       const long at = valid ? (((long)it.slot * args.Hkv + kvh) * 2 * kT + r) * args.Dr + c0 : -1;
       pa::store_rows32<D / 2>(buf, tDV + lane_off + c0, 1.0f, args.part, at, left, lane);
-      pa::store_rows32<D / 2>(buf, tDK + lane_off + c0, args.scale, args.part + (long)kT * args.Dr, at, left, lane);
+      pa::store_rows32<D / 2>(buf, tDK + lane_off + c0, one ? 0.f : args.scale, args.part + (long)kT * args.Dr, at, left, lane);
     }
   }
   tc_fence_before();
@@ -592,7 +592,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const float c2 = args.scale * pa::kLog2e;
     const int pos = min(r / G, it.n_q - 1);
     const bool in = r < G * P && r / G < it.n_q;
-    const int limit = args.causal ? min(it.n_keys, it.limit + pos) : it.n_keys;
+    int limit = args.causal ? min(it.n_keys, it.limit + pos) : it.n_keys;
+    if (limit == 1) limit = 0;                              // one key: dS is 0, not what dP - delta leaves
     const long row = (long)(it.q_row + r / G) * args.Hq + kvh * G + r % G;
     const float lse2 = in ? args.lse[row] * pa::kLog2e : 0.f;
     const float dlt = in ? args.delta[row] : 0.f;

@@ -250,7 +250,7 @@ def key_items(pack, group, kv_heads, causal, sms):
     begin = first[at] + part * size[at] * per
     n_q = np.where(cut[at], np.minimum(lq[at] - begin, size[at] * per), lq[at] - begin)
     out = np.stack([k_row[at], n_k[at], begin, pack.starts[seq][at] + begin, n_q, sees[at] - begin,
-                    np.where(cut[at], slot0[at] + part, -1), np.zeros_like(begin)], 1).reshape(-1, 8)
+                    np.where(cut[at], slot0[at] + part, -1), lk[at]], 1).reshape(-1, 8)
     return _longest_first(out, -(-n_q // per)), joins, int(parts[cut].sum())
 
 

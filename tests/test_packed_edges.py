@@ -205,3 +205,24 @@ def test_gpu_gradients_of_short_sequences(lengths, heads, kv, dim, causal):
     for g, w, r, n in zip(got, want, rounded, ("dq", "dk")):
         assert (g.double() - w).norm() <= 1.1 * (r - w).norm(), n
     ops.check_device_errors()
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,keys", [([1] * 11, None), ([1, 40, 1], [1, 1, 1]), ([3000], [1]), ([300, 1, 20], None)])
+def test_gpu_gradients_of_rows_with_one_key(lengths, keys, causal):
+    """A row that sees one key weighs it by 1 whatever the scores: its dq is zero, and the dk of a sequence of one
+    key.  Zero, not what two sums over the same products leave."""
+    pack = ops.SequencePack(lengths, keys)
+    q, k, v, do = tensors(pack, 8, 2, 128, "cuda", std=3.0)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(Fn.packed_attention(*leaves, pack, causal=causal), leaves, do)
+    for a0, a, b0, b in zip(pack.starts, pack.lengths, pack.key_starts, pack.key_lengths):
+        sees = torch.arange(b - a + 1, b + 1).clamp(min=0) if causal else torch.full((a,), int(b))
+        at = torch.arange(a0, a0 + a)[sees <= 1]
+        assert not dq[at.cuda()].any()
+        rest = torch.arange(a0, a0 + a)[sees > 1]
+        assert len(rest) == 0 or dq[rest.cuda()].any(2).all()
+        if b == 1:
+            assert not dk[b0:b0 + 1].any() and dv[b0:b0 + 1].any()
+    ops.check_device_errors()
