@@ -435,8 +435,9 @@ class _PackedAttnFn(torch.autograd.Function):
 def packed_attention(q, k, v, pack, causal: bool = True, scale=None, rel_bias=None):
     """Attention inside the sequences of ``pack`` (see :func:`ops.packed_attention`), under autograd
     too: q [Nq, heads, D], k and v [Nk, key heads, D] -> [Nq, heads, D], bf16 on the GPU.  The gradient
-    of a shared key head is the sum over its query heads.  ``rel_bias`` has no gradient and allows
-    none: with it, call without autograd.  First derivatives only."""
+    of a shared key head is the sum over its query heads.  On the GPU a call with ``rel_bias`` records no
+    graph and raises where one is asked for (the CPU's form gives all gradients), and derivatives are first ones
+    only."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if not q.is_cuda or transformed(q, k, v, rel_bias):
         ops.packed.check_packed(q, k, v, pack, rel_bias, scale=scale)

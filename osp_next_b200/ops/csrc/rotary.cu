@@ -9,8 +9,8 @@
 // serve all heads of q and k.  A warp takes one token: its lanes hold the cosines and sines of the
 // vector pieces that they own in registers and pass over the heads, so that a table entry is read once
 // per token and not once per head, with four heads' loads in flight.  The inverse (gradients) turns by -s.
-// 80640 tokens x 80 heads of 128 in bf16: 493 us, 6.8 TB/s (one head at a time 570); 14039 x 20 in fp32,
-// half of each head: 51 us, 5.7 TB/s (67).
+// 80640 tokens x 80 heads of 128 in bf16: 492 us, 6.8 TB/s (one head at a time 570); 14039 x 20 in fp32,
+// half of each head: 53 us, 5.4 TB/s (67).
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>

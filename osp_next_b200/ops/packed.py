@@ -47,8 +47,8 @@ class SequencePack:
     Sequences must not overlap.  Rows of no sequence are zeros in results.
 
     Work lists for the kernels are laid out on the device at the first call with each kind (forward,
-    backward, number of heads) and kept here: make that call before capturing a graph, and keep the
-    pack as long as the graph."""
+    backward, number of heads), which waits for their upload, and kept here: make that call before
+    capturing a graph, and keep the pack as long as the graph."""
 
     def __init__(self, lengths: Sequence[int], key_lengths: Optional[Sequence[int]] = None,
                  starts: Optional[Sequence[int]] = None, key_starts: Optional[Sequence[int]] = None, device="cuda"):
