@@ -320,7 +320,8 @@ def qk_norm_rope_packed(qkv, wq, wk, pos, freqs, num_heads: int, eps: float):
 
 
 def _rope_kernel(*ts) -> bool:
-    return all(t.is_cuda and t.dtype in (_BF16, torch.float16, torch.float32) for t in ts) and not transformed(*ts)
+    return not transformed(*ts) and all(t.is_cuda and t.dtype in (_BF16, torch.float16, torch.float32)
+                                        and t.shape[-1] <= 256 for t in ts)
 
 
 def apply_rope(x, pos, freqs):
@@ -332,9 +333,9 @@ def apply_rope(x, pos, freqs):
 
 
 def apply_rope_qk(q, k, pos, freqs):
-    """:func:`apply_rope` of heads without q/k norm in one launch, forward and backward; in q's own type on the
-    GPU, which spares the rounding of fp32 results."""
-    if not _rope_kernel(q, k) or q.dtype != k.dtype:
+    """:func:`apply_rope` of heads without q/k norm; q and k in bf16 on the GPU in one launch and as bf16, which
+    spares the rounding of fp32 results."""
+    if not _rope_kernel(q, k) or not q.dtype == k.dtype == _BF16:
         return apply_rope(q, pos, freqs), apply_rope(k, pos, freqs)
     return rotary(q, k, pos.to(q.device), ops.rope_cos_sin(freqs, q.device), "interleaved", ref.rope_split(q.shape[-1]))
 
@@ -460,8 +461,9 @@ def computes_bf16(x) -> bool:
 def as_made(m, cls) -> bool:
     """Whether a layer computes what its class does: that class itself (no adapter, no quantised or
     parametrised form), no hooks, no forward of its own.  Its parameters may then stand for it."""
-    return (type(m) is cls and not torch.nn.modules.module._has_any_global_hook() and "forward" not in m.__dict__ and not m._forward_hooks and not m._forward_pre_hooks
-            and not m._backward_hooks and not m._backward_pre_hooks)
+    hooks = (m._forward_hooks, m._forward_pre_hooks, m._backward_hooks, m._backward_pre_hooks) if type(m) is cls else ()
+    return (type(m) is cls and "forward" not in m.__dict__ and not any(hooks)
+            and not torch.nn.modules.module._has_any_global_hook())
 
 
 def plain_linears(*ms) -> bool:
@@ -514,8 +516,9 @@ class _GatedFFNFn(torch.autograd.Function):
 
 def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu"):
     """``(act(x W_gate^T) * (x W_up^T)) W_down^T`` (see :func:`ops.gated_ffn`), under autograd too; bf16 on
-    the GPU, where gradients come in their tensor's type (second derivatives by elementary operations).  The projections are kept
-    for them in 16 bits, within 2^-10 of values from 2^-20 to 2^16 and 2^-7 of smaller and larger ones."""
+    the GPU, where gradients come in their tensor's type (second derivatives by elementary operations).
+    The projections are kept for them in 16 bits, within 2^-10 of values from 2^-20 to 2^16 and 2^-7 of
+    smaller and larger ones."""
     if not x.is_cuda or transformed(x, w_gate, w_up, w_down):
         ops.gated.check_gated(x, w_gate, w_up, act, w_down, "gated_ffn")
         return ref.gated_ffn(x, w_gate, w_up, w_down, act)

@@ -299,8 +299,9 @@ def packed_attention(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
 
     q [Nq, heads, D], k and v [Nk, key heads, D] (bf16 on the GPU; rows of any stride, views of a
     fused projection among them).  Heads h G .. (h + 1) G - 1 of q read key head h, G = heads / key
-    heads.  D: multiples of 8 up to 128.  ``scale``: any finite number.  Query i of a sequence with lq queries and lk keys stands at
-    position i + lk - lq; ``causal`` queries see the keys up to their position.  ``rel_bias`` fp32
+    heads.  D: multiples of 8 up to 128.  ``scale``: any finite number (1 / sqrt(D) without one).  Query i of
+    a sequence with lq queries and lk keys stands at position i + lk - lq; ``causal`` queries see the keys up
+    to their position.  ``rel_bias`` fp32
     [heads, 2 M - 1] adds ``rel_bias[h, key position - query position + M - 1]``, finite values; on the GPU
     those beyond +-6.9e37 count as that, so that the type's lowest value hides a key.
     A query that sees no key gives zeros and a log-sum-exp of -inf; so do rows of no sequence.

@@ -422,7 +422,7 @@ def rotary(x, pos, table, layout: str, sections, inverse: bool = False):
         raise IndexError(f"rotary: positions 0 to {table.shape[0] - 1}, got {int(pos.min())} to {int(pos.max())}")
     axis = torch.repeat_interleave(torch.tensor(sections, device=pos.device))
     pair = torch.arange(table.shape[1], device=pos.device)
-    cs = table[pos[:, axis], pair[None]]                                     # [n, pairs, 2]
+    cs = table[pos[:, axis], pair[None]]                                            # [n, pairs, 2]
     acc = torch.float64 if x.dtype == torch.float64 else torch.float32
     c, s = cs[:, None, :, 0].to(acc), cs[:, None, :, 1].to(acc)
     s = -s if inverse else s

@@ -310,8 +310,8 @@ ATTENTION_NAME = "osp_packed"          # the packed kernel's name among transfor
 
 class _PackedMask:
     """What the text layers get in the place of a mask tensor: each row's tokens as one packed sequence.  It
-    is an argument of every layer, so that a layer recomputed in the backward pass sees the same one.  ``library``: makes
-    the mask of a layer that the packed kernel does not take."""
+    is an argument of every layer, so that a layer recomputed in the backward pass sees the same one.
+    ``library``: makes the mask of a layer that the packed kernel does not take."""
 
     def __init__(self, first, lengths, width: int, library):
         self._rows = (lengths, [i * width + f for i, f in enumerate(first)])

@@ -428,3 +428,24 @@ def test_gpu_t5_feed_forward_as_its_layers_would(how):
         assert got.dtype == want.dtype == torch.float16 and torch.equal(got, want)
         with torch.autocast("cuda", torch.bfloat16):
             assert ffn(x).dtype == torch.bfloat16
+
+
+@gpu
+@pytest.mark.parametrize("dim", [96, 288])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gpu_apply_rope_qk(dtype, dim):
+    """One launch for q and k in bf16, and the same bf16 values as from fp32; heads of any size."""
+    from osp_next_b200.models import functional as Fn
+    from osp_next_b200.ops import reference as ref
+    pos, freqs = torch.randint(0, 60, (50, 3), device="cuda"), ref.rope_freqs(dim).cuda()
+    q, k = (torch.randn(2, 50, 3, dim, device="cuda").to(dtype) for _ in range(2))
+    n0 = ops._ext.launch_count()
+    got = Fn.apply_rope_qk(q, k, pos, freqs)
+    launches = ops._ext.launch_count() - n0
+    assert launches == (0 if dim > 256 else 1 if dtype == torch.bfloat16 else 2)
+    for g, x in zip(got, (q, k)):
+        one = Fn.apply_rope(x, pos, freqs)
+        assert one.dtype == torch.float32 and torch.equal(g.bfloat16(), one.bfloat16())
+        # angles to 60 in fp32 on one side: half a step of 2^-18 each
+        assert torch.allclose(one, ref.apply_rope(x, pos, freqs), atol=1e-4)
+    ops.check_device_errors()
