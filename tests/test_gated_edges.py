@@ -123,3 +123,31 @@ def test_gpu_tiled_form(act, M, K, F, C):
             assert got.dtype == dtype
             close(got, want[n], n)
     ops.check_device_errors()
+
+
+@gpu
+def test_gpu_calls_at_once():
+    """Both forms of the block, rotary and packed attention on streams of their own at once: what they give alone."""
+    w = [ffn_tensors(1, K, F, seed=i)[1:4] for i, (K, F) in enumerate(((1024, 2048), (512, 4096), (2048, 512)))]
+    xs = [[ffn_tensors(m, k[0].shape[1], 8, seed=m)[0] for m in (1, 40, 154, 256, 3000)] for k in w]
+    pack = ops.SequencePack([300, 5, 77])
+    q = torch.randn(382, 8, 64, device="cuda").bfloat16()
+    table, pos = ops.rotary_table(64, 400), torch.arange(382, device="cuda")
+
+    def work(i):
+        out = [ops.gated_ffn(x, *w[i]) for x in xs[i]]
+        z = ops.rotary(q, None, pos, table)[0]
+        return out + [z, ops.packed_attention(z, z, z, pack, causal=bool(i % 2))]
+    want = [work(i) for i in range(3)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[], [], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(3):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+    ops.check_device_errors()
